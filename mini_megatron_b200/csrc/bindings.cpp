@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <climits>
 #include <cmath>
 #include <vector>
 
@@ -365,6 +366,216 @@ Tensor flash_attn_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, 
 Tensor flash_attn_bwd_v1(const Tensor& dout, const Tensor& qkv, const Tensor& out, const Tensor& lse, int64_t B,
                          int64_t S, int64_t nh, int64_t d) {
   return flash_attn_bwd_impl(dout, qkv, out, lse, B, S, nh, d, true);
+}
+
+// ----------------------------------------------------------------- packed rows of documents
+// ids [B, S] int64 (tokens, or document ids with by_change) or none, marks [B, S] bool / uint8 or none, lengths [B]
+// int32 or none -> positions, start, end [B, S] int32 and the attention kernels' tile tables (rows, qstat, krange).
+std::vector<Tensor> document_plan(const c10::optional<Tensor>& ids, int64_t eod, bool by_change,
+                                  const c10::optional<Tensor>& marks, const c10::optional<Tensor>& lengths, int64_t B,
+                                  int64_t S, const at::Device& device) {
+  TORCH_CHECK(device.is_cuda(), "document_plan: device must be CUDA");
+  TORCH_CHECK(B >= 1 && S >= 1 && S <= mmb::document_plan_max_len(), "document_plan: rows of 1 to ",
+              mmb::document_plan_max_len(), " tokens, got B = ", B, ", S = ", S);
+  TORCH_CHECK(B <= (1 << 24), "document_plan: too many rows");
+  const at::cuda::CUDAGuard guard(device);
+  const long* ip = nullptr;
+  long ld_ids = 0, ld_marks = 0;
+  const unsigned char* mp = nullptr;
+  const int* lp = nullptr;
+  if (ids.has_value()) {
+    TORCH_CHECK(ids->device() == device && ids->scalar_type() == at::kLong && ids->dim() == 2 && ids->size(0) == B &&
+                    ids->size(1) == S && (S == 1 || ids->stride(1) == 1),
+                "document_plan: ids must be [B, S] int64 on the device, dense in the last dimension");
+    ip = reinterpret_cast<const long*>(ids->data_ptr<int64_t>());
+    ld_ids = ids->stride(0);
+  }
+  if (marks.has_value()) {
+    TORCH_CHECK(marks->device() == device && (marks->scalar_type() == at::kBool || marks->scalar_type() == at::kByte) &&
+                    marks->dim() == 2 && marks->size(0) == B && marks->size(1) == S && (S == 1 || marks->stride(1) == 1),
+                "document_plan: marks must be [B, S] bool on the device, dense in the last dimension");
+    mp = static_cast<const unsigned char*>(marks->data_ptr());
+    ld_marks = marks->stride(0);
+  }
+  if (lengths.has_value()) {
+    TORCH_CHECK(lengths->device() == device && lengths->scalar_type() == at::kInt && lengths->dim() == 1 &&
+                    lengths->size(0) == B && lengths->is_contiguous(),
+                "document_plan: lengths must be [B] int32 on the device");
+    lp = lengths->data_ptr<int>();
+  }
+  const auto opt = at::TensorOptions().dtype(at::kInt).device(device);
+  const int64_t n_t = (S + 127) / 128;
+  Tensor positions = at::empty({B, S}, opt), start = at::empty({B, S}, opt), end = at::empty({B, S}, opt);
+  Tensor rows = at::empty({B, n_t, 2, 128}, opt), qstat = at::empty({B, n_t, 4}, opt),
+         krange = at::empty({B, n_t, 2}, opt);
+  MMB_CHECK_RC(mmb::document_plan(ip, ld_ids, eod, by_change ? 1 : 0, mp, ld_marks, lp, (int)B, (int)S,
+                                  positions.data_ptr<int>(), start.data_ptr<int>(), end.data_ptr<int>(),
+                                  rows.data_ptr<int>(), qstat.data_ptr<int>(), krange.data_ptr<int>(), cur_stream()),
+               "document_plan");
+  return {positions, start, end, rows, qstat, krange};
+}
+
+// ----------------------------------------------------------------- rotary positions
+// x, y [B, S, heads * d] bf16 / fp32 (y may be x), positions [B, S] or [S] int32 / int64 or none, freqs [rot / 2] fp64.
+void rotary(const Tensor& x, Tensor& y, const c10::optional<Tensor>& positions, const Tensor& freqs, double magnitude,
+            bool interleaved, int64_t d, int64_t rot, int64_t heads_rot, bool inverse) {
+  check_cuda(x, "x");
+  const bool f32 = x.scalar_type() == at::kFloat;
+  TORCH_CHECK(f32 || x.scalar_type() == at::kBFloat16, "rotary: x must be bf16 or fp32");
+  TORCH_CHECK(x.dim() == 3 && y.dim() == 3 && x.sizes() == y.sizes() && y.scalar_type() == x.scalar_type() &&
+                  y.device() == x.device(),
+              "rotary: x and y must be [B, S, heads * head_dim] of one type and device");
+  const int64_t B = x.size(0), S = x.size(1), W = x.size(2), per = 16 / x.element_size();
+  TORCH_CHECK(d >= 1 && W % d == 0 && d % per == 0, "rotary: head_dim ", d, " does not cut the last dimension ", W,
+              " into heads of whole 16-byte units");
+  const int64_t heads = W / d;
+  TORCH_CHECK(rot >= 2 * per && rot <= d && rot % (2 * per) == 0, "rotary: rotary_dim must be a multiple of ", 2 * per,
+              " up to head_dim for this type, got ", rot);
+  TORCH_CHECK(heads_rot >= 1 && heads_rot <= heads, "rotary: num_heads must be 1 to ", heads, ", got ", heads_rot);
+  TORCH_CHECK(freqs.device() == x.device() && freqs.scalar_type() == at::kDouble && freqs.is_contiguous() &&
+                  freqs.numel() == rot / 2,
+              "rotary: freqs must be [rotary_dim / 2] fp64 on x's device");
+  TORCH_CHECK(S <= INT_MAX && d <= 4096 && heads <= (1 << 20), "rotary: too large");
+  if (B == 0 || S == 0) return;
+  for (const Tensor* t : {&x, static_cast<const Tensor*>(&y)}) {
+    TORCH_CHECK(t->stride(2) == 1 && (S == 1 || t->stride(1) % per == 0) && (B == 1 || t->stride(0) % per == 0) &&
+                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                "rotary: tensors must be dense in the last dimension, with rows on 16-byte boundaries");
+  }
+  if (x.data_ptr() == y.data_ptr()) {
+    TORCH_CHECK(x.strides() == y.strides(), "rotary: in place needs the same strides");
+  } else {
+    const auto first = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+    const auto last = [&](const Tensor& t) {
+      return first(t) + ((B - 1) * t.stride(0) + (S - 1) * t.stride(1) + W) * t.element_size();
+    };
+    TORCH_CHECK(last(x) <= first(y) || last(y) <= first(x),
+                "rotary: x and y must be the same memory or lie apart (their address ranges meet)");
+  }
+  {
+    const int64_t ss = S > 1 ? y.stride(1) : W, sb = B > 1 ? y.stride(0) : W;
+    TORCH_CHECK((ss >= W && (B == 1 || sb >= (S - 1) * ss + W)) || (sb >= W && ss >= (B - 1) * sb + W),
+                "rotary: rows of y overlap one another");
+  }
+  const at::cuda::CUDAGuard guard(x.device());
+  const void* pp = nullptr;
+  int64_t pos_sb = 0;
+  bool pos64 = false;
+  if (positions.has_value()) {
+    const Tensor& p = *positions;
+    pos64 = p.scalar_type() == at::kLong;
+    TORCH_CHECK(p.device() == x.device() && (pos64 || p.scalar_type() == at::kInt) &&
+                    ((p.dim() == 1 && p.size(0) == S) || (p.dim() == 2 && p.size(0) == B && p.size(1) == S)) &&
+                    (S == 1 || p.stride(-1) == 1),
+                "rotary: positions must be [S] or [B, S] int32 or int64 on x's device, dense in the last dimension");
+    pp = p.data_ptr();
+    pos_sb = p.dim() == 2 ? p.stride(0) : 0;
+  }
+  MMB_CHECK_RC(mmb::rotary(x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(), y.stride(0), y.stride(1), f32, pp,
+                           pos64, pos_sb, freqs.data_ptr<double>(), (float)magnitude, inverse ? -1.f : 1.f,
+                           interleaved, B, (int)S, (int)d, (int)rot, (int)heads_rot, (int)heads, num_sms(),
+                           cur_stream()),
+               "rotary");
+}
+
+// ----------------------------------------------------------------- masked attention
+// A [B, S, W] bf16 activation that the kernels can address with TMA; strides of dimensions of size 1 are replaced.
+void token_strides(const Tensor& t, const char* name, int64_t& ss, int64_t& sb) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 3, name, " must be [B, S, heads * head_dim] bf16");
+  const int64_t B = t.size(0), S = t.size(1), W = t.size(2);
+  ss = S > 1 ? t.stride(1) : W;
+  sb = B > 1 ? t.stride(0) : S * ss;
+  TORCH_CHECK(t.stride(2) == 1 && ss >= W && ss % 8 == 0 && sb >= 1 && sb % 8 == 0 && ss < (1ll << 38) &&
+                  sb < (1ll << 38) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              name, " must be dense in the last dimension, with rows on 16-byte boundaries");
+}
+
+mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, const c10::optional<Tensor>& rows,
+                        const c10::optional<Tensor>& qstat, const c10::optional<Tensor>& krange,
+                        const c10::optional<Tensor>& slopes, double cap, double scale) {
+  mmb::AttnCall c{};
+  int64_t ss, sb;
+  TORCH_CHECK(d == 64 || d == 128, "attention supports head_dim 64 and 128, got ", d);
+  TORCH_CHECK(nkv >= 1 && nh >= nkv && nh % nkv == 0, "attention: num_heads (", nh,
+              ") must be a positive multiple of num_kv_heads (", nkv, ")");
+  token_strides(qkv, "qkv", ss, sb);
+  const int64_t B = qkv.size(0), S = qkv.size(1);
+  TORCH_CHECK(qkv.size(2) == (nh + 2 * nkv) * d, "attention: qkv's last dimension must be (num_heads + 2 num_kv_heads)",
+              " * head_dim = ", (nh + 2 * nkv) * d, ", got ", qkv.size(2));
+  TORCH_CHECK(S <= INT_MAX - 256 && B <= INT_MAX && nh <= (1 << 20), "attention: too large");
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "attention: softmax_scale must be positive and finite, got ", scale);
+  TORCH_CHECK(cap >= 0 && cap <= 1000, "attention: softcap must be at most 1000, got ", cap);
+  c.qkv = qkv.data_ptr();
+  c.qkv_ss = ss;
+  c.qkv_sb = sb;
+  c.B = (int)B;
+  c.S = (int)S;
+  c.nh = (int)nh;
+  c.nkv = (int)nkv;
+  c.d = (int)d;
+  c.cap = (float)cap;
+  c.scale = (float)scale;
+  if (rows.has_value()) {
+    const int64_t n_t = (S + 127) / 128;
+    TORCH_CHECK(qstat.has_value() && krange.has_value(), "attention: incomplete plan");
+    for (const Tensor* t : {&*rows, &*qstat, &*krange})
+      TORCH_CHECK(t->device() == qkv.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
+                  "attention: the plan must be on qkv's device");
+    TORCH_CHECK(rows->numel() == B * n_t * 256 && qstat->numel() == B * n_t * 4 && krange->numel() == B * n_t * 2,
+                "attention: the plan was made for other rows than qkv's [", B, ", ", S, "]");
+    c.rows = rows->data_ptr<int>();
+    c.qstat = qstat->data_ptr<int>();
+    c.krange = krange->data_ptr<int>();
+  }
+  if (slopes.has_value()) {
+    TORCH_CHECK(slopes->device() == qkv.device() && slopes->scalar_type() == at::kFloat && slopes->is_contiguous() &&
+                    slopes->dim() == 1 && slopes->size(0) == nh,
+                "attention: alibi_slopes must be [num_heads] fp32 on qkv's device");
+    c.slopes = slopes->data_ptr<float>();
+  }
+  return c;
+}
+
+std::vector<Tensor> masked_attn_fwd(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d,
+                                    const c10::optional<Tensor>& rows, const c10::optional<Tensor>& qstat,
+                                    const c10::optional<Tensor>& krange, const c10::optional<Tensor>& slopes,
+                                    double cap, double scale) {
+  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, rows, qstat, krange, slopes, cap, scale);
+  const at::cuda::CUDAGuard guard(qkv.device());
+  Tensor out = at::empty({c.B, c.S, nh * d}, qkv.options());
+  Tensor lse = at::empty({c.B, nh, c.S}, qkv.options().dtype(at::kFloat));
+  if (out.numel() == 0) return {out, lse};
+  MMB_CHECK_RC(mmb::masked_attn_fwd(c, out.data_ptr(), lse.data_ptr<float>(), error_word(), num_sms(), cur_stream()),
+               "masked_attn_fwd");
+  return {out, lse};
+}
+
+Tensor masked_attn_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, const Tensor& lse, int64_t nh,
+                       int64_t nkv, int64_t d, const c10::optional<Tensor>& rows, const c10::optional<Tensor>& qstat,
+                       const c10::optional<Tensor>& krange, const c10::optional<Tensor>& slopes, double cap,
+                       double scale) {
+  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, rows, qstat, krange, slopes, cap, scale);
+  const at::cuda::CUDAGuard guard(qkv.device());
+  int64_t do_ss, do_sb;
+  token_strides(dout, "dctx", do_ss, do_sb);
+  check_bf16(out, "ctx");
+  check_f32(lse, "lse");
+  TORCH_CHECK(dout.device() == qkv.device() && out.device() == qkv.device() && lse.device() == qkv.device(),
+              "attention: all tensors must be on one device");
+  TORCH_CHECK(dout.size(0) == c.B && dout.size(1) == c.S && dout.size(2) == nh * d && out.sizes() == dout.sizes() &&
+                  lse.dim() == 3 && lse.size(0) == c.B && lse.size(1) == nh && lse.size(2) == c.S,
+              "attention: dctx and ctx must be [B, S, num_heads * head_dim] and lse [B, num_heads, S] of the forward");
+  Tensor dqkv = at::empty({c.B, c.S, (nh + 2 * nkv) * d}, qkv.options());
+  if (dqkv.numel() == 0) return dqkv;
+  Tensor ld = at::empty({c.B, nh, (c.S + 127) / 128, 256}, lse.options());
+  MMB_CHECK_RC(mmb::masked_attn_dq(c, dout.data_ptr(), do_ss, do_sb, out.data_ptr(), lse.data_ptr<float>(),
+                                   ld.data_ptr<float>(), dqkv.data_ptr(), error_word(), num_sms(), cur_stream()),
+               "masked_attn_dq");
+  MMB_CHECK_RC(mmb::masked_attn_dkv(c, dout.data_ptr(), do_ss, do_sb, ld.data_ptr<float>(), dqkv.data_ptr(),
+                                    error_word(), num_sms(), cur_stream()),
+               "masked_attn_dkv");
+  return dqkv;
 }
 
 // ----------------------------------------------------------------- symmetric memory
@@ -865,6 +1076,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("EPI_CE_STATS") = (int)mmb::EPI_CE_STATS;
   m.attr("EPI_PUSH_BF16") = (int)mmb::EPI_PUSH_BF16;
   m.def("num_sms", &num_sms);
+  m.def("document_plan", &document_plan, py::arg("ids"), py::arg("eod"), py::arg("by_change"), py::arg("marks"),
+        py::arg("lengths"), py::arg("B"), py::arg("S"), py::arg("device"));
+  m.def("document_plan_max_len", &mmb::document_plan_max_len);
+  m.def("rotary", &rotary, py::arg("x"), py::arg("y"), py::arg("positions"), py::arg("freqs"), py::arg("magnitude"),
+        py::arg("interleaved"), py::arg("head_dim"), py::arg("rotary_dim"), py::arg("num_heads"),
+        py::arg("inverse") = false);
+  m.def("masked_attn_fwd", &masked_attn_fwd, py::arg("qkv"), py::arg("num_heads"), py::arg("num_kv_heads"),
+        py::arg("head_dim"), py::arg("rows"), py::arg("qstat"), py::arg("krange"), py::arg("slopes"), py::arg("cap"),
+        py::arg("scale"));
+  m.def("masked_attn_bwd", &masked_attn_bwd, py::arg("dctx"), py::arg("qkv"), py::arg("ctx"), py::arg("lse"),
+        py::arg("num_heads"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("rows"), py::arg("qstat"),
+        py::arg("krange"), py::arg("slopes"), py::arg("cap"), py::arg("scale"));
   m.def("flash_attn_fwd", &flash_attn_fwd);
   m.def("flash_attn_fwd_v1", &flash_attn_fwd_v1, "previous one-tile-per-CTA forward (comparison only)");
   m.def("flash_attn_bwd", &flash_attn_bwd);

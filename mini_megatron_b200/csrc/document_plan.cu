@@ -1,0 +1,341 @@
+// Positions and visible key intervals of packed rows.
+//
+// A row of S tokens holds documents one after another and possibly padding at
+// its end.  Token i sees the keys [start_i, end_i) of its own row:
+//
+//   start_i = the largest document start <= i
+//   end_i   = i + 1, or, while every token from start_i to i is marked as
+//             prefix, the first index after i that is unmarked, begins a
+//             document, is padding, or is S
+//   position_i = i - start_i
+//
+// Padding sees nothing: start = end = position = 0.  All three are scans of
+// one row: a running maximum of document starts, a running maximum of
+// unmarked indices (a token is in its prefix iff that is < start_i), and a
+// running minimum from the right of the indices that stop a prefix.
+//
+// For the attention kernels the same pass writes, for every 128-token tile,
+// the extremes of start and end (which key tiles a query tile needs, and which
+// of them need no mask), a tile-padded copy of (start, end) that a bulk copy
+// can fetch, and, for every key tile, the query tiles that see it.
+//
+// One cluster of 1 to 8 CTAs per row, the row cut into as many chunks; a
+// thread owns 4 consecutive tokens, so a warp owns one 128-token tile and the
+// tile statistics are warp reductions.  Each CTA first reduces its chunk, the
+// chunk results cross the cluster through distributed shared memory, and a
+// second sweep (right to left) scans and writes.  The work is a few bytes per
+// token: latency bounds it, so the row is spread over CTAs as soon as one CTA
+// would need more than one sweep step (4096 tokens).
+#include "common.cuh"
+#include "ops.h"
+
+#include <algorithm>
+#include <climits>
+
+namespace mmb {
+namespace docplan {
+
+constexpr int kThreads = 1024;
+constexpr int kPer = 4;                      // tokens per thread: 32 lanes x 4 = one 128-token tile per warp
+constexpr int kStep = kThreads * kPer;       // 4096 tokens per sweep step
+constexpr int kMaxCtas = 8;                  // portable cluster size
+constexpr int kMaxSteps = 64;                // per CTA: rows of up to 2 Mi tokens
+
+struct Args {
+  const long* ids;        // [B, S] tokens or document ids (nullptr: one document per row)
+  long ld_ids;
+  long eod;
+  int by_change;          // 1: a document starts where the id changes; 0: after a token equal to eod
+  const uint8_t* marks;   // [B, S] prefix marks or nullptr
+  long ld_marks;
+  const int* lengths;     // [B] or nullptr
+  int S, n_t, chunk;      // chunk: tokens per CTA (a multiple of kStep)
+  int* positions;         // [B, S]
+  int* start;
+  int* end;
+  int* rows;              // [B, n_t, 2, 128]
+  int4* qstat;            // [B, n_t] {min start, max end, max start, min end}; no visible key: {INT_MAX, 0, ..}
+  int2* krange;           // [B, n_t] {first, last} query tile that sees the key tile (first > last: none)
+};
+
+struct Agg {
+  int ds, lu, stop;  // max document start, max unmarked index, min stopping index
+};
+
+__device__ __forceinline__ int warp_max_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = max(v, u);
+  }
+  return v;
+}
+__device__ __forceinline__ int warp_min_scan_right(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_down_sync(0xffffffffu, v, o);
+    if (lane + o < 32) v = min(v, u);
+  }
+  return v;
+}
+
+// First (document start) and plain (unmarked or padding) flags of the thread's four tokens.
+__device__ __forceinline__ void load_flags(const Args& a, int b, int i0, int len, bool (&first)[kPer],
+                                           bool (&plain)[kPer]) {
+  long prev = 0;
+  if (a.ids && i0 > 0 && i0 < a.S) prev = a.ids[b * a.ld_ids + i0 - 1];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const int i = i0 + e;
+    first[e] = (i == 0);
+    plain[e] = true;
+    if (i < a.S) {
+      if (a.ids) {
+        const long cur = a.ids[b * a.ld_ids + i];
+        if (i > 0) first[e] = a.by_change ? (cur != prev) : (prev == a.eod);
+        prev = cur;
+      }
+      if (a.marks && i < len) plain[e] = a.marks[b * a.ld_marks + i] == 0;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
+  __shared__ Agg s_warp[32];
+  __shared__ Agg s_step[kMaxSteps];  // reduction of every step of this CTA's chunk
+  __shared__ Agg s_cta;              // reduction of the chunk (read by the other CTAs of the cluster)
+  const int n_cta = (a.S + a.chunk - 1) / a.chunk;
+  const int b = blockIdx.x / n_cta, rank = blockIdx.x % n_cta;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int c0 = rank * a.chunk, c1 = min(c0 + a.chunk, a.n_t * 128);
+  const int n_steps = (c1 - c0 + kStep - 1) / kStep;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
+
+  // ---- reduce the chunk, step by step
+  for (int st = 0; st < n_steps; ++st) {
+    const int i0 = c0 + st * kStep + tid * kPer;
+    bool first[kPer], plain[kPer];
+    load_flags(a, b, i0, len, first, plain);
+    Agg g{-1, -1, a.S};
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int i = i0 + e;
+      if (i >= a.S) continue;
+      if (first[e]) g.ds = i;
+      if (plain[e]) g.lu = i;
+      if (first[e] || plain[e]) g.stop = min(g.stop, i);
+    }
+    g.ds = __reduce_max_sync(0xffffffffu, g.ds);
+    g.lu = __reduce_max_sync(0xffffffffu, g.lu);
+    g.stop = __reduce_min_sync(0xffffffffu, g.stop);
+    if (lane == 0) s_warp[warp] = g;
+    __syncthreads();
+    if (warp == 0) {
+      Agg w = s_warp[lane];
+      w.ds = __reduce_max_sync(0xffffffffu, w.ds);
+      w.lu = __reduce_max_sync(0xffffffffu, w.lu);
+      w.stop = __reduce_min_sync(0xffffffffu, w.stop);
+      if (lane == 0) {
+        s_step[st] = w;
+        if (st == 0) {
+          s_cta = w;
+        } else {
+          s_cta.ds = max(s_cta.ds, w.ds);
+          s_cta.lu = max(s_cta.lu, w.lu);
+          s_cta.stop = min(s_cta.stop, w.stop);
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // ---- what lies left and right of this chunk
+  Agg left{-1, -1, a.S}, right{-1, -1, a.S};
+  if (n_cta > 1) {
+    cluster_sync_all();
+    for (int r = 0; r < n_cta; ++r) {
+      if (r == rank) continue;
+      const uint32_t addr = cluster_addr(&s_cta, r);
+      int ds, lu, stop;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(ds) : "r"(addr) : "memory");
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(lu) : "r"(addr + 4) : "memory");
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(stop) : "r"(addr + 8) : "memory");
+      if (r < rank) {
+        left.ds = max(left.ds, ds);
+        left.lu = max(left.lu, lu);
+      } else {
+        right.stop = min(right.stop, stop);
+      }
+    }
+  }
+
+  // ---- scan and write, right to left
+  int stop_right = right.stop;
+  for (int st = n_steps - 1; st >= 0; --st) {
+    int ds_left = left.ds, lu_left = left.lu;
+    for (int u = 0; u < st; ++u) {
+      ds_left = max(ds_left, s_step[u].ds);
+      lu_left = max(lu_left, s_step[u].lu);
+    }
+    const int i0 = c0 + st * kStep + tid * kPer;
+    bool first[kPer], plain[kPer];
+    load_flags(a, b, i0, len, first, plain);
+    int ds[kPer], lu[kPer], stop[kPer];  // inclusive from the left / stop: first stopping index > i
+    int rd = -1, rl = -1;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int i = i0 + e;
+      if (i < a.S && first[e]) rd = i;
+      if (i < a.S && plain[e]) rl = i;
+      ds[e] = rd;
+      lu[e] = rl;
+    }
+    int rs = a.S;
+#pragma unroll
+    for (int e = kPer - 1; e >= 0; --e) {
+      stop[e] = rs;
+      if (i0 + e < a.S && (first[e] || plain[e])) rs = i0 + e;
+    }
+    const int sd = warp_max_scan(rd, lane), sl = warp_max_scan(rl, lane), ss = warp_min_scan_right(rs, lane);
+    __syncthreads();  // s_warp of the previous sweep has been read
+    if (lane == 31) {
+      s_warp[warp].ds = sd;
+      s_warp[warp].lu = sl;
+    }
+    if (lane == 0) s_warp[warp].stop = ss;
+    __syncthreads();
+    int xd = ds_left, xl = lu_left, xs = stop_right;
+    {
+      // the warps left of this one (starts, unmarked) and right of it (stops)
+      const Agg w = s_warp[lane];
+      xd = max(xd, __reduce_max_sync(0xffffffffu, lane < warp ? w.ds : -1));
+      xl = max(xl, __reduce_max_sync(0xffffffffu, lane < warp ? w.lu : -1));
+      xs = min(xs, __reduce_min_sync(0xffffffffu, lane > warp ? w.stop : a.S));
+    }
+    int pd = __shfl_up_sync(0xffffffffu, sd, 1), pl = __shfl_up_sync(0xffffffffu, sl, 1);
+    int ns = __shfl_down_sync(0xffffffffu, ss, 1);
+    if (lane == 0) pd = pl = -1;
+    if (lane == 31) ns = a.S;
+    xd = max(xd, pd);
+    xl = max(xl, pl);
+    xs = min(xs, ns);
+    stop_right = min(stop_right, s_step[st].stop);
+
+    int smin = INT_MAX, emax = 0, smax = 0, emin = INT_MAX;
+    int vs[kPer], ve[kPer], vp[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int i = i0 + e;
+      vs[e] = ve[e] = vp[e] = 0;
+      if (i < len) {
+        vs[e] = max(xd, ds[e]);
+        ve[e] = max(xl, lu[e]) < vs[e] ? min(xs, stop[e]) : i + 1;
+        vp[e] = i - vs[e];
+        smin = min(smin, vs[e]);
+        emax = max(emax, ve[e]);
+      }
+      if (i < a.S) {
+        smax = max(smax, vs[e]);
+        emin = min(emin, ve[e]);
+      }
+    }
+    const int tile = i0 / 128;  // one tile per warp
+    if (tile < a.n_t) {
+      const size_t row0 = (size_t)b * a.S;
+      if (i0 + kPer <= a.S && (a.S & 3) == 0) {
+        *reinterpret_cast<int4*>(a.positions + row0 + i0) = make_int4(vp[0], vp[1], vp[2], vp[3]);
+        *reinterpret_cast<int4*>(a.start + row0 + i0) = make_int4(vs[0], vs[1], vs[2], vs[3]);
+        *reinterpret_cast<int4*>(a.end + row0 + i0) = make_int4(ve[0], ve[1], ve[2], ve[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          if (i0 + e < a.S) {
+            a.positions[row0 + i0 + e] = vp[e];
+            a.start[row0 + i0 + e] = vs[e];
+            a.end[row0 + i0 + e] = ve[e];
+          }
+      }
+      int* tr = a.rows + ((size_t)b * a.n_t + tile) * 256 + lane * kPer;
+      *reinterpret_cast<int4*>(tr) = make_int4(vs[0], vs[1], vs[2], vs[3]);
+      *reinterpret_cast<int4*>(tr + 128) = make_int4(ve[0], ve[1], ve[2], ve[3]);
+      smin = __reduce_min_sync(0xffffffffu, smin);
+      emax = __reduce_max_sync(0xffffffffu, emax);
+      smax = __reduce_max_sync(0xffffffffu, smax);
+      emin = __reduce_min_sync(0xffffffffu, emin);
+      if (lane == 0) a.qstat[(size_t)b * a.n_t + tile] = make_int4(smin, emax, smax, emin);
+    }
+  }
+
+  // ---- query tiles that see each key tile: both bounds are nondecreasing over the tiles that see
+  // anything, and tiles that see nothing come last, so two binary searches find them
+  __threadfence();
+  if (n_cta > 1) {
+    cluster_sync_all();
+  } else {
+    __syncthreads();
+  }
+  const int4* qs = a.qstat + (size_t)b * a.n_t;
+  for (int kt = c0 / 128 + tid; kt < min((c1 + 127) / 128, a.n_t); kt += kThreads) {
+    int lo = 0, hi = a.n_t;  // first tile with max end > kt * 128 (a tile that sees nothing counts as above)
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      const int emax = __ldcg(&qs[mid].y);
+      if (emax == 0 || emax > kt * 128) hi = mid;
+      else lo = mid + 1;
+    }
+    int l2 = 0, h2 = a.n_t;  // first tile with min start >= (kt + 1) * 128
+    while (l2 < h2) {
+      const int mid = (l2 + h2) / 2;
+      if (__ldcg(&qs[mid].x) >= (kt + 1) * 128) h2 = mid;
+      else l2 = mid + 1;
+    }
+    a.krange[(size_t)b * a.n_t + kt] = make_int2(lo, l2 - 1);
+  }
+  if (n_cta > 1) cluster_sync_all();  // no CTA leaves while its s_cta may still be read
+}
+
+}  // namespace docplan
+
+int document_plan_max_len() { return docplan::kMaxCtas * docplan::kMaxSteps * docplan::kStep; }
+
+int document_plan(const long* ids, long ld_ids, long eod, int by_change, const unsigned char* marks, long ld_marks,
+                  const int* lengths, int B, int S, int* positions, int* start, int* end, int* rows, void* qstat,
+                  void* krange, cudaStream_t stream) {
+  using namespace docplan;
+  if (B < 1 || S < 1 || S > document_plan_max_len()) return -1;
+  Args a;
+  a.ids = ids;
+  a.ld_ids = ld_ids;
+  a.eod = eod;
+  a.by_change = by_change;
+  a.marks = marks;
+  a.ld_marks = ld_marks;
+  a.lengths = lengths;
+  a.S = S;
+  a.n_t = (S + 127) / 128;
+  const int steps = (S + kStep - 1) / kStep;
+  const int per_cta = (steps + kMaxCtas - 1) / kMaxCtas;
+  a.chunk = per_cta * kStep;
+  a.positions = positions;
+  a.start = start;
+  a.end = end;
+  a.rows = rows;
+  a.qstat = static_cast<int4*>(qstat);
+  a.krange = static_cast<int2*>(krange);
+  const int n_cta = (S + a.chunk - 1) / a.chunk;
+  if ((long)B * n_cta > INT_MAX) return -2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * n_cta));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = n_cta;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, document_plan_kernel, a);
+}
+
+}  // namespace mmb

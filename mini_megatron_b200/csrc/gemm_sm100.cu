@@ -719,6 +719,22 @@ int make_tmap_f32_2d(CUtensorMap* map, const void* base, long rows, long cols, l
   return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, rows, cols, ld, box_cols, box_rows);
 }
 
+int make_tmap_bf16_3d(CUtensorMap* map, const void* base, long batch, long rows, long cols, long ld_row, long ld_batch,
+                      int box_cols, int box_rows) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return -2;
+  if (ld_row % 8 != 0 || ld_batch % 8 != 0) return -3;
+  PFN_encodeTiled enc = get_encode_fn();
+  if (!enc) return -1;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
+  cuuint64_t strides[2] = {(cuuint64_t)ld_row * 2, (cuuint64_t)ld_batch * 2};
+  cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -4;
+}
+
 // Launch of one instantiation.  `grid` is in CTAs (even for CTA pairs); pairs are
 // launched as 2-CTA clusters, capped at the number of clusters that fit at once.
 template <int BN, bool A_MN, bool B_MN, int EPI, int CG>

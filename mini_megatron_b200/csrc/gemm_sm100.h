@@ -66,6 +66,10 @@ struct GemmProblem {
 int make_tmap_bf16_2d(CUtensorMap* map, const void* base, long rows, long cols, long ld, int box_cols,
                       int box_rows);
 int make_tmap_f32_2d(CUtensorMap* map, const void* base, long rows, long cols, long ld, int box_cols, int box_rows);
+// [batch, rows, cols] bf16 with token stride ld_row and batch stride ld_batch (elements); box rows past `rows` of
+// one batch entry read as zero and are not part of the next entry.
+int make_tmap_bf16_3d(CUtensorMap* map, const void* base, long batch, long rows, long cols, long ld_row, long ld_batch,
+                      int box_cols, int box_rows);
 int gemm_bf16_launch(const GemmProblem& p, cudaStream_t stream);
 int choose_bn(int M, int N, int num_sms);
 int gemm_pairs_default(int K, int epi);

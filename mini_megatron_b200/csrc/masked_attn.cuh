@@ -1,0 +1,212 @@
+// Shared parts of the masked attention kernels (masked_attn_fwd.cu,
+// masked_attn_dq.cu, masked_attn_dkv.cu): the mask, the score transform, bounded
+// waits and the order of work items.
+//
+// Scores in log2 units, query i, key j, head h, C = cap * log2 e:
+//
+//   x_ij = C tanh(s q_i.k_j / cap)  or  s log2 e (q_i.k_j),   minus  slope_h log2 e |i - j|
+//   visible iff start_i <= j < end_i                          (document_plan.cu; causal: 0 and i + 1)
+//
+// tanh is 1 - 2 / (1 + e^{2u}): one exponential and one reciprocal, whose
+// absolute error (a few 2^-23) is what matters inside the softmax's exponent.
+// The single-instruction tanh approximation is off by up to 2^-11 relative, which
+// a cap of 50 turns into 0.02 in the exponent; it is not used.
+#pragma once
+#include "common.cuh"
+#include "ops.h"
+
+#include <algorithm>
+#include <climits>
+
+namespace mmb {
+namespace mattn {
+
+constexpr int BT = 128;  // rows of every query and key tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
+
+struct Mask {
+  const int* rows;     // [B, n_t, 2, 128] start, end (tile-padded), nullptr: causal
+  const int4* qstat;   // [B, n_t] {min start, max end, max start, min end}
+  const int2* krange;  // [B, n_t] {first, last} query tile
+};
+
+// Key tiles [x, y) that query tile t of row b needs.
+__device__ __forceinline__ int2 key_tiles(const Mask& m, int b, int n_t, int t) {
+  if (!m.rows) return make_int2(0, t + 1);
+  const int4 q = m.qstat[(size_t)b * n_t + t];
+  if (q.y == 0) return make_int2(0, 0);
+  return make_int2(q.x / BT, (q.y + BT - 1) / BT);
+}
+
+// The key tiles of query tile t that need no mask: every row of t sees all of them ([x, y)).
+__device__ __forceinline__ int2 full_tiles(const Mask& m, int b, int n_t, int t) {
+  if (!m.rows) return make_int2(0, t);
+  const int4 q = m.qstat[(size_t)b * n_t + t];
+  return make_int2((q.z + BT - 1) / BT, q.w / BT);
+}
+
+// Query tiles [x, y) that see key tile kt of row b.
+__device__ __forceinline__ int2 query_tiles(const Mask& m, int b, int n_t, int kt) {
+  if (!m.rows) return make_int2(kt, n_t);
+  const int2 r = m.krange[(size_t)b * n_t + kt];
+  return make_int2(r.x, max(r.x, r.y + 1));
+}
+
+// Work item of CTA `c` in round `r`: every other round runs backwards over the CTAs, so that
+// with items sorted by weight the CTA with the heaviest item of one round takes the lightest of the next.
+__device__ __forceinline__ int snake_item(int r) {
+  return r * (int)gridDim.x + ((r & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Constants of the score transform.
+struct Score {
+  float mul;  // plain: s log2 e;  capped: 2 s log2 e / cap (the exponent of e^{2u} in log2 units)
+  float cap;  // C
+};
+
+template <bool CAP>
+__device__ __forceinline__ float score(float s, const Score& k) {
+  if constexpr (CAP) return fmaf(-2.f * k.cap, rcp_approx(1.f + fast_exp2(s * k.mul)), k.cap);
+  return s * k.mul;
+}
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Bounded wait on an mbarrier phase.  The clock is read only after many polls: a read of the
+// global timer costs more than most of these waits.
+__device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  unsigned long long t0 = 0;
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((n & 255u) == 0) {
+      if (*abort_flag) return false;
+      const unsigned long long now = globaltimer();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > kWaitTimeoutNs) {
+        if (err) atomicExch(err, (int)kErrAttnWait);
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+
+// Warp-wide: the warp goes on only if every lane saw the phase complete.
+__device__ __forceinline__ bool wwait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  const bool ok = bwait(bar, parity, err, abort_flag);
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+
+// Bounded wait used while winding down after an abort (does not look at the abort flag).
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < 20000000ull) {
+  }
+}
+
+// One arrival per warp on `bar`, after every lane's tcgen05 loads / stores are ordered before it.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// A [rows, 128-byte chunks] tile of D columns, as CHUNKS boxes of 64 columns x 128 rows.
+template <int D>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int col, int row,
+                                          int batch) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) tma_load_3d(dst + c * 16384, map, bar, col + 64 * c, row, batch);
+}
+
+// 128 x 128 (+)= A [128 x D] B [128 x D]^T, both K-major in shared memory.
+template <int D>
+__device__ __forceinline__ void mma_abt(uint32_t dst, uint32_t a_addr, uint32_t b_addr) {
+  constexpr uint32_t idesc = make_idesc_bf16(BT, BT, false, false);
+  const uint64_t ad = make_sdesc_sw128(a_addr, 16, 1024), bd = make_sdesc_sw128(b_addr, 16, 1024);
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+    umma_bf16_ss(dst, ad + off, bd + off, idesc, k != 0 ? 1u : 0u);
+  }
+}
+
+// 128 x D (+)= A [128 x 128, bf16 in TMEM] B [128 x D] (rows are the reduction: MN-major).  A's 128
+// columns lie in two runs of 64 (32 TMEM columns each) that start `hi` columns apart.
+template <int D>
+__device__ __forceinline__ void mma_tmem_b(uint32_t dst, uint32_t a_tmem, uint32_t hi, uint32_t b_addr, bool acc) {
+  constexpr uint32_t idesc = make_idesc_bf16(BT, D, false, true);
+  const uint64_t bd = make_sdesc_sw128(b_addr, 16384, 1024);
+#pragma unroll
+  for (int k = 0; k < BT / 16; ++k)
+    umma_bf16_ts(dst, a_tmem + (k >> 2) * hi + (k & 3) * 8, bd + (uint64_t)(k * (2048 >> 4)), idesc,
+                 (acc || k != 0) ? 1u : 0u);
+}
+
+// Stores 32 fp32 accumulator values as bf16 (64 bytes of one row).
+__device__ __forceinline__ void store_row32(__nv_bfloat16* p, const uint32_t (&v)[32], float mul) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    uint4 w;
+    w.x = pack_bf16x2(__uint_as_float(v[8 * u + 0]) * mul, __uint_as_float(v[8 * u + 1]) * mul);
+    w.y = pack_bf16x2(__uint_as_float(v[8 * u + 2]) * mul, __uint_as_float(v[8 * u + 3]) * mul);
+    w.z = pack_bf16x2(__uint_as_float(v[8 * u + 4]) * mul, __uint_as_float(v[8 * u + 5]) * mul);
+    w.w = pack_bf16x2(__uint_as_float(v[8 * u + 6]) * mul, __uint_as_float(v[8 * u + 7]) * mul);
+    reinterpret_cast<uint4*>(p)[u] = w;
+  }
+}
+__device__ __forceinline__ void store_zero32(__nv_bfloat16* p) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) reinterpret_cast<uint4*>(p)[u] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+}  // namespace mattn
+
+// Host-side description of one call (ops.h declares the launchers).
+inline int score_constants(float scale, float cap, float* mul, float* c) {
+  if (cap > 0.f) {
+    *mul = 2.f * scale * mattn::kLog2e / cap;
+    *c = cap * mattn::kLog2e;
+  } else {
+    *mul = scale * mattn::kLog2e;
+    *c = 0.f;
+  }
+  return 0;
+}
+
+}  // namespace mmb

@@ -1,0 +1,451 @@
+// Masked attention backward, key side: dK and dV.
+//
+//   dV_j = sum_i P_ij dO_i,  dK_j = s sum_i dS_ij q_i   (P, dS: masked_attn_dq.cu)
+//
+// The sums run over every query that sees key j, in all heads that share the K/V
+// head, in a fixed order in 32-bit TMEM accumulators: shared heads need no
+// reduction afterwards and the result does not depend on scheduling.
+//
+// Persistent grid, one CTA per SM; a work item is (batch, K/V head, 128-row key
+// tile).  Scores are computed transposed (a thread owns a key row), so P^T and dS^T
+// go back into TMEM as the first operands of the two sums and never touch shared
+// memory; LSE, Delta and the visible intervals of the query rows arrive with the
+// Q / dO tiles by bulk copies from tile-padded arrays.  Roles (10 warps):
+//
+//   warp 0     TMA: K_j, V_j per item; Q_i, dO_i and their row data into a ring
+//   warp 1     TMEM allocation; one thread issues S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//   warps 2-9  softmax gradient: warps w and w + 4 share 32 key rows and split the 128 queries
+//
+// d = 64: S^T has two TMEM buffers, the next tile's scores are computed while this tile's
+// softmax runs.  d = 128: S^T, dP^T, dV and dK fill TMEM; the next S^T follows dV and the next
+// dP^T follows dK, each overlapping the other half of the softmax gradient.
+#include "masked_attn.cuh"
+
+namespace mmb {
+namespace mattn {
+namespace dkv {
+
+constexpr int kThreads = 320;
+
+template <int D>
+struct Cfg {
+  static constexpr int TILE = BT * D * 2;
+  static constexpr int KB = (D == 64) ? 2 : 1;  // K / V buffers
+  static constexpr int NQ = (D == 64) ? 3 : 2;  // Q / dO ring stages
+  static constexpr int SB = (D == 64) ? 2 : 1;  // S^T buffers in TMEM
+  static constexpr int K_OFF = 0;               // [KB][K, V]
+  static constexpr int Q_OFF = KB * 2 * TILE;   // [NQ][Q, dO]
+  static constexpr int LD_OFF = Q_OFF + NQ * 2 * TILE;  // [NQ][LSE log2 e 128, Delta 128, start 128, end 128]
+  static constexpr int BAR_OFF = LD_OFF + NQ * 2048;
+  static constexpr int SMEM = 1024 + BAR_OFF + 256;
+  static constexpr uint32_t T_S = 0, T_DP = SB * 128, T_DV = T_DP + 128, T_DK = T_DV + D;
+};
+static_assert(Cfg<128>::SMEM <= 227 * 1024 && Cfg<64>::SMEM <= 227 * 1024, "shared memory of one CTA");
+static_assert(Cfg<128>::T_DK + 128 <= 512 && Cfg<64>::T_DK + 64 <= 512, "TMEM columns");
+
+struct Args {
+  int B, S, nh, nkv, n_t;
+  Mask mask;
+  const float* slopes;
+  Score score;
+  float scale;
+  const float* ld;      // [B, nh, n_t, 2, 128]
+  __nv_bfloat16* dqkv;  // [B, S, (nh + 2 nkv) * D]
+  int* err;
+};
+
+struct Item {
+  int b, hk, t;
+  int2 r;  // query tiles
+};
+
+__device__ __forceinline__ Item decode(const Args& a, int item) {
+  const int BH = a.B * a.nkv;
+  Item it;
+  it.t = item / BH;  // causal rows: the first key tile is seen by the most queries
+  const int bh = item - it.t * BH;
+  it.b = bh / a.nkv;
+  it.hk = bh - it.b * a.nkv;
+  it.r = query_tiles(a.mask, it.b, a.n_t, it.t);
+  return it;
+}
+
+// (head of the group, query tile) pairs of this CTA's items, one after another.
+struct Walk {
+  int round = -1, it = -1, g = 0, i = 0;
+  Item w;
+  bool valid = true;
+  __device__ __forceinline__ void next(const Args& a, int n_items, int group) {
+    if (round >= 0) {
+      if (++i < w.r.y) return;
+      if (++g < group) {
+        i = w.r.x;
+        return;
+      }
+    }
+    while (true) {
+      const int item = snake_item(++round);
+      if (item >= n_items) {
+        valid = false;
+        return;
+      }
+      w = decode(a, item);
+      if (w.r.x < w.r.y) {
+        g = 0;
+        i = w.r.x;
+        ++it;
+        return;
+      }
+    }
+  }
+  __device__ __forceinline__ bool first() const { return g == 0 && i == w.r.x; }
+  __device__ __forceinline__ bool last(int group) const { return g == group - 1 && i == w.r.y - 1; }
+};
+
+template <int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+    masked_attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
+                           const Args a) {
+  pdl_trigger();
+  using C = Cfg<D>;
+  constexpr int KB = C::KB, NQ = C::NQ, SB = C::SB;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* sKV = smem + C::K_OFF;
+  uint8_t* sQ = smem + C::Q_OFF;
+  uint8_t* sLD = smem + C::LD_OFF;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* kv_full = bars;        // [2]
+  uint64_t* kv_empty = bars + 2;   // [2]
+  uint64_t* q_full = bars + 4;     // [3]
+  uint64_t* q_empty = bars + 7;    // [3]
+  uint64_t* s_full = bars + 10;    // [2]
+  uint64_t* dp_full = bars + 12;
+  uint64_t* p_full = bars + 13;    // P^T written, S^T read (8 warps)
+  uint64_t* ds_full = bars + 14;   // dS^T written, dP^T and the row data read (8 warps)
+  uint64_t* g_full = bars + 15;    // dK, dV of an item complete
+  uint64_t* g_free = bars + 16;    // ... read (8 warps)
+  uint64_t* drain = bars + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_items = a.B * a.nkv * a.n_t;
+  const int group = a.nh / a.nkv;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+    }
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    mbar_init(dp_full, 1);
+    mbar_init(p_full, 8);
+    mbar_init(ds_full, 8);
+    mbar_init(g_full, 1);
+    mbar_init(g_free, 8);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_qkv);
+    prefetch_tmap(&tm_do);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------------------------------------------------------- TMA
+      int n = 0, kv_issued = -1;
+      bool ok = true;
+      Walk x;
+      for (x.next(a, n_items, group); x.valid; x.next(a, n_items, group), ++n) {
+        if (x.first()) {
+          const int kb = x.it % KB;
+          if (x.it >= KB && !bwait(&kv_empty[kb], ((x.it / KB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&kv_full[kb], 2 * C::TILE);
+          load_tile<D>(sKV + kb * 2 * C::TILE, &tm_qkv, &kv_full[kb], (a.nh + x.w.hk) * D, x.w.t * BT, x.w.b);
+          load_tile<D>(sKV + kb * 2 * C::TILE + C::TILE, &tm_qkv, &kv_full[kb], (a.nh + a.nkv + x.w.hk) * D,
+                       x.w.t * BT, x.w.b);
+          kv_issued = x.it;
+        }
+        const int st = n % NQ;
+        if (n >= NQ && !bwait(&q_empty[st], ((n / NQ) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+        const int h = x.w.hk * group + x.g;
+        mbar_expect_tx(&q_full[st], 2 * C::TILE + 1024 + (a.mask.rows ? 1024 : 0));
+        load_tile<D>(sQ + st * 2 * C::TILE, &tm_qkv, &q_full[st], h * D, x.i * BT, x.w.b);
+        load_tile<D>(sQ + st * 2 * C::TILE + C::TILE, &tm_do, &q_full[st], h * D, x.i * BT, x.w.b);
+        bulk_load(sLD + st * 2048, a.ld + (((size_t)x.w.b * a.nh + h) * a.n_t + x.i) * (2 * BT), 1024, &q_full[st]);
+        if (a.mask.rows)
+          bulk_load(sLD + st * 2048 + 1024, a.mask.rows + ((size_t)x.w.b * a.n_t + x.i) * (2 * BT), 1024,
+                    &q_full[st]);
+      }
+      if (!ok) {
+        for (int u = max(0, kv_issued - KB + 1); u <= kv_issued; ++u) drain_wait(&kv_full[u % KB], (u / KB) & 1);
+        for (int u = max(0, n - NQ); u < n; ++u) drain_wait(&q_full[u % NQ], (u / NQ) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---------------------------------------------------------------- MMA
+      bool ok = true;
+      int n = 0;
+      Walk cur, nxt;
+      auto issue_s = [&](const Walk& x, int u) -> bool {
+        const int kb = x.it % KB;
+        if (x.first() && !bwait(&kv_full[kb], (x.it / KB) & 1, a.err, abort_flag)) return false;
+        if (!bwait(&q_full[u % NQ], (u / NQ) & 1, a.err, abort_flag)) return false;
+        tc_fence_after();
+        mma_abt<D>(tmem + C::T_S + (u % SB) * 128, smem_u32(sKV + kb * 2 * C::TILE),
+                   smem_u32(sQ + (u % NQ) * 2 * C::TILE));
+        umma_commit(&s_full[u % SB]);
+        return true;
+      };
+      auto issue_dp = [&](const Walk& x, int u) {
+        const int kb = x.it % KB;
+        mma_abt<D>(tmem + C::T_DP, smem_u32(sKV + kb * 2 * C::TILE + C::TILE),
+                   smem_u32(sQ + (u % NQ) * 2 * C::TILE + C::TILE));
+        umma_commit(dp_full);
+      };
+      nxt.next(a, n_items, group);
+      if (nxt.valid) {
+        ok = issue_s(nxt, 0);
+        if (ok) issue_dp(nxt, 0);
+      }
+      while (ok && nxt.valid) {
+        cur = nxt;
+        nxt.next(a, n_items, group);
+        // one K / V buffer: the next item's tiles can only be loaded once this item's products are done
+        const bool early = nxt.valid && (KB == 2 || nxt.it == cur.it);
+        const uint32_t q_addr = smem_u32(sQ + (n % NQ) * 2 * C::TILE);
+        if (SB == 2 && early && !issue_s(nxt, n + 1)) { ok = false; break; }
+        if (!bwait(p_full, n & 1, a.err, abort_flag)) { ok = false; break; }
+        if (cur.first() && cur.it > 0 && !bwait(g_free, (cur.it - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        mma_tmem_b<D>(tmem + C::T_DV, tmem + C::T_S + (n % SB) * 128, 64, q_addr + C::TILE, !cur.first());
+        if (SB == 1 && early && !issue_s(nxt, n + 1)) { ok = false; break; }  // over P^T, in issue order after dV
+        if (!bwait(ds_full, n & 1, a.err, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        mma_tmem_b<D>(tmem + C::T_DK, tmem + C::T_DP, 64, q_addr, !cur.first());
+        umma_commit(&q_empty[n % NQ]);
+        if (cur.last(group)) {
+          umma_commit(g_full);
+          umma_commit(&kv_empty[cur.it % KB]);
+        }
+        if (nxt.valid && !early && !issue_s(nxt, n + 1)) { ok = false; break; }
+        if (nxt.valid) issue_dp(nxt, n + 1);  // over dS^T, in issue order after dK
+        ++n;
+      }
+      if (!ok) {
+        umma_commit(drain);
+        drain_wait(drain, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax gradient, dK / dV store
+    const int half = (warp - 2) >> 2;
+    const int row = (warp & 3) * 32 + lane;  // key row within the tile (TMEM lane)
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const Score k = a.score;
+    int n = 0, it = 0;
+    bool ok = true;
+    for (int r = 0, item; ok && (item = snake_item(r)) < n_items; ++r) {
+      const Item w = decode(a, item);
+      const int key = w.t * BT + row;
+      const bool in = key < a.S;
+      const size_t width = (size_t)(a.nh + 2 * a.nkv) * D;
+      __nv_bfloat16* dk = a.dqkv + ((size_t)w.b * a.S + key) * width + (size_t)(a.nh + w.hk) * D + half * (D / 2);
+      __nv_bfloat16* dv = dk + (size_t)a.nkv * D;
+      if (w.r.x >= w.r.y) {
+        if (in) {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            store_zero32(dk + c * 32);
+            store_zero32(dv + c * 32);
+          }
+        }
+        continue;
+      }
+      for (int g = 0; ok && g < group; ++g) {
+        float slope = 0.f;
+        if (BIAS) slope = a.slopes[w.hk * group + g] * kLog2e;
+        for (int i = w.r.x; i < w.r.y; ++i, ++n) {
+          const int st = n % NQ;
+          const int2 full = full_tiles(a.mask, w.b, a.n_t, i);
+          const bool masked = w.t < full.x || w.t >= full.y;
+          const uint32_t t_s = tmem + C::T_S + (n % SB) * 128 + lane_off + half * 64;
+          const uint32_t t_dp = tmem + C::T_DP + lane_off + half * 64;
+          const float* l2 = reinterpret_cast<const float*>(sLD + st * 2048) + half * 64;
+          const int* start = reinterpret_cast<const int*>(l2 + 2 * BT);
+          if (!wwait(&q_full[st], (n / NQ) & 1, a.err, abort_flag)) { ok = false; break; }
+          if (!wwait(&s_full[n % SB], (n / SB) & 1, a.err, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          float pf[64];  // P (1 - tanh^2)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            uint32_t s[32];
+            tmem_ld_32x32b_x32(t_s + hh * 32, s);
+            tmem_wait_ld();
+            const int q0 = i * BT + half * 64 + hh * 32;  // query of column 0
+            uint32_t seen = 0xffffffffu;
+            if (masked) {
+              if (a.mask.rows) {
+                seen = 0;
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                  const int4 lo = *reinterpret_cast<const int4*>(start + hh * 32 + e);
+                  const int4 hi = *reinterpret_cast<const int4*>(start + BT + hh * 32 + e);
+                  seen |= (key >= lo.x && key < hi.x ? 1u : 0u) << e;
+                  seen |= (key >= lo.y && key < hi.y ? 2u : 0u) << e;
+                  seen |= (key >= lo.z && key < hi.z ? 4u : 0u) << e;
+                  seen |= (key >= lo.w && key < hi.w ? 8u : 0u) << e;
+                }
+              } else {
+                const int l0 = min(max(key - q0, 0), 32);  // query q sees the key iff q >= key
+                seen = ~(l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u);
+              }
+            }
+            const float dist = (float)(q0 - key);
+            uint32_t pp[16];
+#pragma unroll
+            for (int e4 = 0; e4 < 32; e4 += 4) {
+              const float4 lv = *reinterpret_cast<const float4*>(l2 + hh * 32 + e4);
+              const float ls[4] = {lv.x, lv.y, lv.z, lv.w};
+              float pr[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const int e = e4 + u;
+                float x, f = 1.f;
+                if (CAP) {
+                  const float z = rcp_approx(1.f + fast_exp2(__uint_as_float(s[e]) * k.mul));
+                  x = fmaf(-2.f * k.cap, z, k.cap);
+                  f = 4.f * z * (1.f - z);  // 1 - tanh^2
+                }
+                if (BIAS) x = fmaf(-slope, fabsf(dist + (float)e), CAP ? x : __uint_as_float(s[e]) * k.mul);
+                float p;
+                if (CAP || BIAS) p = fast_exp2(x - ls[u]);
+                else p = fast_exp2(fmaf(__uint_as_float(s[e]), k.mul, -ls[u]));
+                if (masked && !(seen & (1u << e))) p = 0.f;
+                pr[u] = p;
+                pf[hh * 32 + e] = CAP ? p * f : p;
+              }
+              pp[e4 / 2] = pack_bf16x2(pr[0], pr[1]);
+              pp[e4 / 2 + 1] = pack_bf16x2(pr[2], pr[3]);
+            }
+            tmem_st_32x32b_x16(t_s + hh * 16, pp);  // over S^T columns already read
+          }
+          tmem_wait_st();
+          warp_arrive(p_full);
+          if (!wwait(dp_full, n & 1, a.err, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const float* delta = l2 + BT;
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            uint32_t dp[32];
+            tmem_ld_32x32b_x32(t_dp + hh * 32, dp);
+            tmem_wait_ld();
+            uint32_t ds[16];
+#pragma unroll
+            for (int e4 = 0; e4 < 32; e4 += 4) {
+              const float4 dl = *reinterpret_cast<const float4*>(delta + hh * 32 + e4);
+              ds[e4 / 2] = pack_bf16x2(pf[hh * 32 + e4] * (__uint_as_float(dp[e4]) - dl.x),
+                                       pf[hh * 32 + e4 + 1] * (__uint_as_float(dp[e4 + 1]) - dl.y));
+              ds[e4 / 2 + 1] = pack_bf16x2(pf[hh * 32 + e4 + 2] * (__uint_as_float(dp[e4 + 2]) - dl.z),
+                                           pf[hh * 32 + e4 + 3] * (__uint_as_float(dp[e4 + 3]) - dl.w));
+            }
+            tmem_st_32x32b_x16(t_dp + hh * 16, ds);  // over dP^T columns already read
+          }
+          tmem_wait_st();
+          warp_arrive(ds_full);
+        }
+      }
+      if (!ok) break;
+      if (!wwait(g_full, it & 1, a.err, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem + C::T_DV + lane_off + half * (D / 2) + c * 32, v);
+        tmem_wait_ld();
+        if (in) store_row32(dv + c * 32, v, 1.f);
+        tmem_ld_32x32b_x32(tmem + C::T_DK + lane_off + half * (D / 2) + c * 32, v);
+        tmem_wait_ld();
+        if (c == D / 64 - 1) warp_arrive(g_free);
+        if (in) store_row32(dk + c * 32, v, a.scale);
+      }
+      ++it;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, bool CAP, bool BIAS>
+int launch(const CUtensorMap& tq, const CUtensorMap& to, const Args& a, int grid, cudaStream_t stream) {
+  auto k = masked_attn_dkv_kernel<D, CAP, BIAS>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  if (e != cudaSuccess) return (int)e;
+  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, a);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace dkv
+}  // namespace mattn
+
+int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb, const float* ld, void* dqkv, int* err,
+                    int num_sms, cudaStream_t stream) {
+  using namespace mattn;
+  const int n_t = (c.S + BT - 1) / BT;
+  const long items = (long)c.B * c.nkv * n_t;
+  if (items > INT_MAX / 2) return -1;
+  CUtensorMap tq, to;
+  int rc = make_tmap_bf16_3d(&tq, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
+  if (rc) return rc - 10;
+  rc = make_tmap_bf16_3d(&to, dout, c.B, c.S, (long)c.nh * c.d, do_ss, do_sb, 64, BT);
+  if (rc) return rc - 20;
+  dkv::Args a;
+  a.B = c.B;
+  a.S = c.S;
+  a.nh = c.nh;
+  a.nkv = c.nkv;
+  a.n_t = n_t;
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange)};
+  a.slopes = c.slopes;
+  score_constants(c.scale, c.cap, &a.score.mul, &a.score.cap);
+  a.scale = c.scale;
+  a.ld = ld;
+  a.dqkv = static_cast<__nv_bfloat16*>(dqkv);
+  a.err = err;
+  const int grid = (int)std::max(1L, std::min(items, (long)num_sms));
+  const bool cap = c.cap > 0.f, bias = c.slopes != nullptr;
+  if (c.d == 64) {
+    if (cap) return bias ? dkv::launch<64, true, true>(tq, to, a, grid, stream) : dkv::launch<64, true, false>(tq, to, a, grid, stream);
+    return bias ? dkv::launch<64, false, true>(tq, to, a, grid, stream) : dkv::launch<64, false, false>(tq, to, a, grid, stream);
+  }
+  if (c.d == 128) {
+    if (cap) return bias ? dkv::launch<128, true, true>(tq, to, a, grid, stream) : dkv::launch<128, true, false>(tq, to, a, grid, stream);
+    return bias ? dkv::launch<128, false, true>(tq, to, a, grid, stream) : dkv::launch<128, false, false>(tq, to, a, grid, stream);
+  }
+  return -2;
+}
+
+}  // namespace mmb

@@ -1,0 +1,481 @@
+// Masked attention backward, query side: dQ, and the row statistics of the key side.
+//
+//   P_ij = exp(x_ij - LSE_i),  Delta_i = sum_c dO_ic O_ic
+//   dS_ij = P_ij (dO_i.v_j - Delta_i) (1 - tanh^2 u_ij),  dQ_i = s sum_j dS_ij k_j
+//
+// The backward is two passes over the visible tiles, one that stays with a query
+// tile (this file) and one that stays with a key tile (masked_attn_dkv.cu).  Scores
+// are computed twice, but each gradient is summed in one place in one order, in
+// 32-bit TMEM accumulators: no atomics, no zeroed 32-bit copy of dQ, no conversion
+// pass, and the same inputs give the same bits.  dS is rounded to bf16 once, as
+// the operand of its products.
+//
+// Persistent grid, one CTA per SM; a work item is (batch, head, 128-row query tile).
+// Roles (12 warps):
+//
+//   warp 0      TMA: Q, dO per item; K_j and V_j into rings
+//   warp 1      TMEM allocation; one thread issues S = Q K_j^T (two TMEM buffers), dP = dO V_j^T
+//               and dQ += dS K_j (dS read from TMEM): S of the next tile before dS of this one is
+//               ready, dP of the next as soon as this one has been read
+//   warps 2-3   Delta and LSE of the next item's rows: into shared memory for the warps below and
+//               into the tile-padded workspace the key side reads with bulk copies
+//   warps 4-11  dS: warps w and w + 4 share 32 query rows and split the 128 keys
+//
+// dS overwrites the S columns it came from; the halves of a row are 64 columns apart.
+#include "masked_attn.cuh"
+
+namespace mmb {
+namespace mattn {
+namespace dq {
+
+constexpr int kThreads = 384;
+
+template <int D>
+struct Cfg {
+  static constexpr int TILE = BT * D * 2;
+  static constexpr int QB = (D == 64) ? 2 : 1;  // Q / dO buffers
+  static constexpr int NK = (D == 64) ? 4 : 3;  // K ring: held from S(j) to dQ(j), one tile longer than V
+  static constexpr int NV = (D == 64) ? 4 : 2;
+  static constexpr int SB = QB;                 // row-statistics buffers
+  static constexpr int Q_OFF = 0;               // [QB][Q, dO]
+  static constexpr int K_OFF = QB * 2 * TILE;
+  static constexpr int V_OFF = K_OFF + NK * TILE;
+  static constexpr int ST_OFF = V_OFF + NV * TILE;  // [SB][128] (LSE log2 e, Delta)
+  static constexpr int BAR_OFF = ST_OFF + SB * BT * 8;
+  static constexpr int SMEM = 1024 + BAR_OFF + 384;
+  static constexpr uint32_t T_S = 0, T_DP = 256, T_DQ = 384;  // S: two buffers of 128 columns
+};
+static_assert(Cfg<128>::SMEM <= 227 * 1024 && Cfg<64>::SMEM <= 227 * 1024, "shared memory of one CTA");
+
+struct Args {
+  int B, S, nh, nkv, n_t;
+  Mask mask;
+  const float* slopes;
+  Score score;
+  float scale;
+  const __nv_bfloat16* dout;  // [B, S, nh * D] with strides
+  long do_ss, do_sb;
+  const __nv_bfloat16* out;   // [B, S, nh * D]
+  const float* lse;           // [B, nh, S]
+  float* ld;                  // [B, nh, n_t, 2, 128] LSE log2 e (+inf: the row takes no part), Delta
+  __nv_bfloat16* dqkv;        // [B, S, (nh + 2 nkv) * D]
+  int* err;
+};
+
+struct Item {
+  int b, h, t;
+  int2 r;  // key tiles
+};
+
+__device__ __forceinline__ Item decode(const Args& a, int item) {
+  const int BH = a.B * a.nh;
+  const int p = item / BH, bh = item - p * BH;
+  Item it;
+  it.t = a.n_t - 1 - p;  // causal rows: the longest first
+  it.b = bh / a.nh;
+  it.h = bh - it.b * a.nh;
+  it.r = key_tiles(a.mask, it.b, a.n_t, it.t);
+  return it;
+}
+
+// The tiles of this CTA one after another, across items (items without keys are skipped).
+struct Walk {
+  int round = -1, it = -1, j = 0;  // it: items with keys so far
+  Item w;
+  bool valid = true;
+  __device__ __forceinline__ void next(const Args& a, int n_items) {
+    if (round >= 0 && j + 1 < w.r.y) {
+      ++j;
+      return;
+    }
+    while (true) {
+      const int item = snake_item(++round);
+      if (item >= n_items) {
+        valid = false;
+        return;
+      }
+      w = decode(a, item);
+      if (w.r.x < w.r.y) {
+        j = w.r.x;
+        ++it;
+        return;
+      }
+    }
+  }
+  __device__ __forceinline__ bool first() const { return j == w.r.x; }
+  __device__ __forceinline__ bool last() const { return j == w.r.y - 1; }
+};
+
+template <int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+    masked_attn_dq_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
+                          const Args a) {
+  pdl_trigger();
+  using C = Cfg<D>;
+  constexpr int QB = C::QB, NK = C::NK, NV = C::NV, SB = C::SB;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* sQ = smem + C::Q_OFF;
+  uint8_t* sK = smem + C::K_OFF;
+  uint8_t* sV = smem + C::V_OFF;
+  float2* sST = reinterpret_cast<float2*>(smem + C::ST_OFF);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* q_full = bars;            // [2]
+  uint64_t* q_empty = bars + 2;       // [2]
+  uint64_t* st_full = bars + 4;       // [2]  row statistics written (2 warps)
+  uint64_t* st_empty = bars + 6;      // [2]  ... read (8 warps)
+  uint64_t* s_full = bars + 8;        // [2]  S computed
+  uint64_t* k_full = bars + 10;       // [4]
+  uint64_t* k_empty = bars + 14;      // [4]
+  uint64_t* v_full = bars + 18;       // [4]
+  uint64_t* v_empty = bars + 22;      // [4]
+  uint64_t* dp_full = bars + 26;      // dP computed
+  uint64_t* ds_full = bars + 27;      // dS written, dP read (8 warps)
+  uint64_t* dq_full = bars + 28;      // dQ of an item complete
+  uint64_t* dq_free = bars + 29;      // ... read (8 warps)
+  uint64_t* drain = bars + 30;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_items = a.B * a.nh * a.n_t;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&st_full[i], 2);
+      mbar_init(&st_empty[i], 8);
+      mbar_init(&s_full[i], 1);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 8);
+    mbar_init(dq_full, 1);
+    mbar_init(dq_free, 8);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_qkv);
+    prefetch_tmap(&tm_do);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem = *tmem_slot;
+  const int group = a.nh / a.nkv;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------------------------------------------------------- TMA
+      int n = 0, q_issued = -1, k_issued = 0, v_issued = 0;
+      bool ok = true;
+      Walk x;
+      for (x.next(a, n_items); x.valid; x.next(a, n_items), ++n) {
+        const int hk = x.w.h / group;
+        if (x.first()) {
+          const int qb = x.it % QB;
+          if (x.it >= QB && !bwait(&q_empty[qb], ((x.it / QB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          uint8_t* qd = sQ + qb * 2 * C::TILE;
+          mbar_expect_tx(&q_full[qb], 2 * C::TILE);
+          load_tile<D>(qd, &tm_qkv, &q_full[qb], x.w.h * D, x.w.t * BT, x.w.b);
+          load_tile<D>(qd + C::TILE, &tm_do, &q_full[qb], x.w.h * D, x.w.t * BT, x.w.b);
+          q_issued = x.it;
+        }
+        const int ks = n % NK, vs = n % NV;
+        if (n >= NK && !bwait(&k_empty[ks], ((n / NK) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+        mbar_expect_tx(&k_full[ks], C::TILE);
+        load_tile<D>(sK + ks * C::TILE, &tm_qkv, &k_full[ks], (a.nh + hk) * D, x.j * BT, x.w.b);
+        k_issued = n + 1;
+        if (n >= NV && !bwait(&v_empty[vs], ((n / NV) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+        mbar_expect_tx(&v_full[vs], C::TILE);
+        load_tile<D>(sV + vs * C::TILE, &tm_qkv, &v_full[vs], (a.nh + a.nkv + hk) * D, x.j * BT, x.w.b);
+        v_issued = n + 1;
+      }
+      if (!ok) {
+        for (int u = max(0, q_issued - QB + 1); u <= q_issued; ++u) drain_wait(&q_full[u % QB], (u / QB) & 1);
+        for (int u = max(0, k_issued - NK); u < k_issued; ++u) drain_wait(&k_full[u % NK], (u / NK) & 1);
+        for (int u = max(0, v_issued - NV); u < v_issued; ++u) drain_wait(&v_full[u % NV], (u / NV) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---------------------------------------------------------------- MMA
+      bool ok = true;
+      int n = 0;
+      Walk cur, nxt;
+      auto issue_s = [&](const Walk& x, int u) -> bool {
+        const int qb = x.it % QB;
+        if (x.first() && !bwait(&q_full[qb], (x.it / QB) & 1, a.err, abort_flag)) return false;
+        if (!bwait(&k_full[u % NK], (u / NK) & 1, a.err, abort_flag)) return false;
+        tc_fence_after();
+        mma_abt<D>(tmem + C::T_S + (u & 1) * 128, smem_u32(sQ + qb * 2 * C::TILE), smem_u32(sK + (u % NK) * C::TILE));
+        umma_commit(&s_full[u & 1]);
+        return true;
+      };
+      auto issue_dp = [&](const Walk& x, int u) -> bool {
+        const int qb = x.it % QB;
+        if (!bwait(&v_full[u % NV], (u / NV) & 1, a.err, abort_flag)) return false;
+        tc_fence_after();
+        mma_abt<D>(tmem + C::T_DP, smem_u32(sQ + qb * 2 * C::TILE + C::TILE), smem_u32(sV + (u % NV) * C::TILE));
+        umma_commit(dp_full);
+        umma_commit(&v_empty[u % NV]);
+        if (x.last()) umma_commit(&q_empty[qb]);  // every product of this item that reads Q or dO is issued
+        return true;
+      };
+      nxt.next(a, n_items);
+      if (nxt.valid) ok = issue_s(nxt, 0) && issue_dp(nxt, 0);
+      while (ok && nxt.valid) {
+        cur = nxt;
+        nxt.next(a, n_items);
+        // one Q buffer: the next item's Q can only be loaded once this item's products are done with it,
+        // and this tile's dQ should not wait for that load
+        const bool early = nxt.valid && (QB == 2 || nxt.it == cur.it);
+        if (early && !issue_s(nxt, n + 1)) { ok = false; break; }
+        if (!bwait(ds_full, n & 1, a.err, abort_flag)) { ok = false; break; }
+        if (early && !issue_dp(nxt, n + 1)) { ok = false; break; }
+        if (cur.first() && cur.it > 0 && !bwait(dq_free, (cur.it - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        mma_tmem_b<D>(tmem + C::T_DQ, tmem + C::T_S + (n & 1) * 128, 64, smem_u32(sK + (n % NK) * C::TILE),
+                      !cur.first());
+        umma_commit(&k_empty[n % NK]);
+        if (cur.last()) umma_commit(dq_full);
+        if (nxt.valid && !early && !(issue_s(nxt, n + 1) && issue_dp(nxt, n + 1))) { ok = false; break; }
+        ++n;
+      }
+      if (!ok) {
+        umma_commit(drain);
+        drain_wait(drain, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ row statistics
+    constexpr int G = D / 8;        // lanes per row
+    constexpr int R = 32 / G;       // rows per pass
+    const int part = lane % G, sub = lane / G;
+    Walk x;
+    x.next(a, n_items);
+    while (x.valid) {
+      const Item& w = x.w;
+      const int sb = x.it % SB;
+      if (x.it >= SB && !wwait(&st_empty[sb], ((x.it / SB) - 1) & 1, a.err, abort_flag)) break;
+      const float* lse = a.lse + ((size_t)w.b * a.nh + w.h) * a.S;
+      float* ld = a.ld + (((size_t)w.b * a.nh + w.h) * a.n_t + w.t) * (2 * BT);
+#pragma unroll 4
+      for (int p = 0; p < 64 / R; ++p) {
+        const int row = (warp - 2) * 64 + p * R + sub;
+        const int i = w.t * BT + row;
+        float acc = 0.f;
+        if (i < a.S) {
+          const uint4 u = *reinterpret_cast<const uint4*>(a.dout + w.b * a.do_sb + i * a.do_ss + w.h * D + part * 8);
+          const uint4 v = *reinterpret_cast<const uint4*>(a.out + ((size_t)w.b * a.S + i) * ((size_t)a.nh * D) +
+                                                          (size_t)w.h * D + part * 8);
+          const uint32_t* uw = reinterpret_cast<const uint32_t*>(&u);
+          const uint32_t* vw = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack_bf16x2(uw[e]), g = unpack_bf16x2(vw[e]);
+            acc = fmaf(f.x, g.x, fmaf(f.y, g.y, acc));
+          }
+        }
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+        if (part == 0) {
+          float l2 = INFINITY;
+          if (i < a.S) {
+            const float l = lse[i];
+            if (l != -INFINITY) l2 = l * kLog2e;
+          }
+          if (l2 == INFINITY) acc = 0.f;  // a row that sees nothing, or lies behind the end, gives no gradient
+          sST[sb * BT + row] = make_float2(l2, acc);
+          ld[row] = l2;
+          ld[BT + row] = acc;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st_full[sb]);
+      x.j = x.w.r.y - 1;  // on to the next item
+      x.next(a, n_items);
+    }
+  } else {
+    // ------------------------------------------------------------------ dS, dQ store
+    const int half = (warp - 4) >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const Score k = a.score;
+    int n = 0, it = 0;
+    bool ok = true;
+    for (int r = 0, item; ok && (item = snake_item(r)) < n_items; ++r) {
+      const Item w = decode(a, item);
+      const int i = w.t * BT + row;
+      const bool in = i < a.S;
+      __nv_bfloat16* dst = a.dqkv + ((size_t)w.b * a.S + i) * ((size_t)(a.nh + 2 * a.nkv) * D) + (size_t)w.h * D +
+                           half * (D / 2);
+      if (w.r.x >= w.r.y) {
+        if (in) {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) store_zero32(dst + c * 32);
+        }
+        continue;
+      }
+      const int2 full = full_tiles(a.mask, w.b, a.n_t, w.t);
+      int start = 0, end = i + 1;
+      if (a.mask.rows) {
+        const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + w.t) * (2 * BT) + row;
+        start = tr[0];
+        end = tr[BT];
+      }
+      float slope = 0.f;
+      if (BIAS) slope = a.slopes[w.h] * kLog2e;
+      const int sb = it % SB;
+      if (!wwait(&st_full[sb], (it / SB) & 1, a.err, abort_flag)) { ok = false; break; }
+      const float2 st = sST[sb * BT + row];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st_empty[sb]);
+      for (int j = w.r.x; j < w.r.y; ++j, ++n) {
+        const uint32_t t_s = tmem + C::T_S + (n & 1) * 128 + lane_off + half * 64;
+        if (!wwait(&s_full[n & 1], (n >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const bool masked = j < full.x || j >= full.y;
+        float pf[64];  // P (1 - tanh^2)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t s[32];
+          tmem_ld_32x32b_x32(t_s + hh * 32, s);
+          tmem_wait_ld();
+          const int j0 = j * BT + half * 64 + hh * 32;  // key of column 0
+          uint32_t seen = 0xffffffffu;
+          if (masked) {
+            const int l0 = min(max(start - j0, 0), 32), h0 = min(max(end - j0, 0), 32);
+            seen = (h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u) & ~(l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u);
+          }
+          const float dist = (float)(j0 - i);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float x, f = 1.f;
+            if (CAP) {
+              const float z = rcp_approx(1.f + fast_exp2(__uint_as_float(s[e]) * k.mul));
+              x = fmaf(-2.f * k.cap, z, k.cap);
+              f = 4.f * z * (1.f - z);  // 1 - tanh^2
+            }
+            if (BIAS) x = fmaf(-slope, fabsf(dist + (float)e), CAP ? x : __uint_as_float(s[e]) * k.mul);
+            float p;
+            if (CAP || BIAS) p = fast_exp2(x - st.x);
+            else p = fast_exp2(fmaf(__uint_as_float(s[e]), k.mul, -st.x));
+            if (CAP) p *= f;
+            pf[hh * 32 + e] = p;
+          }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen & (1u << e))) pf[hh * 32 + e] = 0.f;
+          }
+        }
+        if (!wwait(dp_full, n & 1, a.err, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t dp[32];
+          tmem_ld_32x32b_x32(tmem + C::T_DP + lane_off + half * 64 + hh * 32, dp);
+          tmem_wait_ld();
+          uint32_t ds[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            ds[e] = pack_bf16x2(pf[hh * 32 + 2 * e] * (__uint_as_float(dp[2 * e]) - st.y),
+                                pf[hh * 32 + 2 * e + 1] * (__uint_as_float(dp[2 * e + 1]) - st.y));
+          tmem_st_32x32b_x16(t_s + hh * 16, ds);
+        }
+        tmem_wait_st();
+        warp_arrive(ds_full);
+      }
+      if (!ok) break;
+      if (!wwait(dq_full, it & 1, a.err, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem + C::T_DQ + lane_off + half * (D / 2) + c * 32, v);
+        tmem_wait_ld();
+        if (c == D / 64 - 1) warp_arrive(dq_free);
+        if (in) store_row32(dst + c * 32, v, a.scale);
+      }
+      ++it;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, bool CAP, bool BIAS>
+int launch(const CUtensorMap& tq, const CUtensorMap& to, const Args& a, int grid, cudaStream_t stream) {
+  auto k = masked_attn_dq_kernel<D, CAP, BIAS>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  if (e != cudaSuccess) return (int)e;
+  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, a);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace dq
+}  // namespace mattn
+
+int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, const void* out, const float* lse,
+                   float* ld, void* dqkv, int* err, int num_sms, cudaStream_t stream) {
+  using namespace mattn;
+  const int n_t = (c.S + BT - 1) / BT;
+  const long items = (long)c.B * c.nh * n_t;
+  if (items > INT_MAX / 2) return -1;
+  CUtensorMap tq, to;
+  int rc = make_tmap_bf16_3d(&tq, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
+  if (rc) return rc - 10;
+  rc = make_tmap_bf16_3d(&to, dout, c.B, c.S, (long)c.nh * c.d, do_ss, do_sb, 64, BT);
+  if (rc) return rc - 20;
+  dq::Args a;
+  a.B = c.B;
+  a.S = c.S;
+  a.nh = c.nh;
+  a.nkv = c.nkv;
+  a.n_t = n_t;
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange)};
+  a.slopes = c.slopes;
+  score_constants(c.scale, c.cap, &a.score.mul, &a.score.cap);
+  a.scale = c.scale;
+  a.dout = static_cast<const __nv_bfloat16*>(dout);
+  a.do_ss = do_ss;
+  a.do_sb = do_sb;
+  a.out = static_cast<const __nv_bfloat16*>(out);
+  a.lse = lse;
+  a.ld = ld;
+  a.dqkv = static_cast<__nv_bfloat16*>(dqkv);
+  a.err = err;
+  const int grid = (int)std::max(1L, std::min(items, (long)num_sms));
+  const bool cap = c.cap > 0.f, bias = c.slopes != nullptr;
+  if (c.d == 64) {
+    if (cap) return bias ? dq::launch<64, true, true>(tq, to, a, grid, stream) : dq::launch<64, true, false>(tq, to, a, grid, stream);
+    return bias ? dq::launch<64, false, true>(tq, to, a, grid, stream) : dq::launch<64, false, false>(tq, to, a, grid, stream);
+  }
+  if (c.d == 128) {
+    if (cap) return bias ? dq::launch<128, true, true>(tq, to, a, grid, stream) : dq::launch<128, true, false>(tq, to, a, grid, stream);
+    return bias ? dq::launch<128, false, true>(tq, to, a, grid, stream) : dq::launch<128, false, false>(tq, to, a, grid, stream);
+  }
+  return -2;
+}
+
+}  // namespace mmb

@@ -1,0 +1,523 @@
+// Masked attention forward for sm_100a: document and prefix masks, scores capped
+// by a tanh, a bias linear in the distance, shared K/V heads, any sequence length.
+//
+//   O_i = sum_j softmax_j(x_ij) v_j,  LSE_i = log sum_j exp(x_ij)   (x: masked_attn.cuh)
+//
+// A row that sees nothing gives O = 0 and LSE = -inf.  The running maximum, the
+// row sum and O stay in 32 bits; P is rounded to bf16 once, as the operand of
+// P V, relative to a maximum at most 2^8 stale.
+//
+// Persistent grid, one CTA per SM.  A work item is (batch, head, two adjacent
+// 128-row query tiles); both tiles share the K/V tiles they both need, so a
+// K/V tile is fetched once per 256 queries.  Only the key tiles that a query tile's
+// rows can see are visited, and only those that some row does not see completely
+// pay for a mask.  Roles (16 warps):
+//
+//   warp 0       TMA: Q tiles per item; K_j / V_j into an NS-stage ring
+//   warp 1       TMEM allocation; one thread issues S_i = Q_i K_j^T and O_i += P_i V_j
+//   warps 4-7,   softmax of tile 0 / tile 1, a thread per query row: scores out of
+//   warps 8-11   TMEM, transform, mask, running maximum, P back into TMEM as bf16
+//   warps 12-15  epilogue of both tiles: O / row sum -> bf16, LSE; it runs while the
+//                softmax warps are in the next item
+//
+// O is rescaled in TMEM only when a row's maximum grew by more than 2^8; until then
+// P, O and the row sum share the stale maximum, so nothing is approximated.
+//
+// d = 64: P has its own TMEM columns and Q two buffers, so S_i(j+1) is computed while
+// P_i(j) is.  d = 128: S and O of two tiles fill TMEM, P overwrites S, and the two tiles
+// alternate between the tensor core and the softmax.
+//
+// Every wait is bounded; on a time-out the kernel records an error code, all roles wind
+// down, loads and MMAs in flight are waited for (bounded), TMEM is freed and the CTA returns.
+#include "masked_attn.cuh"
+
+namespace mmb {
+namespace mattn {
+namespace fwd {
+
+constexpr int kThreads = 512;
+constexpr float kRescaleLog2 = 8.0f;
+
+template <int D>
+struct Cfg {
+  static constexpr int TILE = BT * D * 2;
+  static constexpr int NS = (D == 64) ? 4 : 2;  // K/V ring stages
+  static constexpr bool SEP = (D == 64);        // P in its own TMEM columns
+  static constexpr int QB = SEP ? 2 : 1;
+  static constexpr int Q_OFF = 0;  // [QB][Q0, Q1]
+  static constexpr int K_OFF = QB * 2 * TILE;
+  static constexpr int V_OFF = K_OFF + NS * TILE;
+  static constexpr int ML_OFF = V_OFF + NS * TILE;  // [2][128] (maximum, row sum)
+  static constexpr int BAR_OFF = ML_OFF + 2 * BT * 8;
+  static constexpr int SMEM = 1024 + BAR_OFF + 512;
+  static constexpr uint32_t T_S0 = 0, T_S1 = 128, T_O0 = 256, T_O1 = 256 + D;
+  static constexpr uint32_t T_P0 = SEP ? 384 : T_S0, T_P1 = SEP ? 448 : T_S1;
+};
+
+struct Args {
+  int B, S, nh, nkv, n_t;
+  Mask mask;
+  const float* slopes;  // [nh] or nullptr
+  Score score;
+  __nv_bfloat16* out;   // [B, S, nh * D]
+  float* lse;           // [B, nh, S] natural log
+  int* err;
+};
+
+struct Item {
+  int b, h, t0, t1;  // t0 < 0: only tile t1 (odd number of tiles)
+  int2 r0, r1;       // key tiles of t0, t1
+  int lo, hi;        // their union
+};
+
+__device__ __forceinline__ Item decode(const Args& a, int item) {
+  const int BH = a.B * a.nh;
+  const int n_pairs = (a.n_t + 1) / 2;
+  const int pr = item / BH, bh = item - pr * BH;
+  const int p = n_pairs - 1 - pr;  // causal rows: the longest first
+  Item it;
+  it.b = bh / a.nh;
+  it.h = bh - it.b * a.nh;
+  it.t1 = (a.n_t & 1) ? 2 * p : 2 * p + 1;
+  it.t0 = it.t1 - 1;
+  it.r0 = it.t0 >= 0 ? key_tiles(a.mask, it.b, a.n_t, it.t0) : make_int2(0, 0);
+  it.r1 = key_tiles(a.mask, it.b, a.n_t, it.t1);
+  const bool a0 = it.r0.y > it.r0.x, a1 = it.r1.y > it.r1.x;
+  it.lo = a0 ? (a1 ? min(it.r0.x, it.r1.x) : it.r0.x) : it.r1.x;
+  it.hi = max(it.r0.y, it.r1.y);
+  if (!a0 && !a1) it.hi = it.lo;
+  return it;
+}
+
+template <int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+    masked_attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const Args a) {
+  pdl_trigger();
+  using C = Cfg<D>;
+  constexpr int NS = C::NS;
+  constexpr int QB = C::QB;
+  constexpr bool SEP = C::SEP;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* sQ = smem + C::Q_OFF;
+  uint8_t* sK = smem + C::K_OFF;
+  uint8_t* sV = smem + C::V_OFF;
+  float2* sML = reinterpret_cast<float2*>(smem + C::ML_OFF);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* q_full = bars;            // [2]
+  uint64_t* q_empty = bars + 2;       // [2]
+  uint64_t* k_full = bars + 4;        // [NS]
+  uint64_t* k_empty = k_full + NS;    // [NS]
+  uint64_t* v_full = k_empty + NS;    // [NS]
+  uint64_t* v_empty = v_full + NS;    // [NS]
+  uint64_t* s_full = v_empty + NS;    // [2]  S_i computed
+  uint64_t* s_free = s_full + 2;      // [2]  S_i in registers (SEP; 4 warps)
+  uint64_t* p_full = s_free + 2;      // [2]  P_i written (4 warps)
+  uint64_t* p_free = p_full + 2;      // [2]  PV_i that read P_i complete (SEP)
+  uint64_t* o_full = p_free + 2;      // [2]  last PV_i of the item complete
+  uint64_t* o_free = o_full + 2;      // [2]  O_i and its statistics read by the epilogue (4 warps)
+  uint64_t* ml_full = o_free + 2;     // [2]  statistics of the item written (4 warps)
+  uint64_t* drain = ml_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_items = a.B * a.nh * ((a.n_t + 1) / 2);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&p_free[i], 1);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_free[i], 4);
+      mbar_init(&ml_full[i], 4);
+    }
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_qkv);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem = *tmem_slot;
+  const int group = a.nh / a.nkv;
+
+  if (warp < 4) {
+    reg_dec<64>();
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------------- TMA
+      int kv = 0, it = 0, q_issued = -1;
+      bool ok = true;
+      for (int r = 0, item; (item = snake_item(r)) < n_items; ++r) {
+        const Item w = decode(a, item);
+        if (w.lo >= w.hi) continue;
+        const bool a0 = w.r0.y > w.r0.x, a1 = w.r1.y > w.r1.x;
+        const int hk = w.h / group;
+        const int qx = w.h * D, kx = (a.nh + hk) * D, vx = (a.nh + a.nkv + hk) * D;
+        const int qb = it % QB;
+        if (it >= QB && !bwait(&q_empty[qb], ((it / QB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+        uint8_t* qd = sQ + qb * 2 * C::TILE;
+        mbar_expect_tx(&q_full[qb], ((a0 ? 1 : 0) + (a1 ? 1 : 0)) * C::TILE);
+        if (a0) load_tile<D>(qd, &tm_qkv, &q_full[qb], qx, w.t0 * BT, w.b);
+        if (a1) load_tile<D>(qd + C::TILE, &tm_qkv, &q_full[qb], qx, w.t1 * BT, w.b);
+        q_issued = it;
+        for (int j = w.lo; j < w.hi; ++j, ++kv) {
+          const int s = kv % NS, n = kv / NS;
+          if (n > 0 && !bwait(&k_empty[s], (n - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&k_full[s], C::TILE);
+          load_tile<D>(sK + s * C::TILE, &tm_qkv, &k_full[s], kx, j * BT, w.b);
+          if (n > 0 && !bwait(&v_empty[s], (n - 1) & 1, a.err, abort_flag)) {
+            ++kv;  // the K load of this slot is in flight
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&v_full[s], C::TILE);
+          load_tile<D>(sV + s * C::TILE, &tm_qkv, &v_full[s], vx, j * BT, w.b);
+        }
+        if (!ok) break;
+        ++it;
+      }
+      if (!ok) {
+        // let the loads in flight land before the CTA's shared memory goes away
+        for (int u = max(0, q_issued - QB + 1); u <= q_issued; ++u) drain_wait(&q_full[u % QB], (u / QB) & 1);
+        for (int u = max(0, kv - NS); u < kv; ++u) {
+          drain_wait(&k_full[u % NS], (u / NS) & 1);
+          drain_wait(&v_full[u % NS], (u / NS) & 1);
+        }
+      }
+    } else if (warp == 1 && lane == 0) {
+      // ---------------------------------------------------------------- MMA
+      int kv = 0, it = 0;
+      int sc[2] = {0, 0};  // S_i issued (s_free phases)
+      int pc[2] = {0, 0};  // P_i consumed (p_full phases)
+      int ic[2] = {0, 0};  // items with an active tile (o_free phases)
+      bool ok = true;
+      auto issue_s = [&](int i, uint32_t q_addr, int stage) -> bool {
+        if (SEP && sc[i] > 0 && !bwait(&s_free[i], (sc[i] - 1) & 1, a.err, abort_flag)) return false;
+        ++sc[i];
+        tc_fence_after();
+        mma_abt<D>(tmem + (i == 0 ? C::T_S0 : C::T_S1), q_addr, smem_u32(sK + stage * C::TILE));
+        umma_commit(&s_full[i]);
+        return true;
+      };
+      auto issue_pv = [&](int i, int stage, bool first, bool last) -> bool {
+        if (!bwait(&p_full[i], pc[i] & 1, a.err, abort_flag)) return false;
+        ++pc[i];
+        if (first && ic[i] > 0 && !bwait(&o_free[i], (ic[i] - 1) & 1, a.err, abort_flag)) return false;
+        tc_fence_after();
+        mma_tmem_b<D>(tmem + (i == 0 ? C::T_O0 : C::T_O1), tmem + (i == 0 ? C::T_P0 : C::T_P1), 32,
+                      smem_u32(sV + stage * C::TILE), !first);
+        if (SEP) umma_commit(&p_free[i]);
+        if (last) umma_commit(&o_full[i]);
+        return true;
+      };
+      for (int r = 0, item; (item = snake_item(r)) < n_items; ++r) {
+        const Item w = decode(a, item);
+        if (w.lo >= w.hi) continue;
+        const int J = w.hi - w.lo;
+        const int qb = it % QB;
+        const uint32_t q0 = smem_u32(sQ + qb * 2 * C::TILE), q1 = q0 + C::TILE;
+        auto on0 = [&](int j) { return j >= w.r0.x && j < w.r0.y; };
+        auto on1 = [&](int j) { return j >= w.r1.x && j < w.r1.y; };
+        if (!bwait(&q_full[qb], (it / QB) & 1, a.err, abort_flag)) { ok = false; break; }
+        if (!bwait(&k_full[kv % NS], (kv / NS) & 1, a.err, abort_flag)) { ok = false; break; }
+        if (on0(w.lo) && !issue_s(0, q0, kv % NS)) { ok = false; break; }
+        if (on1(w.lo) && !issue_s(1, q1, kv % NS)) { ok = false; break; }
+        umma_commit(&k_empty[kv % NS]);
+        for (int u = 0; u < J && ok; ++u) {
+          const int j = w.lo + u;
+          const int st = (kv + u) % NS, ph = ((kv + u) / NS) & 1;
+          const int st1 = (kv + u + 1) % NS, ph1 = ((kv + u + 1) / NS) & 1;
+          const bool more = u + 1 < J;
+          const bool n0 = more && on0(j + 1), n1 = more && on1(j + 1);
+          if (SEP) {
+            // next scores first: they only need the softmax to have read the current ones
+            if (more) {
+              if (!bwait(&k_full[st1], ph1, a.err, abort_flag)) { ok = false; break; }
+              if (n0 && !issue_s(0, q0, st1)) { ok = false; break; }
+              if (n1 && !issue_s(1, q1, st1)) { ok = false; break; }
+              umma_commit(&k_empty[st1]);
+            }
+            if (!bwait(&v_full[st], ph, a.err, abort_flag)) { ok = false; break; }
+            if (on0(j) && !issue_pv(0, st, j == w.r0.x, j == w.r0.y - 1)) { ok = false; break; }
+            if (on1(j) && !issue_pv(1, st, j == w.r1.x, j == w.r1.y - 1)) { ok = false; break; }
+            umma_commit(&v_empty[st]);
+          } else {
+            // P_i overwrites S_i: PV0_j, S0_{j+1}, PV1_j, S1_{j+1}
+            if (!bwait(&v_full[st], ph, a.err, abort_flag)) { ok = false; break; }
+            if (on0(j) && !issue_pv(0, st, j == w.r0.x, j == w.r0.y - 1)) { ok = false; break; }
+            if (n0) {
+              if (!bwait(&k_full[st1], ph1, a.err, abort_flag)) { ok = false; break; }
+              if (!issue_s(0, q0, st1)) { ok = false; break; }
+            }
+            if (on1(j) && !issue_pv(1, st, j == w.r1.x, j == w.r1.y - 1)) { ok = false; break; }
+            umma_commit(&v_empty[st]);
+            if (more) {
+              if (!bwait(&k_full[st1], ph1, a.err, abort_flag)) { ok = false; break; }
+              if (n1 && !issue_s(1, q1, st1)) { ok = false; break; }
+              umma_commit(&k_empty[st1]);
+            }
+          }
+        }
+        if (!ok) break;
+        umma_commit(&q_empty[qb]);  // every S of this item has been issued
+        kv += J;
+        ++it;
+        if (w.r0.y > w.r0.x) ++ic[0];
+        if (w.r1.y > w.r1.x) ++ic[1];
+      }
+      if (!ok) {
+        umma_commit(drain);
+        drain_wait(drain, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ softmax
+    reg_inc<184>();
+    const int grp = (warp - 4) >> 2;
+    const int row = (warp & 3) * 32 + lane;  // query row within the tile (TMEM lane)
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + (grp == 0 ? C::T_S0 : C::T_S1) + lane_off;
+    const uint32_t t_p = tmem + (grp == 0 ? C::T_P0 : C::T_P1) + lane_off;
+    const uint32_t t_o = tmem + (grp == 0 ? C::T_O0 : C::T_O1) + lane_off;
+    const Score k = a.score;
+    int sc = 0, pc = 0, ic = 0;
+    bool ok = true;
+    for (int r = 0, item; (item = snake_item(r)) < n_items; ++r) {
+      const Item w = decode(a, item);
+      const int t = grp == 0 ? w.t0 : w.t1;
+      const int2 range = grp == 0 ? w.r0 : w.r1;
+      if (range.x >= range.y) continue;
+      const int2 full = full_tiles(a.mask, w.b, a.n_t, t);
+      const int i = t * BT + row;
+      int start = 0, end = i + 1;
+      if (a.mask.rows) {
+        const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + t) * (2 * BT) + row;
+        start = tr[0];
+        end = tr[BT];
+      }
+      float slope = 0.f;
+      if (BIAS) slope = a.slopes[w.h] * kLog2e;
+      float m = -INFINITY, l = 0.f;
+      for (int j = range.x; j < range.y; ++j) {
+        if (!wwait(&s_full[grp], sc & 1, a.err, abort_flag)) { ok = false; break; }
+        ++sc;
+        tc_fence_after();
+        uint32_t s[128];
+        tmem_ld_32x32b_x32(t_s + 0, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        tmem_ld_32x32b_x32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+        tmem_ld_32x32b_x32(t_s + 64, *reinterpret_cast<uint32_t(*)[32]>(&s[64]));
+        tmem_ld_32x32b_x32(t_s + 96, *reinterpret_cast<uint32_t(*)[32]>(&s[96]));
+        tmem_wait_ld();
+        if (SEP) warp_arrive(&s_free[grp]);  // the next S_i may be computed into these columns
+        if (CAP || BIAS) {
+          const float dist = (float)(j * BT - i);
+#pragma unroll
+          for (int c = 0; c < 128; ++c) {
+            float x = score<CAP>(__uint_as_float(s[c]), k);
+            if (BIAS) x = fmaf(-slope, fabsf(dist + (float)c), x);
+            s[c] = __float_as_uint(x);
+          }
+        }
+        if (j < full.x || j >= full.y) {
+          const int lo = start - j * BT, hi = end - j * BT;  // visible columns [lo, hi)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int l0 = min(max(lo - 32 * g, 0), 32), h0 = min(max(hi - 32 * g, 0), 32);
+            const uint32_t below_h = h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u;
+            const uint32_t below_l = l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u;
+            const uint32_t seen = below_h & ~below_l;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen & (1u << e))) s[32 * g + e] = 0xff800000u;  // -inf
+          }
+        }
+        float mx[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mx[u] = __uint_as_float(s[u]);
+#pragma unroll
+        for (int c = 8; c < 128; ++c) mx[c & 7] = fmaxf(mx[c & 7], __uint_as_float(s[c]));
+        float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                         fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+        if (!CAP && !BIAS) mt *= k.mul;
+        const bool need = mt > m + kRescaleLog2;
+        const bool any_need = __any_sync(0xffffffffu, need) != 0;
+        float alpha = 1.f;
+        if (need) {
+          alpha = fast_exp2(m - mt);  // m = -inf (nothing seen yet): 0
+          m = mt;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;  // a row that has seen nothing: every exponential is 0
+        if (SEP) {
+          // the PV that read the previous P_i (and last wrote O_i) must be complete
+          if (pc > 0 && !wwait(&p_free[grp], (pc - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+        }
+        ++pc;
+        float rs[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) rs[u] = 0.f;
+#pragma unroll
+        for (int hcol = 0; hcol < 2; ++hcol) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int c = hcol * 64 + 2 * e;
+            float p0, p1;
+            if (CAP || BIAS) {
+              p0 = fast_exp2(__uint_as_float(s[c]) - mu);
+              p1 = fast_exp2(__uint_as_float(s[c + 1]) - mu);
+            } else {
+              p0 = fast_exp2(fmaf(__uint_as_float(s[c]), k.mul, -mu));
+              p1 = fast_exp2(fmaf(__uint_as_float(s[c + 1]), k.mul, -mu));
+            }
+            rs[e & 7] += p0 + p1;
+            pk[e] = pack_bf16x2(p0, p1);
+          }
+          tmem_st_x32(t_p + hcol * 32, pk);
+        }
+        l = l * alpha + (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7])));
+        if (any_need && j > range.x) {
+          // PV_i(j-1) is complete (SEP: waited above; otherwise it was issued before S_i(j))
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(t_o + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_x32(t_o + c * 32, o);
+          }
+        }
+        tmem_wait_st();
+        warp_arrive(&p_full[grp]);
+      }
+      if (!ok) break;
+      // hand the statistics to the epilogue
+      if (ic > 0 && !wwait(&o_free[grp], (ic - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+      ++ic;
+      sML[grp * BT + row] = make_float2(m, l);
+      warp_arrive(&ml_full[grp]);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    reg_dec<80>();
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    int ic[2] = {0, 0};
+    bool ok = true;
+    for (int r = 0, item; ok && (item = snake_item(r)) < n_items; ++r) {
+      const Item w = decode(a, item);
+#pragma unroll
+      for (int grp = 0; grp < 2; ++grp) {
+        const int t = grp == 0 ? w.t0 : w.t1;
+        if (t < 0) continue;
+        const int2 range = grp == 0 ? w.r0 : w.r1;
+        const int i = t * BT + row;
+        const bool in = i < a.S;
+        __nv_bfloat16* orow = a.out + ((size_t)w.b * a.S + i) * ((size_t)a.nh * D) + (size_t)w.h * D;
+        float* lse = a.lse + ((size_t)w.b * a.nh + w.h) * a.S + i;
+        if (range.x >= range.y) {  // no row of the tile sees anything
+          if (in) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) store_zero32(orow + c * 32);
+            *lse = -INFINITY;
+          }
+          continue;
+        }
+        if (!wwait(&ml_full[grp], ic[grp] & 1, a.err, abort_flag) ||
+            !wwait(&o_full[grp], ic[grp] & 1, a.err, abort_flag)) {
+          ok = false;
+          break;
+        }
+        ++ic[grp];
+        tc_fence_after();
+        const float2 ml = sML[grp * BT + row];
+        const bool seen = ml.y != 0.f;
+        const float inv = seen ? 1.f / ml.y : 0.f;
+        const uint32_t t_o = tmem + (grp == 0 ? C::T_O0 : C::T_O1) + lane_off;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_o + c * 32, o);
+          tmem_wait_ld();
+          if (c == D / 32 - 1) warp_arrive(&o_free[grp]);  // O and the statistics are in registers
+          if (in) store_row32(orow + c * 32, o, inv);
+        }
+        if (in) *lse = seen ? ml.x * kLn2 + logf(ml.y) : -INFINITY;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, bool CAP, bool BIAS>
+int launch(const CUtensorMap& tm, const Args& a, int grid, cudaStream_t stream) {
+  auto k = masked_attn_fwd_kernel<D, CAP, BIAS>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  if (e != cudaSuccess) return (int)e;
+  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tm, a);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace fwd
+}  // namespace mattn
+
+int masked_attn_fwd(const AttnCall& c, void* out, float* lse, int* err, int num_sms, cudaStream_t stream) {
+  using namespace mattn;
+  const int n_t = (c.S + BT - 1) / BT;
+  const long items = (long)c.B * c.nh * ((n_t + 1) / 2);
+  if (items > INT_MAX / 2) return -1;
+  CUtensorMap tm;
+  const int rc = make_tmap_bf16_3d(&tm, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
+  if (rc) return rc - 10;
+  fwd::Args a;
+  a.B = c.B;
+  a.S = c.S;
+  a.nh = c.nh;
+  a.nkv = c.nkv;
+  a.n_t = n_t;
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange)};
+  a.slopes = c.slopes;
+  score_constants(c.scale, c.cap, &a.score.mul, &a.score.cap);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.err = err;
+  const int grid = (int)std::max(1L, std::min(items, (long)num_sms));
+  const bool cap = c.cap > 0.f, bias = c.slopes != nullptr;
+  if (c.d == 64) {
+    if (cap) return bias ? fwd::launch<64, true, true>(tm, a, grid, stream) : fwd::launch<64, true, false>(tm, a, grid, stream);
+    return bias ? fwd::launch<64, false, true>(tm, a, grid, stream) : fwd::launch<64, false, false>(tm, a, grid, stream);
+  }
+  if (c.d == 128) {
+    if (cap) return bias ? fwd::launch<128, true, true>(tm, a, grid, stream) : fwd::launch<128, true, false>(tm, a, grid, stream);
+    return bias ? fwd::launch<128, false, true>(tm, a, grid, stream) : fwd::launch<128, false, false>(tm, a, grid, stream);
+  }
+  return -2;
+}
+
+}  // namespace mmb

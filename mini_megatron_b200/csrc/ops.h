@@ -99,6 +99,35 @@ int flash_attn_bwd_sm100_d64(const __nv_bfloat16* dout, long ld_do, const __nv_b
                              const float* lse, const float* delta, float* dq_acc, __nv_bfloat16* dqkv, long ld_dqkv,
                              int B, int S, int nh, float softmax_scale, int* err, int num_sms, cudaStream_t stream);
 
+// Packed rows of documents (document_plan.cu): positions, visible key intervals and their tile statistics.
+int document_plan_max_len();
+int document_plan(const long* ids, long ld_ids, long eod, int by_change, const unsigned char* marks, long ld_marks,
+                  const int* lengths, int B, int S, int* positions, int* start, int* end, int* rows, void* qstat,
+                  void* krange, cudaStream_t stream);
+
+// Rotary positions (rotary.cu): heads [0, heads_rot) of x rotated into y (y may be x), the rest copied.
+int rotary(const void* x, long x_sb, long x_ss, void* y, long y_sb, long y_ss, int is_f32, const void* positions,
+           int pos64, long pos_sb, const double* freqs, float magnitude, float sign, int interleaved, long B, int S,
+           int d, int rot, int heads_rot, int heads, int num_sms, cudaStream_t stream);
+
+// Masked attention (masked_attn_*.cu) over the packed [B, S, (nh + 2 nkv) * d] bf16 activation.
+struct AttnCall {
+  const void* qkv;
+  long qkv_ss, qkv_sb;   // token and batch strides (elements)
+  int B, S, nh, nkv, d;
+  const int* rows;       // of document_plan, or nullptr: causal
+  const void* qstat;
+  const void* krange;
+  const float* slopes;   // [nh] or nullptr
+  float cap;             // 0: scores are not capped
+  float scale;
+};
+int masked_attn_fwd(const AttnCall& c, void* out, float* lse, int* err, int num_sms, cudaStream_t stream);
+int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, const void* out, const float* lse,
+                   float* ld, void* dqkv, int* err, int num_sms, cudaStream_t stream);
+int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb, const float* ld, void* dqkv, int* err,
+                    int num_sms, cudaStream_t stream);
+
 // Fused DP step (fused_dp.cu)
 struct DpPeersHost {
   int world, rank;

@@ -1,0 +1,145 @@
+"""Packed rows -> positions and visible intervals, against the definition token by token."""
+import pytest
+import torch
+
+from packed_ref import plan_ref, row_tensors, split_rows
+
+CASES = [  # B, S, mean document, prefix, pad, empty last row
+    (1, 1, 0, False, False, False),
+    (1, 1, 0, True, False, False),
+    (2, 7, 2, True, True, False),
+    (3, 128, 20, False, False, False),
+    (2, 129, 1, True, False, False),
+    (3, 257, 60, True, True, True),
+    (2, 1000, 300, True, True, False),
+    (1, 4096, 100, True, False, False),
+    (2, 4097, 1500, True, True, False),
+    (2, 9001, 4000, True, True, True),
+]
+
+
+def _check(device, B, S, doc, prefix, pad, empty, by_ids):
+    from mini_megatron_b200.ops.documents import document_plan
+    rows = split_rows(B, S, doc, prefix, pad, seed=S + B, empty_row=empty)
+    tokens, ids, marks, lengths = row_tensors(rows, S, seed=1)
+    kw = dict(prefix_mask=marks.to(device) if prefix else None,
+              lengths=lengths.to(device) if pad or empty else None)
+    if by_ids:
+        plan = document_plan(document_ids=ids.to(device), **kw)
+    else:
+        plan = document_plan(tokens.to(device), eod=0, **kw)
+    for got, want in zip((plan.positions, plan.start, plan.end), plan_ref(rows, S, prefix)):
+        assert got.dtype == torch.int32 and torch.equal(got.cpu(), want)
+    assert plan.shape == (B, S)
+    return plan
+
+
+@pytest.mark.parametrize("by_ids", [False, True])
+@pytest.mark.parametrize("B,S,doc,prefix,pad,empty", CASES)
+def test_plan_cpu(B, S, doc, prefix, pad, empty, by_ids):
+    _check("cpu", B, S, doc, prefix, pad, empty, by_ids)
+
+
+def _tile_tables(plan):
+    """What the attention kernels read, by its definition."""
+    B, S = plan.shape
+    n_t = (S + 127) // 128
+    start = torch.zeros(B, n_t * 128, dtype=torch.int32)
+    end = torch.zeros(B, n_t * 128, dtype=torch.int32)
+    start[:, :S], end[:, :S] = plan.start.cpu(), plan.end.cpu()
+    rows = torch.stack([start.view(B, n_t, 128), end.view(B, n_t, 128)], 2)
+    qstat = torch.empty(B, n_t, 4, dtype=torch.int32)
+    seen = torch.zeros(B, n_t, n_t, dtype=torch.bool)
+    for b in range(B):
+        for t in range(n_t):
+            s, e = start[b, t * 128:min(S, t * 128 + 128)], end[b, t * 128:min(S, t * 128 + 128)]
+            some = e > s
+            qstat[b, t] = torch.tensor([s[some].min() if some.any() else 2 ** 31 - 1, e[some].max() if some.any() else 0,
+                                        s.max(), e.min()])
+            for k in range(n_t):
+                seen[b, t, k] = bool(((s < k * 128 + 128) & (e > k * 128) & some).any())
+    return rows, qstat, seen
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by_ids", [False, True])
+@pytest.mark.parametrize("B,S,doc,prefix,pad,empty", CASES + [
+    (2, 40000, 9000, True, True, False), (1, 70001, 300, True, True, False), (1, 140000, 50000, True, False, False)])
+def test_plan_gpu(B, S, doc, prefix, pad, empty, by_ids):
+    plan = _check("cuda", B, S, doc, prefix, pad, empty, by_ids)
+    if S > 10000:
+        return
+    rows, qstat, seen = _tile_tables(plan)
+    got_rows, got_stat, got_range = (t.cpu() for t in plan.tiles)
+    assert torch.equal(got_rows, rows)
+    assert torch.equal(got_stat, qstat)
+    n_t = seen.shape[1]
+    for b in range(B):
+        for k in range(n_t):
+            lo, hi = got_range[b, k].tolist()
+            want = seen[b, :, k].nonzero().flatten().tolist()
+            # every tile that sees the key tile is in the range (a range may hold a tile that does not)
+            assert all(lo <= t <= hi for t in want), (b, k, lo, hi, want)
+            assert 0 <= lo and hi < n_t
+            if not want:
+                assert lo > hi or not seen[b, lo:hi + 1, k].any()
+
+
+@pytest.mark.gpu
+def test_plan_strided_rows_other_stream_and_graph():
+    from mini_megatron_b200.ops.documents import document_plan
+    rows = split_rows(3, 500, 90, True, True, seed=3)
+    tokens, _, marks, lengths = row_tensors(rows, 500, seed=2)
+    wide = torch.zeros(3, 777, dtype=torch.int64)
+    wide[:, 5:505] = tokens
+    want = plan_ref(rows, 500, True)
+    s = torch.cuda.Stream()
+    d_tok, d_marks, d_len = wide.cuda()[:, 5:505], marks.cuda(), lengths.cuda()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        plan = document_plan(d_tok, eod=0, prefix_mask=d_marks, lengths=d_len)
+    s.synchronize()
+    assert all(torch.equal(g.cpu(), w) for g, w in zip((plan.positions, plan.start, plan.end), want))
+    # captured once, replayed on new tokens
+    buf = torch.zeros(3, 500, dtype=torch.int64, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        plan = document_plan(buf, eod=0)
+    for seed in (5, 6):
+        rows = split_rows(3, 500, 40, False, False, seed=seed)
+        buf.copy_(row_tensors(rows, 500, seed=seed)[0])
+        g.replay()
+        assert all(torch.equal(x.cpu(), w) for x, w in
+                   zip((plan.positions, plan.start, plan.end), plan_ref(rows, 500, False)))
+
+
+def test_lengths_are_clamped_and_marks_may_be_bytes():
+    from mini_megatron_b200.ops.documents import document_plan
+    tok = torch.ones(2, 4, dtype=torch.int64)
+    for dtype in (torch.int32, torch.int64):
+        plan = document_plan(tok, eod=0, lengths=torch.tensor([-3, 9], dtype=dtype),
+                             prefix_mask=torch.ones(2, 4, dtype=torch.uint8))
+        assert plan.end.tolist() == [[0] * 4, [4] * 4]
+    assert plan.visible()[1].all() and not plan.visible()[0].any()
+
+
+def test_plan_refusals():
+    from mini_megatron_b200.ops.documents import document_plan
+    tok = torch.ones(2, 4, dtype=torch.int64)
+    for args, kw in [((), {}), ((tok,), {}), ((tok, 0), {"document_ids": tok}), ((), {"document_ids": tok, "eod": 1}),
+                     ((tok.int(), 0), {}), ((tok[0], 0), {}), ((tok[:, :0], 0), {}),
+                     ((tok, 0), {"prefix_mask": tok}), ((tok, 0), {"prefix_mask": torch.ones(2, 3, dtype=torch.bool)}),
+                     ((tok, 0), {"lengths": torch.ones(3, dtype=torch.int32)}),
+                     ((tok, 0), {"lengths": torch.ones(2)})]:
+        with pytest.raises(ValueError):
+            document_plan(*args, **kw)
+
+
+@pytest.mark.gpu
+def test_plan_refusals_gpu():
+    from mini_megatron_b200.ops.documents import document_plan
+    tok = torch.ones(2, 4, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError):
+        document_plan(tok, eod=0, lengths=torch.ones(2, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        document_plan(tok, eod=0, prefix_mask=torch.ones(2, 4, dtype=torch.bool))

@@ -1,0 +1,270 @@
+"""Masked attention (documents, prefixes, padding, capped scores, distance bias, shared heads) against 64 bits."""
+import pytest
+import torch
+
+from packed_ref import attention_ref, plan_ref, row_tensors, split_rows
+
+
+def _slopes(nh, device):
+    return torch.tensor([2.0 ** (-8.0 * (h + 1) / nh) for h in range(nh)], device=device)
+
+
+def _case(B, S, nh, nkv, d, doc, prefix, pad, amp, device, dtype, seed=0, empty_row=False):
+    from mini_megatron_b200.ops.documents import document_plan
+    g = torch.Generator().manual_seed(seed + S)
+    qkv = torch.randn(B, S, (nh + 2 * nkv) * d, generator=g)
+    qkv[..., :nh * d] *= amp
+    dctx = torch.randn(B, S, nh * d, generator=g)
+    plan = start = end = None
+    if doc is not None:
+        rows = split_rows(B, S, doc, prefix, pad, seed=seed + S, empty_row=empty_row)
+        tokens, _, marks, lengths = row_tensors(rows, S, seed=seed)
+        _, start, end = (t.to(device) for t in plan_ref(rows, S, prefix))
+        plan = document_plan(tokens.to(device), eod=0, prefix_mask=marks.to(device) if prefix else None,
+                             lengths=lengths.to(device))
+    return qkv.to(device, dtype), dctx.to(device, dtype), plan, start, end
+
+
+def _near(got, want, bound, what):
+    got, want = got.double(), want.double()
+    same = torch.isfinite(want)
+    assert torch.equal(same, torch.isfinite(got)) and torch.equal(got[~same], want[~same]), what
+    off = ((got - want).abs() - bound)[same]
+    assert (off <= 0).all(), f"{what}: {off.max().item():.3g} over the bound"
+
+
+def _rel(a, b):
+    return ((a.double() - b).norm() / b.norm().clamp_min(1e-30)).item()
+
+
+# B, S, nh, nkv, d, mean document (None: causal, 0: one per row), prefix, pad, cap, alibi, amp
+GRID = [
+    (1, 1, 1, 1, 64, None, False, False, 0.0, False, 1.0),
+    (1, 1, 2, 1, 128, 0, True, False, 20.0, True, 1.0),
+    (3, 2, 2, 2, 64, 1, False, True, 0.0, False, 1.0),
+    (2, 127, 3, 3, 64, None, False, False, 0.0, False, 2.0),
+    (2, 128, 2, 1, 128, None, False, False, 0.0, True, 1.0),
+    (2, 129, 4, 2, 64, 30, False, True, 30.0, False, 4.0),
+    (1, 255, 2, 2, 128, 40, True, True, 0.0, True, 1.0),
+    (2, 256, 4, 1, 64, 0, True, False, 0.0, False, 1.0),
+    (2, 300, 6, 2, 128, 100, True, True, 50.0, True, 3.0),
+    (1, 513, 2, 2, 64, None, False, False, 15.0, True, 4.0),
+    (1, 640, 3, 3, 128, None, False, False, 0.0, False, 3.0),
+    (3, 777, 2, 2, 64, 5, False, True, 0.0, False, 1.0),
+    (2, 1000, 4, 4, 128, 350, True, True, 25.0, False, 2.0),
+    (1, 1537, 2, 1, 64, 600, False, True, 0.0, True, 2.0),
+    (5, 384, 12, 12, 64, 200, True, False, 0.0, False, 1.0),
+    (40, 130, 5, 5, 64, 50, False, True, 0.0, False, 1.0),
+    (9, 260, 10, 2, 128, 0, False, True, 0.0, False, 1.0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,nh,nkv,d,doc,prefix,pad,cap,alibi,amp", GRID)
+def test_forward_and_backward(B, S, nh, nkv, d, doc, prefix, pad, cap, alibi, amp):
+    from mini_megatron_b200.ops import check_errors
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    qkv, dctx, plan, start, end = _case(B, S, nh, nkv, d, doc, prefix, pad, amp, "cuda", torch.bfloat16,
+                                        empty_row=pad and B > 2)
+    slopes = _slopes(nh, "cuda") if alibi else None
+    opts = dict(num_kv_heads=nkv, plan=plan, softcap=cap or None, alibi_slopes=slopes)
+    ctx, lse = attention_fwd(qkv, nh, d, **opts)
+    dqkv = attention_bwd(dctx, qkv, ctx, lse, nh, d, **opts)
+    check_errors()
+    (r_ctx, r_lse, r_grad), (b_ctx, b_lse, b_grad) = attention_ref(qkv, dctx, nh, nkv, d, start, end, cap, slopes)
+    _near(ctx, r_ctx, b_ctx, "ctx")
+    _near(lse, r_lse, b_lse, "lse")
+    _near(dqkv, r_grad, b_grad, "dqkv")
+    # three or four independent roundings of at most 2^-8 each (rms at most 2^-8 / sqrt 3): 2 * 2^-8 / sqrt 3 at most
+    assert _rel(ctx, r_ctx) < 4.6e-3 and _rel(dqkv, r_grad) < 4.6e-3 or r_grad.norm() < 1e-6 * dctx.norm().double()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_scale_and_large_scores(d):
+    """Scores spread over hundreds of log2 units: the running maximum moves and rows are nearly one-hot."""
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    qkv, dctx, plan, start, end = _case(2, 700, 2, 2, d, 300, True, False, 6.0, "cuda", torch.bfloat16, seed=5)
+    ctx, lse = attention_fwd(qkv, 2, d, plan=plan, softmax_scale=0.3)
+    grad = attention_bwd(dctx, qkv, ctx, lse, 2, d, plan=plan, softmax_scale=0.3)
+    want, bound = attention_ref(qkv, dctx, 2, 2, d, start, end, scale=0.3)
+    for g, w, b, n in zip((ctx, lse, grad), want, bound, ("ctx", "lse", "dqkv")):
+        _near(g, w, b, n)
+
+
+@pytest.mark.gpu
+def test_same_bits_twice_and_on_another_stream():
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    qkv, dctx, plan, _, _ = _case(3, 900, 8, 2, 64, 250, True, True, 1.0, "cuda", torch.bfloat16)
+    outs = []
+    for k in range(3):
+        s = torch.cuda.Stream() if k else torch.cuda.current_stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            ctx, lse = attention_fwd(qkv, 8, 64, num_kv_heads=2, plan=plan, softcap=30.0)
+            outs.append((ctx, lse, attention_bwd(dctx, qkv, ctx, lse, 8, 64, num_kv_heads=2, plan=plan, softcap=30.0)))
+        torch.cuda.current_stream().wait_stream(s)
+    for got in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, outs[0]))
+
+
+@pytest.mark.gpu
+def test_strides_and_neighbours():
+    """Rows inside wider buffers, a token-major batch; padding gives zeros, what lies around is not read into it."""
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    B, S, nh, d = 3, 200, 2, 64
+    qkv, dctx, plan, _, _ = _case(B, S, nh, nh, d, 70, False, True, 1.0, "cuda", torch.bfloat16)
+    want = attention_fwd(qkv, nh, d, plan=plan)
+    grad = attention_bwd(dctx, qkv, *want, nh, d, plan=plan)
+    wide = torch.full((B, S + 9, 3 * nh * d + 24), float("nan"), device="cuda", dtype=torch.bfloat16)
+    view = wide[:, 4:4 + S, 16:16 + 3 * nh * d]
+    view.copy_(qkv)
+    dwide = torch.full((S + 3, B, nh * d + 8), float("nan"), device="cuda", dtype=torch.bfloat16)
+    dview = dwide[1:1 + S, :, 8:].transpose(0, 1)
+    dview.copy_(dctx)
+    got = attention_fwd(view, nh, d, plan=plan)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(attention_bwd(dview, view, *got, nh, d, plan=plan), grad)
+    pad = plan.end == 0
+    assert pad.any()
+    assert (want[0][pad] == 0).all() and (grad[pad] == 0).all()
+    assert (want[1].transpose(1, 2)[pad] == float("-inf")).all()
+
+
+@pytest.mark.gpu
+def test_two_graphs_share_nothing():
+    """Forward and backward captured twice, replayed alternately on new values, against eager calls."""
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    sets = [_case(2, 333, 4, 2, 64, 90, True, True, 1.0, "cuda", torch.bfloat16, seed=s) for s in (1, 2)]
+    graphs = []
+    for qkv, dctx, plan, _, _ in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ctx, lse = attention_fwd(qkv, 4, 64, num_kv_heads=2, plan=plan)
+            grad = attention_bwd(dctx, qkv, ctx, lse, 4, 64, num_kv_heads=2, plan=plan)
+        graphs.append((g, ctx, lse, grad))
+    for k in range(3):
+        for qkv, dctx, *_ in sets:
+            qkv.copy_(torch.randn_like(qkv))
+        for g, *_ in graphs:
+            g.replay()
+        for (qkv, dctx, plan, _, _), (_, ctx, lse, grad) in zip(sets, graphs):
+            c, l = attention_fwd(qkv, 4, 64, num_kv_heads=2, plan=plan)
+            assert torch.equal(c, ctx) and torch.equal(l, lse)
+            assert torch.equal(attention_bwd(dctx, qkv, c, l, 4, 64, num_kv_heads=2, plan=plan), grad)
+
+
+@pytest.mark.gpu
+def test_autograd_and_broadcast_gradient():
+    from mini_megatron_b200.ops.attention import attention, attention_bwd, attention_fwd
+    qkv, _, plan, _, _ = _case(2, 150, 2, 2, 64, 60, False, True, 1.0, "cuda", torch.bfloat16)
+    leaf = qkv.clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(attention(leaf, 2, 64, plan=plan).sum(), leaf)   # an expanded gradient
+    ctx, lse = attention_fwd(qkv, 2, 64, plan=plan)
+    assert torch.equal(got, attention_bwd(torch.ones_like(ctx), qkv, ctx, lse, 2, 64, plan=plan))
+    frozen = attention(qkv, 2, 64, plan=plan)
+    assert not frozen.requires_grad and torch.equal(frozen, ctx)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_matches_plain_causal_attention(d):
+    """No plan, one K/V head per query head: the function of the framework's causal kernels."""
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd, flash_attn_bwd, flash_attn_fwd
+    B, S, nh = 2, 512, 4
+    qkv, dctx, _, _, _ = _case(B, S, nh, nh, d, None, False, False, 1.0, "cuda", torch.bfloat16)
+    ctx, lse = attention_fwd(qkv, nh, d)
+    c2, l2 = flash_attn_fwd(qkv.view(B * S, -1), B, S, nh, d)
+    _, (b_ctx, b_lse, b_grad) = attention_ref(qkv, dctx, nh, nh, d)
+    _near(ctx, c2.view_as(ctx), 2 * b_ctx, "ctx")
+    _near(lse, l2, 2 * b_lse, "lse")
+    g2 = flash_attn_bwd(dctx.view(B * S, -1), qkv.view(B * S, -1), c2, l2, B, S, nh, d)
+    _near(attention_bwd(dctx, qkv, ctx, lse, nh, d), g2.view_as(qkv), 2 * b_grad, "dqkv")
+
+
+@pytest.mark.gpu
+def test_empty_batch():
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    for B, S in ((0, 5), (2, 0)):
+        qkv = torch.zeros(B, S, 192, device="cuda", dtype=torch.bfloat16)
+        ctx, lse = attention_fwd(qkv, 1, 64)
+        assert ctx.shape == (B, S, 64) and lse.shape == (B, 1, S)
+        assert attention_bwd(ctx, qkv, ctx, lse, 1, 64).shape == qkv.shape
+
+
+@pytest.mark.parametrize("B,S,nh,nkv,d,doc,prefix,pad,cap,alibi,amp", GRID[:10])
+def test_cpu_path(B, S, nh, nkv, d, doc, prefix, pad, cap, alibi, amp):
+    from mini_megatron_b200.ops.attention import attention, attention_fwd
+    qkv, dctx, plan, start, end = _case(B, S, nh, nkv, d, doc, prefix, pad, amp, "cpu", torch.float64)
+    slopes = _slopes(nh, "cpu") if alibi else None
+    opts = dict(num_kv_heads=nkv, plan=plan, softcap=cap or None, alibi_slopes=slopes)
+    (r_ctx, r_lse, r_grad), _ = attention_ref(qkv, dctx, nh, nkv, d, start, end, cap, slopes)
+    ctx, lse = attention_fwd(qkv, nh, d, **opts)
+    torch.testing.assert_close(ctx, r_ctx, rtol=1e-9, atol=1e-9)
+    torch.testing.assert_close(lse, r_lse, rtol=1e-9, atol=1e-9)
+    leaf = qkv.clone().requires_grad_(True)
+    (grad,) = torch.autograd.grad(attention(leaf, nh, d, **opts), leaf, dctx)
+    torch.testing.assert_close(grad, r_grad, rtol=1e-7, atol=1e-7)
+
+
+def test_reference_gradient_against_differences():
+    """The formula behind every gradient test, by central differences along random directions."""
+    g = torch.Generator().manual_seed(0)
+    B, S, nh, nkv, d = 2, 23, 4, 2, 8
+    rows = split_rows(B, S, 9, True, True, seed=4)
+    _, start, end = plan_ref(rows, S, True)
+    qkv = torch.randn(B, S, (nh + 2 * nkv) * d, generator=g, dtype=torch.float64)
+    dctx = torch.randn(B, S, nh * d, generator=g, dtype=torch.float64)
+    slopes = _slopes(nh, "cpu")
+
+    def value(x):
+        return (attention_ref(x, None, nh, nkv, d, start, end, 3.0, slopes)[0][0] * dctx).sum().item()
+
+    grad = attention_ref(qkv, dctx, nh, nkv, d, start, end, 3.0, slopes)[0][2]
+    for _ in range(3):
+        z = torch.randn(qkv.shape, generator=g, dtype=torch.float64)
+        slope = (value(qkv + 1e-5 * z) - value(qkv - 1e-5 * z)) / 2e-5
+        assert abs(slope - (grad * z).sum().item()) < 1e-6 * max(1.0, abs(slope))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_refusals(device):
+    from mini_megatron_b200.ops.attention import attention_fwd
+    from mini_megatron_b200.ops.documents import document_plan
+    x = torch.zeros(2, 4, 384, device=device, dtype=torch.bfloat16)
+    plan = document_plan(torch.ones(2, 5, dtype=torch.int64, device=device), eod=0)
+    for args, kw in [((x[0], 2, 64), {}), ((x, 2, 64), {"plan": plan}), ((x, 2, 64), {"softcap": 0.0}),
+                     ((x, 2, 64), {"softcap": -1.0}),
+                     ((x, 2, 64), {"alibi_slopes": torch.ones(2, device=device, requires_grad=True)})]:
+        with pytest.raises(ValueError):
+            attention_fwd(*args, **kw)
+    for args, kw in [((x, 3, 64), {}), ((x, 4, 64), {"num_kv_heads": 3}), ((x, 4, 64), {"num_kv_heads": 0})]:
+        with pytest.raises((ValueError, RuntimeError)):
+            attention_fwd(*args, **kw)
+
+
+@pytest.mark.gpu
+def test_refusals_gpu():
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    from mini_megatron_b200.ops.documents import document_plan
+    x = torch.zeros(2, 4, 384, device="cuda", dtype=torch.bfloat16)
+    wide = torch.zeros(2, 4, 400, device="cuda", dtype=torch.bfloat16)
+    bad = [((x.float(), 2, 64), {}), ((x, 4, 32), {}), ((x, 2, 64), {"softcap": 1e6}),
+           ((x, 2, 64), {"softmax_scale": 0.0}), ((x, 2, 64), {"softmax_scale": float("nan")}),
+           ((x, 2, 64), {"alibi_slopes": torch.ones(3, device="cuda")}),
+           ((x, 2, 64), {"alibi_slopes": torch.ones(2)}),
+           ((x, 2, 64), {"alibi_slopes": torch.ones(2, device="cuda", dtype=torch.float64)}),
+           ((wide[..., 4:388], 2, 64), {}),                                    # rows off the 16-byte boundary
+           ((x.transpose(1, 2).contiguous().transpose(1, 2), 2, 64), {}),       # not dense
+           ((x[:1].expand(2, 4, 384), 2, 64), {})]                             # one row for the whole batch
+    for args, kw in bad:
+        with pytest.raises(RuntimeError):
+            attention_fwd(*args, **kw)
+    with pytest.raises(ValueError):
+        attention_fwd(x, 2, 64, plan=document_plan(torch.ones(2, 4, dtype=torch.int64), eod=0))
+    ctx, lse = attention_fwd(x, 2, 64)
+    for args in [(ctx.float(), x, ctx, lse), (ctx[:, :3], x, ctx, lse), (ctx, x, ctx[:, :, :64], lse),
+                 (ctx, x, ctx, lse[:, :1]), (ctx, x, ctx, lse.double()), (ctx, x, ctx.transpose(0, 1), lse),
+                 (ctx.cpu(), x, ctx, lse), (ctx, x, ctx, lse.cpu())]:
+        with pytest.raises(RuntimeError):
+            attention_bwd(*args, 2, 64)
