@@ -62,6 +62,16 @@ def parse_args(argv=None):
     p.add_argument("--seq-len", type=int)
     p.add_argument("--vocab-pad", type=int, default=None,
                    help="pad the vocabulary tables to a multiple of this times tp (default 128)")
+    p.add_argument("--num-kv-heads", type=int, help="K/V heads, shared by equal groups of query heads (tp = 1)")
+    p.add_argument("--position-embedding", choices=["learned", "rotary", "alibi"])
+    p.add_argument("--rotary-percent", type=float, help="part of each head that is rotated")
+    p.add_argument("--rotary-base", type=float)
+    p.add_argument("--rotary-interleaved", action="store_true", default=None, help="rotate neighbours, not halves")
+    p.add_argument("--rotary-scaling", choices=["linear", "ntk", "yarn"])
+    p.add_argument("--rotary-factor", type=float, help="how far --rotary-scaling stretches the original positions")
+    p.add_argument("--rotary-original-max-positions", type=int)
+    p.add_argument("--attn-softcap", type=float, help="cap attention scores: cap * tanh(score / cap)")
+    p.add_argument("--eod-token", type=int, help="rows are packed documents that end with this token (pp = 1)")
     p.add_argument("--num-microbatches", type=int, default=1)
     p.add_argument("--sequence-parallel", action="store_true")
     p.add_argument("--zero1", action="store_true")
@@ -87,7 +97,9 @@ def parse_args(argv=None):
 
 def model_config(args) -> GPTConfig:
     base = dataclasses.replace(PRESETS[args.model])
-    for f in ("num_layers", "hidden_size", "num_attention_heads", "ffn_hidden_size", "vocab_size"):
+    for f in ("num_layers", "hidden_size", "num_attention_heads", "ffn_hidden_size", "vocab_size", "num_kv_heads",
+              "position_embedding", "rotary_percent", "rotary_base", "rotary_interleaved", "rotary_scaling",
+              "rotary_factor", "rotary_original_max_positions", "attn_softcap", "eod_token"):
         v = getattr(args, f)
         if v is not None:
             setattr(base, f, v)

@@ -52,10 +52,25 @@ class GPTConfig:
     max_seq_len: int = MAX_SEQ_LEN
     vocab_size: int = VOCAB_SIZE
     vocab_pad_multiple: int = 128
+    # attention variants (the defaults are the reference's model)
+    num_kv_heads: int | None = None          # K/V heads, each shared by num_attention_heads / num_kv_heads query heads
+    position_embedding: str = "learned"      # "learned" (table), "rotary" or "alibi" (bias linear in the distance)
+    rotary_percent: float = 1.0              # part of each head that is rotated
+    rotary_base: float = 10000.0
+    rotary_interleaved: bool = False         # pairs are neighbours instead of halves
+    rotary_scaling: str | None = None        # "linear", "ntk" or "yarn": stretch rotary_original_max_positions
+    rotary_factor: float = 1.0               # ... by this factor
+    rotary_original_max_positions: int | None = None
+    attn_softcap: float | None = None        # scores become cap * tanh(score / cap)
+    eod_token: int | None = None             # rows are packed documents that end with this token
 
     @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_attention_heads
+
+    @property
+    def kv_heads(self) -> int:
+        return self.num_attention_heads if self.num_kv_heads is None else self.num_kv_heads
 
     def as_dict(self):
         return dataclasses.asdict(self)
@@ -63,13 +78,16 @@ class GPTConfig:
     def num_params(self, padded_vocab: int | None = None) -> int:
         h, f, L = self.hidden_size, self.ffn_hidden_size, self.num_layers
         v = padded_vocab or self.vocab_size
-        per_layer = 3 * h * h + h * h + 2 * h * f + 4 * h
-        return L * per_layer + 2 * v * h + self.max_seq_len * h + 2 * h
+        qkv = (self.num_attention_heads + 2 * self.kv_heads) * self.head_dim
+        per_layer = qkv * h + h * h + 2 * h * f + 4 * h
+        table = self.max_seq_len * h if self.position_embedding == "learned" else 0
+        return L * per_layer + 2 * v * h + table + 2 * h
 
     def flops_per_token(self, seq_len: int) -> float:
         """Training FLOPs per token (fwd + bwd, causal attention counted at half)."""
         h, f, L, v = self.hidden_size, self.ffn_hidden_size, self.num_layers, self.vocab_size
-        dense = 2 * (3 * h * h + h * h + 2 * h * f) * L + 2 * h * v
+        qkv = (self.num_attention_heads + 2 * self.kv_heads) * self.head_dim
+        dense = 2 * (qkv * h + h * h + 2 * h * f) * L + 2 * h * v
         attn = 2 * 2 * seq_len * h * L / 2
         return 3.0 * (dense + attn)
 

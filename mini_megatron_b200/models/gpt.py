@@ -18,7 +18,7 @@ from ..parallel import process_groups as pg
 from ..parallel.tensor_parallel import ColumnParallelLinear, pad_vocab_size
 from .embedding import Embedding
 from .loss import CrossEntropyLoss
-from .transformer import GPT, Decoder, DecoderLayer, head_forward
+from .transformer import GPT, AttentionSpec, Decoder, DecoderLayer, head_forward
 
 
 def padded_vocab(cfg: GPTConfig) -> int:
@@ -38,16 +38,33 @@ def _lm_head(cfg):
     return head
 
 
+def attention_spec(cfg: GPTConfig) -> AttentionSpec:
+    """The attention variant a configuration asks for."""
+    if cfg.position_embedding not in ("learned", "rotary", "alibi"):
+        raise ValueError(f"position_embedding must be learned, rotary or alibi, got {cfg.position_embedding!r}")
+    rotary = None
+    if cfg.position_embedding == "rotary":
+        from ..ops.rotary import Rotary
+        rotary = Rotary(cfg.head_dim, rotary_dim=int(cfg.head_dim * cfg.rotary_percent), base=cfg.rotary_base,
+                        interleaved=cfg.rotary_interleaved, scaling=cfg.rotary_scaling, factor=cfg.rotary_factor,
+                        original_max_positions=cfg.rotary_original_max_positions)
+    if cfg.attn_softcap is not None and not cfg.attn_softcap > 0:
+        raise ValueError("attn_softcap must be positive (None: scores are not capped)")
+    return AttentionSpec(num_kv_heads=cfg.num_kv_heads, rotary=rotary, alibi=cfg.position_embedding == "alibi",
+                         softcap=cfg.attn_softcap)
+
+
 def build_gpt(cfg: GPTConfig, device=None, sequence_parallel=None, recompute=False) -> GPT:
     vp = padded_vocab(cfg)
-    embedding = Embedding(cfg.vocab_size, cfg.hidden_size, cfg.max_seq_len, vp, sequence_parallel)
+    embedding = Embedding(cfg.vocab_size, cfg.hidden_size, cfg.max_seq_len, vp, sequence_parallel,
+                          learned_positions=cfg.position_embedding == "learned")
     decoder = Decoder(cfg.hidden_size, cfg.num_attention_heads, cfg.ffn_hidden_size, cfg.num_layers,
-                      sequence_parallel=sequence_parallel, recompute=recompute)
+                      sequence_parallel=sequence_parallel, recompute=recompute, spec=attention_spec(cfg))
     ln_f = nn.LayerNorm(cfg.hidden_size)
     sp = pg.sequence_parallel_enabled() if sequence_parallel is None else sequence_parallel
     for p in ln_f.parameters():
         p.sequence_parallel_grad = bool(sp)
-    model = GPT(embedding, decoder, ln_f, _lm_head(cfg), CrossEntropyLoss(cfg.vocab_size))
+    model = GPT(embedding, decoder, ln_f, _lm_head(cfg), CrossEntropyLoss(cfg.vocab_size), eod_token=cfg.eod_token)
     return model.to(device) if device is not None else model
 
 
@@ -63,16 +80,21 @@ class GPTStage(nn.Module):
 
     def __init__(self, cfg: GPTConfig, pp_rank: int, pp_size: int, sequence_parallel=None, recompute=False):
         super().__init__()
+        if cfg.eod_token is not None:
+            raise ValueError("eod_token needs the tokens in every stage: packed documents run with pipeline size 1")
         self.cfg = cfg
         self.pp_rank, self.pp_size = pp_rank, pp_size
         self.is_first, self.is_last = pp_rank == 0, pp_rank == pp_size - 1
         start, end = stage_layer_range(cfg.num_layers, pp_rank, pp_size)
         self.layer_ids = list(range(start, end))
         vp = padded_vocab(cfg)
-        self.embedding = (Embedding(cfg.vocab_size, cfg.hidden_size, cfg.max_seq_len, vp, sequence_parallel)
+        self.embedding = (Embedding(cfg.vocab_size, cfg.hidden_size, cfg.max_seq_len, vp, sequence_parallel,
+                                    learned_positions=cfg.position_embedding == "learned")
                           if self.is_first else None)
+        spec = attention_spec(cfg)
         self.decoder_layers = nn.ModuleList([
-            DecoderLayer(cfg.hidden_size, cfg.num_attention_heads, cfg.ffn_hidden_size, sequence_parallel, recompute)
+            DecoderLayer(cfg.hidden_size, cfg.num_attention_heads, cfg.ffn_hidden_size, sequence_parallel, recompute,
+                         spec)
             for _ in self.layer_ids
         ])
         sp = pg.sequence_parallel_enabled() if sequence_parallel is None else sequence_parallel

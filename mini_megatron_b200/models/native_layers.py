@@ -33,7 +33,6 @@ import torch.distributed as dist
 
 from ..comm import sequence_parallel as spc
 from ..ops import native
-from ..ops.attention import flash_attn_bwd, flash_attn_fwd
 from ..ops.linear import EPI_DGELU, EPI_RESID, linear_dgrad, linear_fwd, linear_gelu_fwd, linear_wgrad
 from ..parallel.param_buffer import bf16_weight, grad_target
 
@@ -90,14 +89,14 @@ def _reduce(t2, B, group, sp):
     return t2
 
 
-def _layer_forward(x2, layer, B, S, group, sp):
+def _layer_forward(x2, layer, B, S, group, sp, plan=None):
     """Forward of one DecoderLayer on [B*S_l, H] fp32; returns (out, saved tensors)."""
     attn, mlp = layer.attn, layer.mlp
     t = _world(group)
     ln1, m1, r1 = _ln_fwd(x2, layer.ln1)
     ln1_full = _gather_seq(ln1, B, group) if sp else ln1
     qkv = linear_fwd(ln1_full, bf16_weight(attn.qkv.weight))
-    ctx_out, lse = flash_attn_fwd(qkv, B, S, attn.num_heads, attn.head_dim)
+    ctx_out, lse, qkv = attn.native_core_fwd(qkv, B, S, plan)
     if t == 1:
         x1 = linear_fwd(ctx_out, bf16_weight(attn.o.weight), out=torch.empty_like(x2), epi=EPI_RESID, resid=x2)
     else:
@@ -115,7 +114,7 @@ def _layer_forward(x2, layer, B, S, group, sp):
     return out, saved
 
 
-def _layer_backward(dout, saved, layer, B, S, group, sp):
+def _layer_backward(dout, saved, layer, B, S, group, sp, plan=None):
     attn, mlp = layer.attn, layer.mlp
     t = _world(group)
     (x2, m1, r1, ln1_full, qkv, ctx_out, lse, x1, m2, r2, ln2_full, gelu_grad, act) = saved
@@ -136,7 +135,7 @@ def _layer_backward(dout, saved, layer, B, S, group, sp):
     wo, wqkv = attn.o.weight, attn.qkv.weight
     d_ctx = linear_dgrad(g_full, bf16_weight(wo))
     linear_wgrad(g_full, ctx_out, grad_target(wo))
-    dqkv = flash_attn_bwd(d_ctx, qkv, ctx_out, lse, B, S, attn.num_heads, attn.head_dim)
+    dqkv = attn.native_core_bwd(d_ctx, qkv, ctx_out, lse, B, S, plan)
     d_ln1 = linear_dgrad(dqkv, bf16_weight(wqkv))
     linear_wgrad(dqkv, ln1_full, grad_target(wqkv))
     if t > 1:
@@ -144,14 +143,14 @@ def _layer_backward(dout, saved, layer, B, S, group, sp):
     return _ln_bwd(d_ln1, x2, m1, r1, layer.ln1, dres=dx1, want_bf16=True)
 
 
-def _layer_forward_fused(x2, layer, B, S, ws):
+def _layer_forward_fused(x2, layer, B, S, ws, plan=None):
     """Sequence-parallel layer forward with the TP collectives fused into the kernels (parallel/fused_tp.py)."""
     attn, mlp = layer.attn, layer.mlp
     slot = layer._mmb_tp_slot
     ln1_full, m1, r1, e1 = ws.ln_fwd_ag(x2, layer.ln1, 2 * slot)
     qkv = torch.empty(ws.rows, attn.qkv.weight.shape[0], device=x2.device, dtype=torch.bfloat16)
     ws.gemm_ag(ln1_full, e1, bf16_weight(attn.qkv.weight), False, qkv)
-    ctx_out, lse = flash_attn_fwd(qkv, B, S, attn.num_heads, attn.head_dim)
+    ctx_out, lse, qkv = attn.native_core_fwd(qkv, B, S, plan)
     x1 = ws.rs_reduce(ws.gemm_rs(ctx_out, bf16_weight(attn.o.weight), False), resid=x2)
     ln2_full, m2, r2, e2 = ws.ln_fwd_ag(x1, layer.ln2, 2 * slot + 1)
     n_ffn = mlp.fc1.weight.shape[0]
@@ -165,7 +164,7 @@ def _layer_forward_fused(x2, layer, B, S, ws):
     return out, saved
 
 
-def _layer_backward_fused(dout, saved, layer, B, S, ws):
+def _layer_backward_fused(dout, saved, layer, B, S, ws, plan=None):
     attn, mlp = layer.attn, layer.mlp
     (x2, m1, r1, ln1_full, qkv, ctx_out, lse, x1, m2, r2, ln2_full, gelu_grad, act) = saved
     w2, w1, wo, wqkv = mlp.fc2.weight, mlp.fc1.weight, attn.o.weight, attn.qkv.weight
@@ -183,7 +182,7 @@ def _layer_backward_fused(dout, saved, layer, B, S, ws):
     d_ctx = torch.empty(ws.rows, wo.shape[1], device=dout.device, dtype=torch.bfloat16)
     ws.gemm_ag(g_full, eg, bf16_weight(wo), True, d_ctx)
     linear_wgrad(g_full, ctx_out, grad_target(wo))
-    dqkv = flash_attn_bwd(d_ctx, qkv, ctx_out, lse, B, S, attn.num_heads, attn.head_dim)
+    dqkv = attn.native_core_bwd(d_ctx, qkv, ctx_out, lse, B, S, plan)
     e_rs = ws.gemm_rs(dqkv, bf16_weight(wqkv), True)
     linear_wgrad(dqkv, ln1_full, grad_target(wqkv))
     d_ln1 = ws.rs_reduce(e_rs, out_bf16=True)
@@ -194,7 +193,7 @@ class DecoderLayerFn(torch.autograd.Function):
     """x_out = x + MLP(LN2(x1)), x1 = x + Attn(LN1(x)) on the native kernels."""
 
     @staticmethod
-    def forward(ctx, x, layer, group, sp, recompute, *params):
+    def forward(ctx, x, layer, group, sp, recompute, plan, *params):
         # ``params`` are passed only so autograd knows the output depends on
         # them; their gradients are accumulated into main_grad by the kernels.
         ctx.n_params = len(params)
@@ -204,10 +203,11 @@ class DecoderLayerFn(torch.autograd.Function):
         ws = getattr(layer, "_mmb_tp_ws", None) if sp else None
         ctx.ws = ws
         if ws is not None:
-            out, saved = _layer_forward_fused(x2, layer, B, S, ws)
+            out, saved = _layer_forward_fused(x2, layer, B, S, ws, plan)
         else:
-            out, saved = _layer_forward(x2, layer, B, S, group, sp)
+            out, saved = _layer_forward(x2, layer, B, S, group, sp, plan)
         ctx.layer, ctx.group, ctx.sp, ctx.B, ctx.S, ctx.recompute = layer, group, sp, B, S, recompute
+        ctx.plan = plan
         if recompute:
             ctx.save_for_backward(x2)
         else:
@@ -224,9 +224,9 @@ class DecoderLayerFn(torch.autograd.Function):
         if ctx.recompute:
             (x2,) = ctx.saved_tensors
             if ws is not None:
-                _, saved = _layer_forward_fused(x2, ctx.layer, ctx.B, ctx.S, ws)
+                _, saved = _layer_forward_fused(x2, ctx.layer, ctx.B, ctx.S, ws, ctx.plan)
             else:
-                _, saved = _layer_forward(x2, ctx.layer, ctx.B, ctx.S, ctx.group, ctx.sp)
+                _, saved = _layer_forward(x2, ctx.layer, ctx.B, ctx.S, ctx.group, ctx.sp, ctx.plan)
         else:
             saved = ctx.saved_tensors
         if getattr(dout, "_mmb_bf16", None) is not None:
@@ -234,9 +234,9 @@ class DecoderLayerFn(torch.autograd.Function):
         if getattr(dout, "_mmb_gathered", None) is not None:
             d2._mmb_gathered = dout._mmb_gathered
         if ws is not None:
-            dx = _layer_backward_fused(d2, saved, ctx.layer, ctx.B, ctx.S, ws)
+            dx = _layer_backward_fused(d2, saved, ctx.layer, ctx.B, ctx.S, ws, ctx.plan)
         else:
-            dx = _layer_backward(d2, saved, ctx.layer, ctx.B, ctx.S, ctx.group, ctx.sp)
+            dx = _layer_backward(d2, saved, ctx.layer, ctx.B, ctx.S, ctx.group, ctx.sp, ctx.plan)
         for hook in getattr(ctx.layer, "_mmb_grad_ready_hooks", ()):
             hook()
         out = dx.view(B, S_l, H)
@@ -244,7 +244,7 @@ class DecoderLayerFn(torch.autograd.Function):
             out._mmb_bf16 = dx._mmb_bf16.view(B, S_l, H)
         if getattr(dx, "_mmb_gathered", None) is not None:
             out._mmb_gathered = dx._mmb_gathered
-        return (out, None, None, None, None) + (None,) * ctx.n_params
+        return (out, None, None, None, None, None) + (None,) * ctx.n_params
 
 
 def run_grad_ready_hooks(module):
@@ -254,7 +254,7 @@ def run_grad_ready_hooks(module):
 
 
 class EmbeddingFn(torch.autograd.Function):
-    """x = tok_emb(ids) (vocab-parallel, TP-summed) + pos_emb; SP keeps the local sequence shard."""
+    """x = tok_emb(ids) (vocab-parallel, TP-summed) + pos_emb (if any); SP keeps the local sequence shard."""
 
     @staticmethod
     def forward(ctx, ids, emb, group, sp, *params):
@@ -267,6 +267,8 @@ class EmbeddingFn(torch.autograd.Function):
         ws = getattr(emb, "_mmb_tp_ws", None) if sp else None
         ctx.ws = ws
         if ws is not None:
+            if emb.position_embedding is None:
+                raise RuntimeError("the fused tensor-parallel embedding adds a learned position table; use tp_impl=nccl")
             # fused TP: each vocabulary owner writes tok + pos of its rows into their sequence owner
             out = ws.emb_fwd(ids_c.view(-1), tok.weight.detach(), emb.position_embedding.weight.detach(),
                              tok.vocab_start_index, tok.vocab_end_index)
@@ -275,7 +277,8 @@ class EmbeddingFn(torch.autograd.Function):
             return out.view(B, -1, H)
         full = torch.empty(B * S, H, device=ids.device, dtype=torch.float32)
         tp_rank = dist.get_rank(group=group) if _world(group) > 1 else 0
-        wpe = emb.position_embedding.weight.detach() if tp_rank == 0 else None
+        pos = emb.position_embedding
+        wpe = pos.weight.detach() if pos is not None and tp_rank == 0 else None
         C.embedding_fwd(ids_c.view(-1), tok.weight.detach(), wpe, full, S, tok.vocab_start_index,
                         tok.vocab_end_index)
         out = _reduce(full, B, group, sp) if _world(group) > 1 else full
@@ -300,7 +303,7 @@ class EmbeddingFn(torch.autograd.Function):
         if ctx.sp:
             d2 = _gather_seq(d2, B, group).contiguous()
         native().embedding_bwd(ids.view(-1), d2, grad_target(tok.weight),
-                               grad_target(pos.weight) if pos.weight.requires_grad else None, B, S,
+                               grad_target(pos.weight) if pos is not None and pos.weight.requires_grad else None, B, S,
                                tok.vocab_start_index, tok.vocab_end_index)
         run_grad_ready_hooks(emb)
         return (None, None, None, None) + (None,) * ctx.n_params

@@ -13,8 +13,16 @@ Two execution paths share these modules:
 * CPU tensors -> the same math in plain PyTorch ops (pre-LN, fused QKV with
   the stride-3 TP layout, causal SDPA, exact GELU, no biases), which is the
   oracle the native path is tested against.
+
+Beyond the reference's model (:class:`AttentionSpec`): rotary positions, a bias linear
+in the distance, capped scores, shared K/V heads, and a
+:class:`~mini_megatron_b200.ops.documents.DocumentPlan` of packed rows passed down with
+the activations.  Plain causal attention over rows of a multiple of 128 tokens runs on the
+causal kernels; everything else on the masked ones.
 """
 from __future__ import annotations
+
+import dataclasses
 
 import torch
 import torch.nn as nn
@@ -24,59 +32,125 @@ from ..parallel import process_groups as pg
 from ..parallel.tensor_parallel import ColumnParallelLinear, RowParallelLinear
 
 
-class Attention(nn.Module):
-    """Causal multi-head self-attention with a fused, TP-sharded QKV projection."""
+@dataclasses.dataclass
+class AttentionSpec:
+    """What an :class:`Attention` does beyond plain causal attention (the defaults are plain)."""
 
-    def __init__(self, hidden_size, num_heads, sequence_parallel=None):
+    num_kv_heads: int | None = None
+    rotary: object = None             # ops.rotary.Rotary
+    alibi: bool = False
+    softcap: float | None = None
+
+
+class Attention(nn.Module):
+    """Multi-head self-attention with a fused, TP-sharded QKV projection, causal unless a plan says otherwise."""
+
+    def __init__(self, hidden_size, num_heads, sequence_parallel=None, spec=None):
         super().__init__()
+        spec = spec or AttentionSpec()
         tp = pg.tp_size()
         if num_heads % tp:
             raise ValueError("num_heads must divide evenly by TP size")
+        kv_heads = num_heads if spec.num_kv_heads is None else spec.num_kv_heads
+        if kv_heads < 1 or num_heads % kv_heads:
+            raise ValueError("num_heads must be a multiple of num_kv_heads")
+        if kv_heads != num_heads and tp > 1:
+            raise ValueError("shared K/V heads need TP size 1: the QKV weight is sharded in equal Q, K and V parts")
         self.num_heads = num_heads // tp
+        self.num_kv_heads = kv_heads // tp
         self.head_dim = hidden_size // num_heads
         self.hidden_size_per_partition = hidden_size // tp
+        self.spec = spec
+        if spec.alibi:
+            from ..ops.attention import alibi_slopes
+            first = pg.tp_rank() * self.num_heads
+            self.register_buffer("alibi_slopes", alibi_slopes(num_heads)[first:first + self.num_heads].clone(),
+                                 persistent=False)
+        else:
+            self.alibi_slopes = None
         # stride 3: each TP rank holds an equal subset of Q, K and V heads
-        self.qkv = ColumnParallelLinear(hidden_size, 3 * hidden_size, bias=False, stride=3,
+        self.qkv = ColumnParallelLinear(hidden_size, (num_heads + 2 * kv_heads) * self.head_dim, bias=False,
+                                        stride=3 if kv_heads == num_heads else 1,
                                         sequence_parallel=sequence_parallel)
         self.o = RowParallelLinear(hidden_size, hidden_size, bias=False, sequence_parallel=sequence_parallel)
 
-    def core_attention(self, qkv):
+    def plain(self, plan):
+        """Whether this is causal attention without anything else."""
+        return (plan is None and self.spec.rotary is None and not self.spec.alibi and self.spec.softcap is None
+                and self.num_kv_heads == self.num_heads)
+
+    def options(self, plan):
+        """Arguments of the masked attention operators."""
+        return dict(num_kv_heads=self.num_kv_heads, plan=plan, softcap=self.spec.softcap,
+                    alibi_slopes=self.alibi_slopes)
+
+    def native_core_fwd(self, qkv, B, S, plan):
+        """(ctx, lse, qkv as the backward needs it) of the [B*S, W] bf16 activation; rotates ``qkv`` in place."""
+        from ..ops import attention as A
+        if self.plain(plan) and S % 128 == 0:
+            return (*A.flash_attn_fwd(qkv, B, S, self.num_heads, self.head_dim), qkv)
+        q3 = qkv.view(B, S, -1)
+        if self.spec.rotary is not None:
+            from ..ops.rotary import rotary_fwd
+            rotary_fwd(q3, self.spec.rotary, self.num_heads + self.num_kv_heads, plan.positions if plan else None,
+                       out=q3)
+        ctx, lse = A.attention_fwd(q3, self.num_heads, self.head_dim, **self.options(plan))
+        return ctx.view(B * S, -1), lse, qkv
+
+    def native_core_bwd(self, dctx, qkv, ctx, lse, B, S, plan):
+        """dqkv [B*S, W] of :meth:`native_core_fwd`."""
+        from ..ops import attention as A
+        if self.plain(plan) and S % 128 == 0:
+            return A.flash_attn_bwd(dctx, qkv, ctx, lse, B, S, self.num_heads, self.head_dim)
+        dqkv = A.attention_bwd(dctx.view(B, S, -1), qkv.view(B, S, -1), ctx.view(B, S, -1), lse, self.num_heads,
+                               self.head_dim, **self.options(plan))
+        if self.spec.rotary is not None:
+            from ..ops.rotary import rotary_bwd
+            rotary_bwd(dqkv, self.spec.rotary, self.num_heads + self.num_kv_heads, plan.positions if plan else None,
+                       out=dqkv)
+        return dqkv.view(B * S, -1)
+
+    def core_attention(self, qkv, plan=None):
         B, S, _ = qkv.shape
+        if not self.plain(plan):
+            from ..ops.attention import attention
+            if self.spec.rotary is not None:
+                from ..ops.rotary import apply_rotary
+                qkv = apply_rotary(qkv, self.spec.rotary, self.num_heads + self.num_kv_heads,
+                                   plan.positions if plan else None)
+            return attention(qkv, self.num_heads, self.head_dim, **self.options(plan))
         qkv = qkv.reshape(B, S, 3, self.num_heads, self.head_dim)
         q, k, v = (t.transpose(1, 2) for t in qkv.unbind(2))
         out = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         return out.transpose(1, 2).reshape(B, S, self.hidden_size_per_partition)
 
-    def forward(self, x):
+    def forward(self, x, plan=None):
         qkv = self.qkv(x)
         if qkv.is_cuda:
-            from ..ops.attention import flash_attn_fwd
-            B, S, _ = qkv.shape
-            ctx = _AttnFn.apply(qkv, self.num_heads, self.head_dim)
-            return self.o(ctx)
-        return self.o(self.core_attention(qkv))
+            return self.o(_AttnFn.apply(qkv, self, plan))
+        return self.o(self.core_attention(qkv, plan))
 
 
 class _AttnFn(torch.autograd.Function):
-    """Native causal attention on a packed [B, S, 3*Hl] qkv tensor (standalone module use)."""
+    """Native attention on a packed [B, S, W] qkv tensor (standalone module use)."""
 
     @staticmethod
-    def forward(ctx, qkv, nh, d):
-        from ..ops.attention import flash_attn_fwd
+    def forward(ctx, qkv, attn, plan):
         B, S, W = qkv.shape
         q2 = qkv.reshape(B * S, W).to(torch.bfloat16).contiguous()
-        out, lse = flash_attn_fwd(q2, B, S, nh, d)
+        if attn.spec.rotary is not None and q2.data_ptr() == qkv.data_ptr():
+            q2 = q2.clone()  # rotated in place below
+        out, lse, q2 = attn.native_core_fwd(q2, B, S, plan)
         ctx.save_for_backward(q2, out, lse)
-        ctx.shape, ctx.nh, ctx.d, ctx.dtype = (B, S, W), nh, d, qkv.dtype
-        return out.view(B, S, nh * d)
+        ctx.shape, ctx.attn, ctx.plan, ctx.dtype = (B, S, W), attn, plan, qkv.dtype
+        return out.view(B, S, -1)
 
     @staticmethod
     def backward(ctx, dout):
-        from ..ops.attention import flash_attn_bwd
         q2, out, lse = ctx.saved_tensors
         B, S, W = ctx.shape
         d2 = dout.reshape(B * S, -1).to(torch.bfloat16).contiguous()
-        dqkv = flash_attn_bwd(d2, q2, out, lse, B, S, ctx.nh, ctx.d)
+        dqkv = ctx.attn.native_core_bwd(d2, q2, out, lse, B, S, ctx.plan)
         return dqkv.view(B, S, W).to(ctx.dtype), None, None
 
 
@@ -93,10 +167,10 @@ class MLP(nn.Module):
 class DecoderLayer(nn.Module):
     """Pre-LN block: x + attn(ln1(x)), then + mlp(ln2(.))."""
 
-    def __init__(self, hidden_size, num_heads, ffn_hidden_size, sequence_parallel=None, recompute=False):
+    def __init__(self, hidden_size, num_heads, ffn_hidden_size, sequence_parallel=None, recompute=False, spec=None):
         super().__init__()
         self.ln1 = nn.LayerNorm(hidden_size)
-        self.attn = Attention(hidden_size, num_heads, sequence_parallel)
+        self.attn = Attention(hidden_size, num_heads, sequence_parallel, spec)
         self.ln2 = nn.LayerNorm(hidden_size)
         self.mlp = MLP(hidden_size, ffn_hidden_size, sequence_parallel)
         self.sequence_parallel = pg.sequence_parallel_enabled() if sequence_parallel is None else sequence_parallel
@@ -106,41 +180,41 @@ class DecoderLayer(nn.Module):
         for p in list(self.ln1.parameters()) + list(self.ln2.parameters()):
             p.sequence_parallel_grad = bool(self.sequence_parallel)
 
-    def _forward(self, x):
-        x = x + self.attn(self.ln1(x))
+    def _forward(self, x, plan=None):
+        x = x + self.attn(self.ln1(x), plan)
         x = x + self.mlp(self.ln2(x))
         return x
 
-    def native_forward(self, x, recompute=None):
+    def native_forward(self, x, recompute=None, plan=None):
         from .native_layers import DecoderLayerFn
         group = pg.tp_group()
         sp = bool(self.sequence_parallel and group is not None)
         rc = self.recompute if recompute is None else recompute
-        return DecoderLayerFn.apply(x.float().contiguous(), self, group, sp, rc, *self.parameters())
+        return DecoderLayerFn.apply(x.float().contiguous(), self, group, sp, rc, plan, *self.parameters())
 
-    def forward(self, x, use_checkpoint=False):
+    def forward(self, x, use_checkpoint=False, plan=None):
         if x.is_cuda:
-            return self.native_forward(x, recompute=use_checkpoint or self.recompute)
+            return self.native_forward(x, recompute=use_checkpoint or self.recompute, plan=plan)
         if use_checkpoint or self.recompute:
-            return torch.utils.checkpoint.checkpoint(self._forward, x, use_reentrant=False)
-        return self._forward(x)
+            return torch.utils.checkpoint.checkpoint(self._forward, x, plan, use_reentrant=False)
+        return self._forward(x, plan)
 
 
 class Decoder(nn.Module):
     """Stack of DecoderLayer blocks (``layer_ids`` is metadata for pipeline stages)."""
 
     def __init__(self, hidden_size, num_heads, ffn_hidden_size, num_layers, layer_ids=None, sequence_parallel=None,
-                 recompute=False):
+                 recompute=False, spec=None):
         super().__init__()
         self.layer_ids = list(range(num_layers)) if layer_ids is None else list(layer_ids)
         self.layers = nn.ModuleList([
-            DecoderLayer(hidden_size, num_heads, ffn_hidden_size, sequence_parallel, recompute)
+            DecoderLayer(hidden_size, num_heads, ffn_hidden_size, sequence_parallel, recompute, spec)
             for _ in self.layer_ids
         ])
 
-    def forward(self, x):
+    def forward(self, x, plan=None):
         for layer in self.layers:
-            x = layer(x)
+            x = layer(x, plan=plan)
         return x
 
 
@@ -154,19 +228,27 @@ class GPT(nn.Module):
     with the package's CrossEntropyLoss the head runs fused
     (``native_layers.HeadLossFn``) and the returned logits buffer is
     overwritten by its gradient during backward.
+
+    With ``eod_token`` rows are packed documents: attention stays inside a document
+    and rotary positions restart with it.  ``forward(..., plan=...)`` takes another
+    :class:`~mini_megatron_b200.ops.documents.DocumentPlan` instead (prefixes, padding).
     """
 
-    def __init__(self, embedding, decoder, ln_f, lm_head, loss_fn=None):
+    def __init__(self, embedding, decoder, ln_f, lm_head, loss_fn=None, eod_token=None):
         super().__init__()
         self.embedding = embedding
         self.decoder = decoder
         self.ln_f = ln_f
         self.lm_head = lm_head
         self.loss_fn = loss_fn
+        self.eod_token = eod_token
 
-    def forward(self, input_ids, labels=None, loss_mask=None):
+    def forward(self, input_ids, labels=None, loss_mask=None, plan=None):
+        if plan is None and self.eod_token is not None:
+            from ..ops.documents import document_plan
+            plan = document_plan(input_ids, eod=self.eod_token)
         x = self.embedding(input_ids)
-        x = self.decoder(x)
+        x = self.decoder(x, plan=plan)
         return head_forward(self.ln_f, self.lm_head, self.loss_fn, x, labels, loss_mask)
 
 

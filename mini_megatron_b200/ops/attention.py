@@ -38,6 +38,11 @@ def flash_attn_bwd(dctx, qkv, ctx, lse, B, S, nh, d):
 # Rows that see nothing give ctx = 0, lse = -inf and no gradients.
 
 
+def alibi_slopes(num_heads):
+    """``[num_heads]`` fp32: ``2 ** (-8 (h + 1) / num_heads)``, the geometric slopes of linear distance biases."""
+    return torch.tensor([2.0 ** (-8.0 * (h + 1) / num_heads) for h in range(num_heads)], dtype=torch.float32)
+
+
 def _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale):
     if qkv.dim() != 3:
         raise ValueError(f"attention needs qkv [B, S, (num_heads + 2 num_kv_heads) * head_dim], got {tuple(qkv.shape)}")

@@ -117,10 +117,14 @@ class Trainer:
         if not dist.is_initialized():
             raise RuntimeError("torch.distributed must be initialised (world size 1 is fine)")
         seq_len = cfg.seq_len or cfg.model.max_seq_len
+        # the fused embedding adds the learned position table: models without one take the NCCL path
         fused_tp = (self.device.type == "cuda" and cfg.tp > 1 and cfg.tp_impl in ("auto", "fused")
-                    and seq_len % cfg.tp == 0 and (seq_len // cfg.tp) % 128 == 0)
+                    and seq_len % cfg.tp == 0 and (seq_len // cfg.tp) % 128 == 0
+                    and cfg.model.position_embedding == "learned")
         if cfg.tp_impl == "fused" and not fused_tp and cfg.tp > 1:
-            raise ValueError("fused TP needs CUDA and seq_len / tp divisible by 128")
+            raise ValueError("fused TP needs CUDA, seq_len / tp divisible by 128 and learned positions")
+        if cfg.pp > 1 and cfg.model.eod_token is not None:
+            raise ValueError("eod_token (packed documents) needs pp = 1")
         self.tp_impl = "fused" if fused_tp else "nccl"
         self.mpu = mpu or pg.init_model_parallel(cfg.tp, cfg.pp, cfg.sequence_parallel or fused_tp)
         pg.set_model_parallel(self.mpu)

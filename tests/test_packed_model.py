@@ -1,0 +1,211 @@
+"""Plan, rotary positions and masked attention together: as a chain, and inside the GPT and its trainer."""
+import copy
+import os
+
+import pytest
+import torch
+import torch.distributed as dist
+
+from packed_ref import attention_ref, plan_ref, rotary_ref, row_tensors, split_rows
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _pg():
+    if not dist.is_initialized():
+        os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
+        os.environ.setdefault("MASTER_PORT", "29567")
+        dist.init_process_group("gloo", rank=0, world_size=1)
+    yield
+
+
+def _rel(a, b):
+    return ((a.double() - b.double()).norm() / (b.double().norm() + 1e-12)).item()
+
+
+def _cfg(**kw):
+    from mini_megatron_b200.config import GPTConfig
+    base = dict(num_layers=2, hidden_size=256, num_attention_heads=4, ffn_hidden_size=512, max_seq_len=256,
+                vocab_size=500)
+    return GPTConfig(**{**base, **kw})
+
+
+VARIANTS = {
+    "rotary_documents": (dict(position_embedding="rotary", eod_token=3), 200),
+    "rotary_part_interleaved_shared_heads": (dict(position_embedding="rotary", rotary_percent=0.5,
+                                                  rotary_interleaved=True, rotary_scaling="yarn", rotary_factor=4.0,
+                                                  rotary_original_max_positions=64, num_kv_heads=2), 129),
+    "distance_bias_capped": (dict(position_embedding="alibi", attn_softcap=20.0, eod_token=3), 256),
+    "learned_capped_head128": (dict(attn_softcap=30.0, hidden_size=256, num_attention_heads=2, num_kv_heads=1), 77),
+    "plain_odd_length": (dict(), 100),
+}
+
+
+def _build(cfg, seed=0):
+    from mini_megatron_b200.models import build_gpt
+    torch.manual_seed(seed)
+    return build_gpt(cfg)
+
+
+def _batch(cfg, B, S, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    toks = torch.randint(0, cfg.vocab_size, (B, S + 1), generator=g)
+    toks[torch.rand(B, S + 1, generator=g) < 0.03] = 3
+    return toks[:, :-1].contiguous(), toks[:, 1:].contiguous(), torch.ones(B, S)
+
+
+def test_packed_documents_equal_separate_documents():
+    """A row of documents gives each of them the logits it has alone (CPU path)."""
+    for pos in ("rotary", "alibi"):
+        model = _build(_cfg(position_embedding=pos, eod_token=3, num_kv_heads=2)).double()
+        g = torch.Generator().manual_seed(5)
+        docs = [torch.cat([torch.randint(4, 500, (n - 1,), generator=g), torch.tensor([3])]) for n in (9, 1, 30, 14)]
+        logits = model(torch.cat(docs)[None])[0]
+        at = 0
+        for doc in docs:
+            torch.testing.assert_close(logits[at:at + len(doc)], model(doc[None])[0], rtol=1e-9, atol=1e-9)
+            at += len(doc)
+
+
+def test_prefix_plan_reaches_the_layers():
+    """With a prefix both ways the first token sees the second; padding changes nothing else (CPU path)."""
+    from mini_megatron_b200.ops.documents import document_plan
+    model = _build(_cfg(position_embedding="rotary")).double()
+    ids = torch.randint(4, 500, (1, 12), generator=torch.Generator().manual_seed(0))
+    marks = torch.arange(12)[None] < 5
+    plan = document_plan(ids, eod=3, prefix_mask=marks, lengths=torch.tensor([9]))
+    base = model(ids, plan=plan)[0]
+    other = ids.clone()
+    other[0, 4] = 77
+    assert not torch.allclose(model(other, plan=plan)[0, 0], base[0])
+    other = ids.clone()
+    other[0, 7] = 77
+    changed = model(other, plan=plan)[0]
+    torch.testing.assert_close(changed[:7], base[:7], rtol=0, atol=0)
+    other = ids.clone()
+    other[0, 10] = 77
+    torch.testing.assert_close(model(other, plan=plan)[0][:9], base[:9], rtol=0, atol=0)
+
+
+def test_model_refusals():
+    from mini_megatron_b200.models import GPTStage
+    from mini_megatron_b200.training import TrainConfig, Trainer
+    for kw in [dict(position_embedding="other"), dict(num_kv_heads=3), dict(num_kv_heads=0), dict(attn_softcap=0.0),
+               dict(position_embedding="rotary", rotary_percent=0.01), dict(position_embedding="rotary",
+                                                                           rotary_scaling="yarn", rotary_factor=2.0)]:
+        with pytest.raises(ValueError):
+            _build(_cfg(**kw))
+    with pytest.raises(ValueError):
+        GPTStage(_cfg(eod_token=3), 0, 2)
+    with pytest.raises(ValueError):
+        Trainer(TrainConfig(model=_cfg(eod_token=3), pp=2), device="cpu", mpu=None)
+
+
+def test_command_line_reaches_the_config():
+    import main
+    args = main.parse_args("--position-embedding rotary --rotary-percent 0.5 --rotary-interleaved --rotary-scaling ntk "
+                           "--rotary-factor 2 --num-kv-heads 4 --attn-softcap 30 --eod-token 0".split())
+    cfg = main.model_config(args)
+    assert (cfg.position_embedding, cfg.rotary_percent, cfg.rotary_interleaved, cfg.rotary_scaling, cfg.rotary_factor,
+            cfg.num_kv_heads, cfg.attn_softcap, cfg.eod_token) == ("rotary", 0.5, True, "ntk", 2.0, 4, 30.0, 0)
+    assert main.model_config(main.parse_args([])) == main.model_config(main.parse_args(["--seq-len", "16"]))
+
+
+@pytest.mark.parametrize("name", sorted(VARIANTS))
+def test_parameter_count(name):
+    cfg = _cfg(**VARIANTS[name][0])
+    model = _build(cfg)
+    assert sum(p.numel() for p in model.parameters()) == cfg.num_params(padded_vocab=512)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,nh,nkv", [(64, 4, 2), (128, 2, 2)])
+def test_chain_against_64_bits(d, nh, nkv):
+    """plan -> rotary -> attention and back, each step against the 64-bit form of that step on the same inputs."""
+    from mini_megatron_b200.ops import check_errors
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    from mini_megatron_b200.ops.documents import document_plan
+    from mini_megatron_b200.ops.rotary import Rotary, rotary_bwd, rotary_fwd
+    B, S = 3, 411
+    rows = split_rows(B, S, 120, True, True, seed=9)
+    tokens, _, marks, lengths = row_tensors(rows, S, seed=9)
+    plan = document_plan(tokens.cuda(), eod=0, prefix_mask=marks.cuda(), lengths=lengths.cuda())
+    pos, start, end = (t.cuda() for t in plan_ref(rows, S, True))
+    assert torch.equal(plan.positions, pos) and torch.equal(plan.start, start) and torch.equal(plan.end, end)
+    r = Rotary(d, rotary_dim=d // 2, scaling="linear", factor=2.0, device="cuda")
+    qkv = torch.randn(B, S, (nh + 2 * nkv) * d, device="cuda").bfloat16()
+    dctx = torch.randn(B, S, nh * d, device="cuda").bfloat16()
+    want = rotary_ref(qkv, d, d // 2, nh + nkv, False, r.radians, 1.0, pos)
+    rotary_fwd(qkv, r, nh + nkv, plan.positions, out=qkv)
+    # a bf16 rounding (2^-8) of values that a 32-bit rotation leaves within 2^-20 of their pair
+    assert ((qkv.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * want.abs().max()).all()
+    opts = dict(num_kv_heads=nkv, plan=plan, softcap=40.0)
+    ctx, lse = attention_fwd(qkv, nh, d, **opts)
+    dqkv = attention_bwd(dctx, qkv, ctx, lse, nh, d, **opts)
+    (r_ctx, _, r_grad), (b_ctx, _, b_grad) = attention_ref(qkv, dctx, nh, nkv, d, start, end, 40.0)
+    assert ((ctx.double() - r_ctx).abs() <= b_ctx).all() and ((dqkv.double() - r_grad).abs() <= b_grad).all()
+    want = rotary_ref(dqkv, d, d // 2, nh + nkv, False, r.radians, 1.0, pos, inverse=True)
+    rotary_bwd(dqkv, r, nh + nkv, plan.positions, out=dqkv)
+    assert ((dqkv.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * want.abs().max()).all()
+    check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", sorted(VARIANTS))
+def test_native_model_matches_cpu(name):
+    """Loss and gradients of the native model against the fp32 CPU path on the same weights.
+
+    The gates are those of the plain model's parity test: bf16 operands in every product (2^-8 each) through two layers.
+    """
+    from mini_megatron_b200.ops import check_errors
+    from mini_megatron_b200.optim import make_param_buffer
+    kw, S = VARIANTS[name]
+    cfg = _cfg(**kw)
+    cpu = _build(cfg)
+    gpu = copy.deepcopy(cpu).cuda()
+    ids, labels, mask = _batch(cfg, 2, S)
+    _, want = cpu(ids, labels, mask)
+    want.backward()
+    make_param_buffer(gpu)
+    _, loss = gpu(ids.cuda(), labels.cuda(), mask.cuda())
+    loss.backward()
+    torch.cuda.synchronize()
+    check_errors()
+    assert abs(loss.item() - want.item()) < 2e-2 * abs(want.item())
+    for (n, a), (_, b) in zip(cpu.named_parameters(), gpu.named_parameters()):
+        assert _rel(b.main_grad.cpu(), a.grad) < 5e-2, n
+
+
+@pytest.mark.gpu
+def test_standalone_attention_module():
+    from mini_megatron_b200.models import Attention, AttentionSpec
+    from mini_megatron_b200.ops.rotary import Rotary
+    torch.manual_seed(0)
+    cpu = Attention(256, 4, spec=AttentionSpec(num_kv_heads=2, rotary=Rotary(64), softcap=20.0))
+    gpu = copy.deepcopy(cpu).cuda()
+    x = torch.randn(2, 90, 256)
+    a, b = x.clone().requires_grad_(True), x.cuda().requires_grad_(True)
+    ya, yb = cpu(a), gpu(b)
+    dy = torch.randn_like(ya)
+    (ga,) = torch.autograd.grad(ya, a, dy)
+    (gb,) = torch.autograd.grad(yb, b, dy.cuda().to(yb.dtype))
+    assert _rel(yb.cpu().detach(), ya.detach()) < 2e-2 and _rel(gb.cpu(), ga) < 5e-2
+
+
+@pytest.mark.gpu
+def test_trainer_graph_recompute_and_eager_agree():
+    """A packed, rotary, capped model: the captured step rebuilds its plan from every batch's tokens."""
+    from mini_megatron_b200.parallel import process_groups as pg
+    from mini_megatron_b200.training import TrainConfig, Trainer, synthetic_batch
+    mc = _cfg(position_embedding="rotary", attn_softcap=30.0, eod_token=7, vocab_size=64, num_kv_heads=2)
+    runs = {}
+    for mode, rc in (("off", False), ("on", False), ("off", True)):
+        t = Trainer(TrainConfig(model=mc, micro_batch_size=2, seq_len=150, num_microbatches=2, lr=1e-3, warmup_steps=2,
+                                num_steps=20, cuda_graph=mode, recompute=rc))
+        losses = [t.train_step(*synthetic_batch(2, 2, 150, 64, seed=s, pin=True)).item() for s in range(5)]
+        t.check_device_errors()
+        runs[mode, rc] = losses
+        t.destroy()
+        pg.set_model_parallel(None)
+    for other in (("on", False), ("off", True)):
+        for a, b in zip(runs["off", False], runs[other]):
+            assert abs(a - b) < 2e-3 * abs(a), runs
