@@ -65,6 +65,35 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+
 // Constants of the score transform.
 struct Score {
   float mul;  // plain: s log2 e;  capped: 2 s log2 e / cap (the exponent of e^{2u} in log2 units)
@@ -87,6 +116,17 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+
+// One thread of the (converged) warp.  tcgen05.mma and TMA take their descriptors from uniform registers:
+// behind elect.sync the compiler knows that a single thread is left and moves them there directly, behind a
+// test of the lane index it has to assume several threads with different values and issues each instruction
+// from a loop (measured in the forward kernel: 8 products took 1100 cycles to issue).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 // Bounded wait on an mbarrier phase.  The clock is read only after many polls: a read of the
@@ -167,21 +207,26 @@ __device__ __forceinline__ void mma_abt(uint32_t dst, uint32_t a_addr, uint32_t 
 }
 
 // 128 x D (+)= A [128 x 128, bf16 in TMEM] B [128 x D] (rows are the reduction: MN-major).  A's 128
-// columns lie in two runs of 64 (32 TMEM columns each) that start `hi` columns apart.
-template <int D>
-__device__ __forceinline__ void mma_tmem_b(uint32_t dst, uint32_t a_tmem, uint32_t hi, uint32_t b_addr, bool acc) {
+// columns lie in runs of RUN (RUN / 2 TMEM columns) that start 32 TMEM columns apart.
+template <int D, int RUN>
+__device__ __forceinline__ void mma_tmem_b(uint32_t dst, uint32_t a_tmem, uint32_t b_addr, bool acc) {
+  constexpr int PER = RUN / 16;
   constexpr uint32_t idesc = make_idesc_bf16(BT, D, false, true);
   const uint64_t bd = make_sdesc_sw128(b_addr, 16384, 1024);
 #pragma unroll
   for (int k = 0; k < BT / 16; ++k)
-    umma_bf16_ts(dst, a_tmem + (k >> 2) * hi + (k & 3) * 8, bd + (uint64_t)(k * (2048 >> 4)), idesc,
+    umma_bf16_ts(dst, a_tmem + (k / PER) * 32 + (k % PER) * 8, bd + (uint64_t)(k * (2048 >> 4)), idesc,
                  (acc || k != 0) ? 1u : 0u);
 }
 
-// Stores 32 fp32 accumulator values as bf16 (64 bytes of one row).
-__device__ __forceinline__ void store_row32(__nv_bfloat16* p, const uint32_t (&v)[32], float mul) {
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
+
+// Stores N fp32 accumulator values as bf16 (2 N bytes of one row).
+template <int N>
+__device__ __forceinline__ void store_row(__nv_bfloat16* p, const uint32_t (&v)[N], float mul) {
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
+  for (int u = 0; u < N / 8; ++u) {
     uint4 w;
     w.x = pack_bf16x2(__uint_as_float(v[8 * u + 0]) * mul, __uint_as_float(v[8 * u + 1]) * mul);
     w.y = pack_bf16x2(__uint_as_float(v[8 * u + 2]) * mul, __uint_as_float(v[8 * u + 3]) * mul);
@@ -190,9 +235,10 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16* p, const uint32_t (&v
     reinterpret_cast<uint4*>(p)[u] = w;
   }
 }
-__device__ __forceinline__ void store_zero32(__nv_bfloat16* p) {
+template <int N>
+__device__ __forceinline__ void store_zero(__nv_bfloat16* p) {
 #pragma unroll
-  for (int u = 0; u < 4; ++u) reinterpret_cast<uint4*>(p)[u] = make_uint4(0u, 0u, 0u, 0u);
+  for (int u = 0; u < N / 8; ++u) reinterpret_cast<uint4*>(p)[u] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 }  // namespace mattn

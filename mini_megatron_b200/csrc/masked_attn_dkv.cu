@@ -10,11 +10,12 @@
 // tile).  Scores are computed transposed (a thread owns a key row), so P^T and dS^T
 // go back into TMEM as the first operands of the two sums and never touch shared
 // memory; LSE, Delta and the visible intervals of the query rows arrive with the
-// Q / dO tiles by bulk copies from tile-padded arrays.  Roles (10 warps):
+// Q / dO tiles by bulk copies from tile-padded arrays.  Roles (20 warps, two of them idle):
 //
 //   warp 0     TMA: K_j, V_j per item; Q_i, dO_i and their row data into a ring
 //   warp 1     TMEM allocation; one thread issues S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
-//   warps 2-9  softmax gradient: warps w and w + 4 share 32 key rows and split the 128 queries
+//   warps 4-19 softmax gradient: four warps share 32 key rows, each has 32 of the 128 queries
+//              (masked_attn_dq.cu says why four: DKVTWO against DKVFOUR cycles a tile at d = 64)
 //
 // d = 64: S^T has two TMEM buffers, the next tile's scores are computed while this tile's
 // softmax runs.  d = 128: S^T, dP^T, dV and dK fill TMEM; the next S^T follows dV and the next
@@ -25,7 +26,8 @@ namespace mmb {
 namespace mattn {
 namespace dkv {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 640;
+constexpr int kWarps = 16;  // of the softmax gradient
 
 template <int D>
 struct Cfg {
@@ -122,12 +124,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_empty = bars + 7;    // [3]
   uint64_t* s_full = bars + 10;    // [2]
   uint64_t* dp_full = bars + 12;
-  uint64_t* p_full = bars + 13;    // P^T written, S^T read (8 warps)
-  uint64_t* ds_full = bars + 14;   // dS^T written, dP^T and the row data read (8 warps)
+  // P^T written, S^T read (16 warps).  Two barriers: a warp may be done with P^T(n+1) before another one is
+  // with P^T(n), and its second arrival must not complete the first one's phase.
+  uint64_t* p_full = bars + 18;    // [2]
+  uint64_t* ds_full = bars + 14;   // dS^T written, dP^T and the row data read (16 warps)
   uint64_t* g_full = bars + 15;    // dK, dV of an item complete
-  uint64_t* g_free = bars + 16;    // ... read (8 warps)
+  uint64_t* g_free = bars + 16;    // ... read (16 warps)
   uint64_t* drain = bars + 17;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -139,16 +143,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
       mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kWarps);
     }
     for (int i = 0; i < 3; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
     }
     mbar_init(dp_full, 1);
-    mbar_init(p_full, 8);
-    mbar_init(ds_full, 8);
+    mbar_init(ds_full, kWarps);
     mbar_init(g_full, 1);
-    mbar_init(g_free, 8);
+    mbar_init(g_free, kWarps);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -165,99 +169,103 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      // ---------------------------------------------------------------- TMA
-      int n = 0, kv_issued = -1;
-      bool ok = true;
-      Walk x;
-      for (x.next(a, n_items, group); x.valid; x.next(a, n_items, group), ++n) {
-        if (x.first()) {
+  if (warp < 4) {
+    reg_dec<64>();
+    if (warp == 0) {
+      if (elect_one()) {
+        // ---------------------------------------------------------------- TMA
+        int n = 0, kv_issued = -1;
+        bool ok = true;
+        Walk x;
+        for (x.next(a, n_items, group); x.valid; x.next(a, n_items, group), ++n) {
+          if (x.first()) {
+            const int kb = x.it % KB;
+            if (x.it >= KB && !bwait(&kv_empty[kb], ((x.it / KB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+            mbar_expect_tx(&kv_full[kb], 2 * C::TILE);
+            load_tile<D>(sKV + kb * 2 * C::TILE, &tm_qkv, &kv_full[kb], (a.nh + x.w.hk) * D, x.w.t * BT, x.w.b);
+            load_tile<D>(sKV + kb * 2 * C::TILE + C::TILE, &tm_qkv, &kv_full[kb], (a.nh + a.nkv + x.w.hk) * D,
+                         x.w.t * BT, x.w.b);
+            kv_issued = x.it;
+          }
+          const int st = n % NQ;
+          if (n >= NQ && !bwait(&q_empty[st], ((n / NQ) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          const int h = x.w.hk * group + x.g;
+          mbar_expect_tx(&q_full[st], 2 * C::TILE + 1024 + (a.mask.rows ? 1024 : 0));
+          load_tile<D>(sQ + st * 2 * C::TILE, &tm_qkv, &q_full[st], h * D, x.i * BT, x.w.b);
+          load_tile<D>(sQ + st * 2 * C::TILE + C::TILE, &tm_do, &q_full[st], h * D, x.i * BT, x.w.b);
+          bulk_load(sLD + st * 2048, a.ld + (((size_t)x.w.b * a.nh + h) * a.n_t + x.i) * (2 * BT), 1024, &q_full[st]);
+          if (a.mask.rows)
+            bulk_load(sLD + st * 2048 + 1024, a.mask.rows + ((size_t)x.w.b * a.n_t + x.i) * (2 * BT), 1024,
+                      &q_full[st]);
+        }
+        if (!ok) {
+          for (int u = max(0, kv_issued - KB + 1); u <= kv_issued; ++u) drain_wait(&kv_full[u % KB], (u / KB) & 1);
+          for (int u = max(0, n - NQ); u < n; ++u) drain_wait(&q_full[u % NQ], (u / NQ) & 1);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (elect_one()) {
+        // ---------------------------------------------------------------- MMA
+        bool ok = true;
+        int n = 0;
+        Walk cur, nxt;
+        auto issue_s = [&](const Walk& x, int u) -> bool {
           const int kb = x.it % KB;
-          if (x.it >= KB && !bwait(&kv_empty[kb], ((x.it / KB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-          mbar_expect_tx(&kv_full[kb], 2 * C::TILE);
-          load_tile<D>(sKV + kb * 2 * C::TILE, &tm_qkv, &kv_full[kb], (a.nh + x.w.hk) * D, x.w.t * BT, x.w.b);
-          load_tile<D>(sKV + kb * 2 * C::TILE + C::TILE, &tm_qkv, &kv_full[kb], (a.nh + a.nkv + x.w.hk) * D,
-                       x.w.t * BT, x.w.b);
-          kv_issued = x.it;
-        }
-        const int st = n % NQ;
-        if (n >= NQ && !bwait(&q_empty[st], ((n / NQ) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-        const int h = x.w.hk * group + x.g;
-        mbar_expect_tx(&q_full[st], 2 * C::TILE + 1024 + (a.mask.rows ? 1024 : 0));
-        load_tile<D>(sQ + st * 2 * C::TILE, &tm_qkv, &q_full[st], h * D, x.i * BT, x.w.b);
-        load_tile<D>(sQ + st * 2 * C::TILE + C::TILE, &tm_do, &q_full[st], h * D, x.i * BT, x.w.b);
-        bulk_load(sLD + st * 2048, a.ld + (((size_t)x.w.b * a.nh + h) * a.n_t + x.i) * (2 * BT), 1024, &q_full[st]);
-        if (a.mask.rows)
-          bulk_load(sLD + st * 2048 + 1024, a.mask.rows + ((size_t)x.w.b * a.n_t + x.i) * (2 * BT), 1024,
-                    &q_full[st]);
-      }
-      if (!ok) {
-        for (int u = max(0, kv_issued - KB + 1); u <= kv_issued; ++u) drain_wait(&kv_full[u % KB], (u / KB) & 1);
-        for (int u = max(0, n - NQ); u < n; ++u) drain_wait(&q_full[u % NQ], (u / NQ) & 1);
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0) {
-      // ---------------------------------------------------------------- MMA
-      bool ok = true;
-      int n = 0;
-      Walk cur, nxt;
-      auto issue_s = [&](const Walk& x, int u) -> bool {
-        const int kb = x.it % KB;
-        if (x.first() && !bwait(&kv_full[kb], (x.it / KB) & 1, a.err, abort_flag)) return false;
-        if (!bwait(&q_full[u % NQ], (u / NQ) & 1, a.err, abort_flag)) return false;
-        tc_fence_after();
-        mma_abt<D>(tmem + C::T_S + (u % SB) * 128, smem_u32(sKV + kb * 2 * C::TILE),
-                   smem_u32(sQ + (u % NQ) * 2 * C::TILE));
-        umma_commit(&s_full[u % SB]);
-        return true;
-      };
-      auto issue_dp = [&](const Walk& x, int u) {
-        const int kb = x.it % KB;
-        mma_abt<D>(tmem + C::T_DP, smem_u32(sKV + kb * 2 * C::TILE + C::TILE),
-                   smem_u32(sQ + (u % NQ) * 2 * C::TILE + C::TILE));
-        umma_commit(dp_full);
-      };
-      nxt.next(a, n_items, group);
-      if (nxt.valid) {
-        ok = issue_s(nxt, 0);
-        if (ok) issue_dp(nxt, 0);
-      }
-      while (ok && nxt.valid) {
-        cur = nxt;
+          if (x.first() && !bwait(&kv_full[kb], (x.it / KB) & 1, a.err, abort_flag)) return false;
+          if (!bwait(&q_full[u % NQ], (u / NQ) & 1, a.err, abort_flag)) return false;
+          tc_fence_after();
+          mma_abt<D>(tmem + C::T_S + (u % SB) * 128, smem_u32(sKV + kb * 2 * C::TILE),
+                     smem_u32(sQ + (u % NQ) * 2 * C::TILE));
+          umma_commit(&s_full[u % SB]);
+          return true;
+        };
+        auto issue_dp = [&](const Walk& x, int u) {
+          const int kb = x.it % KB;
+          mma_abt<D>(tmem + C::T_DP, smem_u32(sKV + kb * 2 * C::TILE + C::TILE),
+                     smem_u32(sQ + (u % NQ) * 2 * C::TILE + C::TILE));
+          umma_commit(dp_full);
+        };
         nxt.next(a, n_items, group);
-        // one K / V buffer: the next item's tiles can only be loaded once this item's products are done
-        const bool early = nxt.valid && (KB == 2 || nxt.it == cur.it);
-        const uint32_t q_addr = smem_u32(sQ + (n % NQ) * 2 * C::TILE);
-        if (SB == 2 && early && !issue_s(nxt, n + 1)) { ok = false; break; }
-        if (!bwait(p_full, n & 1, a.err, abort_flag)) { ok = false; break; }
-        if (cur.first() && cur.it > 0 && !bwait(g_free, (cur.it - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-        tc_fence_after();
-        mma_tmem_b<D>(tmem + C::T_DV, tmem + C::T_S + (n % SB) * 128, 64, q_addr + C::TILE, !cur.first());
-        if (SB == 1 && early && !issue_s(nxt, n + 1)) { ok = false; break; }  // over P^T, in issue order after dV
-        if (!bwait(ds_full, n & 1, a.err, abort_flag)) { ok = false; break; }
-        tc_fence_after();
-        mma_tmem_b<D>(tmem + C::T_DK, tmem + C::T_DP, 64, q_addr, !cur.first());
-        umma_commit(&q_empty[n % NQ]);
-        if (cur.last(group)) {
-          umma_commit(g_full);
-          umma_commit(&kv_empty[cur.it % KB]);
+        if (nxt.valid) {
+          ok = issue_s(nxt, 0);
+          if (ok) issue_dp(nxt, 0);
         }
-        if (nxt.valid && !early && !issue_s(nxt, n + 1)) { ok = false; break; }
-        if (nxt.valid) issue_dp(nxt, n + 1);  // over dS^T, in issue order after dK
-        ++n;
+        while (ok && nxt.valid) {
+          cur = nxt;
+          nxt.next(a, n_items, group);
+          // one K / V buffer: the next item's tiles can only be loaded once this item's products are done
+          const bool early = nxt.valid && (KB == 2 || nxt.it == cur.it);
+          const uint32_t q_addr = smem_u32(sQ + (n % NQ) * 2 * C::TILE);
+          if (SB == 2 && early && !issue_s(nxt, n + 1)) { ok = false; break; }
+          if (!bwait(&p_full[n & 1], (n >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          if (cur.first() && cur.it > 0 && !bwait(g_free, (cur.it - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          mma_tmem_b<D, 32>(tmem + C::T_DV, tmem + C::T_S + (n % SB) * 128, q_addr + C::TILE, !cur.first());
+          if (SB == 1 && early && !issue_s(nxt, n + 1)) { ok = false; break; }  // over P^T, in issue order after dV
+          if (!bwait(ds_full, n & 1, a.err, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          mma_tmem_b<D, 32>(tmem + C::T_DK, tmem + C::T_DP, q_addr, !cur.first());
+          umma_commit(&q_empty[n % NQ]);
+          if (cur.last(group)) {
+            umma_commit(g_full);
+            umma_commit(&kv_empty[cur.it % KB]);
+          }
+          if (nxt.valid && !early && !issue_s(nxt, n + 1)) { ok = false; break; }
+          if (nxt.valid) issue_dp(nxt, n + 1);  // over dS^T, in issue order after dK
+          ++n;
+        }
+        if (!ok) {
+          umma_commit(drain);
+          drain_wait(drain, 0);
+        }
       }
-      if (!ok) {
-        umma_commit(drain);
-        drain_wait(drain, 0);
-      }
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------------ softmax gradient, dK / dV store
-    const int half = (warp - 2) >> 2;
+    reg_inc<104>();
+    const int part = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;  // key row within the tile (TMEM lane)
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const Score k = a.score;
@@ -268,15 +276,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int key = w.t * BT + row;
       const bool in = key < a.S;
       const size_t width = (size_t)(a.nh + 2 * a.nkv) * D;
-      __nv_bfloat16* dk = a.dqkv + ((size_t)w.b * a.S + key) * width + (size_t)(a.nh + w.hk) * D + half * (D / 2);
+      __nv_bfloat16* dk = a.dqkv + ((size_t)w.b * a.S + key) * width + (size_t)(a.nh + w.hk) * D + part * (D / 4);
       __nv_bfloat16* dv = dk + (size_t)a.nkv * D;
       if (w.r.x >= w.r.y) {
         if (in) {
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            store_zero32(dk + c * 32);
-            store_zero32(dv + c * 32);
-          }
+          store_zero<D / 4>(dk);
+          store_zero<D / 4>(dv);
         }
         continue;
       }
@@ -287,28 +292,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int st = n % NQ;
           const int2 full = full_tiles(a.mask, w.b, a.n_t, i);
           const bool masked = w.t < full.x || w.t >= full.y;
-          const uint32_t t_s = tmem + C::T_S + (n % SB) * 128 + lane_off + half * 64;
-          const uint32_t t_dp = tmem + C::T_DP + lane_off + half * 64;
-          const float* l2 = reinterpret_cast<const float*>(sLD + st * 2048) + half * 64;
+          const uint32_t t_s = tmem + C::T_S + (n % SB) * 128 + lane_off + part * 32;
+          const uint32_t t_dp = tmem + C::T_DP + lane_off + part * 32;
+          const float* l2 = reinterpret_cast<const float*>(sLD + st * 2048) + part * 32;
           const int* start = reinterpret_cast<const int*>(l2 + 2 * BT);
           if (!wwait(&q_full[st], (n / NQ) & 1, a.err, abort_flag)) { ok = false; break; }
           if (!wwait(&s_full[n % SB], (n / SB) & 1, a.err, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          float pf[64];  // P (1 - tanh^2)
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
+          float pf[32];  // P (1 - tanh^2)
+          {
             uint32_t s[32];
-            tmem_ld_32x32b_x32(t_s + hh * 32, s);
+            tmem_ld(t_s, s);
             tmem_wait_ld();
-            const int q0 = i * BT + half * 64 + hh * 32;  // query of column 0
+            const int q0 = i * BT + part * 32;  // query of column 0
             uint32_t seen = 0xffffffffu;
             if (masked) {
               if (a.mask.rows) {
                 seen = 0;
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
-                  const int4 lo = *reinterpret_cast<const int4*>(start + hh * 32 + e);
-                  const int4 hi = *reinterpret_cast<const int4*>(start + BT + hh * 32 + e);
+                  const int4 lo = *reinterpret_cast<const int4*>(start + e);
+                  const int4 hi = *reinterpret_cast<const int4*>(start + BT + e);
                   seen |= (key >= lo.x && key < hi.x ? 1u : 0u) << e;
                   seen |= (key >= lo.y && key < hi.y ? 2u : 0u) << e;
                   seen |= (key >= lo.z && key < hi.z ? 4u : 0u) << e;
@@ -323,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t pp[16];
 #pragma unroll
             for (int e4 = 0; e4 < 32; e4 += 4) {
-              const float4 lv = *reinterpret_cast<const float4*>(l2 + hh * 32 + e4);
+              const float4 lv = *reinterpret_cast<const float4*>(l2 + e4);
               const float ls[4] = {lv.x, lv.y, lv.z, lv.w};
               float pr[4];
 #pragma unroll
@@ -341,33 +345,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else p = fast_exp2(fmaf(__uint_as_float(s[e]), k.mul, -ls[u]));
                 if (masked && !(seen & (1u << e))) p = 0.f;
                 pr[u] = p;
-                pf[hh * 32 + e] = CAP ? p * f : p;
+                pf[e] = CAP ? p * f : p;
               }
               pp[e4 / 2] = pack_bf16x2(pr[0], pr[1]);
               pp[e4 / 2 + 1] = pack_bf16x2(pr[2], pr[3]);
             }
-            tmem_st_32x32b_x16(t_s + hh * 16, pp);  // over S^T columns already read
+            tmem_st_32x32b_x16(t_s, pp);  // over S^T columns already read
           }
           tmem_wait_st();
-          warp_arrive(p_full);
+          warp_arrive(&p_full[n & 1]);
           if (!wwait(dp_full, n & 1, a.err, abort_flag)) { ok = false; break; }
           tc_fence_after();
           const float* delta = l2 + BT;
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
+          {
             uint32_t dp[32];
-            tmem_ld_32x32b_x32(t_dp + hh * 32, dp);
+            tmem_ld(t_dp, dp);
             tmem_wait_ld();
             uint32_t ds[16];
 #pragma unroll
             for (int e4 = 0; e4 < 32; e4 += 4) {
-              const float4 dl = *reinterpret_cast<const float4*>(delta + hh * 32 + e4);
-              ds[e4 / 2] = pack_bf16x2(pf[hh * 32 + e4] * (__uint_as_float(dp[e4]) - dl.x),
-                                       pf[hh * 32 + e4 + 1] * (__uint_as_float(dp[e4 + 1]) - dl.y));
-              ds[e4 / 2 + 1] = pack_bf16x2(pf[hh * 32 + e4 + 2] * (__uint_as_float(dp[e4 + 2]) - dl.z),
-                                           pf[hh * 32 + e4 + 3] * (__uint_as_float(dp[e4 + 3]) - dl.w));
+              const float4 dl = *reinterpret_cast<const float4*>(delta + e4);
+              ds[e4 / 2] = pack_bf16x2(pf[e4] * (__uint_as_float(dp[e4]) - dl.x),
+                                       pf[e4 + 1] * (__uint_as_float(dp[e4 + 1]) - dl.y));
+              ds[e4 / 2 + 1] = pack_bf16x2(pf[e4 + 2] * (__uint_as_float(dp[e4 + 2]) - dl.z),
+                                           pf[e4 + 3] * (__uint_as_float(dp[e4 + 3]) - dl.w));
             }
-            tmem_st_32x32b_x16(t_dp + hh * 16, ds);  // over dP^T columns already read
+            tmem_st_32x32b_x16(t_dp, ds);  // over dP^T columns already read
           }
           tmem_wait_st();
           warp_arrive(ds_full);
@@ -376,16 +379,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (!wwait(g_full, it & 1, a.err, abort_flag)) { ok = false; break; }
       tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tmem + C::T_DV + lane_off + half * (D / 2) + c * 32, v);
+      {
+        uint32_t v[D / 4], u[D / 4];
+        tmem_ld(tmem + C::T_DV + lane_off + part * (D / 4), v);
+        tmem_ld(tmem + C::T_DK + lane_off + part * (D / 4), u);
         tmem_wait_ld();
-        if (in) store_row32(dv + c * 32, v, 1.f);
-        tmem_ld_32x32b_x32(tmem + C::T_DK + lane_off + half * (D / 2) + c * 32, v);
-        tmem_wait_ld();
-        if (c == D / 64 - 1) warp_arrive(g_free);
-        if (in) store_row32(dk + c * 32, v, a.scale);
+        warp_arrive(g_free);
+        if (in) {
+          store_row(dv, v, 1.f);
+          store_row(dk, u, a.scale);
+        }
       }
       ++it;
     }

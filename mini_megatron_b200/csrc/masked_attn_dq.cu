@@ -11,7 +11,7 @@
 // the operand of its products.
 //
 // Persistent grid, one CTA per SM; a work item is (batch, head, 128-row query tile).
-// Roles (12 warps):
+// Roles (20 warps):
 //
 //   warp 0      TMA: Q, dO per item; K_j and V_j into rings
 //   warp 1      TMEM allocation; one thread issues S = Q K_j^T (two TMEM buffers), dP = dO V_j^T
@@ -19,16 +19,20 @@
 //               ready, dP of the next as soon as this one has been read
 //   warps 2-3   Delta and LSE of the next item's rows: into shared memory for the warps below and
 //               into the tile-padded workspace the key side reads with bulk copies
-//   warps 4-11  dS: warps w and w + 4 share 32 query rows and split the 128 keys
+//   warps 4-19  dS: four warps share 32 query rows, each has 32 of the 128 keys
 //
-// dS overwrites the S columns it came from; the halves of a row are 64 columns apart.
+// dS overwrites the S columns it came from: every warp's 32 keys start 32 columns apart.
+// A warp's step is a chain of waits, a TMEM load, exponentials, another wait and load and the
+// store; four warps on each SM sub-partition fill one another's gaps (with two, 64 keys each, the
+// same step took DQTWO cycles a tile instead of DQFOUR at d = 64).
 #include "masked_attn.cuh"
 
 namespace mmb {
 namespace mattn {
 namespace dq {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
+constexpr int kWarps = 16;  // of the softmax gradient
 
 template <int D>
 struct Cfg {
@@ -124,16 +128,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = bars;            // [2]
   uint64_t* q_empty = bars + 2;       // [2]
   uint64_t* st_full = bars + 4;       // [2]  row statistics written (2 warps)
-  uint64_t* st_empty = bars + 6;      // [2]  ... read (8 warps)
+  uint64_t* st_empty = bars + 6;      // [2]  ... read (16 warps)
   uint64_t* s_full = bars + 8;        // [2]  S computed
   uint64_t* k_full = bars + 10;       // [4]
   uint64_t* k_empty = bars + 14;      // [4]
   uint64_t* v_full = bars + 18;       // [4]
   uint64_t* v_empty = bars + 22;      // [4]
   uint64_t* dp_full = bars + 26;      // dP computed
-  uint64_t* ds_full = bars + 27;      // dS written, dP read (8 warps)
+  uint64_t* ds_full = bars + 27;      // dS written, dP read (16 warps)
   uint64_t* dq_full = bars + 28;      // dQ of an item complete
-  uint64_t* dq_free = bars + 29;      // ... read (8 warps)
+  uint64_t* dq_free = bars + 29;      // ... read (16 warps)
   uint64_t* drain = bars + 30;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -146,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&st_full[i], 2);
-      mbar_init(&st_empty[i], 8);
+      mbar_init(&st_empty[i], kWarps);
       mbar_init(&s_full[i], 1);
     }
     for (int s = 0; s < 4; ++s) {
@@ -156,9 +160,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&v_empty[s], 1);
     }
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, 8);
+    mbar_init(ds_full, kWarps);
     mbar_init(dq_full, 1);
-    mbar_init(dq_free, 8);
+    mbar_init(dq_free, kWarps);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -176,143 +180,157 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const int group = a.nh / a.nkv;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      // ---------------------------------------------------------------- TMA
-      int n = 0, q_issued = -1, k_issued = 0, v_issued = 0;
-      bool ok = true;
-      Walk x;
-      for (x.next(a, n_items); x.valid; x.next(a, n_items), ++n) {
-        const int hk = x.w.h / group;
-        if (x.first()) {
-          const int qb = x.it % QB;
-          if (x.it >= QB && !bwait(&q_empty[qb], ((x.it / QB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-          uint8_t* qd = sQ + qb * 2 * C::TILE;
-          mbar_expect_tx(&q_full[qb], 2 * C::TILE);
-          load_tile<D>(qd, &tm_qkv, &q_full[qb], x.w.h * D, x.w.t * BT, x.w.b);
-          load_tile<D>(qd + C::TILE, &tm_do, &q_full[qb], x.w.h * D, x.w.t * BT, x.w.b);
-          q_issued = x.it;
-        }
-        const int ks = n % NK, vs = n % NV;
-        if (n >= NK && !bwait(&k_empty[ks], ((n / NK) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-        mbar_expect_tx(&k_full[ks], C::TILE);
-        load_tile<D>(sK + ks * C::TILE, &tm_qkv, &k_full[ks], (a.nh + hk) * D, x.j * BT, x.w.b);
-        k_issued = n + 1;
-        if (n >= NV && !bwait(&v_empty[vs], ((n / NV) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-        mbar_expect_tx(&v_full[vs], C::TILE);
-        load_tile<D>(sV + vs * C::TILE, &tm_qkv, &v_full[vs], (a.nh + a.nkv + hk) * D, x.j * BT, x.w.b);
-        v_issued = n + 1;
-      }
-      if (!ok) {
-        for (int u = max(0, q_issued - QB + 1); u <= q_issued; ++u) drain_wait(&q_full[u % QB], (u / QB) & 1);
-        for (int u = max(0, k_issued - NK); u < k_issued; ++u) drain_wait(&k_full[u % NK], (u / NK) & 1);
-        for (int u = max(0, v_issued - NV); u < v_issued; ++u) drain_wait(&v_full[u % NV], (u / NV) & 1);
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0) {
-      // ---------------------------------------------------------------- MMA
-      bool ok = true;
-      int n = 0;
-      Walk cur, nxt;
-      auto issue_s = [&](const Walk& x, int u) -> bool {
-        const int qb = x.it % QB;
-        if (x.first() && !bwait(&q_full[qb], (x.it / QB) & 1, a.err, abort_flag)) return false;
-        if (!bwait(&k_full[u % NK], (u / NK) & 1, a.err, abort_flag)) return false;
-        tc_fence_after();
-        mma_abt<D>(tmem + C::T_S + (u & 1) * 128, smem_u32(sQ + qb * 2 * C::TILE), smem_u32(sK + (u % NK) * C::TILE));
-        umma_commit(&s_full[u & 1]);
-        return true;
-      };
-      auto issue_dp = [&](const Walk& x, int u) -> bool {
-        const int qb = x.it % QB;
-        if (!bwait(&v_full[u % NV], (u / NV) & 1, a.err, abort_flag)) return false;
-        tc_fence_after();
-        mma_abt<D>(tmem + C::T_DP, smem_u32(sQ + qb * 2 * C::TILE + C::TILE), smem_u32(sV + (u % NV) * C::TILE));
-        umma_commit(dp_full);
-        umma_commit(&v_empty[u % NV]);
-        if (x.last()) umma_commit(&q_empty[qb]);  // every product of this item that reads Q or dO is issued
-        return true;
-      };
-      nxt.next(a, n_items);
-      if (nxt.valid) ok = issue_s(nxt, 0) && issue_dp(nxt, 0);
-      while (ok && nxt.valid) {
-        cur = nxt;
-        nxt.next(a, n_items);
-        // one Q buffer: the next item's Q can only be loaded once this item's products are done with it,
-        // and this tile's dQ should not wait for that load
-        const bool early = nxt.valid && (QB == 2 || nxt.it == cur.it);
-        if (early && !issue_s(nxt, n + 1)) { ok = false; break; }
-        if (!bwait(ds_full, n & 1, a.err, abort_flag)) { ok = false; break; }
-        if (early && !issue_dp(nxt, n + 1)) { ok = false; break; }
-        if (cur.first() && cur.it > 0 && !bwait(dq_free, (cur.it - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-        tc_fence_after();
-        mma_tmem_b<D>(tmem + C::T_DQ, tmem + C::T_S + (n & 1) * 128, 64, smem_u32(sK + (n % NK) * C::TILE),
-                      !cur.first());
-        umma_commit(&k_empty[n % NK]);
-        if (cur.last()) umma_commit(dq_full);
-        if (nxt.valid && !early && !(issue_s(nxt, n + 1) && issue_dp(nxt, n + 1))) { ok = false; break; }
-        ++n;
-      }
-      if (!ok) {
-        umma_commit(drain);
-        drain_wait(drain, 0);
-      }
-    }
-    __syncwarp();
-  } else if (warp < 4) {
-    // ------------------------------------------------------------------ row statistics
-    constexpr int G = D / 8;        // lanes per row
-    constexpr int R = 32 / G;       // rows per pass
-    const int part = lane % G, sub = lane / G;
-    Walk x;
-    x.next(a, n_items);
-    while (x.valid) {
-      const Item& w = x.w;
-      const int sb = x.it % SB;
-      if (x.it >= SB && !wwait(&st_empty[sb], ((x.it / SB) - 1) & 1, a.err, abort_flag)) break;
-      const float* lse = a.lse + ((size_t)w.b * a.nh + w.h) * a.S;
-      float* ld = a.ld + (((size_t)w.b * a.nh + w.h) * a.n_t + w.t) * (2 * BT);
-#pragma unroll 4
-      for (int p = 0; p < 64 / R; ++p) {
-        const int row = (warp - 2) * 64 + p * R + sub;
-        const int i = w.t * BT + row;
-        float acc = 0.f;
-        if (i < a.S) {
-          const uint4 u = *reinterpret_cast<const uint4*>(a.dout + w.b * a.do_sb + i * a.do_ss + w.h * D + part * 8);
-          const uint4 v = *reinterpret_cast<const uint4*>(a.out + ((size_t)w.b * a.S + i) * ((size_t)a.nh * D) +
-                                                          (size_t)w.h * D + part * 8);
-          const uint32_t* uw = reinterpret_cast<const uint32_t*>(&u);
-          const uint32_t* vw = reinterpret_cast<const uint32_t*>(&v);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack_bf16x2(uw[e]), g = unpack_bf16x2(vw[e]);
-            acc = fmaf(f.x, g.x, fmaf(f.y, g.y, acc));
+  if (warp < 4) {
+    reg_inc<128>();
+    if (warp == 0) {
+      if (elect_one()) {
+        // ---------------------------------------------------------------- TMA
+        int n = 0, q_issued = -1, k_issued = 0, v_issued = 0;
+        bool ok = true;
+        Walk x;
+        for (x.next(a, n_items); x.valid; x.next(a, n_items), ++n) {
+          const int hk = x.w.h / group;
+          if (x.first()) {
+            const int qb = x.it % QB;
+            if (x.it >= QB && !bwait(&q_empty[qb], ((x.it / QB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+            uint8_t* qd = sQ + qb * 2 * C::TILE;
+            mbar_expect_tx(&q_full[qb], 2 * C::TILE);
+            load_tile<D>(qd, &tm_qkv, &q_full[qb], x.w.h * D, x.w.t * BT, x.w.b);
+            load_tile<D>(qd + C::TILE, &tm_do, &q_full[qb], x.w.h * D, x.w.t * BT, x.w.b);
+            q_issued = x.it;
           }
+          const int ks = n % NK, vs = n % NV;
+          if (n >= NK && !bwait(&k_empty[ks], ((n / NK) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&k_full[ks], C::TILE);
+          load_tile<D>(sK + ks * C::TILE, &tm_qkv, &k_full[ks], (a.nh + hk) * D, x.j * BT, x.w.b);
+          k_issued = n + 1;
+          if (n >= NV && !bwait(&v_empty[vs], ((n / NV) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&v_full[vs], C::TILE);
+          load_tile<D>(sV + vs * C::TILE, &tm_qkv, &v_full[vs], (a.nh + a.nkv + hk) * D, x.j * BT, x.w.b);
+          v_issued = n + 1;
         }
-#pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-        if (part == 0) {
-          float l2 = INFINITY;
-          if (i < a.S) {
-            const float l = lse[i];
-            if (l != -INFINITY) l2 = l * kLog2e;
-          }
-          if (l2 == INFINITY) acc = 0.f;  // a row that sees nothing, or lies behind the end, gives no gradient
-          sST[sb * BT + row] = make_float2(l2, acc);
-          ld[row] = l2;
-          ld[BT + row] = acc;
+        if (!ok) {
+          for (int u = max(0, q_issued - QB + 1); u <= q_issued; ++u) drain_wait(&q_full[u % QB], (u / QB) & 1);
+          for (int u = max(0, k_issued - NK); u < k_issued; ++u) drain_wait(&k_full[u % NK], (u / NK) & 1);
+          for (int u = max(0, v_issued - NV); u < v_issued; ++u) drain_wait(&v_full[u % NV], (u / NV) & 1);
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&st_full[sb]);
-      x.j = x.w.r.y - 1;  // on to the next item
+    } else if (warp == 1) {
+      if (elect_one()) {
+        // ---------------------------------------------------------------- MMA
+        bool ok = true;
+        int n = 0;
+        Walk cur, nxt;
+        auto issue_s = [&](const Walk& x, int u) -> bool {
+          const int qb = x.it % QB;
+          if (x.first() && !bwait(&q_full[qb], (x.it / QB) & 1, a.err, abort_flag)) return false;
+          if (!bwait(&k_full[u % NK], (u / NK) & 1, a.err, abort_flag)) return false;
+          tc_fence_after();
+          mma_abt<D>(tmem + C::T_S + (u & 1) * 128, smem_u32(sQ + qb * 2 * C::TILE), smem_u32(sK + (u % NK) * C::TILE));
+          umma_commit(&s_full[u & 1]);
+          return true;
+        };
+        auto issue_dp = [&](const Walk& x, int u) -> bool {
+          const int qb = x.it % QB;
+          if (!bwait(&v_full[u % NV], (u / NV) & 1, a.err, abort_flag)) return false;
+          tc_fence_after();
+          mma_abt<D>(tmem + C::T_DP, smem_u32(sQ + qb * 2 * C::TILE + C::TILE), smem_u32(sV + (u % NV) * C::TILE));
+          umma_commit(dp_full);
+          umma_commit(&v_empty[u % NV]);
+          if (x.last()) umma_commit(&q_empty[qb]);  // every product of this item that reads Q or dO is issued
+          return true;
+        };
+        nxt.next(a, n_items);
+        if (nxt.valid) ok = issue_s(nxt, 0) && issue_dp(nxt, 0);
+        while (ok && nxt.valid) {
+          cur = nxt;
+          nxt.next(a, n_items);
+          // one Q buffer: the next item's Q can only be loaded once this item's products are done with it,
+          // and this tile's dQ should not wait for that load
+          const bool early = nxt.valid && (QB == 2 || nxt.it == cur.it);
+          if (early && !issue_s(nxt, n + 1)) { ok = false; break; }
+          if (!bwait(ds_full, n & 1, a.err, abort_flag)) { ok = false; break; }
+          if (early && !issue_dp(nxt, n + 1)) { ok = false; break; }
+          if (cur.first() && cur.it > 0 && !bwait(dq_free, (cur.it - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          mma_tmem_b<D, 32>(tmem + C::T_DQ, tmem + C::T_S + (n & 1) * 128, smem_u32(sK + (n % NK) * C::TILE),
+                        !cur.first());
+          umma_commit(&k_empty[n % NK]);
+          if (cur.last()) umma_commit(dq_full);
+          if (nxt.valid && !early && !(issue_s(nxt, n + 1) && issue_dp(nxt, n + 1))) { ok = false; break; }
+          ++n;
+        }
+        if (!ok) {
+          umma_commit(drain);
+          drain_wait(drain, 0);
+        }
+      }
+      __syncwarp();
+    } else {
+      // ------------------------------------------------------------------ row statistics
+      constexpr int G = D / 8;        // lanes per row
+      constexpr int R = 32 / G;       // rows per pass
+      const int part = lane % G, sub = lane / G;
+      Walk x;
       x.next(a, n_items);
+      while (x.valid) {
+        const Item& w = x.w;
+        const int sb = x.it % SB;
+        if (x.it >= SB && !wwait(&st_empty[sb], ((x.it / SB) - 1) & 1, a.err, abort_flag)) break;
+        const float* lse = a.lse + ((size_t)w.b * a.nh + w.h) * a.S;
+        float* ld = a.ld + (((size_t)w.b * a.nh + w.h) * a.n_t + w.t) * (2 * BT);
+        // 8 passes' loads in flight at once: 64 threads have to keep up with the 8 warps below
+#pragma unroll 1
+        for (int p0 = 0; p0 < 64 / R; p0 += 8) {
+          uint4 u[8], v[8];
+          float l[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int i = w.t * BT + (warp - 2) * 64 + (p0 + e) * R + sub;
+            u[e] = v[e] = make_uint4(0u, 0u, 0u, 0u);
+            l[e] = -INFINITY;
+            if (i < a.S) {
+              u[e] = *reinterpret_cast<const uint4*>(a.dout + w.b * a.do_sb + i * a.do_ss + w.h * D + part * 8);
+              v[e] = *reinterpret_cast<const uint4*>(a.out + ((size_t)w.b * a.S + i) * ((size_t)a.nh * D) +
+                                                     (size_t)w.h * D + part * 8);
+              l[e] = lse[i];
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int row = (warp - 2) * 64 + (p0 + e) * R + sub;
+            const uint32_t* uw = reinterpret_cast<const uint32_t*>(&u[e]);
+            const uint32_t* vw = reinterpret_cast<const uint32_t*>(&v[e]);
+            float acc = 0.f;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const float2 f = unpack_bf16x2(uw[z]), g = unpack_bf16x2(vw[z]);
+              acc = fmaf(f.x, g.x, fmaf(f.y, g.y, acc));
+            }
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+            if (part == 0) {
+              // a row that sees nothing, or lies behind the end, gives no gradient
+              const bool none = l[e] == -INFINITY;
+              const float l2 = none ? INFINITY : l[e] * kLog2e;
+              acc = none ? 0.f : acc;
+              sST[sb * BT + row] = make_float2(l2, acc);
+              ld[row] = l2;
+              ld[BT + row] = acc;
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&st_full[sb]);
+        x.j = x.w.r.y - 1;  // on to the next item
+        x.next(a, n_items);
+      }
     }
   } else {
     // ------------------------------------------------------------------ dS, dQ store
-    const int half = (warp - 4) >> 2;
+    reg_dec<88>();
+    const int part = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const Score k = a.score;
@@ -323,12 +341,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int i = w.t * BT + row;
       const bool in = i < a.S;
       __nv_bfloat16* dst = a.dqkv + ((size_t)w.b * a.S + i) * ((size_t)(a.nh + 2 * a.nkv) * D) + (size_t)w.h * D +
-                           half * (D / 2);
+                           part * (D / 4);
       if (w.r.x >= w.r.y) {
-        if (in) {
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c) store_zero32(dst + c * 32);
-        }
+        if (in) store_zero<D / 4>(dst);
         continue;
       }
       const int2 full = full_tiles(a.mask, w.b, a.n_t, w.t);
@@ -346,22 +361,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&st_empty[sb]);
       for (int j = w.r.x; j < w.r.y; ++j, ++n) {
-        const uint32_t t_s = tmem + C::T_S + (n & 1) * 128 + lane_off + half * 64;
+        const uint32_t t_s = tmem + C::T_S + (n & 1) * 128 + lane_off + part * 32;
         if (!wwait(&s_full[n & 1], (n >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        const bool masked = j < full.x || j >= full.y;
-        float pf[64];  // P (1 - tanh^2)
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
+        float pf[32];  // P (1 - tanh^2)
+        {
           uint32_t s[32];
-          tmem_ld_32x32b_x32(t_s + hh * 32, s);
+          tmem_ld(t_s, s);
           tmem_wait_ld();
-          const int j0 = j * BT + half * 64 + hh * 32;  // key of column 0
-          uint32_t seen = 0xffffffffu;
-          if (masked) {
-            const int l0 = min(max(start - j0, 0), 32), h0 = min(max(end - j0, 0), 32);
-            seen = (h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u) & ~(l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u);
-          }
+          const int j0 = j * BT + part * 32;  // key of column 0
           const float dist = (float)(j0 - i);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
@@ -375,28 +383,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             float p;
             if (CAP || BIAS) p = fast_exp2(x - st.x);
             else p = fast_exp2(fmaf(__uint_as_float(s[e]), k.mul, -st.x));
-            if (CAP) p *= f;
-            pf[hh * 32 + e] = p;
+            pf[e] = CAP ? p * f : p;
           }
-          if (masked) {
+          if (j < full.x || j >= full.y) {
+            const int l0 = min(max(start - j0, 0), 32), h0 = min(max(end - j0, 0), 32);
+            const uint32_t seen = (h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u) & ~(l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (!(seen & (1u << e))) pf[hh * 32 + e] = 0.f;
+              if (!(seen & (1u << e))) pf[e] = 0.f;
           }
         }
         if (!wwait(dp_full, n & 1, a.err, abort_flag)) { ok = false; break; }
         tc_fence_after();
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
+        {
           uint32_t dp[32];
-          tmem_ld_32x32b_x32(tmem + C::T_DP + lane_off + half * 64 + hh * 32, dp);
+          tmem_ld(tmem + C::T_DP + lane_off + part * 32, dp);
           tmem_wait_ld();
           uint32_t ds[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            ds[e] = pack_bf16x2(pf[hh * 32 + 2 * e] * (__uint_as_float(dp[2 * e]) - st.y),
-                                pf[hh * 32 + 2 * e + 1] * (__uint_as_float(dp[2 * e + 1]) - st.y));
-          tmem_st_32x32b_x16(t_s + hh * 16, ds);
+            ds[e] = pack_bf16x2(pf[2 * e] * (__uint_as_float(dp[2 * e]) - st.y),
+                                pf[2 * e + 1] * (__uint_as_float(dp[2 * e + 1]) - st.y));
+          tmem_st_32x32b_x16(t_s, ds);
         }
         tmem_wait_st();
         warp_arrive(ds_full);
@@ -404,13 +412,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (!wwait(dq_full, it & 1, a.err, abort_flag)) { ok = false; break; }
       tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tmem + C::T_DQ + lane_off + half * (D / 2) + c * 32, v);
+      {
+        uint32_t v[D / 4];
+        tmem_ld(tmem + C::T_DQ + lane_off + part * (D / 4), v);
         tmem_wait_ld();
-        if (c == D / 64 - 1) warp_arrive(dq_free);
-        if (in) store_row32(dst + c * 32, v, a.scale);
+        warp_arrive(dq_free);
+        if (in) store_row(dst, v, a.scale);
       }
       ++it;
     }

@@ -14,7 +14,9 @@
 // pay for a mask.  Roles (16 warps):
 //
 //   warp 0       TMA: Q tiles per item; K_j / V_j into an NS-stage ring
-//   warp 1       TMEM allocation; one thread issues S_i = Q_i K_j^T and O_i += P_i V_j
+//   warps 1, 2   one thread each issues S_i = Q_i K_j^T and O_i += P_i V_j of its tile (warp 1 also
+//                allocates TMEM); with one thread for both, the tile that is ready waited for the
+//                other one's P: 3800 cycles per pair of tiles instead of PAIRCYC at d = 64
 //   warps 4-7,   softmax of tile 0 / tile 1, a thread per query row: scores out of
 //   warps 8-11   TMEM, transform, mask, running maximum, P back into TMEM as bf16
 //   warps 12-15  epilogue of both tiles: O / row sum -> bf16, LSE; it runs while the
@@ -118,17 +120,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_full = p_free + 2;      // [2]  last PV_i of the item complete
   uint64_t* o_free = o_full + 2;      // [2]  O_i and its statistics read by the epilogue (4 warps)
   uint64_t* ml_full = o_free + 2;     // [2]  statistics of the item written (4 warps)
-  uint64_t* drain = ml_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* turn = ml_full + 2;       // [2][4]  exponentials of a joint step issued, per tile and sub-partition
+  uint64_t* drain = turn + 8;         // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_items = a.B * a.nh * ((a.n_t + 1) / 2);
 
   if (threadIdx.x == 0) {
+    for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_empty[i], 2);
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);
       mbar_init(&p_full[i], 4);
@@ -136,14 +140,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 4);
       mbar_init(&ml_full[i], 4);
+      mbar_init(&drain[i], 1);
     }
     for (int s = 0; s < NS; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], 2);
     }
-    mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tm_qkv);
@@ -161,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     reg_dec<64>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
       // ---------------------------------------------------------------- TMA
       int kv = 0, it = 0, q_issued = -1;
       bool ok = true;
@@ -202,90 +206,69 @@ __global__ void __launch_bounds__(kThreads, 1)
           drain_wait(&v_full[u % NS], (u / NS) & 1);
         }
       }
-    } else if (warp == 1 && lane == 0) {
-      // ---------------------------------------------------------------- MMA
+    } else if ((warp == 1 || warp == 2) && elect_one()) {
+      // ---------------------------------------------------------------- MMA, tile grp of every item
+      const int grp = warp - 1;
+      const uint32_t t_s = tmem + (grp == 0 ? C::T_S0 : C::T_S1);
+      const uint32_t t_p = tmem + (grp == 0 ? C::T_P0 : C::T_P1);
+      const uint32_t t_o = tmem + (grp == 0 ? C::T_O0 : C::T_O1);
       int kv = 0, it = 0;
-      int sc[2] = {0, 0};  // S_i issued (s_free phases)
-      int pc[2] = {0, 0};  // P_i consumed (p_full phases)
-      int ic[2] = {0, 0};  // items with an active tile (o_free phases)
+      int sc = 0, pc = 0, ic = 0;  // S issued (s_free phases), P consumed (p_full), items with keys (o_free)
       bool ok = true;
-      auto issue_s = [&](int i, uint32_t q_addr, int stage) -> bool {
-        if (SEP && sc[i] > 0 && !bwait(&s_free[i], (sc[i] - 1) & 1, a.err, abort_flag)) return false;
-        ++sc[i];
-        tc_fence_after();
-        mma_abt<D>(tmem + (i == 0 ? C::T_S0 : C::T_S1), q_addr, smem_u32(sK + stage * C::TILE));
-        umma_commit(&s_full[i]);
+      uint32_t q_addr = 0;
+      // S of the K stage of loop position u; the stage is released either way
+      auto issue_s = [&](int u, bool on) -> bool {
+        const int st = u % NS;
+        if (!bwait(&k_full[st], (u / NS) & 1, a.err, abort_flag)) return false;
+        if (on) {
+          if (SEP && sc > 0 && !bwait(&s_free[grp], (sc - 1) & 1, a.err, abort_flag)) return false;
+          ++sc;
+          tc_fence_after();
+          mma_abt<D>(t_s, q_addr, smem_u32(sK + st * C::TILE));
+          umma_commit(&s_full[grp]);
+        }
+        umma_commit(&k_empty[st]);
         return true;
       };
-      auto issue_pv = [&](int i, int stage, bool first, bool last) -> bool {
-        if (!bwait(&p_full[i], pc[i] & 1, a.err, abort_flag)) return false;
-        ++pc[i];
-        if (first && ic[i] > 0 && !bwait(&o_free[i], (ic[i] - 1) & 1, a.err, abort_flag)) return false;
-        tc_fence_after();
-        mma_tmem_b<D>(tmem + (i == 0 ? C::T_O0 : C::T_O1), tmem + (i == 0 ? C::T_P0 : C::T_P1), 32,
-                      smem_u32(sV + stage * C::TILE), !first);
-        if (SEP) umma_commit(&p_free[i]);
-        if (last) umma_commit(&o_full[i]);
+      auto issue_pv = [&](int u, bool on, bool first, bool last) -> bool {
+        const int st = u % NS;
+        if (!bwait(&v_full[st], (u / NS) & 1, a.err, abort_flag)) return false;
+        if (on) {
+          if (!bwait(&p_full[grp], pc & 1, a.err, abort_flag)) return false;
+          ++pc;
+          if (first && ic > 0 && !bwait(&o_free[grp], (ic - 1) & 1, a.err, abort_flag)) return false;
+          tc_fence_after();
+          mma_tmem_b<D, 64>(t_o, t_p, smem_u32(sV + st * C::TILE), !first);
+          if (SEP) umma_commit(&p_free[grp]);
+          if (last) umma_commit(&o_full[grp]);
+        }
+        umma_commit(&v_empty[st]);
         return true;
       };
       for (int r = 0, item; (item = snake_item(r)) < n_items; ++r) {
         const Item w = decode(a, item);
         if (w.lo >= w.hi) continue;
-        const int J = w.hi - w.lo;
+        const int2 range = grp == 0 ? w.r0 : w.r1;
         const int qb = it % QB;
-        const uint32_t q0 = smem_u32(sQ + qb * 2 * C::TILE), q1 = q0 + C::TILE;
-        auto on0 = [&](int j) { return j >= w.r0.x && j < w.r0.y; };
-        auto on1 = [&](int j) { return j >= w.r1.x && j < w.r1.y; };
+        q_addr = smem_u32(sQ + (qb * 2 + grp) * C::TILE);
         if (!bwait(&q_full[qb], (it / QB) & 1, a.err, abort_flag)) { ok = false; break; }
-        if (!bwait(&k_full[kv % NS], (kv / NS) & 1, a.err, abort_flag)) { ok = false; break; }
-        if (on0(w.lo) && !issue_s(0, q0, kv % NS)) { ok = false; break; }
-        if (on1(w.lo) && !issue_s(1, q1, kv % NS)) { ok = false; break; }
-        umma_commit(&k_empty[kv % NS]);
-        for (int u = 0; u < J && ok; ++u) {
-          const int j = w.lo + u;
-          const int st = (kv + u) % NS, ph = ((kv + u) / NS) & 1;
-          const int st1 = (kv + u + 1) % NS, ph1 = ((kv + u + 1) / NS) & 1;
-          const bool more = u + 1 < J;
-          const bool n0 = more && on0(j + 1), n1 = more && on1(j + 1);
-          if (SEP) {
-            // next scores first: they only need the softmax to have read the current ones
-            if (more) {
-              if (!bwait(&k_full[st1], ph1, a.err, abort_flag)) { ok = false; break; }
-              if (n0 && !issue_s(0, q0, st1)) { ok = false; break; }
-              if (n1 && !issue_s(1, q1, st1)) { ok = false; break; }
-              umma_commit(&k_empty[st1]);
-            }
-            if (!bwait(&v_full[st], ph, a.err, abort_flag)) { ok = false; break; }
-            if (on0(j) && !issue_pv(0, st, j == w.r0.x, j == w.r0.y - 1)) { ok = false; break; }
-            if (on1(j) && !issue_pv(1, st, j == w.r1.x, j == w.r1.y - 1)) { ok = false; break; }
-            umma_commit(&v_empty[st]);
-          } else {
-            // P_i overwrites S_i: PV0_j, S0_{j+1}, PV1_j, S1_{j+1}
-            if (!bwait(&v_full[st], ph, a.err, abort_flag)) { ok = false; break; }
-            if (on0(j) && !issue_pv(0, st, j == w.r0.x, j == w.r0.y - 1)) { ok = false; break; }
-            if (n0) {
-              if (!bwait(&k_full[st1], ph1, a.err, abort_flag)) { ok = false; break; }
-              if (!issue_s(0, q0, st1)) { ok = false; break; }
-            }
-            if (on1(j) && !issue_pv(1, st, j == w.r1.x, j == w.r1.y - 1)) { ok = false; break; }
-            umma_commit(&v_empty[st]);
-            if (more) {
-              if (!bwait(&k_full[st1], ph1, a.err, abort_flag)) { ok = false; break; }
-              if (n1 && !issue_s(1, q1, st1)) { ok = false; break; }
-              umma_commit(&k_empty[st1]);
-            }
-          }
+        auto on = [&](int j) { return j >= range.x && j < range.y; };
+        if (!issue_s(kv, on(w.lo))) { ok = false; break; }
+        for (int j = w.lo; j < w.hi; ++j, ++kv) {
+          // d = 64: the next scores first, they only need the softmax to have read the current ones;
+          // d = 128: P overwrites S, the next scores follow P V
+          if (SEP && j + 1 < w.hi && !issue_s(kv + 1, on(j + 1))) { ok = false; break; }
+          if (!issue_pv(kv, on(j), j == range.x, j == range.y - 1)) { ok = false; break; }
+          if (!SEP && j + 1 < w.hi && !issue_s(kv + 1, on(j + 1))) { ok = false; break; }
         }
         if (!ok) break;
         umma_commit(&q_empty[qb]);  // every S of this item has been issued
-        kv += J;
         ++it;
-        if (w.r0.y > w.r0.x) ++ic[0];
-        if (w.r1.y > w.r1.x) ++ic[1];
+        if (range.x < range.y) ++ic;
       }
       if (!ok) {
-        umma_commit(drain);
-        drain_wait(drain, 0);
+        umma_commit(&drain[grp]);
+        drain_wait(&drain[grp], 0);
       }
     }
     __syncwarp();
@@ -299,12 +282,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_p = tmem + (grp == 0 ? C::T_P0 : C::T_P1) + lane_off;
     const uint32_t t_o = tmem + (grp == 0 ? C::T_O0 : C::T_O1) + lane_off;
     const Score k = a.score;
-    int sc = 0, pc = 0, ic = 0;
+    int sc = 0, pc = 0, ic = 0, nj = 0;  // nj: steps that both tiles take
     bool ok = true;
     for (int r = 0, item; (item = snake_item(r)) < n_items; ++r) {
       const Item w = decode(a, item);
       const int t = grp == 0 ? w.t0 : w.t1;
-      const int2 range = grp == 0 ? w.r0 : w.r1;
+      const int2 range = grp == 0 ? w.r0 : w.r1, other = grp == 0 ? w.r1 : w.r0;
       if (range.x >= range.y) continue;
       const int2 full = full_tiles(a.mask, w.b, a.n_t, t);
       const int i = t * BT + row;
@@ -350,13 +333,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!(seen & (1u << e))) s[32 * g + e] = 0xff800000u;  // -inf
           }
         }
-        float mx[8];
+        float mx[4];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) mx[u] = __uint_as_float(s[u]);
+        for (int u = 0; u < 4; ++u) mx[u] = __uint_as_float(s[u]);
 #pragma unroll
-        for (int c = 8; c < 128; ++c) mx[c & 7] = fmaxf(mx[c & 7], __uint_as_float(s[c]));
-        float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                         fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+        for (int c = 4; c < 124; c += 8) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            mx[u] = max3(mx[u], __uint_as_float(s[c + 2 * u]), __uint_as_float(s[c + 2 * u + 1]));
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], __uint_as_float(s[124 + u]));
+        float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
         if (!CAP && !BIAS) mt *= k.mul;
         const bool need = mt > m + kRescaleLog2;
         const bool any_need = __any_sync(0xffffffffu, need) != 0;
@@ -372,29 +360,43 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
         }
         ++pc;
-        float rs[8];
+        // the exponentials of the two tiles take turns, one warp of each on every SM sub-partition: while one
+        // fills the MUFU pipe the other waits for its scores, takes its maximum and stores its P
+        const bool joint = j >= other.x && j < other.y;
+        if (joint) {
+          if (grp == 1 || nj > 0) {
+            if (!wwait(&turn[(grp ^ 1) * 4 + (warp & 3)], (grp == 1 ? nj : nj - 1) & 1, a.err, abort_flag)) {
+              ok = false;
+              break;
+            }
+          }
+        }
+        float2 rs[4];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) rs[u] = 0.f;
+        for (int u = 0; u < 4; ++u) rs[u] = make_float2(0.f, 0.f);
+        const float2 mul2v = make_float2(k.mul, k.mul), mu2 = make_float2(-mu, -mu);
 #pragma unroll
         for (int hcol = 0; hcol < 2; ++hcol) {
           uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int c = hcol * 64 + 2 * e;
-            float p0, p1;
-            if (CAP || BIAS) {
-              p0 = fast_exp2(__uint_as_float(s[c]) - mu);
-              p1 = fast_exp2(__uint_as_float(s[c + 1]) - mu);
-            } else {
-              p0 = fast_exp2(fmaf(__uint_as_float(s[c]), k.mul, -mu));
-              p1 = fast_exp2(fmaf(__uint_as_float(s[c + 1]), k.mul, -mu));
-            }
-            rs[e & 7] += p0 + p1;
-            pk[e] = pack_bf16x2(p0, p1);
+            float2 x = make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+            x = (CAP || BIAS) ? add2(x, mu2) : fma2(x, mul2v, mu2);
+            x.x = fast_exp2(x.x);
+            x.y = fast_exp2(x.y);
+            rs[e & 3] = add2(rs[e & 3], x);
+            pk[e] = pack_bf16x2(x.x, x.y);
           }
           tmem_st_x32(t_p + hcol * 32, pk);
         }
-        l = l * alpha + (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7])));
+        if (joint) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&turn[grp * 4 + (warp & 3)]);
+          ++nj;
+        }
+        rs[0] = add2(add2(rs[0], rs[1]), add2(rs[2], rs[3]));
+        l = l * alpha + (rs[0].x + rs[0].y);
         if (any_need && j > range.x) {
           // PV_i(j-1) is complete (SEP: waited above; otherwise it was issued before S_i(j))
 #pragma unroll 1
@@ -438,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (range.x >= range.y) {  // no row of the tile sees anything
           if (in) {
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) store_zero32(orow + c * 32);
+            for (int c = 0; c < D / 32; ++c) store_zero<32>(orow + c * 32);
             *lse = -INFINITY;
           }
           continue;
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_32x32b_x32(t_o + c * 32, o);
           tmem_wait_ld();
           if (c == D / 32 - 1) warp_arrive(&o_free[grp]);  // O and the statistics are in registers
-          if (in) store_row32(orow + c * 32, o, inv);
+          if (in) store_row(orow + c * 32, o, inv);
         }
         if (in) *lse = seen ? ml.x * kLn2 + logf(ml.y) : -INFINITY;
       }
