@@ -194,6 +194,32 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
   for (int c = 0; c < D / 64; ++c) tma_load_3d(dst + c * 16384, map, bar, col + 64 * c, row, batch);
 }
 
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
+// N fp32 values of one row, from column col0 on, as bf16 into a staged tile (chunks of 64 columns, `chunk`
+// bytes apart, rows of 128 bytes in the 128-byte swizzle) for a tensor store.  A thread owns a row of an
+// accumulator, so direct stores would touch 32 rows per instruction and hold the load/store pipe, and
+// every barrier poll behind it, for thousands of cycles per tile.
+template <int N>
+__device__ __forceinline__ void stage_row(uint8_t* tile, int chunk, int row, int col0, const uint32_t (&v)[N],
+                                          float mul) {
+#pragma unroll
+  for (int u = 0; u < N / 8; ++u) {
+    const int unit = col0 / 8 + u;
+    uint4 w;
+    w.x = pack_bf16x2(__uint_as_float(v[8 * u + 0]) * mul, __uint_as_float(v[8 * u + 1]) * mul);
+    w.y = pack_bf16x2(__uint_as_float(v[8 * u + 2]) * mul, __uint_as_float(v[8 * u + 3]) * mul);
+    w.z = pack_bf16x2(__uint_as_float(v[8 * u + 4]) * mul, __uint_as_float(v[8 * u + 5]) * mul);
+    w.w = pack_bf16x2(__uint_as_float(v[8 * u + 6]) * mul, __uint_as_float(v[8 * u + 7]) * mul);
+    *reinterpret_cast<uint4*>(tile + (unit >> 3) * chunk + row * 128 + (((unit & 7) ^ (row & 7)) << 4)) = w;
+  }
+}
+
 // 128 x 128 (+)= A [128 x D] B [128 x D]^T, both K-major in shared memory.
 template <int D>
 __device__ __forceinline__ void mma_abt(uint32_t dst, uint32_t a_addr, uint32_t b_addr) {
@@ -222,19 +248,6 @@ __device__ __forceinline__ void mma_tmem_b(uint32_t dst, uint32_t a_tmem, uint32
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
 
-// Stores N fp32 accumulator values as bf16 (2 N bytes of one row).
-template <int N>
-__device__ __forceinline__ void store_row(__nv_bfloat16* p, const uint32_t (&v)[N], float mul) {
-#pragma unroll
-  for (int u = 0; u < N / 8; ++u) {
-    uint4 w;
-    w.x = pack_bf16x2(__uint_as_float(v[8 * u + 0]) * mul, __uint_as_float(v[8 * u + 1]) * mul);
-    w.y = pack_bf16x2(__uint_as_float(v[8 * u + 2]) * mul, __uint_as_float(v[8 * u + 3]) * mul);
-    w.z = pack_bf16x2(__uint_as_float(v[8 * u + 4]) * mul, __uint_as_float(v[8 * u + 5]) * mul);
-    w.w = pack_bf16x2(__uint_as_float(v[8 * u + 6]) * mul, __uint_as_float(v[8 * u + 7]) * mul);
-    reinterpret_cast<uint4*>(p)[u] = w;
-  }
-}
 template <int N>
 __device__ __forceinline__ void store_zero(__nv_bfloat16* p) {
 #pragma unroll

@@ -107,7 +107,7 @@ struct Walk {
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
     masked_attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
-                           const Args a) {
+                           const __grid_constant__ CUtensorMap tm_dqkv, const Args a) {
   pdl_trigger();
   using C = Cfg<D>;
   constexpr int KB = C::KB, NQ = C::NQ, SB = C::SB;
@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* g_full = bars + 15;    // dK, dV of an item complete
   uint64_t* g_free = bars + 16;    // ... read (16 warps)
   uint64_t* drain = bars + 17;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* out_full = bars + 20;  // dK, dV of an item staged (16 warps)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -153,11 +154,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(ds_full, kWarps);
     mbar_init(g_full, 1);
     mbar_init(g_free, kWarps);
+    mbar_init(out_full, kWarps);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tm_qkv);
     prefetch_tmap(&tm_do);
+    prefetch_tmap(&tm_dqkv);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -248,8 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_tmem_b<D, 32>(tmem + C::T_DK, tmem + C::T_DP, q_addr, !cur.first());
           umma_commit(&q_empty[n % NQ]);
           if (cur.last(group)) {
-            umma_commit(g_full);
-            umma_commit(&kv_empty[cur.it % KB]);
+            umma_commit(g_full);  // K and V become the staging tiles of dK and dV, whose store releases them
           }
           if (nxt.valid && !early && !issue_s(nxt, n + 1)) { ok = false; break; }
           if (nxt.valid) issue_dp(nxt, n + 1);  // over dS^T, in issue order after dK
@@ -385,13 +387,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld(tmem + C::T_DK + lane_off + part * (D / 4), u);
         tmem_wait_ld();
         warp_arrive(g_free);
-        if (in) {
-          store_row(dv, v, 1.f);
-          store_row(dk, u, a.scale);
+        uint8_t* stg = sKV + (it % KB) * 2 * C::TILE;
+        stage_row(stg, 16384, row, part * (D / 4), u, a.scale);
+        stage_row(stg + C::TILE, 16384, row, part * (D / 4), v, 1.f);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(out_full);
+        if (warp == 4) {
+          if (!wwait(out_full, it & 1, a.err, abort_flag)) { ok = false; break; }
+          if (lane == 0) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              tma_store_3d(&tm_dqkv, stg + c * 16384, (a.nh + w.hk) * D + c * 64, w.t * BT, w.b);
+              tma_store_3d(&tm_dqkv, stg + C::TILE + c * 16384, (a.nh + a.nkv + w.hk) * D + c * 64, w.t * BT, w.b);
+            }
+            bulk_commit();
+            bulk_wait_read<0>();
+            mbar_arrive(&kv_empty[it % KB]);
+          }
+          __syncwarp();
         }
       }
       ++it;
     }
+    if (lane == 0) bulk_wait<0>();
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -403,11 +423,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int D, bool CAP, bool BIAS>
-int launch(const CUtensorMap& tq, const CUtensorMap& to, const Args& a, int grid, cudaStream_t stream) {
+int launch(const CUtensorMap& tq, const CUtensorMap& to, const CUtensorMap& td, const Args& a, int grid, cudaStream_t stream) {
   auto k = masked_attn_dkv_kernel<D, CAP, BIAS>;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, a);
+  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, td, a);
   return (int)cudaGetLastError();
 }
 
@@ -420,11 +440,14 @@ int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb,
   const int n_t = (c.S + BT - 1) / BT;
   const long items = (long)c.B * c.nkv * n_t;
   if (items > INT_MAX / 2) return -1;
-  CUtensorMap tq, to;
+  CUtensorMap tq, to, td;
   int rc = make_tmap_bf16_3d(&tq, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
   if (rc) return rc - 10;
   rc = make_tmap_bf16_3d(&to, dout, c.B, c.S, (long)c.nh * c.d, do_ss, do_sb, 64, BT);
   if (rc) return rc - 20;
+  const long width = (long)(c.nh + 2 * c.nkv) * c.d;
+  rc = make_tmap_bf16_3d(&td, dqkv, c.B, c.S, width, width, width * c.S, 64, BT);
+  if (rc) return rc - 30;
   dkv::Args a;
   a.B = c.B;
   a.S = c.S;
@@ -441,12 +464,12 @@ int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb,
   const int grid = (int)std::max(1L, std::min(items, (long)num_sms));
   const bool cap = c.cap > 0.f, bias = c.slopes != nullptr;
   if (c.d == 64) {
-    if (cap) return bias ? dkv::launch<64, true, true>(tq, to, a, grid, stream) : dkv::launch<64, true, false>(tq, to, a, grid, stream);
-    return bias ? dkv::launch<64, false, true>(tq, to, a, grid, stream) : dkv::launch<64, false, false>(tq, to, a, grid, stream);
+    if (cap) return bias ? dkv::launch<64, true, true>(tq, to, td, a, grid, stream) : dkv::launch<64, true, false>(tq, to, td, a, grid, stream);
+    return bias ? dkv::launch<64, false, true>(tq, to, td, a, grid, stream) : dkv::launch<64, false, false>(tq, to, td, a, grid, stream);
   }
   if (c.d == 128) {
-    if (cap) return bias ? dkv::launch<128, true, true>(tq, to, a, grid, stream) : dkv::launch<128, true, false>(tq, to, a, grid, stream);
-    return bias ? dkv::launch<128, false, true>(tq, to, a, grid, stream) : dkv::launch<128, false, false>(tq, to, a, grid, stream);
+    if (cap) return bias ? dkv::launch<128, true, true>(tq, to, td, a, grid, stream) : dkv::launch<128, true, false>(tq, to, td, a, grid, stream);
+    return bias ? dkv::launch<128, false, true>(tq, to, td, a, grid, stream) : dkv::launch<128, false, false>(tq, to, td, a, grid, stream);
   }
   return -2;
 }

@@ -113,7 +113,7 @@ struct Walk {
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
     masked_attn_dq_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
-                          const Args a) {
+                          const __grid_constant__ CUtensorMap tm_dqkv, const Args a) {
   pdl_trigger();
   using C = Cfg<D>;
   constexpr int QB = C::QB, NK = C::NK, NV = C::NV, SB = C::SB;
@@ -138,8 +138,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* ds_full = bars + 27;      // dS written, dP read (16 warps)
   uint64_t* dq_full = bars + 28;      // dQ of an item complete
   uint64_t* dq_free = bars + 29;      // ... read (16 warps)
-  uint64_t* drain = bars + 30;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
+  uint64_t* out_full = bars + 30;     // dQ of an item staged (16 warps)
+  uint64_t* drain = bars + 31;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -163,11 +164,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(ds_full, kWarps);
     mbar_init(dq_full, 1);
     mbar_init(dq_free, kWarps);
+    mbar_init(out_full, kWarps);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tm_qkv);
     prefetch_tmap(&tm_do);
+    prefetch_tmap(&tm_dqkv);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -256,8 +259,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           mma_tmem_b<D, 32>(tmem + C::T_DQ, tmem + C::T_S + (n & 1) * 128, smem_u32(sK + (n % NK) * C::TILE),
                         !cur.first());
-          umma_commit(&k_empty[n % NK]);
+          // the K stage of an item's last tile becomes the staging tile of its dQ, which then releases it
           if (cur.last()) umma_commit(dq_full);
+          else umma_commit(&k_empty[n % NK]);
           if (nxt.valid && !early && !(issue_s(nxt, n + 1) && issue_dp(nxt, n + 1))) { ok = false; break; }
           ++n;
         }
@@ -417,10 +421,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld(tmem + C::T_DQ + lane_off + part * (D / 4), v);
         tmem_wait_ld();
         warp_arrive(dq_free);
-        if (in) store_row(dst, v, a.scale);
+        const int ks = (n - 1) % NK;
+        uint8_t* stg = sK + ks * C::TILE;
+        stage_row(stg, 16384, row, part * (D / 4), v, a.scale);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(out_full);
+        if (warp == 4) {
+          if (!wwait(out_full, it & 1, a.err, abort_flag)) { ok = false; break; }
+          if (lane == 0) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_store_3d(&tm_dqkv, stg + c * 16384, w.h * D + c * 64, w.t * BT, w.b);
+            bulk_commit();
+            bulk_wait_read<0>();
+            mbar_arrive(&k_empty[ks]);
+          }
+          __syncwarp();
+        }
       }
       ++it;
     }
+    if (lane == 0) bulk_wait<0>();
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -432,11 +455,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int D, bool CAP, bool BIAS>
-int launch(const CUtensorMap& tq, const CUtensorMap& to, const Args& a, int grid, cudaStream_t stream) {
+int launch(const CUtensorMap& tq, const CUtensorMap& to, const CUtensorMap& td, const Args& a, int grid, cudaStream_t stream) {
   auto k = masked_attn_dq_kernel<D, CAP, BIAS>;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, a);
+  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, td, a);
   return (int)cudaGetLastError();
 }
 
@@ -449,11 +472,14 @@ int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, 
   const int n_t = (c.S + BT - 1) / BT;
   const long items = (long)c.B * c.nh * n_t;
   if (items > INT_MAX / 2) return -1;
-  CUtensorMap tq, to;
+  CUtensorMap tq, to, td;
   int rc = make_tmap_bf16_3d(&tq, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
   if (rc) return rc - 10;
   rc = make_tmap_bf16_3d(&to, dout, c.B, c.S, (long)c.nh * c.d, do_ss, do_sb, 64, BT);
   if (rc) return rc - 20;
+  const long width = (long)(c.nh + 2 * c.nkv) * c.d;
+  rc = make_tmap_bf16_3d(&td, dqkv, c.B, c.S, width, width, width * c.S, 64, BT);
+  if (rc) return rc - 30;
   dq::Args a;
   a.B = c.B;
   a.S = c.S;
@@ -475,12 +501,12 @@ int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, 
   const int grid = (int)std::max(1L, std::min(items, (long)num_sms));
   const bool cap = c.cap > 0.f, bias = c.slopes != nullptr;
   if (c.d == 64) {
-    if (cap) return bias ? dq::launch<64, true, true>(tq, to, a, grid, stream) : dq::launch<64, true, false>(tq, to, a, grid, stream);
-    return bias ? dq::launch<64, false, true>(tq, to, a, grid, stream) : dq::launch<64, false, false>(tq, to, a, grid, stream);
+    if (cap) return bias ? dq::launch<64, true, true>(tq, to, td, a, grid, stream) : dq::launch<64, true, false>(tq, to, td, a, grid, stream);
+    return bias ? dq::launch<64, false, true>(tq, to, td, a, grid, stream) : dq::launch<64, false, false>(tq, to, td, a, grid, stream);
   }
   if (c.d == 128) {
-    if (cap) return bias ? dq::launch<128, true, true>(tq, to, a, grid, stream) : dq::launch<128, true, false>(tq, to, a, grid, stream);
-    return bias ? dq::launch<128, false, true>(tq, to, a, grid, stream) : dq::launch<128, false, false>(tq, to, a, grid, stream);
+    if (cap) return bias ? dq::launch<128, true, true>(tq, to, td, a, grid, stream) : dq::launch<128, true, false>(tq, to, td, a, grid, stream);
+    return bias ? dq::launch<128, false, true>(tq, to, td, a, grid, stream) : dq::launch<128, false, false>(tq, to, td, a, grid, stream);
   }
   return -2;
 }

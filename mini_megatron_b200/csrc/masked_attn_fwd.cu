@@ -50,7 +50,8 @@ struct Cfg {
   static constexpr int K_OFF = QB * 2 * TILE;
   static constexpr int V_OFF = K_OFF + NS * TILE;
   static constexpr int ML_OFF = V_OFF + NS * TILE;  // [2][128] (maximum, row sum)
-  static constexpr int BAR_OFF = ML_OFF + 2 * BT * 8;
+  static constexpr int OUT_OFF = ML_OFF + 2 * BT * 8;  // 4 epilogue warps x 32 rows x 64 columns bf16
+  static constexpr int BAR_OFF = OUT_OFF + 4 * 4096;
   static constexpr int SMEM = 1024 + BAR_OFF + 512;
   static constexpr uint32_t T_S0 = 0, T_S1 = 128, T_O0 = 256, T_O1 = 256 + D;
   static constexpr uint32_t T_P0 = SEP ? 384 : T_S0, T_P1 = SEP ? 448 : T_S1;
@@ -93,7 +94,8 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
 
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
-    masked_attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const Args a) {
+    masked_attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_out,
+                           const Args a) {
   pdl_trigger();
   using C = Cfg<D>;
   constexpr int NS = C::NS;
@@ -151,6 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tm_qkv);
+    prefetch_tmap(&tm_out);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -424,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     reg_dec<80>();
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    uint8_t* stg = smem + C::OUT_OFF + (warp & 3) * 4096;
     int ic[2] = {0, 0};
     bool ok = true;
     for (int r = 0, item; ok && (item = snake_item(r)) < n_items; ++r) {
@@ -460,13 +464,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(t_o + c * 32, o);
+          if ((c & 1) == 0 && lane == 0) bulk_wait_read<0>();  // the last store has read the staged rows
           tmem_wait_ld();
+          __syncwarp();
           if (c == D / 32 - 1) warp_arrive(&o_free[grp]);  // O and the statistics are in registers
-          if (in) store_row(orow + c * 32, o, inv);
+          stage_row(stg, 0, lane, (c & 1) * 32, o, inv);
+          if (c & 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            const int row0 = t * BT + (warp & 3) * 32;
+            if (lane == 0 && row0 < a.S) {
+              tma_store_3d(&tm_out, stg, w.h * D + (c / 2) * 64, row0, w.b);
+              bulk_commit();
+            }
+          }
         }
         if (in) *lse = seen ? ml.x * kLn2 + logf(ml.y) : -INFINITY;
       }
     }
+    if (lane == 0) bulk_wait<0>();
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -478,11 +495,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int D, bool CAP, bool BIAS>
-int launch(const CUtensorMap& tm, const Args& a, int grid, cudaStream_t stream) {
+int launch(const CUtensorMap& tm, const CUtensorMap& to, const Args& a, int grid, cudaStream_t stream) {
   auto k = masked_attn_fwd_kernel<D, CAP, BIAS>;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tm, a);
+  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tm, to, a);
   return (int)cudaGetLastError();
 }
 
@@ -494,9 +511,11 @@ int masked_attn_fwd(const AttnCall& c, void* out, float* lse, int* err, int num_
   const int n_t = (c.S + BT - 1) / BT;
   const long items = (long)c.B * c.nh * ((n_t + 1) / 2);
   if (items > INT_MAX / 2) return -1;
-  CUtensorMap tm;
-  const int rc = make_tmap_bf16_3d(&tm, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
+  CUtensorMap tm, to;
+  int rc = make_tmap_bf16_3d(&tm, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
   if (rc) return rc - 10;
+  rc = make_tmap_bf16_3d(&to, out, c.B, c.S, (long)c.nh * c.d, (long)c.nh * c.d, (long)c.S * c.nh * c.d, 64, 32);
+  if (rc) return rc - 20;
   fwd::Args a;
   a.B = c.B;
   a.S = c.S;
@@ -512,12 +531,12 @@ int masked_attn_fwd(const AttnCall& c, void* out, float* lse, int* err, int num_
   const int grid = (int)std::max(1L, std::min(items, (long)num_sms));
   const bool cap = c.cap > 0.f, bias = c.slopes != nullptr;
   if (c.d == 64) {
-    if (cap) return bias ? fwd::launch<64, true, true>(tm, a, grid, stream) : fwd::launch<64, true, false>(tm, a, grid, stream);
-    return bias ? fwd::launch<64, false, true>(tm, a, grid, stream) : fwd::launch<64, false, false>(tm, a, grid, stream);
+    if (cap) return bias ? fwd::launch<64, true, true>(tm, to, a, grid, stream) : fwd::launch<64, true, false>(tm, to, a, grid, stream);
+    return bias ? fwd::launch<64, false, true>(tm, to, a, grid, stream) : fwd::launch<64, false, false>(tm, to, a, grid, stream);
   }
   if (c.d == 128) {
-    if (cap) return bias ? fwd::launch<128, true, true>(tm, a, grid, stream) : fwd::launch<128, true, false>(tm, a, grid, stream);
-    return bias ? fwd::launch<128, false, true>(tm, a, grid, stream) : fwd::launch<128, false, false>(tm, a, grid, stream);
+    if (cap) return bias ? fwd::launch<128, true, true>(tm, to, a, grid, stream) : fwd::launch<128, true, false>(tm, to, a, grid, stream);
+    return bias ? fwd::launch<128, false, true>(tm, to, a, grid, stream) : fwd::launch<128, false, false>(tm, to, a, grid, stream);
   }
   return -2;
 }
