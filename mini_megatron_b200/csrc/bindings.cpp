@@ -370,7 +370,7 @@ Tensor flash_attn_bwd_v1(const Tensor& dout, const Tensor& qkv, const Tensor& ou
 
 // ----------------------------------------------------------------- packed rows of documents
 // ids [B, S] int64 (tokens, or document ids with by_change) or none, marks [B, S] bool / uint8 or none, lengths [B]
-// int32 or none -> positions, start, end [B, S] int32 and the attention kernels' tile tables (rows, qstat, krange).
+// int32 or none -> positions, start, end [B, S] int32 and the attention kernels' tile tables (rows, qstat, krange, order).
 std::vector<Tensor> document_plan(const c10::optional<Tensor>& ids, int64_t eod, bool by_change,
                                   const c10::optional<Tensor>& marks, const c10::optional<Tensor>& lengths, int64_t B,
                                   int64_t S, const at::Device& device) {
@@ -407,12 +407,13 @@ std::vector<Tensor> document_plan(const c10::optional<Tensor>& ids, int64_t eod,
   const int64_t n_t = (S + 127) / 128;
   Tensor positions = at::empty({B, S}, opt), start = at::empty({B, S}, opt), end = at::empty({B, S}, opt);
   Tensor rows = at::empty({B, n_t, 2, 128}, opt), qstat = at::empty({B, n_t, 4}, opt),
-         krange = at::empty({B, n_t, 2}, opt);
+         krange = at::empty({B, n_t, 2}, opt), order = at::empty({B * ((n_t + 1) / 2 + 2 * n_t)}, opt);
   MMB_CHECK_RC(mmb::document_plan(ip, ld_ids, eod, by_change ? 1 : 0, mp, ld_marks, lp, (int)B, (int)S,
                                   positions.data_ptr<int>(), start.data_ptr<int>(), end.data_ptr<int>(),
-                                  rows.data_ptr<int>(), qstat.data_ptr<int>(), krange.data_ptr<int>(), cur_stream()),
+                                  rows.data_ptr<int>(), qstat.data_ptr<int>(), krange.data_ptr<int>(),
+                                  order.data_ptr<int>(), cur_stream()),
                "document_plan");
-  return {positions, start, end, rows, qstat, krange};
+  return {positions, start, end, rows, qstat, krange, order};
 }
 
 // ----------------------------------------------------------------- rotary positions
@@ -493,7 +494,8 @@ void token_strides(const Tensor& t, const char* name, int64_t& ss, int64_t& sb) 
 
 mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, const c10::optional<Tensor>& rows,
                         const c10::optional<Tensor>& qstat, const c10::optional<Tensor>& krange,
-                        const c10::optional<Tensor>& slopes, double cap, double scale) {
+                        const c10::optional<Tensor>& order, const c10::optional<Tensor>& slopes, double cap,
+                        double scale) {
   mmb::AttnCall c{};
   int64_t ss, sb;
   TORCH_CHECK(d == 64 || d == 128, "attention supports head_dim 64 and 128, got ", d);
@@ -518,15 +520,19 @@ mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, c
   c.scale = (float)scale;
   if (rows.has_value()) {
     const int64_t n_t = (S + 127) / 128;
-    TORCH_CHECK(qstat.has_value() && krange.has_value(), "attention: incomplete plan");
-    for (const Tensor* t : {&*rows, &*qstat, &*krange})
+    TORCH_CHECK(qstat.has_value() && krange.has_value() && order.has_value(), "attention: incomplete plan");
+    for (const Tensor* t : {&*rows, &*qstat, &*krange, &*order})
       TORCH_CHECK(t->device() == qkv.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
                   "attention: the plan must be on qkv's device");
-    TORCH_CHECK(rows->numel() == B * n_t * 256 && qstat->numel() == B * n_t * 4 && krange->numel() == B * n_t * 2,
+    TORCH_CHECK(rows->numel() == B * n_t * 256 && qstat->numel() == B * n_t * 4 && krange->numel() == B * n_t * 2 &&
+                    order->numel() == B * ((n_t + 1) / 2 + 2 * n_t),
                 "attention: the plan was made for other rows than qkv's [", B, ", ", S, "]");
     c.rows = rows->data_ptr<int>();
     c.qstat = qstat->data_ptr<int>();
     c.krange = krange->data_ptr<int>();
+    c.order_p = order->data_ptr<int>();
+    c.order_q = c.order_p + B * ((n_t + 1) / 2);
+    c.order_k = c.order_q + B * n_t;
   }
   if (slopes.has_value()) {
     TORCH_CHECK(slopes->device() == qkv.device() && slopes->scalar_type() == at::kFloat && slopes->is_contiguous() &&
@@ -539,9 +545,10 @@ mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, c
 
 std::vector<Tensor> masked_attn_fwd(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d,
                                     const c10::optional<Tensor>& rows, const c10::optional<Tensor>& qstat,
-                                    const c10::optional<Tensor>& krange, const c10::optional<Tensor>& slopes,
+                                    const c10::optional<Tensor>& krange, const c10::optional<Tensor>& order,
+                       const c10::optional<Tensor>& slopes,
                                     double cap, double scale) {
-  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, rows, qstat, krange, slopes, cap, scale);
+  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, rows, qstat, krange, order, slopes, cap, scale);
   const at::cuda::CUDAGuard guard(qkv.device());
   Tensor out = at::empty({c.B, c.S, nh * d}, qkv.options());
   Tensor lse = at::empty({c.B, nh, c.S}, qkv.options().dtype(at::kFloat));
@@ -553,9 +560,10 @@ std::vector<Tensor> masked_attn_fwd(const Tensor& qkv, int64_t nh, int64_t nkv, 
 
 Tensor masked_attn_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, const Tensor& lse, int64_t nh,
                        int64_t nkv, int64_t d, const c10::optional<Tensor>& rows, const c10::optional<Tensor>& qstat,
-                       const c10::optional<Tensor>& krange, const c10::optional<Tensor>& slopes, double cap,
+                       const c10::optional<Tensor>& krange, const c10::optional<Tensor>& order,
+                       const c10::optional<Tensor>& slopes, double cap,
                        double scale) {
-  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, rows, qstat, krange, slopes, cap, scale);
+  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, rows, qstat, krange, order, slopes, cap, scale);
   const at::cuda::CUDAGuard guard(qkv.device());
   int64_t do_ss, do_sb;
   token_strides(dout, "dctx", do_ss, do_sb);
@@ -572,7 +580,11 @@ Tensor masked_attn_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out,
   MMB_CHECK_RC(mmb::masked_attn_dq(c, dout.data_ptr(), do_ss, do_sb, out.data_ptr(), lse.data_ptr<float>(),
                                    ld.data_ptr<float>(), dqkv.data_ptr(), error_word(), num_sms(), cur_stream()),
                "masked_attn_dq");
-  MMB_CHECK_RC(mmb::masked_attn_dkv(c, dout.data_ptr(), do_ss, do_sb, ld.data_ptr<float>(), dqkv.data_ptr(),
+  const int parts = mmb::masked_attn_dkv_parts(c.B, c.S, c.nh, c.nkv, num_sms());
+  Tensor partial;
+  if (parts > 1) partial = at::empty({parts, c.B, c.S, 2 * nkv * d}, lse.options());
+  MMB_CHECK_RC(mmb::masked_attn_dkv(c, dout.data_ptr(), do_ss, do_sb, ld.data_ptr<float>(),
+                                    parts > 1 ? partial.data_ptr<float>() : nullptr, parts, dqkv.data_ptr(),
                                     error_word(), num_sms(), cur_stream()),
                "masked_attn_dkv");
   return dqkv;
@@ -1083,11 +1095,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("interleaved"), py::arg("head_dim"), py::arg("rotary_dim"), py::arg("num_heads"),
         py::arg("inverse") = false);
   m.def("masked_attn_fwd", &masked_attn_fwd, py::arg("qkv"), py::arg("num_heads"), py::arg("num_kv_heads"),
-        py::arg("head_dim"), py::arg("rows"), py::arg("qstat"), py::arg("krange"), py::arg("slopes"), py::arg("cap"),
+        py::arg("head_dim"), py::arg("rows"), py::arg("qstat"), py::arg("krange"), py::arg("order"), py::arg("slopes"), py::arg("cap"),
         py::arg("scale"));
   m.def("masked_attn_bwd", &masked_attn_bwd, py::arg("dctx"), py::arg("qkv"), py::arg("ctx"), py::arg("lse"),
         py::arg("num_heads"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("rows"), py::arg("qstat"),
-        py::arg("krange"), py::arg("slopes"), py::arg("cap"), py::arg("scale"));
+        py::arg("krange"), py::arg("order"), py::arg("slopes"), py::arg("cap"), py::arg("scale"));
   m.def("flash_attn_fwd", &flash_attn_fwd);
   m.def("flash_attn_fwd_v1", &flash_attn_fwd_v1, "previous one-tile-per-CTA forward (comparison only)");
   m.def("flash_attn_bwd", &flash_attn_bwd);

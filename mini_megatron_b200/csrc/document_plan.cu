@@ -294,15 +294,84 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
   if (n_cta > 1) cluster_sync_all();  // no CTA leaves while its s_cta may still be read
 }
 
+// Order in which the attention kernels take the tiles of all rows, heaviest first: a persistent grid hands tiles out
+// in rounds, so the long ones have to come first and neighbours in a round be alike.  Counting sort by weight (key or
+// query tiles to visit), one CTA for each of: pairs of query tiles, query tiles, key tiles.  The order of equals is
+// left open; it changes when a tile is computed, not what is computed.
+constexpr int kBins = 2048;
+struct OrderArgs {
+  const int4* qstat;
+  const int2* krange;
+  int B, n_t, n_pairs, shift;  // weight >> shift < kBins
+  int* out[3];
+};
+
+__device__ __forceinline__ int tile_weight(const OrderArgs& a, int b, int t) {
+  const int4 q = a.qstat[(size_t)b * a.n_t + t];
+  return q.y == 0 ? 0 : (q.y + 127) / 128 - q.x / 128;
+}
+
+__global__ void __launch_bounds__(kThreads) plan_order_kernel(const OrderArgs a) {
+  __shared__ int s_bin[kBins];
+  __shared__ int s_warp[32];
+  const int which = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = which == 0 ? a.n_pairs : a.n_t;
+  const int n = a.B * per;
+  auto bin = [&](int e) {  // heaviest first
+    const int b = e / per, t = e - b * per;
+    int w;
+    if (which == 0) {
+      const int t1 = (a.n_t & 1) ? 2 * t : 2 * t + 1;
+      w = tile_weight(a, b, t1) + (t1 > 0 ? tile_weight(a, b, t1 - 1) : 0);
+    } else if (which == 1) {
+      w = tile_weight(a, b, t);
+    } else {
+      const int2 r = a.krange[(size_t)b * a.n_t + t];
+      w = max(0, r.y + 1 - r.x);
+    }
+    return kBins - 1 - (w >> a.shift);
+  };
+  for (int k = tid; k < kBins; k += kThreads) s_bin[k] = 0;
+  __syncthreads();
+  for (int e = tid; e < n; e += kThreads) atomicAdd(&s_bin[bin(e)], 1);
+  __syncthreads();
+  // exclusive scan over the bins, two to a thread
+  const int c0 = s_bin[2 * tid], c1 = s_bin[2 * tid + 1];
+  int v = c0 + c1;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) s_warp[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    int w = s_warp[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += u;
+    }
+    s_warp[lane] = w;
+  }
+  __syncthreads();
+  const int base = v - c0 - c1 + (warp > 0 ? s_warp[warp - 1] : 0);
+  s_bin[2 * tid] = base;
+  s_bin[2 * tid + 1] = base + c0;
+  __syncthreads();
+  for (int e = tid; e < n; e += kThreads) a.out[which][atomicAdd(&s_bin[bin(e)], 1)] = e;
+}
+static_assert(kBins == 2 * kThreads, "two bins to a thread");
+
 }  // namespace docplan
 
 int document_plan_max_len() { return docplan::kMaxCtas * docplan::kMaxSteps * docplan::kStep; }
 
 int document_plan(const long* ids, long ld_ids, long eod, int by_change, const unsigned char* marks, long ld_marks,
                   const int* lengths, int B, int S, int* positions, int* start, int* end, int* rows, void* qstat,
-                  void* krange, cudaStream_t stream) {
+                  void* krange, int* order, cudaStream_t stream) {
   using namespace docplan;
-  if (B < 1 || S < 1 || S > document_plan_max_len()) return -1;
+  if (B < 1 || S < 1 || S > document_plan_max_len() || (long)B * ((S + 127) / 128) > INT_MAX / 8) return -1;
   Args a;
   a.ids = ids;
   a.ld_ids = ld_ids;
@@ -335,7 +404,21 @@ int document_plan(const long* ids, long ld_ids, long eod, int by_change, const u
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, document_plan_kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, document_plan_kernel, a);
+  if (e != cudaSuccess || !order) return (int)e;
+  OrderArgs o;
+  o.qstat = a.qstat;
+  o.krange = a.krange;
+  o.B = B;
+  o.n_t = a.n_t;
+  o.n_pairs = (a.n_t + 1) / 2;
+  o.shift = 0;
+  while ((2 * a.n_t) >> o.shift >= kBins) ++o.shift;
+  o.out[0] = order;
+  o.out[1] = order + (size_t)B * o.n_pairs;
+  o.out[2] = o.out[1] + (size_t)B * a.n_t;
+  plan_order_kernel<<<3, kThreads, 0, stream>>>(o);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace mmb

@@ -29,6 +29,7 @@ struct Mask {
   const int* rows;     // [B, n_t, 2, 128] start, end (tile-padded), nullptr: causal
   const int4* qstat;   // [B, n_t] {min start, max end, max start, min end}
   const int2* krange;  // [B, n_t] {first, last} query tile
+  const int* order;    // this kernel's tiles of all rows, heaviest first, or nullptr: by position
 };
 
 // Key tiles [x, y) that query tile t of row b needs.
@@ -53,11 +54,38 @@ __device__ __forceinline__ int2 query_tiles(const Mask& m, int b, int n_t, int k
   return make_int2(r.x, max(r.x, r.y + 1));
 }
 
-// Work item of CTA `c` in round `r`: every other round runs backwards over the CTAs, so that
-// with items sorted by weight the CTA with the heaviest item of one round takes the lightest of the next.
+// Item of this CTA in round `r`: every other round runs backwards over the CTAs, so that with items
+// sorted by weight the CTA with the heaviest item of one round takes the lightest of the next.
 __device__ __forceinline__ int snake_item(int r) {
   return r * (int)gridDim.x + ((r & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
 }
+
+// n / d for 0 <= n < 2^31 by a multiplication (the round-up method: m = ceil(2^(31 + l) / d), 2^(l-1) < d <= 2^l).
+struct FastDiv {
+  uint32_t m, l, d;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : l(0), d(div) {
+    while ((1ull << l) < div) ++l;
+    m = (uint32_t)(((1ull << (31 + l)) + div - 1) / div);
+  }
+  __device__ __forceinline__ int quot(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> (31 + l)); }
+};
+
+// Work items travel from one scheduling thread to the roles through a ring in shared memory: decoding an item
+// (divisions, loads of the mask's tile tables) takes about a thousand cycles, which every role would otherwise
+// spend between two items.
+constexpr int kRing = 4;
+template <typename Item>
+struct Ring {
+  Item* items;
+  uint64_t* full;   // [kRing] 1 arrival
+  uint64_t* empty;  // [kRing] one arrival per consumer
+  // consumer side, item number k: a whole warp / one thread
+  __device__ __forceinline__ bool get_warp(Item& w, int k, int* err, volatile int* abort_flag) const;
+  __device__ __forceinline__ bool get_thread(Item& w, int k, int* err, volatile int* abort_flag) const;
+  // producer side
+  __device__ __forceinline__ bool put(const Item& w, int k, int* err, volatile int* abort_flag) const;
+};
 
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
@@ -94,16 +122,22 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&d);
 }
 
+__device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
+__device__ __forceinline__ float2 pair(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float2 pair(uint32_t a, uint32_t b) {
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+
 // Constants of the score transform.
 struct Score {
   float mul;  // plain: s log2 e;  capped: 2 s log2 e / cap (the exponent of e^{2u} in log2 units)
   float cap;  // C
 };
 
-template <bool CAP>
-__device__ __forceinline__ float score(float s, const Score& k) {
-  if constexpr (CAP) return fmaf(-2.f * k.cap, rcp_approx(1.f + fast_exp2(s * k.mul)), k.cap);
-  return s * k.mul;
+// 1 / (1 + e^{2u}) of a pair of scores; C tanh u = C - 2 C z, 1 - tanh^2 u = 4 z (1 - z).
+__device__ __forceinline__ float2 cap_z(float2 s, const Score& k) {
+  const float2 e = add2(exp2_pair(mul2(s, pair(k.mul))), pair(1.f));
+  return make_float2(rcp_approx(e.x), rcp_approx(e.y));
 }
 
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -160,6 +194,29 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
   const unsigned long long t0 = globaltimer();
   while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < 20000000ull) {
   }
+}
+
+template <typename Item>
+__device__ __forceinline__ bool Ring<Item>::get_thread(Item& w, int k, int* err, volatile int* abort_flag) const {
+  if (!bwait(&full[k % kRing], (k / kRing) & 1, err, abort_flag)) return false;
+  w = items[k % kRing];
+  mbar_arrive(&empty[k % kRing]);
+  return true;
+}
+template <typename Item>
+__device__ __forceinline__ bool Ring<Item>::get_warp(Item& w, int k, int* err, volatile int* abort_flag) const {
+  if (!wwait(&full[k % kRing], (k / kRing) & 1, err, abort_flag)) return false;
+  w = items[k % kRing];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&empty[k % kRing]);
+  return true;
+}
+template <typename Item>
+__device__ __forceinline__ bool Ring<Item>::put(const Item& w, int k, int* err, volatile int* abort_flag) const {
+  if (k >= kRing && !bwait(&empty[k % kRing], ((k / kRing) - 1) & 1, err, abort_flag)) return false;
+  items[k % kRing] = w;
+  mbar_arrive(&full[k % kRing]);
+  return true;
 }
 
 // One arrival per warp on `bar`, after every lane's tcgen05 loads / stores are ordered before it.

@@ -37,9 +37,11 @@ struct Cfg {
   static constexpr int SB = (D == 64) ? 2 : 1;  // S^T buffers in TMEM
   static constexpr int K_OFF = 0;               // [KB][K, V]
   static constexpr int Q_OFF = KB * 2 * TILE;   // [NQ][Q, dO]
-  static constexpr int LD_OFF = Q_OFF + NQ * 2 * TILE;  // [NQ][LSE log2 e 128, Delta 128, start 128, end 128]
-  static constexpr int BAR_OFF = LD_OFF + NQ * 2048;
-  static constexpr int SMEM = 1024 + BAR_OFF + 256;
+  // [NQ][-LSE log2 e 128, -Delta 128, start 128, end 128, {min start, max end, max start, min end}]
+  static constexpr int LD_OFF = Q_OFF + NQ * 2 * TILE, LD = 2176;
+  static constexpr int ITEM_OFF = LD_OFF + NQ * LD;  // [kRing] work items
+  static constexpr int BAR_OFF = ITEM_OFF + kRing * 32;
+  static constexpr int SMEM = 1024 + BAR_OFF + 320;
   static constexpr uint32_t T_S = 0, T_DP = SB * 128, T_DV = T_DP + 128, T_DK = T_DV + D;
 };
 static_assert(Cfg<128>::SMEM <= 227 * 1024 && Cfg<64>::SMEM <= 227 * 1024, "shared memory of one CTA");
@@ -47,61 +49,72 @@ static_assert(Cfg<128>::T_DK + 128 <= 512 && Cfg<64>::T_DK + 64 <= 512, "TMEM co
 
 struct Args {
   int B, S, nh, nkv, n_t;
+  int parts, heads;     // an item's share: `heads` = nh / nkv / parts query heads
+  FastDiv by_parts, by_nkv, by_B, by_tiles;
   Mask mask;
   const float* slopes;
   Score score;
   float scale;
   const float* ld;      // [B, nh, n_t, 2, 128]
   __nv_bfloat16* dqkv;  // [B, S, (nh + 2 nkv) * D]
+  float* partial;       // parts > 1: [parts, B, S, 2 nkv * D] sums of each share
   int* err;
 };
 
-struct Item {
-  int b, hk, t;
-  int2 r;  // query tiles
+struct alignas(16) Item {
+  int b, hk, t;  // b < 0: no more items
+  int part;      // which share of the K/V head's query heads
+  int2 r;        // query tiles
 };
+static_assert(sizeof(Item) <= 32, "ring entry");
+constexpr int kConsumers = 1 + 1 + kWarps;  // TMA and MMA threads, softmax warps
 
 __device__ __forceinline__ Item decode(const Args& a, int item) {
-  const int BH = a.B * a.nkv;
+  const int q = a.by_parts.quot(item);
+  const int li = a.by_nkv.quot(q);
   Item it;
-  it.t = item / BH;  // causal rows: the first key tile is seen by the most queries
-  const int bh = item - it.t * BH;
-  it.b = bh / a.nkv;
-  it.hk = bh - it.b * a.nkv;
+  it.part = item - q * a.parts;
+  it.hk = q - li * a.nkv;
+  if (a.mask.order) {
+    const int e = a.mask.order[li];
+    it.b = a.by_tiles.quot(e);
+    it.t = e - it.b * a.n_t;
+  } else {  // causal rows: the first key tile is seen by the most queries
+    it.t = a.by_B.quot(li);
+    it.b = li - it.t * a.B;
+  }
   it.r = query_tiles(a.mask, it.b, a.n_t, it.t);
   return it;
 }
 
-// (head of the group, query tile) pairs of this CTA's items, one after another.
+// (head of the item's share, query tile) pairs of this CTA's items, one after another.
 struct Walk {
-  int round = -1, it = -1, g = 0, i = 0;
+  int k = 0, it = -1, g = 0, i = 0;  // it: items with queries so far
   Item w;
-  bool valid = true;
-  __device__ __forceinline__ void next(const Args& a, int n_items, int group) {
-    if (round >= 0) {
-      if (++i < w.r.y) return;
-      if (++g < group) {
+  bool started = false;
+  // 1: at the next pair, 0: no more, -1: the wait for an item ran out
+  __device__ __forceinline__ int next(const Ring<Item>& ring, int heads, int* err, volatile int* abort_flag) {
+    if (started) {
+      if (++i < w.r.y) return 1;
+      if (++g < heads) {
         i = w.r.x;
-        return;
+        return 1;
       }
     }
+    started = true;
     while (true) {
-      const int item = snake_item(++round);
-      if (item >= n_items) {
-        valid = false;
-        return;
-      }
-      w = decode(a, item);
+      if (!ring.get_thread(w, k++, err, abort_flag)) return -1;
+      if (w.b < 0) return 0;
       if (w.r.x < w.r.y) {
         g = 0;
         i = w.r.x;
         ++it;
-        return;
+        return 1;
       }
     }
   }
   __device__ __forceinline__ bool first() const { return g == 0 && i == w.r.x; }
-  __device__ __forceinline__ bool last(int group) const { return g == group - 1 && i == w.r.y - 1; }
+  __device__ __forceinline__ bool last(int heads) const { return g == heads - 1 && i == w.r.y - 1; }
 };
 
 template <int D, bool CAP, bool BIAS>
@@ -132,12 +145,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* g_free = bars + 16;    // ... read (16 warps)
   uint64_t* drain = bars + 17;
   uint64_t* out_full = bars + 20;  // dK, dV of an item staged (16 warps)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);  // bars + 21 ..: the ring of work items
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_items = a.B * a.nkv * a.n_t;
-  const int group = a.nh / a.nkv;
+  const Ring<Item> ring{reinterpret_cast<Item*>(smem + C::ITEM_OFF), bars + 21, bars + 21 + kRing};
+  const int heads = a.heads;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -149,6 +162,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 3; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&bars[21 + i], 1);
+      mbar_init(&bars[21 + kRing + i], kConsumers);
     }
     mbar_init(dp_full, 1);
     mbar_init(ds_full, kWarps);
@@ -180,7 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         int n = 0, kv_issued = -1;
         bool ok = true;
         Walk x;
-        for (x.next(a, n_items, group); x.valid; x.next(a, n_items, group), ++n) {
+        for (int got; (got = x.next(ring, heads, a.err, abort_flag)) != 0; ++n) {
+          if (got < 0) { ok = false; break; }
           if (x.first()) {
             const int kb = x.it % KB;
             if (x.it >= KB && !bwait(&kv_empty[kb], ((x.it / KB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
@@ -192,14 +210,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const int st = n % NQ;
           if (n >= NQ && !bwait(&q_empty[st], ((n / NQ) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-          const int h = x.w.hk * group + x.g;
-          mbar_expect_tx(&q_full[st], 2 * C::TILE + 1024 + (a.mask.rows ? 1024 : 0));
+          const int h = (x.w.hk * a.parts + x.w.part) * heads + x.g;
+          mbar_expect_tx(&q_full[st], 2 * C::TILE + 1024 + (a.mask.rows ? 1040 : 0));
           load_tile<D>(sQ + st * 2 * C::TILE, &tm_qkv, &q_full[st], h * D, x.i * BT, x.w.b);
           load_tile<D>(sQ + st * 2 * C::TILE + C::TILE, &tm_do, &q_full[st], h * D, x.i * BT, x.w.b);
-          bulk_load(sLD + st * 2048, a.ld + (((size_t)x.w.b * a.nh + h) * a.n_t + x.i) * (2 * BT), 1024, &q_full[st]);
-          if (a.mask.rows)
-            bulk_load(sLD + st * 2048 + 1024, a.mask.rows + ((size_t)x.w.b * a.n_t + x.i) * (2 * BT), 1024,
-                      &q_full[st]);
+          bulk_load(sLD + st * C::LD, a.ld + (((size_t)x.w.b * a.nh + h) * a.n_t + x.i) * (2 * BT), 1024, &q_full[st]);
+          if (a.mask.rows) {
+            const size_t bt = (size_t)x.w.b * a.n_t + x.i;
+            bulk_load(sLD + st * C::LD + 1024, a.mask.rows + bt * (2 * BT), 1024, &q_full[st]);
+            bulk_load(sLD + st * C::LD + 2048, a.mask.qstat + bt, 16, &q_full[st]);
+          }
         }
         if (!ok) {
           for (int u = max(0, kv_issued - KB + 1); u <= kv_issued; ++u) drain_wait(&kv_full[u % KB], (u / KB) & 1);
@@ -229,16 +249,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                      smem_u32(sQ + (u % NQ) * 2 * C::TILE + C::TILE));
           umma_commit(dp_full);
         };
-        nxt.next(a, n_items, group);
-        if (nxt.valid) {
+        int more = nxt.next(ring, heads, a.err, abort_flag);
+        ok = more >= 0;
+        if (more > 0) {
           ok = issue_s(nxt, 0);
           if (ok) issue_dp(nxt, 0);
         }
-        while (ok && nxt.valid) {
+        while (ok && more) {
           cur = nxt;
-          nxt.next(a, n_items, group);
+          more = nxt.next(ring, heads, a.err, abort_flag);
+          if (more < 0) { ok = false; break; }
           // one K / V buffer: the next item's tiles can only be loaded once this item's products are done
-          const bool early = nxt.valid && (KB == 2 || nxt.it == cur.it);
+          const bool early = more && (KB == 2 || nxt.it == cur.it);
           const uint32_t q_addr = smem_u32(sQ + (n % NQ) * 2 * C::TILE);
           if (SB == 2 && early && !issue_s(nxt, n + 1)) { ok = false; break; }
           if (!bwait(&p_full[n & 1], (n >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
@@ -250,16 +272,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           mma_tmem_b<D, 32>(tmem + C::T_DK, tmem + C::T_DP, q_addr, !cur.first());
           umma_commit(&q_empty[n % NQ]);
-          if (cur.last(group)) {
+          if (cur.last(heads)) {
             umma_commit(g_full);  // K and V become the staging tiles of dK and dV, whose store releases them
           }
-          if (nxt.valid && !early && !issue_s(nxt, n + 1)) { ok = false; break; }
-          if (nxt.valid) issue_dp(nxt, n + 1);  // over dS^T, in issue order after dK
+          if (more && !early && !issue_s(nxt, n + 1)) { ok = false; break; }
+          if (more) issue_dp(nxt, n + 1);  // over dS^T, in issue order after dK
           ++n;
         }
         if (!ok) {
           umma_commit(drain);
           drain_wait(drain, 0);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 2) {
+      if (elect_one()) {
+        // -------------------------------------------------------------- work items
+        const int n_items = a.B * a.nkv * a.n_t * a.parts;
+        Item w;
+        for (int r = 0, item;; ++r) {
+          item = snake_item(r);
+          if (item < n_items) w = decode(a, item);
+          else w.b = -1;
+          if (!ring.put(w, r, a.err, abort_flag) || w.b < 0) break;
         }
       }
       __syncwarp();
@@ -273,34 +308,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Score k = a.score;
     int n = 0, it = 0;
     bool ok = true;
-    for (int r = 0, item; ok && (item = snake_item(r)) < n_items; ++r) {
-      const Item w = decode(a, item);
+    Item w;
+    for (int u = 0; ok && (ok = ring.get_warp(w, u, a.err, abort_flag)) && w.b >= 0; ++u) {
       const int key = w.t * BT + row;
       const bool in = key < a.S;
-      const size_t width = (size_t)(a.nh + 2 * a.nkv) * D;
-      __nv_bfloat16* dk = a.dqkv + ((size_t)w.b * a.S + key) * width + (size_t)(a.nh + w.hk) * D + part * (D / 4);
-      __nv_bfloat16* dv = dk + (size_t)a.nkv * D;
+      // a share's sums: dK and dV of this warp's columns, [parts, B, S, 2 nkv * D]
+      auto share_row = [&]() {
+        return a.partial + (((size_t)w.part * a.B + w.b) * a.S + key) * ((size_t)2 * a.nkv * D) + (size_t)w.hk * D +
+               part * (D / 4);
+      };
       if (w.r.x >= w.r.y) {
-        if (in) {
+        if (in && a.parts > 1) {
+          float* pk = share_row();
+#pragma unroll
+          for (int c = 0; c < D / 4; c += 4) {
+            *reinterpret_cast<float4*>(pk + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(pk + (size_t)a.nkv * D + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        } else if (in) {
+          __nv_bfloat16* dk = a.dqkv + ((size_t)w.b * a.S + key) * ((size_t)(a.nh + 2 * a.nkv) * D) +
+                              (size_t)(a.nh + w.hk) * D + part * (D / 4);
+          __nv_bfloat16* dv = dk + (size_t)a.nkv * D;
           store_zero<D / 4>(dk);
           store_zero<D / 4>(dv);
         }
         continue;
       }
-      for (int g = 0; ok && g < group; ++g) {
+      for (int g = 0; ok && g < heads; ++g) {
         float slope = 0.f;
-        if (BIAS) slope = a.slopes[w.hk * group + g] * kLog2e;
+        if (BIAS) slope = a.slopes[(w.hk * a.parts + w.part) * heads + g] * kLog2e;
         for (int i = w.r.x; i < w.r.y; ++i, ++n) {
           const int st = n % NQ;
-          const int2 full = full_tiles(a.mask, w.b, a.n_t, i);
-          const bool masked = w.t < full.x || w.t >= full.y;
           const uint32_t t_s = tmem + C::T_S + (n % SB) * 128 + lane_off + part * 32;
           const uint32_t t_dp = tmem + C::T_DP + lane_off + part * 32;
-          const float* l2 = reinterpret_cast<const float*>(sLD + st * 2048) + part * 32;
+          const float* l2 = reinterpret_cast<const float*>(sLD + st * C::LD) + part * 32;
           const int* start = reinterpret_cast<const int*>(l2 + 2 * BT);
           if (!wwait(&q_full[st], (n / NQ) & 1, a.err, abort_flag)) { ok = false; break; }
           if (!wwait(&s_full[n % SB], (n / SB) & 1, a.err, abort_flag)) { ok = false; break; }
           tc_fence_after();
+          bool masked = i == w.t;  // causal: only the diagonal tile
+          if (a.mask.rows) {
+            const int4 q = *reinterpret_cast<const int4*>(sLD + st * C::LD + 2048);
+            masked = q.z > w.t * BT || q.w < (w.t + 1) * BT;
+          }
           float pf[32];  // P (1 - tanh^2)
           {
             uint32_t s[32];
@@ -330,27 +380,32 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e4 = 0; e4 < 32; e4 += 4) {
               const float4 lv = *reinterpret_cast<const float4*>(l2 + e4);
-              const float ls[4] = {lv.x, lv.y, lv.z, lv.w};
-              float pr[4];
 #pragma unroll
-              for (int u = 0; u < 4; ++u) {
+              for (int u = 0; u < 4; u += 2) {
                 const int e = e4 + u;
-                float x, f = 1.f;
+                float2 x = pair(s[e], s[e + 1]), f;
+                const float2 ls = u == 0 ? make_float2(lv.x, lv.y) : make_float2(lv.z, lv.w);
                 if (CAP) {
-                  const float z = rcp_approx(1.f + fast_exp2(__uint_as_float(s[e]) * k.mul));
-                  x = fmaf(-2.f * k.cap, z, k.cap);
-                  f = 4.f * z * (1.f - z);  // 1 - tanh^2
+                  const float2 z = cap_z(x, k);
+                  x = fma2(z, pair(-2.f * k.cap), pair(k.cap));
+                  f = mul2(mul2(z, pair(4.f)), fma2(z, pair(-1.f), pair(1.f)));  // 1 - tanh^2
                 }
-                if (BIAS) x = fmaf(-slope, fabsf(dist + (float)e), CAP ? x : __uint_as_float(s[e]) * k.mul);
-                float p;
-                if (CAP || BIAS) p = fast_exp2(x - ls[u]);
-                else p = fast_exp2(fmaf(__uint_as_float(s[e]), k.mul, -ls[u]));
-                if (masked && !(seen & (1u << e))) p = 0.f;
-                pr[u] = p;
-                pf[e] = CAP ? p * f : p;
+                if (BIAS) {
+                  if (!CAP) x = mul2(x, pair(k.mul));
+                  x.x = fmaf(-slope, fabsf(dist + (float)e), x.x);
+                  x.y = fmaf(-slope, fabsf(dist + (float)(e + 1)), x.y);
+                }
+                x = (CAP || BIAS) ? add2(x, ls) : fma2(x, pair(k.mul), ls);
+                x = exp2_pair(x);
+                if (masked) {
+                  if (!(seen & (1u << e))) x.x = 0.f;
+                  if (!(seen & (2u << e))) x.y = 0.f;
+                }
+                pp[e / 2] = pack_bf16x2(x.x, x.y);
+                if (CAP) x = mul2(x, f);
+                pf[e] = x.x;
+                pf[e + 1] = x.y;
               }
-              pp[e4 / 2] = pack_bf16x2(pr[0], pr[1]);
-              pp[e4 / 2 + 1] = pack_bf16x2(pr[2], pr[3]);
             }
             tmem_st_32x32b_x16(t_s, pp);  // over S^T columns already read
           }
@@ -367,10 +422,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e4 = 0; e4 < 32; e4 += 4) {
               const float4 dl = *reinterpret_cast<const float4*>(delta + e4);
-              ds[e4 / 2] = pack_bf16x2(pf[e4] * (__uint_as_float(dp[e4]) - dl.x),
-                                       pf[e4 + 1] * (__uint_as_float(dp[e4 + 1]) - dl.y));
-              ds[e4 / 2 + 1] = pack_bf16x2(pf[e4 + 2] * (__uint_as_float(dp[e4 + 2]) - dl.z),
-                                           pf[e4 + 3] * (__uint_as_float(dp[e4 + 3]) - dl.w));
+              const float2 v = mul2(make_float2(pf[e4], pf[e4 + 1]), add2(pair(dp[e4], dp[e4 + 1]), make_float2(dl.x, dl.y)));
+              const float2 z = mul2(make_float2(pf[e4 + 2], pf[e4 + 3]),
+                                    add2(pair(dp[e4 + 2], dp[e4 + 3]), make_float2(dl.z, dl.w)));
+              ds[e4 / 2] = pack_bf16x2(v.x, v.y);
+              ds[e4 / 2 + 1] = pack_bf16x2(z.x, z.y);
             }
             tmem_st_32x32b_x16(t_dp, ds);  // over dP^T columns already read
           }
@@ -388,16 +444,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
         warp_arrive(g_free);
         uint8_t* stg = sKV + (it % KB) * 2 * C::TILE;
-        stage_row(stg, 16384, row, part * (D / 4), u, a.scale);
-        stage_row(stg + C::TILE, 16384, row, part * (D / 4), v, 1.f);
-        fence_proxy_async_smem();
+        if (a.parts > 1) {
+          if (in) {
+            float* pk = share_row();
+#pragma unroll
+            for (int c = 0; c < D / 4; c += 4) {
+              *reinterpret_cast<float4*>(pk + c) =
+                  make_float4(__uint_as_float(u[c]) * a.scale, __uint_as_float(u[c + 1]) * a.scale,
+                              __uint_as_float(u[c + 2]) * a.scale, __uint_as_float(u[c + 3]) * a.scale);
+              *reinterpret_cast<float4*>(pk + (size_t)a.nkv * D + c) =
+                  make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
+                              __uint_as_float(v[c + 3]));
+            }
+          }
+        } else {
+          stage_row(stg, 16384, row, part * (D / 4), u, a.scale);
+          stage_row(stg + C::TILE, 16384, row, part * (D / 4), v, 1.f);
+          fence_proxy_async_smem();
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(out_full);
         if (warp == 4) {
           if (!wwait(out_full, it & 1, a.err, abort_flag)) { ok = false; break; }
           if (lane == 0) {
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
+            for (int c = 0; c < (a.parts > 1 ? 0 : D / 64); ++c) {
               tma_store_3d(&tm_dqkv, stg + c * 16384, (a.nh + w.hk) * D + c * 64, w.t * BT, w.b);
               tma_store_3d(&tm_dqkv, stg + C::TILE + c * 16384, (a.nh + a.nkv + w.hk) * D + c * 64, w.t * BT, w.b);
             }
@@ -431,14 +502,48 @@ int launch(const CUtensorMap& tq, const CUtensorMap& to, const CUtensorMap& td, 
   return (int)cudaGetLastError();
 }
 
+// dK and dV of a token = the shares' sums, added in order and rounded once.
+__global__ void join_parts_kernel(const float* __restrict__ partial, int parts, long stride, long tokens, int width,
+                                  __nv_bfloat16* __restrict__ dqkv, long ld, long col0) {
+  pdl_trigger();
+  pdl_wait();
+  const long n = tokens * (width / 8);
+  for (long u = blockIdx.x * (long)blockDim.x + threadIdx.x; u < n; u += (long)gridDim.x * blockDim.x) {
+    const long tok = u / (width / 8);
+    const int c = (int)(u - tok * (width / 8)) * 8;
+    const float* p = partial + tok * width + c;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    for (int k = 0; k < parts; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(p + k * stride), w = *reinterpret_cast<const float4*>(p + k * stride + 4);
+      x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+      y = make_float4(y.x + w.x, y.y + w.y, y.z + w.z, y.w + w.w);
+    }
+    *reinterpret_cast<uint4*>(dqkv + tok * ld + col0 + c) =
+        make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w), pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+  }
+}
+
 }  // namespace dkv
 }  // namespace mattn
 
-int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb, const float* ld, void* dqkv, int* err,
-                    int num_sms, cudaStream_t stream) {
+// Few key tiles and shared heads: an item is a share of the K/V head's query heads, so that every SM gets work
+// (about three items each, which leaves the heaviest-first order something to balance); the shares' 32-bit sums are
+// joined afterwards.  One K/V head of 128 key tiles (S = 16384, 4 query heads) took DKVONE us as 128 items and
+// DKVSPLIT us with the join as 512.
+int masked_attn_dkv_parts(int B, int S, int nh, int nkv, int num_sms) {
+  const long items = (long)B * nkv * ((S + mattn::BT - 1) / mattn::BT);
+  const int group = nh / nkv;
+  for (int p = 1; p < group; ++p)
+    if (group % p == 0 && items * p >= 3L * num_sms) return p;
+  return group;
+}
+
+int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb, const float* ld, float* partial,
+                    int parts, void* dqkv, int* err, int num_sms, cudaStream_t stream) {
   using namespace mattn;
   const int n_t = (c.S + BT - 1) / BT;
-  const long items = (long)c.B * c.nkv * n_t;
+  const long items = (long)c.B * c.nkv * n_t * parts;
+  if (parts < 1 || (c.nh / c.nkv) % parts || (parts > 1 && !partial)) return -3;
   if (items > INT_MAX / 2) return -1;
   CUtensorMap tq, to, td;
   int rc = make_tmap_bf16_3d(&tq, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
@@ -454,7 +559,14 @@ int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb,
   a.nh = c.nh;
   a.nkv = c.nkv;
   a.n_t = n_t;
-  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange)};
+  a.parts = parts;
+  a.heads = c.nh / c.nkv / parts;
+  a.by_parts = FastDiv(parts);
+  a.by_nkv = FastDiv(c.nkv);
+  a.by_B = FastDiv(c.B);
+  a.by_tiles = FastDiv(n_t);
+  a.partial = partial;
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange), c.order_k};
   a.slopes = c.slopes;
   score_constants(c.scale, c.cap, &a.score.mul, &a.score.cap);
   a.scale = c.scale;
@@ -464,14 +576,20 @@ int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb,
   const int grid = (int)std::max(1L, std::min(items, (long)num_sms));
   const bool cap = c.cap > 0.f, bias = c.slopes != nullptr;
   if (c.d == 64) {
-    if (cap) return bias ? dkv::launch<64, true, true>(tq, to, td, a, grid, stream) : dkv::launch<64, true, false>(tq, to, td, a, grid, stream);
-    return bias ? dkv::launch<64, false, true>(tq, to, td, a, grid, stream) : dkv::launch<64, false, false>(tq, to, td, a, grid, stream);
+    if (cap) rc = bias ? dkv::launch<64, true, true>(tq, to, td, a, grid, stream) : dkv::launch<64, true, false>(tq, to, td, a, grid, stream);
+    else rc = bias ? dkv::launch<64, false, true>(tq, to, td, a, grid, stream) : dkv::launch<64, false, false>(tq, to, td, a, grid, stream);
+  } else if (c.d == 128) {
+    if (cap) rc = bias ? dkv::launch<128, true, true>(tq, to, td, a, grid, stream) : dkv::launch<128, true, false>(tq, to, td, a, grid, stream);
+    else rc = bias ? dkv::launch<128, false, true>(tq, to, td, a, grid, stream) : dkv::launch<128, false, false>(tq, to, td, a, grid, stream);
+  } else {
+    rc = -2;
   }
-  if (c.d == 128) {
-    if (cap) return bias ? dkv::launch<128, true, true>(tq, to, td, a, grid, stream) : dkv::launch<128, true, false>(tq, to, td, a, grid, stream);
-    return bias ? dkv::launch<128, false, true>(tq, to, td, a, grid, stream) : dkv::launch<128, false, false>(tq, to, td, a, grid, stream);
-  }
-  return -2;
+  if (rc || parts == 1) return rc;
+  const long tokens = (long)c.B * c.S, wid = 2L * c.nkv * c.d;
+  const long units = tokens * (wid / 8);
+  launch_k(dkv::join_parts_kernel, (unsigned)std::min((units + 255) / 256, 8L * num_sms), 256, 0, stream, partial, parts,
+           tokens * wid, tokens, (int)wid, static_cast<__nv_bfloat16*>(dqkv), width, (long)c.nh * c.d);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace mmb

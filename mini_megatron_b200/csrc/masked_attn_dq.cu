@@ -10,15 +10,19 @@
 // pass, and the same inputs give the same bits.  dS is rounded to bf16 once, as
 // the operand of its products.
 //
-// Persistent grid, one CTA per SM; a work item is (batch, head, 128-row query tile).
-// Roles (20 warps):
+// row_stats_kernel: one pass over ctx and dO computes Delta and stores it with LSE, both negated and in the units of
+// the softmax, in an array padded to whole tiles, from which both passes fetch a tile's rows with bulk copies.
+// (Two warps of the query-side kernel computing it for the item ahead kept pace only with batches of loads
+// that took the registers of the softmax warps; as a kernel of its own it is bound by reading ctx and dO.)
 //
-//   warp 0      TMA: Q, dO per item; K_j and V_j into rings
+// masked_attn_dq_kernel: persistent grid, one CTA per SM; a work item is (batch, head, 128-row query tile).
+// Roles (20 warps, one of them idle):
+//
+//   warp 0      TMA: Q, dO and row statistics per item; K_j and V_j into rings
 //   warp 1      TMEM allocation; one thread issues S = Q K_j^T (two TMEM buffers), dP = dO V_j^T
 //               and dQ += dS K_j (dS read from TMEM): S of the next tile before dS of this one is
 //               ready, dP of the next as soon as this one has been read
-//   warps 2-3   Delta and LSE of the next item's rows: into shared memory for the warps below and
-//               into the tile-padded workspace the key side reads with bulk copies
+//   warp 2      hands out the work items
 //   warps 4-19  dS: four warps share 32 query rows, each has 32 of the 128 keys
 //
 // dS overwrites the S columns it came from: every warp's 32 keys start 32 columns apart.
@@ -40,69 +44,73 @@ struct Cfg {
   static constexpr int QB = (D == 64) ? 2 : 1;  // Q / dO buffers
   static constexpr int NK = (D == 64) ? 4 : 3;  // K ring: held from S(j) to dQ(j), one tile longer than V
   static constexpr int NV = (D == 64) ? 4 : 2;
-  static constexpr int SB = QB;                 // row-statistics buffers
   static constexpr int Q_OFF = 0;               // [QB][Q, dO]
   static constexpr int K_OFF = QB * 2 * TILE;
   static constexpr int V_OFF = K_OFF + NK * TILE;
-  static constexpr int ST_OFF = V_OFF + NV * TILE;  // [SB][128] (LSE log2 e, Delta)
-  static constexpr int BAR_OFF = ST_OFF + SB * BT * 8;
-  static constexpr int SMEM = 1024 + BAR_OFF + 384;
+  static constexpr int ST_OFF = V_OFF + NV * TILE;  // [QB][-LSE log2 e 128, -Delta 128]
+  static constexpr int ITEM_OFF = ST_OFF + QB * BT * 8;  // [kRing] work items
+  static constexpr int BAR_OFF = ITEM_OFF + kRing * 32;
+  static constexpr int SMEM = 1024 + BAR_OFF + 352;
   static constexpr uint32_t T_S = 0, T_DP = 256, T_DQ = 384;  // S: two buffers of 128 columns
 };
 static_assert(Cfg<128>::SMEM <= 227 * 1024 && Cfg<64>::SMEM <= 227 * 1024, "shared memory of one CTA");
 
 struct Args {
   int B, S, nh, nkv, n_t;
+  FastDiv by_nh, by_B, by_tiles, by_group;
   Mask mask;
   const float* slopes;
   Score score;
   float scale;
-  const __nv_bfloat16* dout;  // [B, S, nh * D] with strides
-  long do_ss, do_sb;
-  const __nv_bfloat16* out;   // [B, S, nh * D]
-  const float* lse;           // [B, nh, S]
-  float* ld;                  // [B, nh, n_t, 2, 128] LSE log2 e (+inf: the row takes no part), Delta
+  const float* ld;            // [B, nh, n_t, 2, 128] -LSE log2 e (-inf: the row takes no part), -Delta
   __nv_bfloat16* dqkv;        // [B, S, (nh + 2 nkv) * D]
   int* err;
 };
 
-struct Item {
-  int b, h, t;
-  int2 r;  // key tiles
+struct alignas(16) Item {
+  int b, h, t;  // b < 0: no more items
+  int2 r, f;    // key tiles, and those of them that need no mask
 };
+static_assert(sizeof(Item) <= 32, "ring entry");
+constexpr int kConsumers = 1 + 1 + kWarps;  // TMA and MMA threads, softmax warps
 
 __device__ __forceinline__ Item decode(const Args& a, int item) {
-  const int BH = a.B * a.nh;
-  const int p = item / BH, bh = item - p * BH;
+  const int li = a.by_nh.quot(item);
   Item it;
-  it.t = a.n_t - 1 - p;  // causal rows: the longest first
-  it.b = bh / a.nh;
-  it.h = bh - it.b * a.nh;
+  it.h = item - li * a.nh;
+  if (a.mask.order) {
+    const int e = a.mask.order[li];
+    it.b = a.by_tiles.quot(e);
+    it.t = e - it.b * a.n_t;
+  } else {  // causal rows: the longest first
+    const int q = a.by_B.quot(li);
+    it.b = li - q * a.B;
+    it.t = a.n_t - 1 - q;
+  }
   it.r = key_tiles(a.mask, it.b, a.n_t, it.t);
+  it.f = full_tiles(a.mask, it.b, a.n_t, it.t);
   return it;
 }
 
 // The tiles of this CTA one after another, across items (items without keys are skipped).
 struct Walk {
-  int round = -1, it = -1, j = 0;  // it: items with keys so far
+  int k = 0, it = -1, j = 0;  // it: items with keys so far
   Item w;
-  bool valid = true;
-  __device__ __forceinline__ void next(const Args& a, int n_items) {
-    if (round >= 0 && j + 1 < w.r.y) {
+  bool started = false;
+  // 1: at the next tile, 0: no more, -1: the wait for an item ran out
+  __device__ __forceinline__ int next(const Ring<Item>& ring, int* err, volatile int* abort_flag) {
+    if (started && j + 1 < w.r.y) {
       ++j;
-      return;
+      return 1;
     }
+    started = true;
     while (true) {
-      const int item = snake_item(++round);
-      if (item >= n_items) {
-        valid = false;
-        return;
-      }
-      w = decode(a, item);
+      if (!ring.get_thread(w, k++, err, abort_flag)) return -1;
+      if (w.b < 0) return 0;
       if (w.r.x < w.r.y) {
         j = w.r.x;
         ++it;
-        return;
+        return 1;
       }
     }
   }
@@ -116,19 +124,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                           const __grid_constant__ CUtensorMap tm_dqkv, const Args a) {
   pdl_trigger();
   using C = Cfg<D>;
-  constexpr int QB = C::QB, NK = C::NK, NV = C::NV, SB = C::SB;
+  constexpr int QB = C::QB, NK = C::NK, NV = C::NV;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
   uint8_t* sQ = smem + C::Q_OFF;
   uint8_t* sK = smem + C::K_OFF;
   uint8_t* sV = smem + C::V_OFF;
-  float2* sST = reinterpret_cast<float2*>(smem + C::ST_OFF);
+  float* sST = reinterpret_cast<float*>(smem + C::ST_OFF);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint64_t* q_full = bars;            // [2]
   uint64_t* q_empty = bars + 2;       // [2]
-  uint64_t* st_full = bars + 4;       // [2]  row statistics written (2 warps)
-  uint64_t* st_empty = bars + 6;      // [2]  ... read (16 warps)
+  uint64_t* st_empty = bars + 6;      // [2]  row statistics read (16 warps)
   uint64_t* s_full = bars + 8;        // [2]  S computed
   uint64_t* k_full = bars + 10;       // [4]
   uint64_t* k_empty = bars + 14;      // [4]
@@ -139,18 +146,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* dq_full = bars + 28;      // dQ of an item complete
   uint64_t* dq_free = bars + 29;      // ... read (16 warps)
   uint64_t* out_full = bars + 30;     // dQ of an item staged (16 warps)
-  uint64_t* drain = bars + 31;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
+  uint64_t* ring_full = bars + 31;    // [kRing]
+  uint64_t* ring_empty = bars + 35;   // [kRing]
+  uint64_t* drain = bars + 39;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 40);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_items = a.B * a.nh * a.n_t;
+  const Ring<Item> ring{reinterpret_cast<Item*>(smem + C::ITEM_OFF), ring_full, ring_empty};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
-      mbar_init(&st_full[i], 2);
       mbar_init(&st_empty[i], kWarps);
       mbar_init(&s_full[i], 1);
     }
@@ -159,6 +167,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
+    }
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&ring_full[i], 1);
+      mbar_init(&ring_empty[i], kConsumers);
     }
     mbar_init(dp_full, 1);
     mbar_init(ds_full, kWarps);
@@ -181,23 +193,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   pdl_wait();
   const uint32_t tmem = *tmem_slot;
-  const int group = a.nh / a.nkv;
 
   if (warp < 4) {
-    reg_inc<128>();
+    reg_dec<64>();
     if (warp == 0) {
       if (elect_one()) {
         // ---------------------------------------------------------------- TMA
         int n = 0, q_issued = -1, k_issued = 0, v_issued = 0;
         bool ok = true;
         Walk x;
-        for (x.next(a, n_items); x.valid; x.next(a, n_items), ++n) {
-          const int hk = x.w.h / group;
+        for (int got; (got = x.next(ring, a.err, abort_flag)) != 0; ++n) {
+          if (got < 0) { ok = false; break; }
+          const int hk = a.by_group.quot(x.w.h);
           if (x.first()) {
             const int qb = x.it % QB;
             if (x.it >= QB && !bwait(&q_empty[qb], ((x.it / QB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+            if (x.it >= QB && !bwait(&st_empty[qb], ((x.it / QB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
             uint8_t* qd = sQ + qb * 2 * C::TILE;
-            mbar_expect_tx(&q_full[qb], 2 * C::TILE);
+            mbar_expect_tx(&q_full[qb], 2 * C::TILE + 1024);
+            bulk_load(sST + qb * 256, a.ld + (((size_t)x.w.b * a.nh + x.w.h) * a.n_t + x.w.t) * (2 * BT), 1024, &q_full[qb]);
             load_tile<D>(qd, &tm_qkv, &q_full[qb], x.w.h * D, x.w.t * BT, x.w.b);
             load_tile<D>(qd + C::TILE, &tm_do, &q_full[qb], x.w.h * D, x.w.t * BT, x.w.b);
             q_issued = x.it;
@@ -244,14 +258,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (x.last()) umma_commit(&q_empty[qb]);  // every product of this item that reads Q or dO is issued
           return true;
         };
-        nxt.next(a, n_items);
-        if (nxt.valid) ok = issue_s(nxt, 0) && issue_dp(nxt, 0);
-        while (ok && nxt.valid) {
+        int more = nxt.next(ring, a.err, abort_flag);
+        ok = more >= 0 && (more == 0 || (issue_s(nxt, 0) && issue_dp(nxt, 0)));
+        while (ok && more) {
           cur = nxt;
-          nxt.next(a, n_items);
+          more = nxt.next(ring, a.err, abort_flag);
+          if (more < 0) { ok = false; break; }
           // one Q buffer: the next item's Q can only be loaded once this item's products are done with it,
           // and this tile's dQ should not wait for that load
-          const bool early = nxt.valid && (QB == 2 || nxt.it == cur.it);
+          const bool early = more && (QB == 2 || nxt.it == cur.it);
           if (early && !issue_s(nxt, n + 1)) { ok = false; break; }
           if (!bwait(ds_full, n & 1, a.err, abort_flag)) { ok = false; break; }
           if (early && !issue_dp(nxt, n + 1)) { ok = false; break; }
@@ -262,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // the K stage of an item's last tile becomes the staging tile of its dQ, which then releases it
           if (cur.last()) umma_commit(dq_full);
           else umma_commit(&k_empty[n % NK]);
-          if (nxt.valid && !early && !(issue_s(nxt, n + 1) && issue_dp(nxt, n + 1))) { ok = false; break; }
+          if (more && !early && !(issue_s(nxt, n + 1) && issue_dp(nxt, n + 1))) { ok = false; break; }
           ++n;
         }
         if (!ok) {
@@ -271,86 +286,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       __syncwarp();
-    } else {
-      // ------------------------------------------------------------------ row statistics
-      constexpr int G = D / 8;        // lanes per row
-      constexpr int R = 32 / G;       // rows per pass
-      const int part = lane % G, sub = lane / G;
-      Walk x;
-      x.next(a, n_items);
-      while (x.valid) {
-        const Item& w = x.w;
-        const int sb = x.it % SB;
-        if (x.it >= SB && !wwait(&st_empty[sb], ((x.it / SB) - 1) & 1, a.err, abort_flag)) break;
-        const float* lse = a.lse + ((size_t)w.b * a.nh + w.h) * a.S;
-        float* ld = a.ld + (((size_t)w.b * a.nh + w.h) * a.n_t + w.t) * (2 * BT);
-        // 8 passes' loads in flight at once: 64 threads have to keep up with the 8 warps below
-#pragma unroll 1
-        for (int p0 = 0; p0 < 64 / R; p0 += 8) {
-          uint4 u[8], v[8];
-          float l[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = w.t * BT + (warp - 2) * 64 + (p0 + e) * R + sub;
-            u[e] = v[e] = make_uint4(0u, 0u, 0u, 0u);
-            l[e] = -INFINITY;
-            if (i < a.S) {
-              u[e] = *reinterpret_cast<const uint4*>(a.dout + w.b * a.do_sb + i * a.do_ss + w.h * D + part * 8);
-              v[e] = *reinterpret_cast<const uint4*>(a.out + ((size_t)w.b * a.S + i) * ((size_t)a.nh * D) +
-                                                     (size_t)w.h * D + part * 8);
-              l[e] = lse[i];
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int row = (warp - 2) * 64 + (p0 + e) * R + sub;
-            const uint32_t* uw = reinterpret_cast<const uint32_t*>(&u[e]);
-            const uint32_t* vw = reinterpret_cast<const uint32_t*>(&v[e]);
-            float acc = 0.f;
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              const float2 f = unpack_bf16x2(uw[z]), g = unpack_bf16x2(vw[z]);
-              acc = fmaf(f.x, g.x, fmaf(f.y, g.y, acc));
-            }
-#pragma unroll
-            for (int o = G / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-            if (part == 0) {
-              // a row that sees nothing, or lies behind the end, gives no gradient
-              const bool none = l[e] == -INFINITY;
-              const float l2 = none ? INFINITY : l[e] * kLog2e;
-              acc = none ? 0.f : acc;
-              sST[sb * BT + row] = make_float2(l2, acc);
-              ld[row] = l2;
-              ld[BT + row] = acc;
-            }
-          }
+    } else if (warp == 2) {
+      if (elect_one()) {
+        // -------------------------------------------------------------- work items
+        const int n_items = a.B * a.nh * a.n_t;
+        Item w;
+        for (int r = 0, item;; ++r) {
+          item = snake_item(r);
+          if (item < n_items) w = decode(a, item);
+          else w.b = -1;
+          if (!ring.put(w, r, a.err, abort_flag) || w.b < 0) break;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&st_full[sb]);
-        x.j = x.w.r.y - 1;  // on to the next item
-        x.next(a, n_items);
       }
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------------ dS, dQ store
-    reg_dec<88>();
+    reg_inc<104>();
     const int part = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const Score k = a.score;
     int n = 0, it = 0;
     bool ok = true;
-    for (int r = 0, item; ok && (item = snake_item(r)) < n_items; ++r) {
-      const Item w = decode(a, item);
+    Item w;
+    for (int u = 0; ok && (ok = ring.get_warp(w, u, a.err, abort_flag)) && w.b >= 0; ++u) {
       const int i = w.t * BT + row;
-      const bool in = i < a.S;
-      __nv_bfloat16* dst = a.dqkv + ((size_t)w.b * a.S + i) * ((size_t)(a.nh + 2 * a.nkv) * D) + (size_t)w.h * D +
-                           part * (D / 4);
       if (w.r.x >= w.r.y) {
-        if (in) store_zero<D / 4>(dst);
+        if (i < a.S)
+          store_zero<D / 4>(a.dqkv + ((size_t)w.b * a.S + i) * ((size_t)(a.nh + 2 * a.nkv) * D) + (size_t)w.h * D +
+                            part * (D / 4));
         continue;
       }
-      const int2 full = full_tiles(a.mask, w.b, a.n_t, w.t);
       int start = 0, end = i + 1;
       if (a.mask.rows) {
         const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + w.t) * (2 * BT) + row;
@@ -359,11 +326,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float slope = 0.f;
       if (BIAS) slope = a.slopes[w.h] * kLog2e;
-      const int sb = it % SB;
-      if (!wwait(&st_full[sb], (it / SB) & 1, a.err, abort_flag)) { ok = false; break; }
-      const float2 st = sST[sb * BT + row];
+      const int qb = it % QB;
+      if (!wwait(&q_full[qb], (it / QB) & 1, a.err, abort_flag)) { ok = false; break; }
+      const float2 st = make_float2(sST[qb * 256 + row], sST[qb * 256 + BT + row]);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&st_empty[sb]);
+      if (lane == 0) mbar_arrive(&st_empty[qb]);
       for (int j = w.r.x; j < w.r.y; ++j, ++n) {
         const uint32_t t_s = tmem + C::T_S + (n & 1) * 128 + lane_off + part * 32;
         if (!wwait(&s_full[n & 1], (n >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
@@ -376,20 +343,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int j0 = j * BT + part * 32;  // key of column 0
           const float dist = (float)(j0 - i);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float x, f = 1.f;
+          for (int e = 0; e < 32; e += 2) {
+            float2 x = pair(s[e], s[e + 1]), f;
             if (CAP) {
-              const float z = rcp_approx(1.f + fast_exp2(__uint_as_float(s[e]) * k.mul));
-              x = fmaf(-2.f * k.cap, z, k.cap);
-              f = 4.f * z * (1.f - z);  // 1 - tanh^2
+              const float2 z = cap_z(x, k);
+              x = fma2(z, pair(-2.f * k.cap), pair(k.cap));
+              f = mul2(mul2(z, pair(4.f)), fma2(z, pair(-1.f), pair(1.f)));  // 1 - tanh^2
             }
-            if (BIAS) x = fmaf(-slope, fabsf(dist + (float)e), CAP ? x : __uint_as_float(s[e]) * k.mul);
-            float p;
-            if (CAP || BIAS) p = fast_exp2(x - st.x);
-            else p = fast_exp2(fmaf(__uint_as_float(s[e]), k.mul, -st.x));
-            pf[e] = CAP ? p * f : p;
+            if (BIAS) {
+              if (!CAP) x = mul2(x, pair(k.mul));
+              x.x = fmaf(-slope, fabsf(dist + (float)e), x.x);
+              x.y = fmaf(-slope, fabsf(dist + (float)(e + 1)), x.y);
+            }
+            x = (CAP || BIAS) ? add2(x, pair(st.x)) : fma2(x, pair(k.mul), pair(st.x));
+            x = exp2_pair(x);
+            if (CAP) x = mul2(x, f);
+            pf[e] = x.x;
+            pf[e + 1] = x.y;
           }
-          if (j < full.x || j >= full.y) {
+          if (j < w.f.x || j >= w.f.y) {
             const int l0 = min(max(start - j0, 0), 32), h0 = min(max(end - j0, 0), 32);
             const uint32_t seen = (h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u) & ~(l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u);
 #pragma unroll
@@ -406,8 +378,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t ds[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            ds[e] = pack_bf16x2(pf[2 * e] * (__uint_as_float(dp[2 * e]) - st.y),
-                                pf[2 * e + 1] * (__uint_as_float(dp[2 * e + 1]) - st.y));
+          {
+            const float2 v = mul2(make_float2(pf[2 * e], pf[2 * e + 1]), add2(pair(dp[2 * e], dp[2 * e + 1]), pair(st.y)));
+            ds[e] = pack_bf16x2(v.x, v.y);
+          }
           tmem_st_32x32b_x16(t_s, ds);
         }
         tmem_wait_st();
@@ -454,6 +428,71 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+constexpr int kStatRows = 32;
+
+// ld[b, h, tile, 0 / 1, row] = -LSE log2 e / -Delta; -inf and 0 for a row that takes no part.  A CTA has 32 tokens
+// of one batch entry, all heads: neighbouring threads read neighbouring 16 bytes, the d / 8 threads of a (token, head)
+// add up with shuffles, and the results leave through shared memory as 128-byte runs per head.
+template <int D>
+__global__ void __launch_bounds__(256)
+    row_stats_kernel(const __nv_bfloat16* __restrict__ dout, long do_ss, long do_sb, const __nv_bfloat16* __restrict__ out,
+                     const float* __restrict__ lse, int S, int nh, int n_t, float* __restrict__ ld) {
+  pdl_trigger();
+  constexpr int G = D / 8;
+  extern __shared__ float s_delta[];  // [nh][kStatRows + 1]
+  const int blocks = n_t * (BT / kStatRows);
+  const int b = blockIdx.x / blocks, row0 = (blockIdx.x % blocks) * kStatRows;
+  const int per_row = nh * G, units = kStatRows * per_row;
+  pdl_wait();
+  // every thread of a warp takes part in the shuffles: units and the block size are multiples of the warp size
+#pragma unroll 4
+  for (int u = threadIdx.x; u < units; u += 256) {
+    const int r = u / per_row, c = u - r * per_row;
+    const int i = row0 + r;
+    float acc = 0.f;
+    if (i < S) {
+      const uint4 x = *reinterpret_cast<const uint4*>(dout + b * do_sb + i * do_ss + c * 8);
+      const uint4 y = *reinterpret_cast<const uint4*>(out + ((size_t)b * S + i) * ((size_t)nh * D) + c * 8);
+      const uint32_t* xw = reinterpret_cast<const uint32_t*>(&x);
+      const uint32_t* yw = reinterpret_cast<const uint32_t*>(&y);
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const float2 f = unpack_bf16x2(xw[z]), g = unpack_bf16x2(yw[z]);
+        acc = fmaf(f.x, g.x, fmaf(f.y, g.y, acc));
+      }
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (c % G == 0) s_delta[(c / G) * (kStatRows + 1) + r] = acc;
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < nh * kStatRows; u += 256) {
+    const int h = u / kStatRows, r = u % kStatRows, i = row0 + r;
+    const float l = i < S ? lse[((size_t)b * nh + h) * S + i] : -INFINITY;
+    const bool none = l == -INFINITY;
+    float* p = ld + (((size_t)b * nh + h) * n_t + row0 / BT) * (2 * BT) + row0 % BT + r;
+    p[0] = none ? -INFINITY : -l * kLog2e;
+    p[BT] = none ? 0.f : -s_delta[h * (kStatRows + 1) + r];
+  }
+}
+
+template <int D>
+int row_stats(const AttnCall& c, const void* dout, long do_ss, long do_sb, const void* out, const float* lse, float* ld,
+              cudaStream_t stream) {
+  const int n_t = (c.S + BT - 1) / BT;
+  const long grid = (long)c.B * n_t * (BT / kStatRows);
+  const size_t smem = (size_t)c.nh * (kStatRows + 1) * sizeof(float);
+  if (grid > INT_MAX || smem > 200 * 1024) return -4;
+  auto k = row_stats_kernel<D>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+  }
+  launch_k(k, (unsigned)grid, 256, smem, stream, static_cast<const __nv_bfloat16*>(dout), do_ss, do_sb,
+           static_cast<const __nv_bfloat16*>(out), lse, c.S, c.nh, n_t, ld);
+  return (int)cudaGetLastError();
+}
+
 template <int D, bool CAP, bool BIAS>
 int launch(const CUtensorMap& tq, const CUtensorMap& to, const CUtensorMap& td, const Args& a, int grid, cudaStream_t stream) {
   auto k = masked_attn_dq_kernel<D, CAP, BIAS>;
@@ -472,8 +511,12 @@ int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, 
   const int n_t = (c.S + BT - 1) / BT;
   const long items = (long)c.B * c.nh * n_t;
   if (items > INT_MAX / 2) return -1;
+  if (c.d != 64 && c.d != 128) return -2;
+  int rc = c.d == 64 ? dq::row_stats<64>(c, dout, do_ss, do_sb, out, lse, ld, stream)
+                     : dq::row_stats<128>(c, dout, do_ss, do_sb, out, lse, ld, stream);
+  if (rc) return rc;
   CUtensorMap tq, to, td;
-  int rc = make_tmap_bf16_3d(&tq, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
+  rc = make_tmap_bf16_3d(&tq, c.qkv, c.B, c.S, (long)(c.nh + 2 * c.nkv) * c.d, c.qkv_ss, c.qkv_sb, 64, BT);
   if (rc) return rc - 10;
   rc = make_tmap_bf16_3d(&to, dout, c.B, c.S, (long)c.nh * c.d, do_ss, do_sb, 64, BT);
   if (rc) return rc - 20;
@@ -486,15 +529,14 @@ int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, 
   a.nh = c.nh;
   a.nkv = c.nkv;
   a.n_t = n_t;
-  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange)};
+  a.by_nh = FastDiv(c.nh);
+  a.by_B = FastDiv(c.B);
+  a.by_tiles = FastDiv(n_t);
+  a.by_group = FastDiv(c.nh / c.nkv);
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange), c.order_q};
   a.slopes = c.slopes;
   score_constants(c.scale, c.cap, &a.score.mul, &a.score.cap);
   a.scale = c.scale;
-  a.dout = static_cast<const __nv_bfloat16*>(dout);
-  a.do_ss = do_ss;
-  a.do_sb = do_sb;
-  a.out = static_cast<const __nv_bfloat16*>(out);
-  a.lse = lse;
   a.ld = ld;
   a.dqkv = static_cast<__nv_bfloat16*>(dqkv);
   a.err = err;

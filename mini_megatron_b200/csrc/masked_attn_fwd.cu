@@ -51,46 +51,66 @@ struct Cfg {
   static constexpr int V_OFF = K_OFF + NS * TILE;
   static constexpr int ML_OFF = V_OFF + NS * TILE;  // [2][128] (maximum, row sum)
   static constexpr int OUT_OFF = ML_OFF + 2 * BT * 8;  // 4 epilogue warps x 32 rows x 64 columns bf16
-  static constexpr int BAR_OFF = OUT_OFF + 4 * 4096;
+  static constexpr int ITEM_OFF = OUT_OFF + 4 * 4096;  // [kRing] work items
+  static constexpr int BAR_OFF = ITEM_OFF + kRing * 64;
   static constexpr int SMEM = 1024 + BAR_OFF + 512;
   static constexpr uint32_t T_S0 = 0, T_S1 = 128, T_O0 = 256, T_O1 = 256 + D;
   static constexpr uint32_t T_P0 = SEP ? 384 : T_S0, T_P1 = SEP ? 448 : T_S1;
 };
 
 struct Args {
-  int B, S, nh, nkv, n_t;
+  int B, S, nh, nkv, n_t, n_pairs;
+  FastDiv by_nh, by_B, by_pairs, by_group;
   Mask mask;
   const float* slopes;  // [nh] or nullptr
   Score score;
+  float* lse;  // [B, nh, S] natural log
   __nv_bfloat16* out;   // [B, S, nh * D]
-  float* lse;           // [B, nh, S] natural log
   int* err;
 };
 
-struct Item {
-  int b, h, t0, t1;  // t0 < 0: only tile t1 (odd number of tiles)
+struct alignas(16) Item {
+  int b, h, t0, t1;  // b < 0: no more items; t0 < 0: only tile t1 (odd number of tiles)
   int2 r0, r1;       // key tiles of t0, t1
-  int lo, hi;        // their union
+  int2 f0, f1;       // those of them that need no mask
+  int lo, hi;        // union of the key tiles
 };
+static_assert(sizeof(Item) <= 64, "ring entry");
+constexpr int kConsumers = 1 + 2 + 8 + 4;  // TMA and MMA threads, softmax and epilogue warps
 
 __device__ __forceinline__ Item decode(const Args& a, int item) {
-  const int BH = a.B * a.nh;
-  const int n_pairs = (a.n_t + 1) / 2;
-  const int pr = item / BH, bh = item - pr * BH;
-  const int p = n_pairs - 1 - pr;  // causal rows: the longest first
+  const int li = a.by_nh.quot(item);
   Item it;
-  it.b = bh / a.nh;
-  it.h = bh - it.b * a.nh;
+  it.h = item - li * a.nh;
+  int p;
+  if (a.mask.order) {
+    const int e = a.mask.order[li];
+    it.b = a.by_pairs.quot(e);
+    p = e - it.b * a.n_pairs;
+  } else {  // causal rows: the longest first
+    const int q = a.by_B.quot(li);
+    it.b = li - q * a.B;
+    p = a.n_pairs - 1 - q;
+  }
   it.t1 = (a.n_t & 1) ? 2 * p : 2 * p + 1;
   it.t0 = it.t1 - 1;
-  it.r0 = it.t0 >= 0 ? key_tiles(a.mask, it.b, a.n_t, it.t0) : make_int2(0, 0);
+  it.r0 = it.f0 = make_int2(0, 0);
+  if (it.t0 >= 0) {
+    it.r0 = key_tiles(a.mask, it.b, a.n_t, it.t0);
+    it.f0 = full_tiles(a.mask, it.b, a.n_t, it.t0);
+  }
   it.r1 = key_tiles(a.mask, it.b, a.n_t, it.t1);
+  it.f1 = full_tiles(a.mask, it.b, a.n_t, it.t1);
   const bool a0 = it.r0.y > it.r0.x, a1 = it.r1.y > it.r1.x;
   it.lo = a0 ? (a1 ? min(it.r0.x, it.r1.x) : it.r0.x) : it.r1.x;
   it.hi = max(it.r0.y, it.r1.y);
   if (!a0 && !a1) it.hi = it.lo;
   return it;
 }
+
+// Whether the exponentials of the two tiles take turns.
+template <int D>
+constexpr bool kTurns = D == 128;
 
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -123,15 +143,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_free = o_full + 2;      // [2]  O_i and its statistics read by the epilogue (4 warps)
   uint64_t* ml_full = o_free + 2;     // [2]  statistics of the item written (4 warps)
   uint64_t* turn = ml_full + 2;       // [2][4]  exponentials of a joint step issued, per tile and sub-partition
-  uint64_t* drain = turn + 8;         // [2]
+  uint64_t* ring_full = turn + 8;     // [kRing]
+  uint64_t* ring_empty = ring_full + kRing;  // [kRing]
+  uint64_t* drain = ring_empty + kRing;      // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_items = a.B * a.nh * ((a.n_t + 1) / 2);
+  const Ring<Item> ring{reinterpret_cast<Item*>(smem + C::ITEM_OFF), ring_full, ring_empty};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&ring_full[i], 1);
+      mbar_init(&ring_empty[i], kConsumers);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 2);
@@ -164,19 +190,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   pdl_wait();
   const uint32_t tmem = *tmem_slot;
-  const int group = a.nh / a.nkv;
 
   if (warp < 4) {
-    reg_dec<64>();
+    reg_dec<56>();
     if (warp == 0 && elect_one()) {
       // ---------------------------------------------------------------- TMA
       int kv = 0, it = 0, q_issued = -1;
       bool ok = true;
-      for (int r = 0, item; (item = snake_item(r)) < n_items; ++r) {
-        const Item w = decode(a, item);
+      Item w;
+      for (int k = 0; (ok = ring.get_thread(w, k, a.err, abort_flag)) && w.b >= 0; ++k) {
         if (w.lo >= w.hi) continue;
         const bool a0 = w.r0.y > w.r0.x, a1 = w.r1.y > w.r1.x;
-        const int hk = w.h / group;
+        const int hk = a.by_group.quot(w.h);
         const int qx = w.h * D, kx = (a.nh + hk) * D, vx = (a.nh + a.nkv + hk) * D;
         const int qb = it % QB;
         if (it >= QB && !bwait(&q_empty[qb], ((it / QB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
@@ -248,8 +273,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         umma_commit(&v_empty[st]);
         return true;
       };
-      for (int r = 0, item; (item = snake_item(r)) < n_items; ++r) {
-        const Item w = decode(a, item);
+      Item w;
+      for (int k = 0; (ok = ring.get_thread(w, k, a.err, abort_flag)) && w.b >= 0; ++k) {
         if (w.lo >= w.hi) continue;
         const int2 range = grp == 0 ? w.r0 : w.r1;
         const int qb = it % QB;
@@ -273,11 +298,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         umma_commit(&drain[grp]);
         drain_wait(&drain[grp], 0);
       }
+    } else if (warp == 3 && elect_one()) {
+      // ---------------------------------------------------------------- work items
+      const int n_items = a.B * a.nh * a.n_pairs;
+      Item w;
+      for (int r = 0, item;; ++r) {
+        item = snake_item(r);
+        if (item < n_items) w = decode(a, item);
+        else w.b = -1;
+        if (!ring.put(w, r, a.err, abort_flag) || w.b < 0) break;
+      }
     }
     __syncwarp();
   } else if (warp < 12) {
     // ------------------------------------------------------------------ softmax
-    reg_inc<184>();
+    reg_inc<192>();
     const int grp = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;  // query row within the tile (TMEM lane)
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
@@ -287,12 +322,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Score k = a.score;
     int sc = 0, pc = 0, ic = 0, nj = 0;  // nj: steps that both tiles take
     bool ok = true;
-    for (int r = 0, item; (item = snake_item(r)) < n_items; ++r) {
-      const Item w = decode(a, item);
+    Item w;
+    for (int n = 0; (ok = ring.get_warp(w, n, a.err, abort_flag)) && w.b >= 0; ++n) {
       const int t = grp == 0 ? w.t0 : w.t1;
-      const int2 range = grp == 0 ? w.r0 : w.r1, other = grp == 0 ? w.r1 : w.r0;
+      const int2 range = grp == 0 ? w.r0 : w.r1, other = grp == 0 ? w.r1 : w.r0, full = grp == 0 ? w.f0 : w.f1;
       if (range.x >= range.y) continue;
-      const int2 full = full_tiles(a.mask, w.b, a.n_t, t);
       const int i = t * BT + row;
       int start = 0, end = i + 1;
       if (a.mask.rows) {
@@ -317,10 +351,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (CAP || BIAS) {
           const float dist = (float)(j * BT - i);
 #pragma unroll
-          for (int c = 0; c < 128; ++c) {
-            float x = score<CAP>(__uint_as_float(s[c]), k);
-            if (BIAS) x = fmaf(-slope, fabsf(dist + (float)c), x);
-            s[c] = __float_as_uint(x);
+          for (int c = 0; c < 128; c += 2) {
+            float2 x = pair(s[c], s[c + 1]);
+            if (CAP) x = fma2(cap_z(x, k), pair(-2.f * k.cap), pair(k.cap));
+            else x = mul2(x, pair(k.mul));
+            if (BIAS) {
+              x.x = fmaf(-slope, fabsf(dist + (float)c), x.x);
+              x.y = fmaf(-slope, fabsf(dist + (float)(c + 1)), x.y);
+            }
+            s[c] = __float_as_uint(x.x);
+            s[c + 1] = __float_as_uint(x.y);
           }
         }
         if (j < full.x || j >= full.y) {
@@ -364,30 +404,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++pc;
         // the exponentials of the two tiles take turns, one warp of each on every SM sub-partition: while one
-        // fills the MUFU pipe the other waits for its scores, takes its maximum and stores its P
-        const bool joint = j >= other.x && j < other.y;
-        if (joint) {
-          if (grp == 1 || nj > 0) {
-            if (!wwait(&turn[(grp ^ 1) * 4 + (warp & 3)], (grp == 1 ? nj : nj - 1) & 1, a.err, abort_flag)) {
-              ok = false;
-              break;
-            }
+        // fills the pipes the other waits for its scores, takes its maximum and stores its P
+        const bool joint = kTurns<D> && j >= other.x && j < other.y;
+        if (joint && (grp == 1 || nj > 0)) {
+          if (!wwait(&turn[(grp ^ 1) * 4 + (warp & 3)], (grp == 1 ? nj : nj - 1) & 1, a.err, abort_flag)) {
+            ok = false;
+            break;
           }
         }
         float2 rs[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) rs[u] = make_float2(0.f, 0.f);
-        const float2 mul2v = make_float2(k.mul, k.mul), mu2 = make_float2(-mu, -mu);
+        for (int u = 0; u < 4; ++u) rs[u] = pair(0.f);
 #pragma unroll
         for (int hcol = 0; hcol < 2; ++hcol) {
           uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int c = hcol * 64 + 2 * e;
-            float2 x = make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-            x = (CAP || BIAS) ? add2(x, mu2) : fma2(x, mul2v, mu2);
-            x.x = fast_exp2(x.x);
-            x.y = fast_exp2(x.y);
+            float2 x = pair(s[c], s[c + 1]);
+            x = (CAP || BIAS) ? add2(x, pair(-mu)) : fma2(x, pair(k.mul), pair(-mu));
+            x = exp2_pair(x);
             rs[e & 3] = add2(rs[e & 3], x);
             pk[e] = pack_bf16x2(x.x, x.y);
           }
@@ -424,14 +460,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ epilogue
-    reg_dec<80>();
+    reg_dec<72>();
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     uint8_t* stg = smem + C::OUT_OFF + (warp & 3) * 4096;
     int ic[2] = {0, 0};
     bool ok = true;
-    for (int r = 0, item; ok && (item = snake_item(r)) < n_items; ++r) {
-      const Item w = decode(a, item);
+    Item w;
+    for (int n = 0; ok && (ok = ring.get_warp(w, n, a.err, abort_flag)) && w.b >= 0; ++n) {
 #pragma unroll
       for (int grp = 0; grp < 2; ++grp) {
         const int t = grp == 0 ? w.t0 : w.t1;
@@ -522,7 +558,12 @@ int masked_attn_fwd(const AttnCall& c, void* out, float* lse, int* err, int num_
   a.nh = c.nh;
   a.nkv = c.nkv;
   a.n_t = n_t;
-  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange)};
+  a.n_pairs = (n_t + 1) / 2;
+  a.by_nh = FastDiv(c.nh);
+  a.by_B = FastDiv(c.B);
+  a.by_pairs = FastDiv(a.n_pairs);
+  a.by_group = FastDiv(c.nh / c.nkv);
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange), c.order_p};
   a.slopes = c.slopes;
   score_constants(c.scale, c.cap, &a.score.mul, &a.score.cap);
   a.out = static_cast<__nv_bfloat16*>(out);

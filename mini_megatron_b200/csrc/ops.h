@@ -103,7 +103,7 @@ int flash_attn_bwd_sm100_d64(const __nv_bfloat16* dout, long ld_do, const __nv_b
 int document_plan_max_len();
 int document_plan(const long* ids, long ld_ids, long eod, int by_change, const unsigned char* marks, long ld_marks,
                   const int* lengths, int B, int S, int* positions, int* start, int* end, int* rows, void* qstat,
-                  void* krange, cudaStream_t stream);
+                  void* krange, int* order, cudaStream_t stream);
 
 // Rotary positions (rotary.cu): heads [0, heads_rot) of x rotated into y (y may be x), the rest copied.
 int rotary(const void* x, long x_sb, long x_ss, void* y, long y_sb, long y_ss, int is_f32, const void* positions,
@@ -118,6 +118,9 @@ struct AttnCall {
   const int* rows;       // of document_plan, or nullptr: causal
   const void* qstat;
   const void* krange;
+  const int* order_p;    // query tile pairs, query tiles and key tiles of all rows, heaviest first
+  const int* order_q;
+  const int* order_k;
   const float* slopes;   // [nh] or nullptr
   float cap;             // 0: scores are not capped
   float scale;
@@ -125,8 +128,9 @@ struct AttnCall {
 int masked_attn_fwd(const AttnCall& c, void* out, float* lse, int* err, int num_sms, cudaStream_t stream);
 int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, const void* out, const float* lse,
                    float* ld, void* dqkv, int* err, int num_sms, cudaStream_t stream);
-int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb, const float* ld, void* dqkv, int* err,
-                    int num_sms, cudaStream_t stream);
+int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb, const float* ld, float* partial,
+                    int parts, void* dqkv, int* err, int num_sms, cudaStream_t stream);
+int masked_attn_dkv_parts(int B, int S, int nh, int nkv, int num_sms);
 
 // Fused DP step (fused_dp.cu)
 struct DpPeersHost {

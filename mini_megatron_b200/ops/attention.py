@@ -68,7 +68,7 @@ def attention_fwd(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, sof
     nkv, cap, scale = _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale)
     if not qkv.is_cuda:
         return _attention_cpu(qkv, num_heads, head_dim, nkv, plan, cap, alibi_slopes, scale)
-    tiles = plan.tiles if plan is not None else (None, None, None)
+    tiles = plan.tiles if plan is not None else (None,) * 4
     return tuple(native().masked_attn_fwd(qkv, num_heads, nkv, head_dim, *tiles, alibi_slopes, cap, scale))
 
 
@@ -77,7 +77,7 @@ def attention_bwd(dctx, qkv, ctx, lse, num_heads, head_dim, *, num_kv_heads=None
     """``dqkv`` (layout of ``qkv``, contiguous) from the gradient of ``ctx`` and what :func:`attention_fwd` returned.
     CUDA only.  The same inputs give the same bits: no atomics."""
     nkv, cap, scale = _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale)
-    tiles = plan.tiles if plan is not None else (None, None, None)
+    tiles = plan.tiles if plan is not None else (None,) * 4
     return native().masked_attn_bwd(dctx, qkv, ctx, lse, num_heads, nkv, head_dim, *tiles, alibi_slopes, cap, scale)
 
 

@@ -70,7 +70,7 @@ def test_plan_gpu(B, S, doc, prefix, pad, empty, by_ids):
     if S > 10000:
         return
     rows, qstat, seen = _tile_tables(plan)
-    got_rows, got_stat, got_range = (t.cpu() for t in plan.tiles)
+    got_rows, got_stat, got_range, order = (t.cpu() for t in plan.tiles)
     assert torch.equal(got_rows, rows)
     assert torch.equal(got_stat, qstat)
     n_t = seen.shape[1]
@@ -83,6 +83,17 @@ def test_plan_gpu(B, S, doc, prefix, pad, empty, by_ids):
             assert 0 <= lo and hi < n_t
             if not want:
                 assert lo > hi or not seen[b, lo:hi + 1, k].any()
+    # every tile once, heaviest first (tiles to visit; a weight per 1024 tiles is one bin)
+    n_p = (n_t + 1) // 2
+    keys = torch.where(qstat[..., 1] == 0, 0, (qstat[..., 1] + 127) // 128 - qstat[..., 0] // 128)
+    pairs = torch.zeros(B, n_p, dtype=torch.int32)
+    for t in range(n_t):
+        pairs[:, (t + 1) // 2 if n_t % 2 else t // 2] += keys[:, t]
+    queries = (got_range[..., 1] + 1 - got_range[..., 0]).clamp_min(0)
+    for part, weight in zip(order.split([B * n_p, B * n_t, B * n_t]), (pairs, keys, queries)):
+        assert torch.equal(part.sort().values, torch.arange(len(part), dtype=torch.int32))
+        along = weight.flatten()[part.long()]
+        assert (along[1:] <= along[:-1]).all()
 
 
 @pytest.mark.gpu
