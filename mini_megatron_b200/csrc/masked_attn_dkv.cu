@@ -33,7 +33,7 @@ template <int D>
 struct Cfg {
   static constexpr int TILE = BT * D * 2;
   static constexpr int KB = (D == 64) ? 2 : 1;  // K / V buffers
-  static constexpr int NQ = (D == 64) ? 3 : 2;  // Q / dO ring stages
+  static constexpr int NQ = (D == 64) ? 4 : 2;  // Q / dO ring stages
   static constexpr int SB = (D == 64) ? 2 : 1;  // S^T buffers in TMEM
   static constexpr int K_OFF = 0;               // [KB][K, V]
   static constexpr int Q_OFF = KB * 2 * TILE;   // [NQ][Q, dO]
@@ -41,7 +41,7 @@ struct Cfg {
   static constexpr int LD_OFF = Q_OFF + NQ * 2 * TILE, LD = 2176;
   static constexpr int ITEM_OFF = LD_OFF + NQ * LD;  // [kRing] work items
   static constexpr int BAR_OFF = ITEM_OFF + kRing * 32;
-  static constexpr int SMEM = 1024 + BAR_OFF + 320;
+  static constexpr int SMEM = 1024 + BAR_OFF + 384;
   static constexpr uint32_t T_S = 0, T_DP = SB * 128, T_DV = T_DP + 128, T_DK = T_DV + D;
 };
 static_assert(Cfg<128>::SMEM <= 227 * 1024 && Cfg<64>::SMEM <= 227 * 1024, "shared memory of one CTA");
@@ -131,10 +131,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sQ = smem + C::Q_OFF;
   uint8_t* sLD = smem + C::LD_OFF;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-  uint64_t* kv_full = bars;        // [2]
-  uint64_t* kv_empty = bars + 2;   // [2]
-  uint64_t* q_full = bars + 4;     // [3]
-  uint64_t* q_empty = bars + 7;    // [3]
+  uint64_t* k_full = bars;         // [2]
+  uint64_t* k_empty = bars + 2;    // [2]
+  uint64_t* v_full = bars + 4;     // [2]
+  uint64_t* v_empty = bars + 6;    // [2]
+  uint64_t* q_full = bars + 30;    // [4]
+  uint64_t* q_empty = bars + 34;   // [4]
   uint64_t* s_full = bars + 10;    // [2]
   uint64_t* dp_full = bars + 12;
   // P^T written, S^T read (16 warps).  Two barriers: a warp may be done with P^T(n+1) before another one is
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* g_free = bars + 16;    // ... read (16 warps)
   uint64_t* drain = bars + 17;
   uint64_t* out_full = bars + 20;  // dK, dV of an item staged (16 warps)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);  // bars + 21 ..: the ring of work items
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);  // bars + 21 ..: the ring of work items
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -154,12 +156,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], kWarps);
     }
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < NQ; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
     }
@@ -194,19 +198,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       if (elect_one()) {
         // ---------------------------------------------------------------- TMA
-        int n = 0, kv_issued = -1;
+        int n = 0, k_issued = -1, v_issued = -1;
         bool ok = true;
         Walk x;
         for (int got; (got = x.next(ring, heads, a.err, abort_flag)) != 0; ++n) {
           if (got < 0) { ok = false; break; }
           if (x.first()) {
             const int kb = x.it % KB;
-            if (x.it >= KB && !bwait(&kv_empty[kb], ((x.it / KB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-            mbar_expect_tx(&kv_full[kb], 2 * C::TILE);
-            load_tile<D>(sKV + kb * 2 * C::TILE, &tm_qkv, &kv_full[kb], (a.nh + x.w.hk) * D, x.w.t * BT, x.w.b);
-            load_tile<D>(sKV + kb * 2 * C::TILE + C::TILE, &tm_qkv, &kv_full[kb], (a.nh + a.nkv + x.w.hk) * D,
-                         x.w.t * BT, x.w.b);
-            kv_issued = x.it;
+            uint8_t* kd = sKV + kb * 2 * C::TILE;
+            if (x.it >= KB && !bwait(&k_empty[kb], ((x.it / KB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+            mbar_expect_tx(&k_full[kb], C::TILE);
+            load_tile<D>(kd, &tm_qkv, &k_full[kb], (a.nh + x.w.hk) * D, x.w.t * BT, x.w.b);
+            k_issued = x.it;
+            if (x.it >= KB && !bwait(&v_empty[kb], ((x.it / KB) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+            mbar_expect_tx(&v_full[kb], C::TILE);
+            load_tile<D>(kd + C::TILE, &tm_qkv, &v_full[kb], (a.nh + a.nkv + x.w.hk) * D, x.w.t * BT, x.w.b);
+            v_issued = x.it;
           }
           const int st = n % NQ;
           if (n >= NQ && !bwait(&q_empty[st], ((n / NQ) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
@@ -222,7 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (!ok) {
-          for (int u = max(0, kv_issued - KB + 1); u <= kv_issued; ++u) drain_wait(&kv_full[u % KB], (u / KB) & 1);
+          for (int u = max(0, k_issued - KB + 1); u <= k_issued; ++u) drain_wait(&k_full[u % KB], (u / KB) & 1);
+          for (int u = max(0, v_issued - KB + 1); u <= v_issued; ++u) drain_wait(&v_full[u % KB], (u / KB) & 1);
           for (int u = max(0, n - NQ); u < n; ++u) drain_wait(&q_full[u % NQ], (u / NQ) & 1);
         }
       }
@@ -233,50 +241,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         int n = 0;
         Walk cur, nxt;
+        // K is only read by S^T and V only by dP^T: after an item's last one the next item's tile may load
         auto issue_s = [&](const Walk& x, int u) -> bool {
           const int kb = x.it % KB;
-          if (x.first() && !bwait(&kv_full[kb], (x.it / KB) & 1, a.err, abort_flag)) return false;
+          if (x.first() && !bwait(&k_full[kb], (x.it / KB) & 1, a.err, abort_flag)) return false;
           if (!bwait(&q_full[u % NQ], (u / NQ) & 1, a.err, abort_flag)) return false;
           tc_fence_after();
           mma_abt<D>(tmem + C::T_S + (u % SB) * 128, smem_u32(sKV + kb * 2 * C::TILE),
                      smem_u32(sQ + (u % NQ) * 2 * C::TILE));
           umma_commit(&s_full[u % SB]);
+          if (x.last(heads)) umma_commit(&k_empty[kb]);
           return true;
         };
-        auto issue_dp = [&](const Walk& x, int u) {
+        auto issue_dp = [&](const Walk& x, int u) -> bool {
           const int kb = x.it % KB;
+          if (x.first() && !bwait(&v_full[kb], (x.it / KB) & 1, a.err, abort_flag)) return false;
+          tc_fence_after();
           mma_abt<D>(tmem + C::T_DP, smem_u32(sKV + kb * 2 * C::TILE + C::TILE),
                      smem_u32(sQ + (u % NQ) * 2 * C::TILE + C::TILE));
           umma_commit(dp_full);
+          if (x.last(heads)) umma_commit(&v_empty[kb]);
+          return true;
         };
         int more = nxt.next(ring, heads, a.err, abort_flag);
-        ok = more >= 0;
-        if (more > 0) {
-          ok = issue_s(nxt, 0);
-          if (ok) issue_dp(nxt, 0);
-        }
+        ok = more >= 0 && (more == 0 || (issue_s(nxt, 0) && issue_dp(nxt, 0)));
         while (ok && more) {
           cur = nxt;
           more = nxt.next(ring, heads, a.err, abort_flag);
           if (more < 0) { ok = false; break; }
-          // one K / V buffer: the next item's tiles can only be loaded once this item's products are done
-          const bool early = more && (KB == 2 || nxt.it == cur.it);
           const uint32_t q_addr = smem_u32(sQ + (n % NQ) * 2 * C::TILE);
-          if (SB == 2 && early && !issue_s(nxt, n + 1)) { ok = false; break; }
+          if (SB == 2 && more && !issue_s(nxt, n + 1)) { ok = false; break; }
           if (!bwait(&p_full[n & 1], (n >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
           if (cur.first() && cur.it > 0 && !bwait(g_free, (cur.it - 1) & 1, a.err, abort_flag)) { ok = false; break; }
           tc_fence_after();
           mma_tmem_b<D, 32>(tmem + C::T_DV, tmem + C::T_S + (n % SB) * 128, q_addr + C::TILE, !cur.first());
-          if (SB == 1 && early && !issue_s(nxt, n + 1)) { ok = false; break; }  // over P^T, in issue order after dV
+          if (SB == 1 && more && !issue_s(nxt, n + 1)) { ok = false; break; }  // over P^T, in issue order after dV
           if (!bwait(ds_full, n & 1, a.err, abort_flag)) { ok = false; break; }
           tc_fence_after();
           mma_tmem_b<D, 32>(tmem + C::T_DK, tmem + C::T_DP, q_addr, !cur.first());
-          umma_commit(&q_empty[n % NQ]);
-          if (cur.last(heads)) {
-            umma_commit(g_full);  // K and V become the staging tiles of dK and dV, whose store releases them
-          }
-          if (more && !early && !issue_s(nxt, n + 1)) { ok = false; break; }
-          if (more) issue_dp(nxt, n + 1);  // over dS^T, in issue order after dK
+          // the Q / dO stage of an item's last pair becomes the staging tile of its dK and dV, which releases it
+          if (cur.last(heads)) umma_commit(g_full);
+          else umma_commit(&q_empty[n % NQ]);
+          if (more && !issue_dp(nxt, n + 1)) { ok = false; break; }  // over dS^T, in issue order after dK
           ++n;
         }
         if (!ok) {
@@ -443,7 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld(tmem + C::T_DK + lane_off + part * (D / 4), u);
         tmem_wait_ld();
         warp_arrive(g_free);
-        uint8_t* stg = sKV + (it % KB) * 2 * C::TILE;
+        const int qs = (n - 1) % NQ;
+        uint8_t* stg = sQ + qs * 2 * C::TILE;
         if (a.parts > 1) {
           if (in) {
             float* pk = share_row();
@@ -474,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             bulk_commit();
             bulk_wait_read<0>();
-            mbar_arrive(&kv_empty[it % KB]);
+            mbar_arrive(&q_empty[qs]);
           }
           __syncwarp();
         }

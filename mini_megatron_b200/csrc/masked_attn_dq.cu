@@ -428,11 +428,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-constexpr int kStatRows = 32;
+constexpr int kStatRows = 8;
 
-// ld[b, h, tile, 0 / 1, row] = -LSE log2 e / -Delta; -inf and 0 for a row that takes no part.  A CTA has 32 tokens
+// ld[b, h, tile, 0 / 1, row] = -LSE log2 e / -Delta; -inf and 0 for a row that takes no part.  A CTA has 8 tokens
 // of one batch entry, all heads: neighbouring threads read neighbouring 16 bytes, the d / 8 threads of a (token, head)
-// add up with shuffles, and the results leave through shared memory as 128-byte runs per head.
+// add up with shuffles, and the results leave through shared memory as 32-byte runs per head.
 template <int D>
 __global__ void __launch_bounds__(256)
     row_stats_kernel(const __nv_bfloat16* __restrict__ dout, long do_ss, long do_sb, const __nv_bfloat16* __restrict__ out,
