@@ -7,10 +7,11 @@
 //   x_ij = C tanh(s q_i.k_j / cap)  or  s log2 e (q_i.k_j),   minus  slope_h log2 e |i - j|
 //   visible iff start_i <= j < end_i                          (document_plan.cu; causal: 0 and i + 1)
 //
-// tanh is 1 - 2 / (1 + e^{2u}): one exponential and one reciprocal, whose
-// absolute error (a few 2^-23) is what matters inside the softmax's exponent.
-// The single-instruction tanh approximation is off by up to 2^-11 relative, which
-// a cap of 50 turns into 0.02 in the exponent; it is not used.
+// tanh u of a warp whose scores all have |u| <= 1 (the cap well above them, the usual case) is u times a polynomial
+// in u^2: it runs on the FMA pipe, while 1 - 2 / (1 + e^{2u}), used otherwise, takes two of the three MUFU
+// operations of a score, and those bound the capped kernels (16 a cycle and SM; CAPOLD).  Both are
+// exact to a few 2^-23.  The single-instruction tanh approximation is off by up to 2^-11 relative, which a cap of 50
+// turns into 0.02 in the exponent; it is not used.
 #pragma once
 #include "common.cuh"
 #include "ops.h"
@@ -87,6 +88,15 @@ struct Ring {
   __device__ __forceinline__ bool put(const Item& w, int k, int* err, volatile int* abort_flag) const;
 };
 
+__device__ __forceinline__ void st_shared(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ float ld_shared(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -130,14 +140,57 @@ __device__ __forceinline__ float2 pair(uint32_t a, uint32_t b) {
 
 // Constants of the score transform.
 struct Score {
-  float mul;  // plain: s log2 e;  capped: 2 s log2 e / cap (the exponent of e^{2u} in log2 units)
-  float cap;  // C
+  float mul;    // plain: s log2 e;  capped: s / cap (u = mul q.k)
+  float twice;  // capped: 2 s log2 e / cap (e^{2u} = 2^(twice q.k))
+  float cap;    // C
 };
 
-// 1 / (1 + e^{2u}) of a pair of scores; C tanh u = C - 2 C z, 1 - tanh^2 u = 4 z (1 - z).
-__device__ __forceinline__ float2 cap_z(float2 s, const Score& k) {
-  const float2 e = add2(exp2_pair(mul2(s, pair(k.mul))), pair(1.f));
-  return make_float2(rcp_approx(e.x), rcp_approx(e.y));
+// tanh u for |u| <= 1: u times a polynomial of degree 6 in u^2, fitted for the least relative error (1.6e-7).
+__device__ __forceinline__ float2 tanh_small(float2 u) {
+  const float2 z = mul2(u, u);
+  float2 p = fma2(z, pair(1.041017706e-03f), pair(-6.203362253e-03f));
+  p = fma2(p, z, pair(2.028995939e-02f));
+  p = fma2(p, z, pair(-5.345701799e-02f));
+  p = fma2(p, z, pair(1.332520396e-01f));
+  p = fma2(p, z, pair(-3.333283961e-01f));
+  p = fma2(p, z, pair(9.999999404e-01f));
+  return mul2(u, p);
+}
+// tanh of a pair of scores.
+template <bool SMALL>
+__device__ __forceinline__ float2 cap_tanh(float2 s, const Score& k) {
+  if constexpr (SMALL) return tanh_small(mul2(s, pair(k.mul)));
+  const float2 e = add2(exp2_pair(mul2(s, pair(k.twice))), pair(1.f));
+  return fma2(make_float2(rcp_approx(e.x), rcp_approx(e.y)), pair(-2.f), pair(1.f));
+}
+// Whether every |u| of the warp's N scores a thread is at most 1 (false for a NaN).
+template <int N>
+__device__ __forceinline__ bool cap_small(const uint32_t (&s)[N], const Score& k) {
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < N; c += 2)
+    m[(c / 2) & 3] = max3(m[(c / 2) & 3], fabsf(__uint_as_float(s[c])), fabsf(__uint_as_float(s[c + 1])));
+  return __all_sync(0xffffffffu, max3(fmaxf(m[0], m[1]), m[2], m[3]) * k.mul <= 1.f) != 0;
+}
+
+// The warp's scores replaced by their tanh u.
+template <int N>
+__device__ __forceinline__ void cap_in_place(uint32_t (&s)[N], const Score& k) {
+  if (cap_small(s, k)) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      const float2 t = cap_tanh<true>(pair(s[c], s[c + 1]), k);
+      s[c] = __float_as_uint(t.x);
+      s[c + 1] = __float_as_uint(t.y);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      const float2 t = cap_tanh<false>(pair(s[c], s[c + 1]), k);
+      s[c] = __float_as_uint(t.x);
+      s[c + 1] = __float_as_uint(t.y);
+    }
+  }
 }
 
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -290,15 +343,15 @@ __device__ __forceinline__ void mma_abt(uint32_t dst, uint32_t a_addr, uint32_t 
 }
 
 // 128 x D (+)= A [128 x 128, bf16 in TMEM] B [128 x D] (rows are the reduction: MN-major).  A's 128
-// columns lie in runs of RUN (RUN / 2 TMEM columns) that start 32 TMEM columns apart.
-template <int D, int RUN>
+// columns lie in runs of RUN (RUN / 2 TMEM columns) that start STRIDE TMEM columns apart.
+template <int D, int RUN, int STRIDE = 32>
 __device__ __forceinline__ void mma_tmem_b(uint32_t dst, uint32_t a_tmem, uint32_t b_addr, bool acc) {
   constexpr int PER = RUN / 16;
   constexpr uint32_t idesc = make_idesc_bf16(BT, D, false, true);
   const uint64_t bd = make_sdesc_sw128(b_addr, 16384, 1024);
 #pragma unroll
   for (int k = 0; k < BT / 16; ++k)
-    umma_bf16_ts(dst, a_tmem + (k / PER) * 32 + (k % PER) * 8, bd + (uint64_t)(k * (2048 >> 4)), idesc,
+    umma_bf16_ts(dst, a_tmem + (k / PER) * STRIDE + (k % PER) * 8, bd + (uint64_t)(k * (2048 >> 4)), idesc,
                  (acc || k != 0) ? 1u : 0u);
 }
 
@@ -314,15 +367,9 @@ __device__ __forceinline__ void store_zero(__nv_bfloat16* p) {
 }  // namespace mattn
 
 // Host-side description of one call (ops.h declares the launchers).
-inline int score_constants(float scale, float cap, float* mul, float* c) {
-  if (cap > 0.f) {
-    *mul = 2.f * scale * mattn::kLog2e / cap;
-    *c = cap * mattn::kLog2e;
-  } else {
-    *mul = scale * mattn::kLog2e;
-    *c = 0.f;
-  }
-  return 0;
+inline mattn::Score score_constants(float scale, float cap) {
+  if (cap > 0.f) return {scale / cap, 2.f * scale * mattn::kLog2e / cap, cap * mattn::kLog2e};
+  return {scale * mattn::kLog2e, 0.f, 0.f};
 }
 
 }  // namespace mmb

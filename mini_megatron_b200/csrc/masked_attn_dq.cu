@@ -340,15 +340,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t s[32];
           tmem_ld(t_s, s);
           tmem_wait_ld();
+          if (CAP) cap_in_place(s, k);
           const int j0 = j * BT + part * 32;  // key of column 0
           const float dist = (float)(j0 - i);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             float2 x = pair(s[e], s[e + 1]), f;
             if (CAP) {
-              const float2 z = cap_z(x, k);
-              x = fma2(z, pair(-2.f * k.cap), pair(k.cap));
-              f = mul2(mul2(z, pair(4.f)), fma2(z, pair(-1.f), pair(1.f)));  // 1 - tanh^2
+              f = fma2(mul2(x, pair(-1.f)), x, pair(1.f));  // 1 - tanh^2
+              x = mul2(x, pair(k.cap));
             }
             if (BIAS) {
               if (!CAP) x = mul2(x, pair(k.mul));
@@ -535,7 +535,7 @@ int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, 
   a.by_group = FastDiv(c.nh / c.nkv);
   a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange), c.order_q};
   a.slopes = c.slopes;
-  score_constants(c.scale, c.cap, &a.score.mul, &a.score.cap);
+  a.score = score_constants(c.scale, c.cap);
   a.scale = c.scale;
   a.ld = ld;
   a.dqkv = static_cast<__nv_bfloat16*>(dqkv);

@@ -348,13 +348,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_32x32b_x32(t_s + 96, *reinterpret_cast<uint32_t(*)[32]>(&s[96]));
         tmem_wait_ld();
         if (SEP) warp_arrive(&s_free[grp]);  // the next S_i may be computed into these columns
+        if (CAP) cap_in_place(s, k);
         if (CAP || BIAS) {
           const float dist = (float)(j * BT - i);
 #pragma unroll
           for (int c = 0; c < 128; c += 2) {
-            float2 x = pair(s[c], s[c + 1]);
-            if (CAP) x = fma2(cap_z(x, k), pair(-2.f * k.cap), pair(k.cap));
-            else x = mul2(x, pair(k.mul));
+            float2 x = mul2(pair(s[c], s[c + 1]), pair(CAP ? k.cap : k.mul));
             if (BIAS) {
               x.x = fmaf(-slope, fabsf(dist + (float)c), x.x);
               x.y = fmaf(-slope, fabsf(dist + (float)(c + 1)), x.y);
@@ -565,7 +564,7 @@ int masked_attn_fwd(const AttnCall& c, void* out, float* lse, int* err, int num_
   a.by_group = FastDiv(c.nh / c.nkv);
   a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange), c.order_p};
   a.slopes = c.slopes;
-  score_constants(c.scale, c.cap, &a.score.mul, &a.score.cap);
+  a.score = score_constants(c.scale, c.cap);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
   a.err = err;
