@@ -369,27 +369,36 @@ Tensor flash_attn_bwd_v1(const Tensor& dout, const Tensor& qkv, const Tensor& ou
 }
 
 // ----------------------------------------------------------------- packed rows of documents
-// ids [B, S] int64 (tokens, or document ids with by_change) or none, marks [B, S] bool / uint8 or none, lengths [B]
-// int32 or none -> positions, start, end [B, S] int32 and the attention kernels' tile tables (rows, qstat, krange, order).
-std::vector<Tensor> document_plan(const c10::optional<Tensor>& ids, int64_t eod, bool by_change,
-                                  const c10::optional<Tensor>& marks, const c10::optional<Tensor>& lengths, int64_t B,
-                                  int64_t S, const at::Device& device) {
-  TORCH_CHECK(device.is_cuda(), "document_plan: device must be CUDA");
+// The attention kernels' tile tables of a plan, in one int32 buffer: rows [B, n_t, 2, 128], qstat [B, n_t, 4],
+// krange [B, n_t, 2] and, for rows of more than kUnorderedTiles tiles, the order of pairs, query and key tiles.
+struct PlanTables {
+  int64_t rows, qstat, krange, order, total;
+  PlanTables(int64_t B, int64_t S) {
+    const int64_t n_t = (S + 127) / 128;
+    rows = 0;
+    qstat = rows + B * n_t * 256;
+    krange = qstat + B * n_t * 4;
+    order = krange + B * n_t * 2;
+    total = order + (n_t > mmb::kUnorderedTiles ? B * ((n_t + 1) / 2 + 2 * n_t) : 0);
+  }
+};
+
+// ids [B, S] int64 (tokens, or document ids with by_change), marks [B, S] bool / uint8 or none, lengths [B]
+// int32 or none -> positions, start, end [B, S] int32 and the tile tables.
+std::vector<Tensor> document_plan(const Tensor& ids, int64_t eod, bool by_change, const c10::optional<Tensor>& marks,
+                                  const c10::optional<Tensor>& lengths) {
+  check_cuda(ids, "ids");
+  TORCH_CHECK(ids.scalar_type() == at::kLong && ids.dim() == 2, "document_plan: ids must be [B, S] int64");
+  const int64_t B = ids.size(0), S = ids.size(1);
+  const at::Device device = ids.device();
   TORCH_CHECK(B >= 1 && S >= 1 && S <= mmb::document_plan_max_len(), "document_plan: rows of 1 to ",
               mmb::document_plan_max_len(), " tokens, got B = ", B, ", S = ", S);
   TORCH_CHECK(B <= (1 << 24), "document_plan: too many rows");
+  TORCH_CHECK(S == 1 || ids.stride(1) == 1, "document_plan: ids must be dense in the last dimension");
   const at::cuda::CUDAGuard guard(device);
-  const long* ip = nullptr;
-  long ld_ids = 0, ld_marks = 0;
+  int64_t ld_marks = 0;
   const unsigned char* mp = nullptr;
   const int* lp = nullptr;
-  if (ids.has_value()) {
-    TORCH_CHECK(ids->device() == device && ids->scalar_type() == at::kLong && ids->dim() == 2 && ids->size(0) == B &&
-                    ids->size(1) == S && (S == 1 || ids->stride(1) == 1),
-                "document_plan: ids must be [B, S] int64 on the device, dense in the last dimension");
-    ip = reinterpret_cast<const long*>(ids->data_ptr<int64_t>());
-    ld_ids = ids->stride(0);
-  }
   if (marks.has_value()) {
     TORCH_CHECK(marks->device() == device && (marks->scalar_type() == at::kBool || marks->scalar_type() == at::kByte) &&
                     marks->dim() == 2 && marks->size(0) == B && marks->size(1) == S && (S == 1 || marks->stride(1) == 1),
@@ -404,24 +413,27 @@ std::vector<Tensor> document_plan(const c10::optional<Tensor>& ids, int64_t eod,
     lp = lengths->data_ptr<int>();
   }
   const auto opt = at::TensorOptions().dtype(at::kInt).device(device);
-  const int64_t n_t = (S + 127) / 128;
-  Tensor positions = at::empty({B, S}, opt), start = at::empty({B, S}, opt), end = at::empty({B, S}, opt);
-  Tensor rows = at::empty({B, n_t, 2, 128}, opt), qstat = at::empty({B, n_t, 4}, opt),
-         krange = at::empty({B, n_t, 2}, opt), order = at::empty({B * ((n_t + 1) / 2 + 2 * n_t)}, opt);
-  MMB_CHECK_RC(mmb::document_plan(ip, ld_ids, eod, by_change ? 1 : 0, mp, ld_marks, lp, (int)B, (int)S,
-                                  positions.data_ptr<int>(), start.data_ptr<int>(), end.data_ptr<int>(),
-                                  rows.data_ptr<int>(), qstat.data_ptr<int>(), krange.data_ptr<int>(),
-                                  order.data_ptr<int>(), cur_stream()),
+  const PlanTables at_(B, S);
+  Tensor out = at::empty({3, B, S}, opt), tables = at::empty({at_.total}, opt);
+  int* o = out.data_ptr<int>();
+  int* t = tables.data_ptr<int>();
+  MMB_CHECK_RC(mmb::document_plan(reinterpret_cast<const long*>(ids.data_ptr<int64_t>()), ids.stride(0), eod,
+                                  by_change ? 1 : 0, mp, ld_marks, lp, (int)B, (int)S, o, o + B * S, o + 2 * B * S,
+                                  t + at_.rows, t + at_.qstat, t + at_.krange,
+                                  at_.total > at_.order ? t + at_.order : nullptr, cur_stream()),
                "document_plan");
-  return {positions, start, end, rows, qstat, krange, order};
+  return {out.select(0, 0), out.select(0, 1), out.select(0, 2), tables};
 }
 
 // ----------------------------------------------------------------- rotary positions
-// x, y [B, S, heads * d] bf16 / fp32 (y may be x), positions [B, S] or [S] int32 / int64 or none, freqs [rot / 2] fp64.
-void rotary(const Tensor& x, Tensor& y, const c10::optional<Tensor>& positions, const Tensor& freqs, double magnitude,
-            bool interleaved, int64_t d, int64_t rot, int64_t heads_rot, bool inverse) {
+// x, y [B, S, heads * d] bf16 / fp32 (y may be x; none: a new tensor), positions [B, S] or [S] int32 / int64 or none, freqs [rot / 2] fp64.
+Tensor rotary(const Tensor& x, const c10::optional<Tensor>& out, const c10::optional<Tensor>& positions,
+              const Tensor& freqs, double magnitude, bool interleaved, int64_t d, int64_t rot, int64_t heads_rot,
+              bool inverse) {
   check_cuda(x, "x");
   const bool f32 = x.scalar_type() == at::kFloat;
+  const at::cuda::CUDAGuard guard(x.device());
+  const Tensor y = out.has_value() ? *out : at::empty(x.sizes(), x.options());
   TORCH_CHECK(f32 || x.scalar_type() == at::kBFloat16, "rotary: x must be bf16 or fp32");
   TORCH_CHECK(x.dim() == 3 && y.dim() == 3 && x.sizes() == y.sizes() && y.scalar_type() == x.scalar_type() &&
                   y.device() == x.device(),
@@ -437,8 +449,8 @@ void rotary(const Tensor& x, Tensor& y, const c10::optional<Tensor>& positions, 
                   freqs.numel() == rot / 2,
               "rotary: freqs must be [rotary_dim / 2] fp64 on x's device");
   TORCH_CHECK(S <= INT_MAX && d <= 4096 && heads <= (1 << 20), "rotary: too large");
-  if (B == 0 || S == 0) return;
-  for (const Tensor* t : {&x, static_cast<const Tensor*>(&y)}) {
+  if (B == 0 || S == 0) return y;
+  for (const Tensor* t : {&x, &y}) {
     TORCH_CHECK(t->stride(2) == 1 && (S == 1 || t->stride(1) % per == 0) && (B == 1 || t->stride(0) % per == 0) &&
                     reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                 "rotary: tensors must be dense in the last dimension, with rows on 16-byte boundaries");
@@ -458,7 +470,6 @@ void rotary(const Tensor& x, Tensor& y, const c10::optional<Tensor>& positions, 
     TORCH_CHECK((ss >= W && (B == 1 || sb >= (S - 1) * ss + W)) || (sb >= W && ss >= (B - 1) * sb + W),
                 "rotary: rows of y overlap one another");
   }
-  const at::cuda::CUDAGuard guard(x.device());
   const void* pp = nullptr;
   int64_t pos_sb = 0;
   bool pos64 = false;
@@ -477,6 +488,7 @@ void rotary(const Tensor& x, Tensor& y, const c10::optional<Tensor>& positions, 
                            interleaved, B, (int)S, (int)d, (int)rot, (int)heads_rot, (int)heads, num_sms(),
                            cur_stream()),
                "rotary");
+  return y;
 }
 
 // ----------------------------------------------------------------- masked attention
@@ -492,10 +504,8 @@ void token_strides(const Tensor& t, const char* name, int64_t& ss, int64_t& sb) 
               name, " must be dense in the last dimension, with rows on 16-byte boundaries");
 }
 
-mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, const c10::optional<Tensor>& rows,
-                        const c10::optional<Tensor>& qstat, const c10::optional<Tensor>& krange,
-                        const c10::optional<Tensor>& order, const c10::optional<Tensor>& slopes, double cap,
-                        double scale) {
+mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, const c10::optional<Tensor>& tables,
+                        const c10::optional<Tensor>& slopes, double cap, double scale) {
   mmb::AttnCall c{};
   int64_t ss, sb;
   TORCH_CHECK(d == 64 || d == 128, "attention supports head_dim 64 and 128, got ", d);
@@ -518,21 +528,21 @@ mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, c
   c.d = (int)d;
   c.cap = (float)cap;
   c.scale = (float)scale;
-  if (rows.has_value()) {
-    const int64_t n_t = (S + 127) / 128;
-    TORCH_CHECK(qstat.has_value() && krange.has_value() && order.has_value(), "attention: incomplete plan");
-    for (const Tensor* t : {&*rows, &*qstat, &*krange, &*order})
-      TORCH_CHECK(t->device() == qkv.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
-                  "attention: the plan must be on qkv's device");
-    TORCH_CHECK(rows->numel() == B * n_t * 256 && qstat->numel() == B * n_t * 4 && krange->numel() == B * n_t * 2 &&
-                    order->numel() == B * ((n_t + 1) / 2 + 2 * n_t),
-                "attention: the plan was made for other rows than qkv's [", B, ", ", S, "]");
-    c.rows = rows->data_ptr<int>();
-    c.qstat = qstat->data_ptr<int>();
-    c.krange = krange->data_ptr<int>();
-    c.order_p = order->data_ptr<int>();
-    c.order_q = c.order_p + B * ((n_t + 1) / 2);
-    c.order_k = c.order_q + B * n_t;
+  if (tables.has_value()) {
+    const PlanTables at_(B, S);
+    TORCH_CHECK(tables->device() == qkv.device() && tables->scalar_type() == at::kInt && tables->is_contiguous() &&
+                    tables->numel() == at_.total,
+                "attention: the plan was made for other rows than qkv's [", B, ", ", S, "] or on another device");
+    const int* t = tables->data_ptr<int>();
+    c.rows = t + at_.rows;
+    c.qstat = t + at_.qstat;
+    c.krange = t + at_.krange;
+    if (at_.total > at_.order) {
+      const int64_t n_t = (S + 127) / 128;
+      c.order_p = t + at_.order;
+      c.order_q = c.order_p + B * ((n_t + 1) / 2);
+      c.order_k = c.order_q + B * n_t;
+    }
   }
   if (slopes.has_value()) {
     TORCH_CHECK(slopes->device() == qkv.device() && slopes->scalar_type() == at::kFloat && slopes->is_contiguous() &&
@@ -544,11 +554,9 @@ mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, c
 }
 
 std::vector<Tensor> masked_attn_fwd(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d,
-                                    const c10::optional<Tensor>& rows, const c10::optional<Tensor>& qstat,
-                                    const c10::optional<Tensor>& krange, const c10::optional<Tensor>& order,
-                       const c10::optional<Tensor>& slopes,
+                                    const c10::optional<Tensor>& tables, const c10::optional<Tensor>& slopes,
                                     double cap, double scale) {
-  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, rows, qstat, krange, order, slopes, cap, scale);
+  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, tables, slopes, cap, scale);
   const at::cuda::CUDAGuard guard(qkv.device());
   Tensor out = at::empty({c.B, c.S, nh * d}, qkv.options());
   Tensor lse = at::empty({c.B, nh, c.S}, qkv.options().dtype(at::kFloat));
@@ -559,11 +567,9 @@ std::vector<Tensor> masked_attn_fwd(const Tensor& qkv, int64_t nh, int64_t nkv, 
 }
 
 Tensor masked_attn_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, const Tensor& lse, int64_t nh,
-                       int64_t nkv, int64_t d, const c10::optional<Tensor>& rows, const c10::optional<Tensor>& qstat,
-                       const c10::optional<Tensor>& krange, const c10::optional<Tensor>& order,
-                       const c10::optional<Tensor>& slopes, double cap,
+                       int64_t nkv, int64_t d, const c10::optional<Tensor>& tables, const c10::optional<Tensor>& slopes, double cap,
                        double scale) {
-  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, rows, qstat, krange, order, slopes, cap, scale);
+  const mmb::AttnCall c = attn_call(qkv, nh, nkv, d, tables, slopes, cap, scale);
   const at::cuda::CUDAGuard guard(qkv.device());
   int64_t do_ss, do_sb;
   token_strides(dout, "dctx", do_ss, do_sb);
@@ -1089,17 +1095,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("EPI_PUSH_BF16") = (int)mmb::EPI_PUSH_BF16;
   m.def("num_sms", &num_sms);
   m.def("document_plan", &document_plan, py::arg("ids"), py::arg("eod"), py::arg("by_change"), py::arg("marks"),
-        py::arg("lengths"), py::arg("B"), py::arg("S"), py::arg("device"));
+        py::arg("lengths"));
   m.def("document_plan_max_len", &mmb::document_plan_max_len);
-  m.def("rotary", &rotary, py::arg("x"), py::arg("y"), py::arg("positions"), py::arg("freqs"), py::arg("magnitude"),
+  m.def("rotary", &rotary, py::arg("x"), py::arg("out"), py::arg("positions"), py::arg("freqs"), py::arg("magnitude"),
         py::arg("interleaved"), py::arg("head_dim"), py::arg("rotary_dim"), py::arg("num_heads"),
         py::arg("inverse") = false);
   m.def("masked_attn_fwd", &masked_attn_fwd, py::arg("qkv"), py::arg("num_heads"), py::arg("num_kv_heads"),
-        py::arg("head_dim"), py::arg("rows"), py::arg("qstat"), py::arg("krange"), py::arg("order"), py::arg("slopes"), py::arg("cap"),
+        py::arg("head_dim"), py::arg("tables"), py::arg("slopes"), py::arg("cap"),
         py::arg("scale"));
   m.def("masked_attn_bwd", &masked_attn_bwd, py::arg("dctx"), py::arg("qkv"), py::arg("ctx"), py::arg("lse"),
-        py::arg("num_heads"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("rows"), py::arg("qstat"),
-        py::arg("krange"), py::arg("order"), py::arg("slopes"), py::arg("cap"), py::arg("scale"));
+        py::arg("num_heads"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("tables"), py::arg("slopes"), py::arg("cap"), py::arg("scale"));
   m.def("flash_attn_fwd", &flash_attn_fwd);
   m.def("flash_attn_fwd_v1", &flash_attn_fwd_v1, "previous one-tile-per-CTA forward (comparison only)");
   m.def("flash_attn_bwd", &flash_attn_bwd);

@@ -50,6 +50,7 @@ struct Args {
   long ld_marks;
   const int* lengths;     // [B] or nullptr
   int S, n_t, chunk;      // chunk: tokens per CTA (a multiple of kStep)
+  int staged;             // 1: the row's tile bounds fit into shared memory
   int* positions;         // [B, S]
   int* start;
   int* end;
@@ -82,21 +83,45 @@ __device__ __forceinline__ int warp_min_scan_right(int v, int lane) {
 // First (document start) and plain (unmarked or padding) flags of the thread's four tokens.
 __device__ __forceinline__ void load_flags(const Args& a, int b, int i0, int len, bool (&first)[kPer],
                                            bool (&plain)[kPer]) {
+  long id[kPer] = {0, 0, 0, 0};
+  uint8_t mark[kPer] = {0, 0, 0, 0};
   long prev = 0;
-  if (a.ids && i0 > 0 && i0 < a.S) prev = a.ids[b * a.ld_ids + i0 - 1];
+  const bool whole = i0 + kPer <= a.S;
+  if (a.ids && i0 < a.S) {
+    const long* p = a.ids + b * a.ld_ids + i0;
+    if (i0 > 0) prev = p[-1];
+    if (whole && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      const longlong2 u = *reinterpret_cast<const longlong2*>(p), v = *reinterpret_cast<const longlong2*>(p + 2);
+      id[0] = u.x;
+      id[1] = u.y;
+      id[2] = v.x;
+      id[3] = v.y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (i0 + e < a.S) id[e] = p[e];
+    }
+  }
+  if (a.marks && i0 < len) {
+    const uint8_t* p = a.marks + b * a.ld_marks + i0;
+    if (whole && (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+      const uchar4 u = *reinterpret_cast<const uchar4*>(p);
+      mark[0] = u.x;
+      mark[1] = u.y;
+      mark[2] = u.z;
+      mark[3] = u.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (i0 + e < a.S) mark[e] = p[e];
+    }
+  }
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int i = i0 + e;
-    first[e] = (i == 0);
-    plain[e] = true;
-    if (i < a.S) {
-      if (a.ids) {
-        const long cur = a.ids[b * a.ld_ids + i];
-        if (i > 0) first[e] = a.by_change ? (cur != prev) : (prev == a.eod);
-        prev = cur;
-      }
-      if (a.marks && i < len) plain[e] = a.marks[b * a.ld_marks + i] == 0;
-    }
+    const long before = e == 0 ? prev : id[e - 1];
+    first[e] = i == 0 || (a.ids && (a.by_change ? id[e] != before : before == a.eod));
+    plain[e] = !(i < len && mark[e]);
   }
 }
 
@@ -111,8 +136,9 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
   const int n_steps = (c1 - c0 + kStep - 1) / kStep;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
 
-  // ---- reduce the chunk, step by step
-  for (int st = 0; st < n_steps; ++st) {
+  // ---- reduce the chunk, step by step (a row of one step has nothing to carry over)
+  const bool alone = n_cta == 1 && n_steps == 1;
+  for (int st = 0; !alone && st < n_steps; ++st) {
     const int i0 = c0 + st * kStep + tid * kPer;
     bool first[kPer], plain[kPer];
     load_flags(a, b, i0, len, first, plain);
@@ -219,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
     xd = max(xd, pd);
     xl = max(xl, pl);
     xs = min(xs, ns);
-    stop_right = min(stop_right, s_step[st].stop);
+    if (!alone) stop_right = min(stop_right, s_step[st].stop);
 
     int smin = INT_MAX, emax = 0, smax = 0, emin = INT_MAX;
     int vs[kPer], ve[kPer], vp[kPer];
@@ -275,18 +301,26 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
     __syncthreads();
   }
   const int4* qs = a.qstat + (size_t)b * a.n_t;
+  extern __shared__ int2 s_bounds[];  // [n_t] (min start, max end) where that fits, to search without global loads
+  if (a.staged) {
+    for (int t = tid; t < a.n_t; t += kThreads) {
+      const int2 v = __ldcg(reinterpret_cast<const int2*>(qs + t));
+      s_bounds[t] = v;
+    }
+    __syncthreads();
+  }
   for (int kt = c0 / 128 + tid; kt < min((c1 + 127) / 128, a.n_t); kt += kThreads) {
     int lo = 0, hi = a.n_t;  // first tile with max end > kt * 128 (a tile that sees nothing counts as above)
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
-      const int emax = __ldcg(&qs[mid].y);
+      const int emax = a.staged ? s_bounds[mid].y : __ldcg(&qs[mid].y);
       if (emax == 0 || emax > kt * 128) hi = mid;
       else lo = mid + 1;
     }
     int l2 = 0, h2 = a.n_t;  // first tile with min start >= (kt + 1) * 128
     while (l2 < h2) {
       const int mid = (l2 + h2) / 2;
-      if (__ldcg(&qs[mid].x) >= (kt + 1) * 128) h2 = mid;
+      if ((a.staged ? s_bounds[mid].x : __ldcg(&qs[mid].x)) >= (kt + 1) * 128) h2 = mid;
       else l2 = mid + 1;
     }
     a.krange[(size_t)b * a.n_t + kt] = make_int2(lo, l2 - 1);
@@ -396,6 +430,8 @@ int document_plan(const long* ids, long ld_ids, long eod, int by_change, const u
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * n_cta));
   cfg.blockDim = dim3(kThreads);
+  a.staged = a.n_t <= 4096;
+  cfg.dynamicSmemBytes = a.staged ? a.n_t * sizeof(int2) : 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -405,6 +441,7 @@ int document_plan(const long* ids, long ld_ids, long eod, int by_change, const u
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, document_plan_kernel, a);
+  // rows of a few tiles: no tile is much heavier than another
   if (e != cudaSuccess || !order) return (int)e;
   OrderArgs o;
   o.qstat = a.qstat;

@@ -101,6 +101,8 @@ int flash_attn_bwd_sm100_d64(const __nv_bfloat16* dout, long ld_do, const __nv_b
 
 // Packed rows of documents (document_plan.cu): positions, visible key intervals and their tile statistics.
 int document_plan_max_len();
+// Rows of up to this many 128-token tiles get no order: their tiles weigh much the same.
+constexpr int kUnorderedTiles = 4;
 int document_plan(const long* ids, long ld_ids, long eod, int by_change, const unsigned char* marks, long ld_marks,
                   const int* lengths, int B, int S, int* positions, int* start, int* end, int* rows, void* qstat,
                   void* krange, int* order, cudaStream_t stream);

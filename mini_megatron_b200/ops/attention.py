@@ -47,7 +47,7 @@ def _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes
     if qkv.dim() != 3:
         raise ValueError(f"attention needs qkv [B, S, (num_heads + 2 num_kv_heads) * head_dim], got {tuple(qkv.shape)}")
     nkv = num_heads if num_kv_heads is None else num_kv_heads
-    if plan is not None and (plan.shape != tuple(qkv.shape[:2]) or plan.device != qkv.device):
+    if plan is not None and (plan.shape != qkv.shape[:2] or (plan.tables is None) == qkv.is_cuda):
         raise ValueError(f"the plan was made for rows of {plan.shape} on {plan.device}, qkv has "
                          f"{tuple(qkv.shape[:2])} on {qkv.device}")
     if softcap is not None and not softcap > 0:
@@ -68,8 +68,8 @@ def attention_fwd(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, sof
     nkv, cap, scale = _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale)
     if not qkv.is_cuda:
         return _attention_cpu(qkv, num_heads, head_dim, nkv, plan, cap, alibi_slopes, scale)
-    tiles = plan.tiles if plan is not None else (None,) * 4
-    return tuple(native().masked_attn_fwd(qkv, num_heads, nkv, head_dim, *tiles, alibi_slopes, cap, scale))
+    return tuple(native().masked_attn_fwd(qkv, num_heads, nkv, head_dim, None if plan is None else plan.tables,
+                                          alibi_slopes, cap, scale))
 
 
 def attention_bwd(dctx, qkv, ctx, lse, num_heads, head_dim, *, num_kv_heads=None, plan=None, softcap=None,
@@ -77,8 +77,8 @@ def attention_bwd(dctx, qkv, ctx, lse, num_heads, head_dim, *, num_kv_heads=None
     """``dqkv`` (layout of ``qkv``, contiguous) from the gradient of ``ctx`` and what :func:`attention_fwd` returned.
     CUDA only.  The same inputs give the same bits: no atomics."""
     nkv, cap, scale = _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale)
-    tiles = plan.tiles if plan is not None else (None,) * 4
-    return native().masked_attn_bwd(dctx, qkv, ctx, lse, num_heads, nkv, head_dim, *tiles, alibi_slopes, cap, scale)
+    return native().masked_attn_bwd(dctx, qkv, ctx, lse, num_heads, nkv, head_dim, None if plan is None else plan.tables,
+                                          alibi_slopes, cap, scale)
 
 
 class _AttentionFn(torch.autograd.Function):

@@ -20,25 +20,19 @@ rebuild the plan from new tokens.
 """
 from __future__ import annotations
 
-import dataclasses
-
 import torch
 
 from . import native
 
 
-@dataclasses.dataclass(frozen=True)
 class DocumentPlan:
-    """``positions``, ``start``, ``end``: ``[B, S]`` int32.  ``tiles`` belongs to the attention kernels."""
+    """``positions``, ``start``, ``end``: ``[B, S]`` int32.  ``tables`` belongs to the attention kernels."""
 
-    positions: torch.Tensor
-    start: torch.Tensor
-    end: torch.Tensor
-    tiles: tuple = ()
+    __slots__ = ("positions", "start", "end", "tables", "shape")
 
-    @property
-    def shape(self):
-        return tuple(self.positions.shape)
+    def __init__(self, positions, start, end, tables=None):
+        self.positions, self.start, self.end, self.tables = positions, start, end, tables
+        self.shape = tuple(positions.shape)
 
     @property
     def device(self):
@@ -87,9 +81,8 @@ def document_plan(tokens=None, eod=None, *, document_ids=None, prefix_mask=None,
     ids = ids if ids.stride(1) == 1 else ids.contiguous()
     if prefix_mask is not None and prefix_mask.stride(1) != 1:
         prefix_mask = prefix_mask.contiguous()
-    positions, start, end, *tiles = native().document_plan(ids, 0 if eod is None else int(eod), document_ids is not None,
-                                                           prefix_mask, lengths, B, S, ids.device)
-    return DocumentPlan(positions, start, end, tuple(tiles))
+    return DocumentPlan(*native().document_plan(ids, 0 if eod is None else eod, document_ids is not None, prefix_mask,
+                                                lengths))
 
 
 def _plan_cpu(ids, eod, prefix_mask, lengths):

@@ -91,11 +91,11 @@ def _run(x, rotary, num_heads, positions, out, inverse):
     if not x.is_cuda:
         y = _rotary_cpu(x, rotary, num_heads, positions, inverse)
         return y if out is None else out.copy_(y)
-    if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    native().rotary(x, out, positions, rotary.turns(x.device), rotary.magnitude, rotary.interleaved, rotary.head_dim,
-                    rotary.rotary_dim, num_heads, inverse)
-    return out
+    freqs = rotary._turns.get(x.device)
+    if freqs is None:
+        freqs = rotary.turns(x.device)
+    return native().rotary(x, out, positions, freqs, rotary.magnitude, rotary.interleaved, rotary.head_dim,
+                           rotary.rotary_dim, num_heads, inverse)
 
 
 def rotary_fwd(x, rotary, num_heads, positions=None, out=None):
