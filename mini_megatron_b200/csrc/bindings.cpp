@@ -369,16 +369,16 @@ Tensor flash_attn_bwd_v1(const Tensor& dout, const Tensor& qkv, const Tensor& ou
 }
 
 // ----------------------------------------------------------------- packed rows of documents
-// The attention kernels' tile tables of a plan, in one int32 buffer: rows [B, n_t, 2, 128], qstat [B, n_t, 4],
-// krange [B, n_t, 2] and, for rows of more than kUnorderedTiles tiles, the order of pairs, query and key tiles.
+// The attention kernels' tile tables of a plan, in one int32 buffer: rows [B, n_t, 4, 128], qstat [B, n_t, 4],
+// kstat [B, n_t, 4] and, for rows of more than kUnorderedTiles tiles, the order of pairs, query and key tiles.
 struct PlanTables {
-  int64_t rows, qstat, krange, order, total;
+  int64_t rows, qstat, kstat, order, total;
   PlanTables(int64_t B, int64_t S) {
     const int64_t n_t = (S + 127) / 128;
     rows = 0;
-    qstat = rows + B * n_t * 256;
-    krange = qstat + B * n_t * 4;
-    order = krange + B * n_t * 2;
+    qstat = rows + B * n_t * 512;
+    kstat = qstat + B * n_t * 4;
+    order = kstat + B * n_t * 4;
     total = order + (n_t > mmb::kUnorderedTiles ? B * ((n_t + 1) / 2 + 2 * n_t) : 0);
   }
 };
@@ -419,7 +419,7 @@ std::vector<Tensor> document_plan(const Tensor& ids, int64_t eod, bool by_change
   int* t = tables.data_ptr<int>();
   MMB_CHECK_RC(mmb::document_plan(reinterpret_cast<const long*>(ids.data_ptr<int64_t>()), ids.stride(0), eod,
                                   by_change ? 1 : 0, mp, ld_marks, lp, (int)B, (int)S, o, o + B * S, o + 2 * B * S,
-                                  t + at_.rows, t + at_.qstat, t + at_.krange,
+                                  t + at_.rows, t + at_.qstat, t + at_.kstat,
                                   at_.total > at_.order ? t + at_.order : nullptr, cur_stream()),
                "document_plan");
   return {out.select(0, 0), out.select(0, 1), out.select(0, 2), tables};
@@ -536,7 +536,7 @@ mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, c
     const int* t = tables->data_ptr<int>();
     c.rows = t + at_.rows;
     c.qstat = t + at_.qstat;
-    c.krange = t + at_.krange;
+    c.kstat = t + at_.kstat;
     if (at_.total > at_.order) {
       const int64_t n_t = (S + 127) / 128;
       c.order_p = t + at_.order;

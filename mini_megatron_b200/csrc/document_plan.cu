@@ -9,15 +9,16 @@
 //             document, is padding, or is S
 //   position_i = i - start_i
 //
-// Padding sees nothing: start = end = position = 0.  All three are scans of
-// one row: a running maximum of document starts, a running maximum of
-// unmarked indices (a token is in its prefix iff that is < start_i), and a
-// running minimum from the right of the indices that stop a prefix.
+// Padding sees nothing: start = end = position = 0.  Seen from the keys, key j is
+// visible to the queries [j, document end), or, as part of a prefix, to its whole
+// document: an interval again.  All of it comes from scans of one row: a running
+// maximum of document starts, a running maximum of unmarked indices (a token is in
+// its prefix iff that is < start_i), and running minima from the right of the
+// document starts and of the indices that stop a prefix.
 //
-// For the attention kernels the same pass writes, for every 128-token tile,
-// the extremes of start and end (which key tiles a query tile needs, and which
-// of them need no mask), a tile-padded copy of (start, end) that a bulk copy
-// can fetch, and, for every key tile, the query tiles that see it.
+// For the attention kernels the same pass writes tile-padded copies of both intervals
+// and, for every 128-token tile, the extremes of their bounds: which key tiles a query
+// tile needs, which query tiles a key tile, and which of them need no mask.
 //
 // One cluster of 1 to 8 CTAs per row, the row cut into as many chunks; a
 // thread owns 4 consecutive tokens, so a warp owns one 128-token tile and the
@@ -50,17 +51,16 @@ struct Args {
   long ld_marks;
   const int* lengths;     // [B] or nullptr
   int S, n_t, chunk;      // chunk: tokens per CTA (a multiple of kStep)
-  int staged;             // 1: the row's tile bounds fit into shared memory
   int* positions;         // [B, S]
   int* start;
   int* end;
-  int* rows;              // [B, n_t, 2, 128]
+  int* rows;              // [B, n_t, 4, 128] start, end; first and one past the last query that sees the token
   int4* qstat;            // [B, n_t] {min start, max end, max start, min end}; no visible key: {INT_MAX, 0, ..}
-  int2* krange;           // [B, n_t] {first, last} query tile that sees the key tile (first > last: none)
+  int4* kstat;            // [B, n_t] the same of the query intervals
 };
 
 struct Agg {
-  int ds, lu, stop;  // max document start, max unmarked index, min stopping index
+  int ds, lu, stop, nf;  // max document start, max unmarked index, min stopping index, min document start
 };
 
 __device__ __forceinline__ int warp_max_scan(int v, int lane) {
@@ -142,18 +142,20 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
     const int i0 = c0 + st * kStep + tid * kPer;
     bool first[kPer], plain[kPer];
     load_flags(a, b, i0, len, first, plain);
-    Agg g{-1, -1, a.S};
+    Agg g{-1, -1, a.S, a.S};
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const int i = i0 + e;
       if (i >= a.S) continue;
       if (first[e]) g.ds = i;
+      if (first[e]) g.nf = min(g.nf, i);
       if (plain[e]) g.lu = i;
       if (first[e] || plain[e]) g.stop = min(g.stop, i);
     }
     g.ds = __reduce_max_sync(0xffffffffu, g.ds);
     g.lu = __reduce_max_sync(0xffffffffu, g.lu);
     g.stop = __reduce_min_sync(0xffffffffu, g.stop);
+    g.nf = __reduce_min_sync(0xffffffffu, g.nf);
     if (lane == 0) s_warp[warp] = g;
     __syncthreads();
     if (warp == 0) {
@@ -161,6 +163,7 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
       w.ds = __reduce_max_sync(0xffffffffu, w.ds);
       w.lu = __reduce_max_sync(0xffffffffu, w.lu);
       w.stop = __reduce_min_sync(0xffffffffu, w.stop);
+      w.nf = __reduce_min_sync(0xffffffffu, w.nf);
       if (lane == 0) {
         s_step[st] = w;
         if (st == 0) {
@@ -169,6 +172,7 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
           s_cta.ds = max(s_cta.ds, w.ds);
           s_cta.lu = max(s_cta.lu, w.lu);
           s_cta.stop = min(s_cta.stop, w.stop);
+          s_cta.nf = min(s_cta.nf, w.nf);
         }
       }
     }
@@ -176,27 +180,29 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
   }
 
   // ---- what lies left and right of this chunk
-  Agg left{-1, -1, a.S}, right{-1, -1, a.S};
+  Agg left{-1, -1, a.S, a.S}, right{-1, -1, a.S, a.S};
   if (n_cta > 1) {
     cluster_sync_all();
     for (int r = 0; r < n_cta; ++r) {
       if (r == rank) continue;
       const uint32_t addr = cluster_addr(&s_cta, r);
-      int ds, lu, stop;
+      int ds, lu, stop, nf;
       asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(ds) : "r"(addr) : "memory");
       asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(lu) : "r"(addr + 4) : "memory");
       asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(stop) : "r"(addr + 8) : "memory");
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(nf) : "r"(addr + 12) : "memory");
       if (r < rank) {
         left.ds = max(left.ds, ds);
         left.lu = max(left.lu, lu);
       } else {
         right.stop = min(right.stop, stop);
+        right.nf = min(right.nf, nf);
       }
     }
   }
 
   // ---- scan and write, right to left
-  int stop_right = right.stop;
+  int stop_right = right.stop, first_right = right.nf;
   for (int st = n_steps - 1; st >= 0; --st) {
     int ds_left = left.ds, lu_left = left.lu;
     for (int u = 0; u < st; ++u) {
@@ -206,7 +212,7 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
     const int i0 = c0 + st * kStep + tid * kPer;
     bool first[kPer], plain[kPer];
     load_flags(a, b, i0, len, first, plain);
-    int ds[kPer], lu[kPer], stop[kPer];  // inclusive from the left / stop: first stopping index > i
+    int ds[kPer], lu[kPer], stop[kPer], nf[kPer];  // inclusive from the left / first stop and document start > i
     int rd = -1, rl = -1;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
@@ -216,46 +222,63 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
       ds[e] = rd;
       lu[e] = rl;
     }
-    int rs = a.S;
+    int rs = a.S, rf = a.S;
 #pragma unroll
     for (int e = kPer - 1; e >= 0; --e) {
       stop[e] = rs;
+      nf[e] = rf;
+      if (i0 + e < a.S && first[e]) rf = i0 + e;
       if (i0 + e < a.S && (first[e] || plain[e])) rs = i0 + e;
     }
-    const int sd = warp_max_scan(rd, lane), sl = warp_max_scan(rl, lane), ss = warp_min_scan_right(rs, lane);
+    const int sd = warp_max_scan(rd, lane), sl = warp_max_scan(rl, lane), ss = warp_min_scan_right(rs, lane),
+              sf = warp_min_scan_right(rf, lane);
     __syncthreads();  // s_warp of the previous sweep has been read
     if (lane == 31) {
       s_warp[warp].ds = sd;
       s_warp[warp].lu = sl;
     }
-    if (lane == 0) s_warp[warp].stop = ss;
+    if (lane == 0) {
+      s_warp[warp].stop = ss;
+      s_warp[warp].nf = sf;
+    }
     __syncthreads();
-    int xd = ds_left, xl = lu_left, xs = stop_right;
+    int xd = ds_left, xl = lu_left, xs = stop_right, xf = first_right;
     {
       // the warps left of this one (starts, unmarked) and right of it (stops)
       const Agg w = s_warp[lane];
       xd = max(xd, __reduce_max_sync(0xffffffffu, lane < warp ? w.ds : -1));
       xl = max(xl, __reduce_max_sync(0xffffffffu, lane < warp ? w.lu : -1));
       xs = min(xs, __reduce_min_sync(0xffffffffu, lane > warp ? w.stop : a.S));
+      xf = min(xf, __reduce_min_sync(0xffffffffu, lane > warp ? w.nf : a.S));
     }
     int pd = __shfl_up_sync(0xffffffffu, sd, 1), pl = __shfl_up_sync(0xffffffffu, sl, 1);
-    int ns = __shfl_down_sync(0xffffffffu, ss, 1);
+    int ns = __shfl_down_sync(0xffffffffu, ss, 1), nn = __shfl_down_sync(0xffffffffu, sf, 1);
     if (lane == 0) pd = pl = -1;
-    if (lane == 31) ns = a.S;
+    if (lane == 31) ns = nn = a.S;
     xd = max(xd, pd);
     xl = max(xl, pl);
     xs = min(xs, ns);
-    if (!alone) stop_right = min(stop_right, s_step[st].stop);
+    xf = min(xf, nn);
+    if (!alone) {
+      stop_right = min(stop_right, s_step[st].stop);
+      first_right = min(first_right, s_step[st].nf);
+    }
 
     int smin = INT_MAX, emax = 0, smax = 0, emin = INT_MAX;
-    int vs[kPer], ve[kPer], vp[kPer];
+    int qmin = INT_MAX, qemax = 0, qmax = 0, qemin = INT_MAX;
+    int vs[kPer], ve[kPer], vp[kPer], ws[kPer], we[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const int i = i0 + e;
-      vs[e] = ve[e] = vp[e] = 0;
+      vs[e] = ve[e] = vp[e] = ws[e] = we[e] = 0;
       if (i < len) {
         vs[e] = max(xd, ds[e]);
-        ve[e] = max(xl, lu[e]) < vs[e] ? min(xs, stop[e]) : i + 1;
+        const bool in_prefix = max(xl, lu[e]) < vs[e];
+        ve[e] = in_prefix ? min(xs, stop[e]) : i + 1;
+        ws[e] = in_prefix ? vs[e] : i;
+        we[e] = min(min(xf, nf[e]), len);
+        qmin = min(qmin, ws[e]);
+        qemax = max(qemax, we[e]);
         vp[e] = i - vs[e];
         smin = min(smin, vs[e]);
         emax = max(emax, ve[e]);
@@ -263,6 +286,8 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
       if (i < a.S) {
         smax = max(smax, vs[e]);
         emin = min(emin, ve[e]);
+        qmax = max(qmax, ws[e]);
+        qemin = min(qemin, we[e]);
       }
     }
     const int tile = i0 / 128;  // one tile per warp
@@ -281,49 +306,24 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
             a.end[row0 + i0 + e] = ve[e];
           }
       }
-      int* tr = a.rows + ((size_t)b * a.n_t + tile) * 256 + lane * kPer;
+      int* tr = a.rows + ((size_t)b * a.n_t + tile) * 512 + lane * kPer;
       *reinterpret_cast<int4*>(tr) = make_int4(vs[0], vs[1], vs[2], vs[3]);
       *reinterpret_cast<int4*>(tr + 128) = make_int4(ve[0], ve[1], ve[2], ve[3]);
+      *reinterpret_cast<int4*>(tr + 256) = make_int4(ws[0], ws[1], ws[2], ws[3]);
+      *reinterpret_cast<int4*>(tr + 384) = make_int4(we[0], we[1], we[2], we[3]);
       smin = __reduce_min_sync(0xffffffffu, smin);
       emax = __reduce_max_sync(0xffffffffu, emax);
       smax = __reduce_max_sync(0xffffffffu, smax);
       emin = __reduce_min_sync(0xffffffffu, emin);
-      if (lane == 0) a.qstat[(size_t)b * a.n_t + tile] = make_int4(smin, emax, smax, emin);
+      qmin = __reduce_min_sync(0xffffffffu, qmin);
+      qemax = __reduce_max_sync(0xffffffffu, qemax);
+      qmax = __reduce_max_sync(0xffffffffu, qmax);
+      qemin = __reduce_min_sync(0xffffffffu, qemin);
+      if (lane == 0) {
+        a.qstat[(size_t)b * a.n_t + tile] = make_int4(smin, emax, smax, emin);
+        a.kstat[(size_t)b * a.n_t + tile] = make_int4(qmin, qemax, qmax, qemin);
+      }
     }
-  }
-
-  // ---- query tiles that see each key tile: both bounds are nondecreasing over the tiles that see
-  // anything, and tiles that see nothing come last, so two binary searches find them
-  __threadfence();
-  if (n_cta > 1) {
-    cluster_sync_all();
-  } else {
-    __syncthreads();
-  }
-  const int4* qs = a.qstat + (size_t)b * a.n_t;
-  extern __shared__ int2 s_bounds[];  // [n_t] (min start, max end) where that fits, to search without global loads
-  if (a.staged) {
-    for (int t = tid; t < a.n_t; t += kThreads) {
-      const int2 v = __ldcg(reinterpret_cast<const int2*>(qs + t));
-      s_bounds[t] = v;
-    }
-    __syncthreads();
-  }
-  for (int kt = c0 / 128 + tid; kt < min((c1 + 127) / 128, a.n_t); kt += kThreads) {
-    int lo = 0, hi = a.n_t;  // first tile with max end > kt * 128 (a tile that sees nothing counts as above)
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      const int emax = a.staged ? s_bounds[mid].y : __ldcg(&qs[mid].y);
-      if (emax == 0 || emax > kt * 128) hi = mid;
-      else lo = mid + 1;
-    }
-    int l2 = 0, h2 = a.n_t;  // first tile with min start >= (kt + 1) * 128
-    while (l2 < h2) {
-      const int mid = (l2 + h2) / 2;
-      if ((a.staged ? s_bounds[mid].x : __ldcg(&qs[mid].x)) >= (kt + 1) * 128) h2 = mid;
-      else l2 = mid + 1;
-    }
-    a.krange[(size_t)b * a.n_t + kt] = make_int2(lo, l2 - 1);
   }
   if (n_cta > 1) cluster_sync_all();  // no CTA leaves while its s_cta may still be read
 }
@@ -335,13 +335,13 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
 constexpr int kBins = 2048;
 struct OrderArgs {
   const int4* qstat;
-  const int2* krange;
+  const int4* kstat;
   int B, n_t, n_pairs, shift;  // weight >> shift < kBins
   int* out[3];
 };
 
-__device__ __forceinline__ int tile_weight(const OrderArgs& a, int b, int t) {
-  const int4 q = a.qstat[(size_t)b * a.n_t + t];
+__device__ __forceinline__ int tile_weight(const int4* stat, const OrderArgs& a, int b, int t) {
+  const int4 q = stat[(size_t)b * a.n_t + t];
   return q.y == 0 ? 0 : (q.y + 127) / 128 - q.x / 128;
 }
 
@@ -356,12 +356,9 @@ __global__ void __launch_bounds__(kThreads) plan_order_kernel(const OrderArgs a)
     int w;
     if (which == 0) {
       const int t1 = (a.n_t & 1) ? 2 * t : 2 * t + 1;
-      w = tile_weight(a, b, t1) + (t1 > 0 ? tile_weight(a, b, t1 - 1) : 0);
-    } else if (which == 1) {
-      w = tile_weight(a, b, t);
+      w = tile_weight(a.qstat, a, b, t1) + (t1 > 0 ? tile_weight(a.qstat, a, b, t1 - 1) : 0);
     } else {
-      const int2 r = a.krange[(size_t)b * a.n_t + t];
-      w = max(0, r.y + 1 - r.x);
+      w = tile_weight(which == 1 ? a.qstat : a.kstat, a, b, t);
     }
     return kBins - 1 - (w >> a.shift);
   };
@@ -403,7 +400,7 @@ int document_plan_max_len() { return docplan::kMaxCtas * docplan::kMaxSteps * do
 
 int document_plan(const long* ids, long ld_ids, long eod, int by_change, const unsigned char* marks, long ld_marks,
                   const int* lengths, int B, int S, int* positions, int* start, int* end, int* rows, void* qstat,
-                  void* krange, int* order, cudaStream_t stream) {
+                  void* kstat, int* order, cudaStream_t stream) {
   using namespace docplan;
   if (B < 1 || S < 1 || S > document_plan_max_len() || (long)B * ((S + 127) / 128) > INT_MAX / 8) return -1;
   Args a;
@@ -424,14 +421,12 @@ int document_plan(const long* ids, long ld_ids, long eod, int by_change, const u
   a.end = end;
   a.rows = rows;
   a.qstat = static_cast<int4*>(qstat);
-  a.krange = static_cast<int2*>(krange);
+  a.kstat = static_cast<int4*>(kstat);
   const int n_cta = (S + a.chunk - 1) / a.chunk;
   if ((long)B * n_cta > INT_MAX) return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * n_cta));
   cfg.blockDim = dim3(kThreads);
-  a.staged = a.n_t <= 4096;
-  cfg.dynamicSmemBytes = a.staged ? a.n_t * sizeof(int2) : 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -445,7 +440,7 @@ int document_plan(const long* ids, long ld_ids, long eod, int by_change, const u
   if (e != cudaSuccess || !order) return (int)e;
   OrderArgs o;
   o.qstat = a.qstat;
-  o.krange = a.krange;
+  o.kstat = a.kstat;
   o.B = B;
   o.n_t = a.n_t;
   o.n_pairs = (a.n_t + 1) / 2;

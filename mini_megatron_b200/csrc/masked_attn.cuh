@@ -27,32 +27,45 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
 
 struct Mask {
-  const int* rows;     // [B, n_t, 2, 128] start, end (tile-padded), nullptr: causal
-  const int4* qstat;   // [B, n_t] {min start, max end, max start, min end}
-  const int2* krange;  // [B, n_t] {first, last} query tile
-  const int* order;    // this kernel's tiles of all rows, heaviest first, or nullptr: by position
+  const int* rows;    // [B, n_t, 4, 128] start, end; the queries that see the token as a key (tile-padded); nullptr: causal
+  const int4* qstat;  // [B, n_t] {min start, max end, max start, min end}
+  const int4* kstat;  // [B, n_t] the same of the query intervals
+  const int* order;   // this kernel's tiles of all rows, heaviest first, or nullptr: by position
 };
 
-// Key tiles [x, y) that query tile t of row b needs.
-__device__ __forceinline__ int2 key_tiles(const Mask& m, int b, int n_t, int t) {
-  if (!m.rows) return make_int2(0, t + 1);
-  const int4 q = m.qstat[(size_t)b * n_t + t];
-  if (q.y == 0) return make_int2(0, 0);
-  return make_int2(q.x / BT, (q.y + BT - 1) / BT);
+// Tiles [x, y) of the other side that a tile with these bounds needs, and those of them that need no mask: every row
+// sees all of the tile.  (Rows behind the end of the sequence do not count: what they read is zero.)
+__device__ __forceinline__ int2 needed_tiles(const int4& q) {
+  return q.y == 0 ? make_int2(0, 0) : make_int2(q.x / BT, (q.y + BT - 1) / BT);
 }
+__device__ __forceinline__ int2 whole_tiles(const int4& q) { return make_int2((q.z + BT - 1) / BT, q.w / BT); }
 
-// The key tiles of query tile t that need no mask: every row of t sees all of them ([x, y)).
-__device__ __forceinline__ int2 full_tiles(const Mask& m, int b, int n_t, int t) {
-  if (!m.rows) return make_int2(0, t);
+// Key tiles of query tile t of row b.
+__device__ __forceinline__ void key_tiles(const Mask& m, int b, int n_t, int t, int2& need, int2& whole) {
+  if (!m.rows) {
+    need = make_int2(0, t + 1);
+    whole = make_int2(0, t);
+    return;
+  }
   const int4 q = m.qstat[(size_t)b * n_t + t];
-  return make_int2((q.z + BT - 1) / BT, q.w / BT);
+  need = needed_tiles(q);
+  whole = whole_tiles(q);
 }
-
-// Query tiles [x, y) that see key tile kt of row b.
-__device__ __forceinline__ int2 query_tiles(const Mask& m, int b, int n_t, int kt) {
-  if (!m.rows) return make_int2(kt, n_t);
-  const int2 r = m.krange[(size_t)b * n_t + kt];
-  return make_int2(r.x, max(r.x, r.y + 1));
+// Query tiles of key tile t of row b.
+__device__ __forceinline__ void query_tiles(const Mask& m, int b, int n_t, int t, int2& need, int2& whole) {
+  if (!m.rows) {
+    need = make_int2(t, n_t);
+    whole = make_int2(t + 1, n_t);
+    return;
+  }
+  const int4 q = m.kstat[(size_t)b * n_t + t];
+  need = needed_tiles(q);
+  whole = whole_tiles(q);
+}
+// Which of 32 consecutive rows or columns from `first` on lie in [lo, hi).
+__device__ __forceinline__ uint32_t seen_bits(int lo, int hi, int first) {
+  const int l = min(max(lo - first, 0), 32), h = min(max(hi - first, 0), 32);
+  return (h >= 32 ? 0xffffffffu : (1u << h) - 1u) & ~(l >= 32 ? 0xffffffffu : (1u << l) - 1u);
 }
 
 // Item of this CTA in round `r`: every other round runs backwards over the CTAs, so that with items

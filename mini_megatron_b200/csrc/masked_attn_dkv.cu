@@ -9,8 +9,9 @@
 // Persistent grid, one CTA per SM; a work item is (batch, K/V head, 128-row key
 // tile).  Scores are computed transposed (a thread owns a key row), so P^T and dS^T
 // go back into TMEM as the first operands of the two sums and never touch shared
-// memory; LSE, Delta and the visible intervals of the query rows arrive with the
-// Q / dO tiles by bulk copies from tile-padded arrays.  Roles (20 warps, two of them idle):
+// memory; LSE and Delta of the query rows arrive with the Q / dO tiles by bulk copies.
+// The queries that see a key are an interval too (document_plan.cu), so a mask is two
+// numbers per thread here as well.  Roles (20 warps, one of them idle):
 //
 //   warp 0     TMA: K_j, V_j per item; Q_i, dO_i and their row data into a ring
 //   warp 1     TMEM allocation; one thread issues S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
@@ -37,8 +38,7 @@ struct Cfg {
   static constexpr int SB = (D == 64) ? 2 : 1;  // S^T buffers in TMEM
   static constexpr int K_OFF = 0;               // [KB][K, V]
   static constexpr int Q_OFF = KB * 2 * TILE;   // [NQ][Q, dO]
-  // [NQ][-LSE log2 e 128, -Delta 128, start 128, end 128, {min start, max end, max start, min end}]
-  static constexpr int LD_OFF = Q_OFF + NQ * 2 * TILE, LD = 2176;
+  static constexpr int LD_OFF = Q_OFF + NQ * 2 * TILE, LD = 1024;  // [NQ][-LSE log2 e 128, -Delta 128]
   static constexpr int ITEM_OFF = LD_OFF + NQ * LD;  // [kRing] work items
   static constexpr int BAR_OFF = ITEM_OFF + kRing * 32;
   static constexpr int SMEM = 1024 + BAR_OFF + 384;
@@ -64,7 +64,7 @@ struct Args {
 struct alignas(16) Item {
   int b, hk, t;  // b < 0: no more items
   int part;      // which share of the K/V head's query heads
-  int2 r;        // query tiles
+  int2 r, f;     // query tiles, and those of them that need no mask
 };
 static_assert(sizeof(Item) <= 32, "ring entry");
 constexpr int kConsumers = 1 + 1 + kWarps;  // TMA and MMA threads, softmax warps
@@ -83,8 +83,17 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
     it.t = a.by_B.quot(li);
     it.b = li - it.t * a.B;
   }
-  it.r = query_tiles(a.mask, it.b, a.n_t, it.t);
+  query_tiles(a.mask, it.b, a.n_t, it.t, it.r, it.f);
   return it;
+}
+
+// 32 bytes of one row.
+__device__ __forceinline__ void store8(float* p, const uint32_t* v, float mul) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(__uint_as_float(v[0]) * mul),
+               "f"(__uint_as_float(v[1]) * mul), "f"(__uint_as_float(v[2]) * mul), "f"(__uint_as_float(v[3]) * mul),
+               "f"(__uint_as_float(v[4]) * mul), "f"(__uint_as_float(v[5]) * mul), "f"(__uint_as_float(v[6]) * mul),
+               "f"(__uint_as_float(v[7]) * mul)
+               : "memory");
 }
 
 // (head of the item's share, query tile) pairs of this CTA's items, one after another.
@@ -218,15 +227,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int st = n % NQ;
           if (n >= NQ && !bwait(&q_empty[st], ((n / NQ) - 1) & 1, a.err, abort_flag)) { ok = false; break; }
           const int h = (x.w.hk * a.parts + x.w.part) * heads + x.g;
-          mbar_expect_tx(&q_full[st], 2 * C::TILE + 1024 + (a.mask.rows ? 1040 : 0));
+          mbar_expect_tx(&q_full[st], 2 * C::TILE + 1024);
           load_tile<D>(sQ + st * 2 * C::TILE, &tm_qkv, &q_full[st], h * D, x.i * BT, x.w.b);
           load_tile<D>(sQ + st * 2 * C::TILE + C::TILE, &tm_do, &q_full[st], h * D, x.i * BT, x.w.b);
           bulk_load(sLD + st * C::LD, a.ld + (((size_t)x.w.b * a.nh + h) * a.n_t + x.i) * (2 * BT), 1024, &q_full[st]);
-          if (a.mask.rows) {
-            const size_t bt = (size_t)x.w.b * a.n_t + x.i;
-            bulk_load(sLD + st * C::LD + 1024, a.mask.rows + bt * (2 * BT), 1024, &q_full[st]);
-            bulk_load(sLD + st * C::LD + 2048, a.mask.qstat + bt, 16, &q_full[st]);
-          }
         }
         if (!ok) {
           for (int u = max(0, k_issued - KB + 1); u <= k_issued; ++u) drain_wait(&k_full[u % KB], (u / KB) & 1);
@@ -340,6 +344,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         continue;
       }
+      int first = key, last = a.n_t * BT;
+      if (a.mask.rows) {
+        const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + w.t) * (4 * BT) + 2 * BT + row;
+        first = tr[0];
+        last = tr[BT];
+      }
       for (int g = 0; ok && g < heads; ++g) {
         float slope = 0.f;
         if (BIAS) slope = a.slopes[(w.hk * a.parts + w.part) * heads + g] * kLog2e;
@@ -348,15 +358,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t t_s = tmem + C::T_S + (n % SB) * 128 + lane_off + part * 32;
           const uint32_t t_dp = tmem + C::T_DP + lane_off + part * 32;
           const float* l2 = reinterpret_cast<const float*>(sLD + st * C::LD) + part * 32;
-          const int* start = reinterpret_cast<const int*>(l2 + 2 * BT);
           if (!wwait(&q_full[st], (n / NQ) & 1, a.err, abort_flag)) { ok = false; break; }
           if (!wwait(&s_full[n % SB], (n / SB) & 1, a.err, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          bool masked = i == w.t;  // causal: only the diagonal tile
-          if (a.mask.rows) {
-            const int4 q = *reinterpret_cast<const int4*>(sLD + st * C::LD + 2048);
-            masked = q.z > w.t * BT || q.w < (w.t + 1) * BT;
-          }
+          const bool masked = i < w.f.x || i >= w.f.y;
           float pf[32];  // P (1 - tanh^2)
           {
             uint32_t s[32];
@@ -364,24 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_ld();
             if (CAP) cap_in_place(s, k);
             const int q0 = i * BT + part * 32;  // query of column 0
-            uint32_t seen = 0xffffffffu;
-            if (masked) {
-              if (a.mask.rows) {
-                seen = 0;
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                  const int4 lo = *reinterpret_cast<const int4*>(start + e);
-                  const int4 hi = *reinterpret_cast<const int4*>(start + BT + e);
-                  seen |= (key >= lo.x && key < hi.x ? 1u : 0u) << e;
-                  seen |= (key >= lo.y && key < hi.y ? 2u : 0u) << e;
-                  seen |= (key >= lo.z && key < hi.z ? 4u : 0u) << e;
-                  seen |= (key >= lo.w && key < hi.w ? 8u : 0u) << e;
-                }
-              } else {
-                const int l0 = min(max(key - q0, 0), 32);  // query q sees the key iff q >= key
-                seen = ~(l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u);
-              }
-            }
+            const uint32_t seen = masked ? seen_bits(first, last, q0) : 0xffffffffu;
             const float dist = (float)(q0 - key);
             uint32_t pp[16];
 #pragma unroll
@@ -455,13 +443,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (in) {
             float* pk = share_row();
 #pragma unroll
-            for (int c = 0; c < D / 4; c += 4) {
-              *reinterpret_cast<float4*>(pk + c) =
-                  make_float4(__uint_as_float(u[c]) * a.scale, __uint_as_float(u[c + 1]) * a.scale,
-                              __uint_as_float(u[c + 2]) * a.scale, __uint_as_float(u[c + 3]) * a.scale);
-              *reinterpret_cast<float4*>(pk + (size_t)a.nkv * D + c) =
-                  make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
-                              __uint_as_float(v[c + 3]));
+            for (int c = 0; c < D / 4; c += 8) {
+              store8(pk + c, &u[c], a.scale);
+              store8(pk + (size_t)a.nkv * D + c, &v[c], 1.f);
             }
           }
         } else {
@@ -541,7 +525,7 @@ int masked_attn_dkv_parts(int B, int S, int nh, int nkv, int num_sms) {
   const long items = (long)B * nkv * ((S + mattn::BT - 1) / mattn::BT);
   const int group = nh / nkv;
   for (int p = 1; p < group; ++p)
-    if (group % p == 0 && items * p >= 3L * num_sms) return p;
+    if (group % p == 0 && items * p >= 2L * num_sms) return p;
   return group;
 }
 
@@ -573,7 +557,7 @@ int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb,
   a.by_B = FastDiv(c.B);
   a.by_tiles = FastDiv(n_t);
   a.partial = partial;
-  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange), c.order_k};
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int4*>(c.kstat), c.order_k};
   a.slopes = c.slopes;
   a.score = score_constants(c.scale, c.cap);
   a.scale = c.scale;

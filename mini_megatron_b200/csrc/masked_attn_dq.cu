@@ -87,8 +87,7 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
     it.b = li - q * a.B;
     it.t = a.n_t - 1 - q;
   }
-  it.r = key_tiles(a.mask, it.b, a.n_t, it.t);
-  it.f = full_tiles(a.mask, it.b, a.n_t, it.t);
+  key_tiles(a.mask, it.b, a.n_t, it.t, it.r, it.f);
   return it;
 }
 
@@ -320,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       int start = 0, end = i + 1;
       if (a.mask.rows) {
-        const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + w.t) * (2 * BT) + row;
+        const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + w.t) * (4 * BT) + row;
         start = tr[0];
         end = tr[BT];
       }
@@ -362,8 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             pf[e + 1] = x.y;
           }
           if (j < w.f.x || j >= w.f.y) {
-            const int l0 = min(max(start - j0, 0), 32), h0 = min(max(end - j0, 0), 32);
-            const uint32_t seen = (h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u) & ~(l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u);
+            const uint32_t seen = seen_bits(start, end, j0);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!(seen & (1u << e))) pf[e] = 0.f;
@@ -533,7 +531,7 @@ int masked_attn_dq(const AttnCall& c, const void* dout, long do_ss, long do_sb, 
   a.by_B = FastDiv(c.B);
   a.by_tiles = FastDiv(n_t);
   a.by_group = FastDiv(c.nh / c.nkv);
-  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange), c.order_q};
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int4*>(c.kstat), c.order_q};
   a.slopes = c.slopes;
   a.score = score_constants(c.scale, c.cap);
   a.scale = c.scale;

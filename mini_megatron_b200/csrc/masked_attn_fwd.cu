@@ -96,11 +96,9 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
   it.t0 = it.t1 - 1;
   it.r0 = it.f0 = make_int2(0, 0);
   if (it.t0 >= 0) {
-    it.r0 = key_tiles(a.mask, it.b, a.n_t, it.t0);
-    it.f0 = full_tiles(a.mask, it.b, a.n_t, it.t0);
+    key_tiles(a.mask, it.b, a.n_t, it.t0, it.r0, it.f0);
   }
-  it.r1 = key_tiles(a.mask, it.b, a.n_t, it.t1);
-  it.f1 = full_tiles(a.mask, it.b, a.n_t, it.t1);
+  key_tiles(a.mask, it.b, a.n_t, it.t1, it.r1, it.f1);
   const bool a0 = it.r0.y > it.r0.x, a1 = it.r1.y > it.r1.x;
   it.lo = a0 ? (a1 ? min(it.r0.x, it.r1.x) : it.r0.x) : it.r1.x;
   it.hi = max(it.r0.y, it.r1.y);
@@ -330,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int i = t * BT + row;
       int start = 0, end = i + 1;
       if (a.mask.rows) {
-        const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + t) * (2 * BT) + row;
+        const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + t) * (4 * BT) + row;
         start = tr[0];
         end = tr[BT];
       }
@@ -363,13 +361,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (j < full.x || j >= full.y) {
-          const int lo = start - j * BT, hi = end - j * BT;  // visible columns [lo, hi)
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const int l0 = min(max(lo - 32 * g, 0), 32), h0 = min(max(hi - 32 * g, 0), 32);
-            const uint32_t below_h = h0 >= 32 ? 0xffffffffu : (1u << h0) - 1u;
-            const uint32_t below_l = l0 >= 32 ? 0xffffffffu : (1u << l0) - 1u;
-            const uint32_t seen = below_h & ~below_l;
+            const uint32_t seen = seen_bits(start, end, j * BT + 32 * g);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!(seen & (1u << e))) s[32 * g + e] = 0xff800000u;  // -inf
@@ -562,7 +556,7 @@ int masked_attn_fwd(const AttnCall& c, void* out, float* lse, int* err, int num_
   a.by_B = FastDiv(c.B);
   a.by_pairs = FastDiv(a.n_pairs);
   a.by_group = FastDiv(c.nh / c.nkv);
-  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int2*>(c.krange), c.order_p};
+  a.mask = Mask{c.rows, static_cast<const int4*>(c.qstat), static_cast<const int4*>(c.kstat), c.order_p};
   a.slopes = c.slopes;
   a.score = score_constants(c.scale, c.cap);
   a.out = static_cast<__nv_bfloat16*>(out);

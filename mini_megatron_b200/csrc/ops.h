@@ -105,7 +105,7 @@ int document_plan_max_len();
 constexpr int kUnorderedTiles = 4;
 int document_plan(const long* ids, long ld_ids, long eod, int by_change, const unsigned char* marks, long ld_marks,
                   const int* lengths, int B, int S, int* positions, int* start, int* end, int* rows, void* qstat,
-                  void* krange, int* order, cudaStream_t stream);
+                  void* kstat, int* order, cudaStream_t stream);
 
 // Rotary positions (rotary.cu): heads [0, heads_rot) of x rotated into y (y may be x), the rest copied.
 int rotary(const void* x, long x_sb, long x_ss, void* y, long y_sb, long y_ss, int is_f32, const void* positions,
@@ -119,7 +119,7 @@ struct AttnCall {
   int B, S, nh, nkv, d;
   const int* rows;       // of document_plan, or nullptr: causal
   const void* qstat;
-  const void* krange;
+  const void* kstat;
   const int* order_p;    // query tile pairs, query tiles and key tiles of all rows, heaviest first
   const int* order_q;
   const int* order_k;

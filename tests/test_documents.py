@@ -41,24 +41,32 @@ def test_plan_cpu(B, S, doc, prefix, pad, empty, by_ids):
 
 
 def _tile_tables(plan):
-    """What the attention kernels read, by its definition."""
+    """What the attention kernels read, by its definition from the dense mask: intervals of both sides, their bounds."""
     B, S = plan.shape
     n_t = (S + 127) // 128
-    start = torch.zeros(B, n_t * 128, dtype=torch.int32)
-    end = torch.zeros(B, n_t * 128, dtype=torch.int32)
-    start[:, :S], end[:, :S] = plan.start.cpu(), plan.end.cpu()
-    rows = torch.stack([start.view(B, n_t, 128), end.view(B, n_t, 128)], 2)
-    qstat = torch.empty(B, n_t, 4, dtype=torch.int32)
-    seen = torch.zeros(B, n_t, n_t, dtype=torch.bool)
-    for b in range(B):
+    dense = plan.visible().cpu()
+
+    def side(mask):
+        lo = torch.zeros(B, n_t * 128, dtype=torch.int32)
+        hi = torch.zeros(B, n_t * 128, dtype=torch.int32)
+        some = mask.any(2)
+        at = torch.arange(S)
+        lo[:, :S] = torch.where(some, torch.where(mask, at, S).amin(2), 0)
+        hi[:, :S] = torch.where(some, torch.where(mask, at, -1).amax(2) + 1, 0)
+        assert torch.equal(mask.sum(2), (hi - lo)[:, :S].long())      # intervals without holes
+        stat = torch.empty(B, n_t, 4, dtype=torch.int32)
         for t in range(n_t):
-            s, e = start[b, t * 128:min(S, t * 128 + 128)], end[b, t * 128:min(S, t * 128 + 128)]
-            some = e > s
-            qstat[b, t] = torch.tensor([s[some].min() if some.any() else 2 ** 31 - 1, e[some].max() if some.any() else 0,
-                                        s.max(), e.min()])
-            for k in range(n_t):
-                seen[b, t, k] = bool(((s < k * 128 + 128) & (e > k * 128) & some).any())
-    return rows, qstat, seen
+            cut = slice(t * 128, min(S, t * 128 + 128))
+            l, h = lo[:, cut], hi[:, cut]
+            seen = h > l
+            stat[:, t, 0] = torch.where(seen, l, 2 ** 31 - 1).amin(1)
+            stat[:, t, 1] = torch.where(seen, h, 0).amax(1)
+            stat[:, t, 2], stat[:, t, 3] = l.amax(1), h.amin(1)
+        return lo.view(B, n_t, 1, 128), hi.view(B, n_t, 1, 128), stat
+
+    qlo, qhi, qstat = side(dense)
+    klo, khi, kstat = side(dense.transpose(1, 2))
+    return torch.cat([qlo, qhi, klo, khi], 2), qstat, kstat
 
 
 @pytest.mark.gpu
@@ -69,34 +77,21 @@ def test_plan_gpu(B, S, doc, prefix, pad, empty, by_ids):
     plan = _check("cuda", B, S, doc, prefix, pad, empty, by_ids)
     if S > 10000:
         return
-    rows, qstat, seen = _tile_tables(plan)
-    n_t = seen.shape[1]
-    sizes = [rows.numel(), qstat.numel(), B * n_t * 2, B * ((n_t + 1) // 2 + 2 * n_t) if n_t > 4 else 0]
-    got_rows, got_stat, got_range, order = plan.tables.cpu().split(sizes)
-    got_rows, got_stat, got_range = got_rows.view_as(rows), got_stat.view_as(qstat), got_range.view(B, n_t, 2)
-    assert torch.equal(got_rows, rows)
-    assert torch.equal(got_stat, qstat)
-    for b in range(B):
-        for k in range(n_t):
-            lo, hi = got_range[b, k].tolist()
-            want = seen[b, :, k].nonzero().flatten().tolist()
-            # every tile that sees the key tile is in the range (a range may hold a tile that does not)
-            assert all(lo <= t <= hi for t in want), (b, k, lo, hi, want)
-            assert 0 <= lo and hi < n_t
-            if not want:
-                assert lo > hi or not seen[b, lo:hi + 1, k].any()
-    if n_t <= 4:
-        return
-    # every tile once, heaviest first
+    rows, qstat, kstat = _tile_tables(plan)
+    n_t = qstat.shape[1]
     n_p = (n_t + 1) // 2
-    keys = torch.where(qstat[..., 1] == 0, 0, (qstat[..., 1] + 127) // 128 - qstat[..., 0] // 128)
-    pairs = torch.zeros(B, n_p, dtype=torch.int32)
+    parts = [rows.numel(), qstat.numel(), kstat.numel()] + ([B * n_p, B * n_t, B * n_t] if n_t > 4 else [])
+    got_rows, got_q, got_k, *orders = plan.tables.cpu().split(parts)
+    assert torch.equal(got_rows.view_as(rows), rows)
+    assert torch.equal(got_q.view_as(qstat), qstat) and torch.equal(got_k.view_as(kstat), kstat)
+    # every tile once, heaviest first
+    keys, queries = (torch.where(s[..., 1] == 0, 0, (s[..., 1] + 127) // 128 - s[..., 0] // 128) for s in (qstat, kstat))
+    pairs = torch.zeros(B, n_p, dtype=torch.int64)
     for t in range(n_t):
         pairs[:, (t + 1) // 2 if n_t % 2 else t // 2] += keys[:, t]
-    queries = (got_range[..., 1] + 1 - got_range[..., 0]).clamp_min(0)
-    for part, weight in zip(order.split([B * n_p, B * n_t, B * n_t]), (pairs, keys, queries)):
-        assert torch.equal(part.sort().values, torch.arange(len(part), dtype=torch.int32))
-        along = weight.flatten()[part.long()]
+    for order, weight in zip(orders, (pairs, keys, queries)):
+        assert torch.equal(order.sort().values, torch.arange(len(order), dtype=torch.int32))
+        along = weight.flatten()[order.long()]
         assert (along[1:] <= along[:-1]).all()
 
 
