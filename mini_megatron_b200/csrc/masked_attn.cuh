@@ -356,14 +356,15 @@ __device__ __forceinline__ void mma_abt(uint32_t dst, uint32_t a_addr, uint32_t 
 }
 
 // 128 x D (+)= A [128 x 128, bf16 in TMEM] B [128 x D] (rows are the reduction: MN-major).  A's 128
-// columns lie in runs of RUN (RUN / 2 TMEM columns) that start STRIDE TMEM columns apart.
-template <int D, int RUN, int STRIDE = 32>
+// columns lie in runs of RUN (RUN / 2 TMEM columns) that start STRIDE TMEM columns apart.  K0, K1: part of the
+// reduction, in steps of 16.
+template <int D, int RUN, int STRIDE = 32, int K0 = 0, int K1 = BT / 16>
 __device__ __forceinline__ void mma_tmem_b(uint32_t dst, uint32_t a_tmem, uint32_t b_addr, bool acc) {
   constexpr int PER = RUN / 16;
   constexpr uint32_t idesc = make_idesc_bf16(BT, D, false, true);
   const uint64_t bd = make_sdesc_sw128(b_addr, 16384, 1024);
 #pragma unroll
-  for (int k = 0; k < BT / 16; ++k)
+  for (int k = K0; k < K1; ++k)
     umma_bf16_ts(dst, a_tmem + (k / PER) * STRIDE + (k % PER) * 8, bd + (uint64_t)(k * (2048 >> 4)), idesc,
                  (acc || k != 0) ? 1u : 0u);
 }

@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_empty = v_full + NS;    // [NS]
   uint64_t* s_full = v_empty + NS;    // [2]  S_i computed
   uint64_t* s_free = s_full + 2;      // [2]  S_i in registers (SEP; 4 warps)
-  uint64_t* p_full = s_free + 2;      // [2]  P_i written (4 warps)
-  uint64_t* p_free = p_full + 2;      // [2]  PV_i that read P_i complete (SEP)
+  uint64_t* p_full = s_free + 2;      // [2][2]  first / other 64 keys of P_i written (4 warps)
+  uint64_t* p_free = p_full + 4;      // [2]  PV_i that read P_i complete (SEP)
   uint64_t* o_full = p_free + 2;      // [2]  last PV_i of the item complete
   uint64_t* o_free = o_full + 2;      // [2]  O_i and its statistics read by the epilogue (4 warps)
   uint64_t* ml_full = o_free + 2;     // [2]  statistics of the item written (4 warps)
@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_empty[i], 2);
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&p_free[i], 1);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 4);
@@ -260,11 +261,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = u % NS;
         if (!bwait(&v_full[st], (u / NS) & 1, a.err, abort_flag)) return false;
         if (on) {
-          if (!bwait(&p_full[grp], pc & 1, a.err, abort_flag)) return false;
-          ++pc;
+          // the first 64 keys' share runs while the softmax is at the other 64
+          if (!bwait(&p_full[2 * grp], pc & 1, a.err, abort_flag)) return false;
           if (first && ic > 0 && !bwait(&o_free[grp], (ic - 1) & 1, a.err, abort_flag)) return false;
           tc_fence_after();
-          mma_tmem_b<D, 64>(t_o, t_p, smem_u32(sV + st * C::TILE), !first);
+          mma_tmem_b<D, 64, 32, 0, 4>(t_o, t_p, smem_u32(sV + st * C::TILE), !first);
+          if (!bwait(&p_full[2 * grp + 1], pc & 1, a.err, abort_flag)) return false;
+          ++pc;
+          tc_fence_after();
+          mma_tmem_b<D, 64, 32, 4, 8>(t_o, t_p, smem_u32(sV + st * C::TILE), true);
           if (SEP) umma_commit(&p_free[grp]);
           if (last) umma_commit(&o_full[grp]);
         }
@@ -369,18 +374,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!(seen & (1u << e))) s[32 * g + e] = 0xff800000u;  // -inf
           }
         }
-        float mx[4];
+        float mx[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = __uint_as_float(s[u]);
+        for (int u = 0; u < 8; ++u) mx[u] = __uint_as_float(s[u]);
 #pragma unroll
-        for (int c = 4; c < 124; c += 8) {
+        for (int c = 8; c < 120; c += 16) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
+          for (int u = 0; u < 8; ++u)
             mx[u] = max3(mx[u], __uint_as_float(s[c + 2 * u]), __uint_as_float(s[c + 2 * u + 1]));
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], __uint_as_float(s[124 + u]));
-        float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+        for (int u = 0; u < 8; ++u) mx[u] = fmaxf(mx[u], __uint_as_float(s[120 + u]));
+        float mt = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
         if (!CAP && !BIAS) mt *= k.mul;
         const bool need = mt > m + kRescaleLog2;
         const bool any_need = __any_sync(0xffffffffu, need) != 0;
@@ -390,12 +395,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = mt;
         }
         const float mu = m == -INFINITY ? 0.f : m;  // a row that has seen nothing: every exponential is 0
-        if (SEP) {
-          // the PV that read the previous P_i (and last wrote O_i) must be complete
-          if (pc > 0 && !wwait(&p_free[grp], (pc - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-          tc_fence_after();
+        // SEP: before P_i's columns (and O_i) are written, the PV that read the previous P_i (and last wrote O_i) must be
+        // complete; that wait sits behind the first half of the exponentials unless O_i has to be rescaled
+        bool waited = !SEP || pc == 0;
+        if (any_need && j > range.x) {
+          if (!waited) {
+            if (!wwait(&p_free[grp], (pc - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            waited = true;
+          }
+          // otherwise PV_i(j-1) was issued before S_i(j), which is complete
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(t_o + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_x32(t_o + c * 32, o);
+          }
         }
-        ++pc;
         // the exponentials of the two tiles take turns, one warp of each on every SM sub-partition: while one
         // fills the pipes the other waits for its scores, takes its maximum and stores its P
         const bool joint = kTurns<D> && j >= other.x && j < other.y;
@@ -420,8 +439,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             rs[e & 3] = add2(rs[e & 3], x);
             pk[e] = pack_bf16x2(x.x, x.y);
           }
+          if (!waited) {
+            if (!wwait(&p_free[grp], (pc - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            waited = true;
+          }
           tmem_st_x32(t_p + hcol * 32, pk);
+          tmem_wait_st();
+          warp_arrive(&p_full[2 * grp + hcol]);
         }
+        if (!ok) break;
+        ++pc;
         if (joint) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&turn[grp * 4 + (warp & 3)]);
@@ -429,20 +457,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         rs[0] = add2(add2(rs[0], rs[1]), add2(rs[2], rs[3]));
         l = l * alpha + (rs[0].x + rs[0].y);
-        if (any_need && j > range.x) {
-          // PV_i(j-1) is complete (SEP: waited above; otherwise it was issued before S_i(j))
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(t_o + c * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_x32(t_o + c * 32, o);
-          }
-        }
-        tmem_wait_st();
-        warp_arrive(&p_full[grp]);
       }
       if (!ok) break;
       // hand the statistics to the epilogue
