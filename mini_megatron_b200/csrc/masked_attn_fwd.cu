@@ -396,15 +396,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float mu = m == -INFINITY ? 0.f : m;  // a row that has seen nothing: every exponential is 0
         // SEP: before P_i's columns (and O_i) are written, the PV that read the previous P_i (and last wrote O_i) must be
-        // complete; that wait sits behind the first half of the exponentials unless O_i has to be rescaled
+        // complete.  With a cap that wait sits behind the first half of the exponentials unless O_i has to be rescaled
+        // (GPT-125M shape 112 us instead of 123); without one it comes first: the two tiles then fall into step less
+        // (S = 16384: 206 us instead of 225).
         bool waited = !SEP || pc == 0;
+        if (!waited && (!CAP || (any_need && j > range.x))) {
+          if (!wwait(&p_free[grp], (pc - 1) & 1, a.err, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          waited = true;
+        }
         if (any_need && j > range.x) {
-          if (!waited) {
-            if (!wwait(&p_free[grp], (pc - 1) & 1, a.err, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            waited = true;
-          }
-          // otherwise PV_i(j-1) was issued before S_i(j), which is complete
+          // d = 128: PV_i(j-1) was issued before S_i(j), which is complete
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
