@@ -99,6 +99,7 @@ struct Ring {
   __device__ __forceinline__ bool get_thread(Item& w, int k, int* err, volatile int* abort_flag) const;
   // producer side
   __device__ __forceinline__ bool put(const Item& w, int k, int* err, volatile int* abort_flag) const;
+  __device__ __forceinline__ bool put_warp(const Item& w, int k, int* err, volatile int* abort_flag) const;
 };
 
 __device__ __forceinline__ void st_shared(uint32_t addr, float v) {
@@ -285,6 +286,17 @@ __device__ __forceinline__ bool Ring<Item>::put(const Item& w, int k, int* err, 
   return true;
 }
 
+template <typename Item>
+__device__ __forceinline__ bool Ring<Item>::put_warp(const Item& w, int k, int* err, volatile int* abort_flag) const {
+  if (k >= kRing && !wwait(&empty[k % kRing], ((k / kRing) - 1) & 1, err, abort_flag)) return false;
+  if ((threadIdx.x & 31) == 0) {
+    items[k % kRing] = w;
+    mbar_arrive(&full[k % kRing]);
+  }
+  __syncwarp();
+  return true;
+}
+
 // One arrival per warp on `bar`, after every lane's tcgen05 loads / stores are ordered before it.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   tc_fence_before();
@@ -371,6 +383,15 @@ __device__ __forceinline__ void mma_tmem_b(uint32_t dst, uint32_t a_tmem, uint32
 
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
+
+// `rows` rows of BYTES bytes, `stride` bytes apart, set to zero by one warp.
+template <int BYTES>
+__device__ __forceinline__ void zero_rows(void* p, size_t stride, int rows) {
+  constexpr int PER = BYTES / 16;
+  const int lane = threadIdx.x & 31;
+  for (int u = lane; u < rows * PER; u += 32)
+    *reinterpret_cast<uint4*>(static_cast<char*>(p) + (u / PER) * stride + (u % PER) * 16) = make_uint4(0u, 0u, 0u, 0u);
+}
 
 template <int N>
 __device__ __forceinline__ void store_zero(__nv_bfloat16* p) {

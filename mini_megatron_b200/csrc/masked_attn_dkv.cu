@@ -11,10 +11,12 @@
 // go back into TMEM as the first operands of the two sums and never touch shared
 // memory; LSE and Delta of the query rows arrive with the Q / dO tiles by bulk copies.
 // The queries that see a key are an interval too (document_plan.cu), so a mask is two
-// numbers per thread here as well.  Roles (20 warps, one of them idle):
+// numbers per thread here as well.  Roles (20 warps):
 //
 //   warp 0     TMA: K_j, V_j per item; Q_i, dO_i and their row data into a ring
 //   warp 1     TMEM allocation; one thread issues S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//   warp 2     hands out the work items
+//   warp 3     stores finished dK / dV tiles from the Q / dO stage they were staged in
 //   warps 4-19 softmax gradient: four warps share 32 key rows, each has 32 of the 128 queries
 //              (masked_attn_dq.cu says why four: DKVTWO against DKVFOUR cycles a tile at d = 64)
 //
@@ -36,6 +38,9 @@ struct Cfg {
   static constexpr int KB = (D == 64) ? 2 : 1;  // K / V buffers
   static constexpr int NQ = (D == 64) ? 4 : 2;  // Q / dO ring stages
   static constexpr int SB = (D == 64) ? 2 : 1;  // S^T buffers in TMEM
+  // dK and dV of an item leave during the next item's first pair.  d = 128: they leave at once, with two stages the one
+  // they are staged in is needed again by then.
+  static constexpr bool DEFER = (D == 64);
   static constexpr int K_OFF = 0;               // [KB][K, V]
   static constexpr int Q_OFF = KB * 2 * TILE;   // [NQ][Q, dO]
   static constexpr int LD_OFF = Q_OFF + NQ * 2 * TILE, LD = 1024;  // [NQ][-LSE log2 e 128, -Delta 128]
@@ -67,7 +72,7 @@ struct alignas(16) Item {
   int2 r, f;     // query tiles, and those of them that need no mask
 };
 static_assert(sizeof(Item) <= 32, "ring entry");
-constexpr int kConsumers = 1 + 1 + kWarps;  // TMA and MMA threads, softmax warps
+constexpr int kConsumers = 1 + 1 + 1 + kWarps;  // TMA and MMA threads, store and softmax warps
 
 __device__ __forceinline__ Item decode(const Args& a, int item) {
   const int q = a.by_parts.quot(item);
@@ -98,29 +103,21 @@ __device__ __forceinline__ void store8(float* p, const uint32_t* v, float mul) {
 
 // (head of the item's share, query tile) pairs of this CTA's items, one after another.
 struct Walk {
-  int k = 0, it = -1, g = 0, i = 0;  // it: items with queries so far
+  int it = -1, g = 0, i = 0;
   Item w;
-  bool started = false;
   // 1: at the next pair, 0: no more, -1: the wait for an item ran out
   __device__ __forceinline__ int next(const Ring<Item>& ring, int heads, int* err, volatile int* abort_flag) {
-    if (started) {
+    if (it >= 0) {
       if (++i < w.r.y) return 1;
       if (++g < heads) {
         i = w.r.x;
         return 1;
       }
     }
-    started = true;
-    while (true) {
-      if (!ring.get_thread(w, k++, err, abort_flag)) return -1;
-      if (w.b < 0) return 0;
-      if (w.r.x < w.r.y) {
-        g = 0;
-        i = w.r.x;
-        ++it;
-        return 1;
-      }
-    }
+    if (!ring.get_thread(w, ++it, err, abort_flag)) return -1;
+    g = 0;
+    i = w.r.x;
+    return w.b >= 0;
   }
   __device__ __forceinline__ bool first() const { return g == 0 && i == w.r.x; }
   __device__ __forceinline__ bool last(int heads) const { return g == heads - 1 && i == w.r.y - 1; }
@@ -296,17 +293,61 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     } else if (warp == 2) {
-      if (elect_one()) {
-        // -------------------------------------------------------------- work items
-        const int n_items = a.B * a.nkv * a.n_t * a.parts;
-        Item w;
-        for (int r = 0, item;; ++r) {
-          item = snake_item(r);
-          if (item < n_items) w = decode(a, item);
-          else w.b = -1;
-          if (!ring.put(w, r, a.err, abort_flag) || w.b < 0) break;
+      // ---------------------------------------------------------------- work items
+      // Only items with work travel through the ring: the MMA thread takes the next item before the other roles have
+      // finished the current one, so a run of empty ones could fill the ring with nobody left to empty it.
+      const int n_items = a.B * a.nkv * a.n_t * a.parts;
+      Item w;
+      for (int r = 0, k = 0;; ++r) {
+        const int item = snake_item(r);
+        if (item < n_items) {
+          w = decode(a, item);
+          if (w.r.x >= w.r.y) {
+            const int rows = min(BT, a.S - w.t * BT);
+            const size_t tok = (size_t)w.b * a.S + w.t * BT;
+            if (a.parts > 1) {
+              const size_t width = (size_t)2 * a.nkv * D;
+              float* p = a.partial + ((size_t)w.part * a.B * a.S + tok) * width + (size_t)w.hk * D;
+              zero_rows<4 * D>(p, 4 * width, rows);
+              zero_rows<4 * D>(p + (size_t)a.nkv * D, 4 * width, rows);
+            } else {
+              const size_t width = (size_t)(a.nh + 2 * a.nkv) * D;
+              __nv_bfloat16* p = a.dqkv + tok * width + (size_t)(a.nh + w.hk) * D;
+              zero_rows<2 * D>(p, 2 * width, rows);
+              zero_rows<2 * D>(p + (size_t)a.nkv * D, 2 * width, rows);
+            }
+            continue;
+          }
+        } else {
+          w.b = -1;
         }
+        if (!ring.put_warp(w, k++, a.err, abort_flag) || w.b < 0) break;
       }
+    } else {
+      // ---------------------------------------------------------------- stores of staged dK / dV tiles
+      int n = 0, it = 0;
+      Item w;
+      for (int u = 0; ring.get_warp(w, u, a.err, abort_flag) && w.b >= 0; ++u) {
+        n += (w.r.y - w.r.x) * heads;
+        if (!wwait(out_full, it & 1, a.err, abort_flag)) break;
+        if (lane == 0) {
+          const int qs = (n - 1) % NQ;
+          if (a.parts == 1) {
+            uint8_t* stg = sQ + qs * 2 * C::TILE;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              tma_store_3d(&tm_dqkv, stg + c * 16384, (a.nh + w.hk) * D + c * 64, w.t * BT, w.b);
+              tma_store_3d(&tm_dqkv, stg + C::TILE + c * 16384, (a.nh + a.nkv + w.hk) * D + c * 64, w.t * BT, w.b);
+            }
+            bulk_commit();
+            bulk_wait_read<0>();
+          }
+          mbar_arrive(&q_empty[qs]);
+        }
+        __syncwarp();
+        ++it;
+      }
+      if (lane == 0) bulk_wait<0>();
       __syncwarp();
     }
   } else {
@@ -318,32 +359,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Score k = a.score;
     int n = 0, it = 0;
     bool ok = true;
+    // a share's sums: dK and dV of this warp's columns, [parts, B, S, 2 nkv * D]
+    auto share_row = [&](const Item& w) {
+      return a.partial + (((size_t)w.part * a.B + w.b) * a.S + w.t * BT + row) * ((size_t)2 * a.nkv * D) +
+             (size_t)w.hk * D + part * (D / 4);
+    };
+    // dK and dV of item number `of`, whose last pair was number `last`: TMEM -> the Q / dO stage of that pair, for the
+    // store warp, or, where they are a share's, to `pk` (nullptr: the row lies behind the end)
+    auto drain_dkv = [&](int of, int last, float* pk) -> bool {
+      if (!wwait(g_full, of & 1, a.err, abort_flag)) return false;
+      tc_fence_after();
+      uint32_t v[D / 4], u[D / 4];
+      tmem_ld(tmem + C::T_DV + lane_off + part * (D / 4), v);
+      tmem_ld(tmem + C::T_DK + lane_off + part * (D / 4), u);
+      tmem_wait_ld();
+      warp_arrive(g_free);
+      if (a.parts > 1) {
+        if (pk) {
+#pragma unroll
+          for (int c = 0; c < D / 4; c += 8) {
+            store8(pk + c, &u[c], a.scale);
+            store8(pk + (size_t)a.nkv * D + c, &v[c], 1.f);
+          }
+        }
+      } else {
+        uint8_t* stg = sQ + (last % NQ) * 2 * C::TILE;
+        stage_row(stg, 16384, row, part * (D / 4), u, a.scale);
+        stage_row(stg + C::TILE, 16384, row, part * (D / 4), v, 1.f);
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(out_full);
+      return true;
+    };
+    int last_pair = -1;  // last pair of the item whose dK and dV are still in TMEM
+    float* last_pk = nullptr;
     Item w;
     for (int u = 0; ok && (ok = ring.get_warp(w, u, a.err, abort_flag)) && w.b >= 0; ++u) {
       const int key = w.t * BT + row;
       const bool in = key < a.S;
-      // a share's sums: dK and dV of this warp's columns, [parts, B, S, 2 nkv * D]
-      auto share_row = [&]() {
-        return a.partial + (((size_t)w.part * a.B + w.b) * a.S + key) * ((size_t)2 * a.nkv * D) + (size_t)w.hk * D +
-               part * (D / 4);
-      };
-      if (w.r.x >= w.r.y) {
-        if (in && a.parts > 1) {
-          float* pk = share_row();
-#pragma unroll
-          for (int c = 0; c < D / 4; c += 4) {
-            *reinterpret_cast<float4*>(pk + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(pk + (size_t)a.nkv * D + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-        } else if (in) {
-          __nv_bfloat16* dk = a.dqkv + ((size_t)w.b * a.S + key) * ((size_t)(a.nh + 2 * a.nkv) * D) +
-                              (size_t)(a.nh + w.hk) * D + part * (D / 4);
-          __nv_bfloat16* dv = dk + (size_t)a.nkv * D;
-          store_zero<D / 4>(dk);
-          store_zero<D / 4>(dv);
-        }
-        continue;
-      }
       int first = key, last = a.n_t * BT;
       if (a.mask.rows) {
         const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + w.t) * (4 * BT) + 2 * BT + row;
@@ -405,6 +459,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tmem_wait_st();
           warp_arrive(&p_full[n & 1]);
+          // the previous item's dK and dV leave here: its last products ran while this pair's P was computed
+          if (C::DEFER && last_pair >= 0) {
+            if (!drain_dkv(it - 1, last_pair, last_pk)) { ok = false; break; }
+            last_pair = -1;
+          }
           if (!wwait(dp_full, n & 1, a.err, abort_flag)) { ok = false; break; }
           tc_fence_after();
           const float* delta = l2 + BT;
@@ -429,51 +488,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!ok) break;
-      if (!wwait(g_full, it & 1, a.err, abort_flag)) { ok = false; break; }
-      tc_fence_after();
-      {
-        uint32_t v[D / 4], u[D / 4];
-        tmem_ld(tmem + C::T_DV + lane_off + part * (D / 4), v);
-        tmem_ld(tmem + C::T_DK + lane_off + part * (D / 4), u);
-        tmem_wait_ld();
-        warp_arrive(g_free);
-        const int qs = (n - 1) % NQ;
-        uint8_t* stg = sQ + qs * 2 * C::TILE;
-        if (a.parts > 1) {
-          if (in) {
-            float* pk = share_row();
-#pragma unroll
-            for (int c = 0; c < D / 4; c += 8) {
-              store8(pk + c, &u[c], a.scale);
-              store8(pk + (size_t)a.nkv * D + c, &v[c], 1.f);
-            }
-          }
-        } else {
-          stage_row(stg, 16384, row, part * (D / 4), u, a.scale);
-          stage_row(stg + C::TILE, 16384, row, part * (D / 4), v, 1.f);
-          fence_proxy_async_smem();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(out_full);
-        if (warp == 4) {
-          if (!wwait(out_full, it & 1, a.err, abort_flag)) { ok = false; break; }
-          if (lane == 0) {
-#pragma unroll
-            for (int c = 0; c < (a.parts > 1 ? 0 : D / 64); ++c) {
-              tma_store_3d(&tm_dqkv, stg + c * 16384, (a.nh + w.hk) * D + c * 64, w.t * BT, w.b);
-              tma_store_3d(&tm_dqkv, stg + C::TILE + c * 16384, (a.nh + a.nkv + w.hk) * D + c * 64, w.t * BT, w.b);
-            }
-            bulk_commit();
-            bulk_wait_read<0>();
-            mbar_arrive(&q_empty[qs]);
-          }
-          __syncwarp();
-        }
-      }
+      last_pair = n - 1;
+      last_pk = a.parts > 1 && in ? share_row(w) : nullptr;
       ++it;
+      if (!C::DEFER && !drain_dkv(it - 1, last_pair, last_pk)) { ok = false; break; }
     }
-    if (lane == 0) bulk_wait<0>();
-    __syncwarp();
+    if (C::DEFER && ok && last_pair >= 0) drain_dkv(it - 1, last_pair, last_pk);
   }
 
   tc_fence_before();

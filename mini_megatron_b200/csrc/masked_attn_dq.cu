@@ -16,13 +16,14 @@
 // that took the registers of the softmax warps; as a kernel of its own it is bound by reading ctx and dO.)
 //
 // masked_attn_dq_kernel: persistent grid, one CTA per SM; a work item is (batch, head, 128-row query tile).
-// Roles (20 warps, one of them idle):
+// Roles (20 warps):
 //
 //   warp 0      TMA: Q, dO and row statistics per item; K_j and V_j into rings
 //   warp 1      TMEM allocation; one thread issues S = Q K_j^T (two TMEM buffers), dP = dO V_j^T
 //               and dQ += dS K_j (dS read from TMEM): S of the next tile before dS of this one is
 //               ready, dP of the next as soon as this one has been read
 //   warp 2      hands out the work items
+//   warp 3      stores finished dQ tiles from the K stage they were staged in
 //   warps 4-19  dS: four warps share 32 query rows, each has 32 of the 128 keys
 //
 // dS overwrites the S columns it came from: every warp's 32 keys start 32 columns apart.
@@ -72,7 +73,7 @@ struct alignas(16) Item {
   int2 r, f;    // key tiles, and those of them that need no mask
 };
 static_assert(sizeof(Item) <= 32, "ring entry");
-constexpr int kConsumers = 1 + 1 + kWarps;  // TMA and MMA threads, softmax warps
+constexpr int kConsumers = 1 + 1 + 1 + kWarps;  // TMA and MMA threads, store and softmax warps
 
 __device__ __forceinline__ Item decode(const Args& a, int item) {
   const int li = a.by_nh.quot(item);
@@ -91,27 +92,16 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
   return it;
 }
 
-// The tiles of this CTA one after another, across items (items without keys are skipped).
+// The tiles of this CTA one after another, across items.
 struct Walk {
-  int k = 0, it = -1, j = 0;  // it: items with keys so far
+  int it = -1, j = 0;
   Item w;
-  bool started = false;
   // 1: at the next tile, 0: no more, -1: the wait for an item ran out
   __device__ __forceinline__ int next(const Ring<Item>& ring, int* err, volatile int* abort_flag) {
-    if (started && j + 1 < w.r.y) {
-      ++j;
-      return 1;
-    }
-    started = true;
-    while (true) {
-      if (!ring.get_thread(w, k++, err, abort_flag)) return -1;
-      if (w.b < 0) return 0;
-      if (w.r.x < w.r.y) {
-        j = w.r.x;
-        ++it;
-        return 1;
-      }
-    }
+    if (it >= 0 && ++j < w.r.y) return 1;
+    if (!ring.get_thread(w, ++it, err, abort_flag)) return -1;
+    j = w.r.x;
+    return w.b >= 0;
   }
   __device__ __forceinline__ bool first() const { return j == w.r.x; }
   __device__ __forceinline__ bool last() const { return j == w.r.y - 1; }
@@ -286,17 +276,46 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     } else if (warp == 2) {
-      if (elect_one()) {
-        // -------------------------------------------------------------- work items
-        const int n_items = a.B * a.nh * a.n_t;
-        Item w;
-        for (int r = 0, item;; ++r) {
-          item = snake_item(r);
-          if (item < n_items) w = decode(a, item);
-          else w.b = -1;
-          if (!ring.put(w, r, a.err, abort_flag) || w.b < 0) break;
+      // ---------------------------------------------------------------- work items
+      // Only items with work travel through the ring: the MMA thread takes the next item before the other roles have
+      // finished the current one, so a run of empty ones could fill the ring with nobody left to empty it.
+      const int n_items = a.B * a.nh * a.n_t;
+      Item w;
+      for (int r = 0, k = 0;; ++r) {
+        const int item = snake_item(r);
+        if (item < n_items) {
+          w = decode(a, item);
+          if (w.r.x >= w.r.y) {
+            const size_t width = (size_t)(a.nh + 2 * a.nkv) * D;
+            zero_rows<2 * D>(a.dqkv + ((size_t)w.b * a.S + w.t * BT) * width + (size_t)w.h * D, 2 * width,
+                             min(BT, a.S - w.t * BT));
+            continue;
+          }
+        } else {
+          w.b = -1;
         }
+        if (!ring.put_warp(w, k++, a.err, abort_flag) || w.b < 0) break;
       }
+    } else {
+      // ---------------------------------------------------------------- stores of staged dQ tiles
+      int n = 0, it = 0;
+      Item w;
+      for (int u = 0; ring.get_warp(w, u, a.err, abort_flag) && w.b >= 0; ++u) {
+        n += w.r.y - w.r.x;
+        if (!wwait(out_full, it & 1, a.err, abort_flag)) break;
+        if (lane == 0) {
+          const int ks = (n - 1) % NK;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_store_3d(&tm_dqkv, sK + ks * C::TILE + c * 16384, w.h * D + c * 64, w.t * BT, w.b);
+          bulk_commit();
+          bulk_wait_read<0>();
+          mbar_arrive(&k_empty[ks]);
+        }
+        __syncwarp();
+        ++it;
+      }
+      if (lane == 0) bulk_wait<0>();
       __syncwarp();
     }
   } else {
@@ -308,15 +327,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Score k = a.score;
     int n = 0, it = 0;
     bool ok = true;
+    // dQ of item number `of`, whose last tile was number `last`: TMEM -> the K stage of that tile, for the store warp
+    auto drain_dq = [&](int of, int last) -> bool {
+      if (!wwait(dq_full, of & 1, a.err, abort_flag)) return false;
+      tc_fence_after();
+      uint32_t v[D / 4];
+      tmem_ld(tmem + C::T_DQ + lane_off + part * (D / 4), v);
+      tmem_wait_ld();
+      warp_arrive(dq_free);
+      stage_row(sK + (last % NK) * C::TILE, 16384, row, part * (D / 4), v, a.scale);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(out_full);
+      return true;
+    };
+    int last = -1;  // last tile of the item whose dQ is still in TMEM
     Item w;
     for (int u = 0; ok && (ok = ring.get_warp(w, u, a.err, abort_flag)) && w.b >= 0; ++u) {
       const int i = w.t * BT + row;
-      if (w.r.x >= w.r.y) {
-        if (i < a.S)
-          store_zero<D / 4>(a.dqkv + ((size_t)w.b * a.S + i) * ((size_t)(a.nh + 2 * a.nkv) * D) + (size_t)w.h * D +
-                            part * (D / 4));
-        continue;
-      }
       int start = 0, end = i + 1;
       if (a.mask.rows) {
         const int* tr = a.mask.rows + ((size_t)w.b * a.n_t + w.t) * (4 * BT) + row;
@@ -367,6 +395,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!(seen & (1u << e))) pf[e] = 0.f;
           }
         }
+        // the previous item's dQ leaves here: its last product ran while this tile's P was computed
+        if (last >= 0) {
+          if (!drain_dq(it - 1, last)) { ok = false; break; }
+          last = -1;
+        }
         if (!wwait(dp_full, n & 1, a.err, abort_flag)) { ok = false; break; }
         tc_fence_after();
         {
@@ -375,8 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
           uint32_t ds[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-          {
+          for (int e = 0; e < 16; ++e) {
             const float2 v = mul2(make_float2(pf[2 * e], pf[2 * e + 1]), add2(pair(dp[2 * e], dp[2 * e + 1]), pair(st.y)));
             ds[e] = pack_bf16x2(v.x, v.y);
           }
@@ -386,36 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         warp_arrive(ds_full);
       }
       if (!ok) break;
-      if (!wwait(dq_full, it & 1, a.err, abort_flag)) { ok = false; break; }
-      tc_fence_after();
-      {
-        uint32_t v[D / 4];
-        tmem_ld(tmem + C::T_DQ + lane_off + part * (D / 4), v);
-        tmem_wait_ld();
-        warp_arrive(dq_free);
-        const int ks = (n - 1) % NK;
-        uint8_t* stg = sK + ks * C::TILE;
-        stage_row(stg, 16384, row, part * (D / 4), v, a.scale);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(out_full);
-        if (warp == 4) {
-          if (!wwait(out_full, it & 1, a.err, abort_flag)) { ok = false; break; }
-          if (lane == 0) {
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c)
-              tma_store_3d(&tm_dqkv, stg + c * 16384, w.h * D + c * 64, w.t * BT, w.b);
-            bulk_commit();
-            bulk_wait_read<0>();
-            mbar_arrive(&k_empty[ks]);
-          }
-          __syncwarp();
-        }
-      }
+      last = n - 1;
       ++it;
     }
-    if (lane == 0) bulk_wait<0>();
-    __syncwarp();
+    if (ok && last >= 0) drain_dq(it - 1, last);
   }
 
   tc_fence_before();

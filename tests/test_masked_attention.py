@@ -132,6 +132,35 @@ def test_strides_and_neighbours():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d,nh,nkv", [(64, 4, 4), (64, 4, 1), (128, 2, 1)])
+@pytest.mark.parametrize("S", [200, 900])
+def test_many_empty_rows(d, nh, nkv, S):
+    """A batch of mostly empty rows: a CTA then has one tile of work among dozens without any."""
+    from mini_megatron_b200.ops import check_errors
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    from mini_megatron_b200.ops.documents import document_plan
+    B = 400
+    g = torch.Generator().manual_seed(S)
+    lengths = torch.zeros(B, dtype=torch.int32)
+    lengths[[3, 150, 151, 399]] = torch.tensor([S, 1, 130, S - 1], dtype=torch.int32)
+    tokens = torch.randint(0, 40, (B, S), generator=g)
+    qkv = torch.randn(B, S, (nh + 2 * nkv) * d, generator=g).bfloat16().cuda()
+    dctx = torch.randn(B, S, nh * d, generator=g).bfloat16().cuda()
+    plan = document_plan(tokens.cuda(), eod=0, lengths=lengths.cuda())
+    ctx, lse = attention_fwd(qkv, nh, d, num_kv_heads=nkv, plan=plan)
+    grad = attention_bwd(dctx, qkv, ctx, lse, nh, d, num_kv_heads=nkv, plan=plan)
+    check_errors()
+    some = lengths.nonzero().flatten().tolist()
+    start, end = plan.start[some], plan.end[some]
+    (r_ctx, r_lse, r_grad), (b_ctx, b_lse, b_grad) = attention_ref(qkv[some], dctx[some], nh, nkv, d, start, end)
+    _near(ctx[some], r_ctx, b_ctx, "ctx")
+    _near(lse[some], r_lse, b_lse, "lse")
+    _near(grad[some], r_grad, b_grad, "dqkv")
+    none = [b for b in range(B) if b not in some]
+    assert not ctx[none].any() and not grad[none].any() and (lse[none] == float("-inf")).all()
+
+
+@pytest.mark.gpu
 def test_two_graphs_share_nothing():
     """Forward and backward captured twice, replayed alternately on new values, against eager calls."""
     from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
