@@ -515,9 +515,10 @@ mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, c
   const int64_t B = qkv.size(0), S = qkv.size(1);
   TORCH_CHECK(qkv.size(2) == (nh + 2 * nkv) * d, "attention: qkv's last dimension must be (num_heads + 2 num_kv_heads)",
               " * head_dim = ", (nh + 2 * nkv) * d, ", got ", qkv.size(2));
-  TORCH_CHECK(S <= INT_MAX - 256 && B <= INT_MAX && nh <= (1 << 20), "attention: too large");
-  TORCH_CHECK(scale > 0 && std::isfinite(scale), "attention: softmax_scale must be positive and finite, got ", scale);
-  TORCH_CHECK(cap >= 0 && cap <= 1000, "attention: softcap must be at most 1000, got ", cap);
+  TORCH_CHECK(S <= INT_MAX - 256 && B <= INT_MAX && nh <= 4096, "attention: at most 4096 heads, got ", nh);
+  // in 32 bits neither the scale nor its quotient by the cap overflows or vanishes
+  TORCH_CHECK(scale >= 1e-15 && scale <= 1e15, "attention: softmax_scale must be from 1e-15 to 1e15, got ", scale);
+  TORCH_CHECK(cap == 0 || (cap >= 1e-3 && cap <= 1000), "attention: softcap must be from 0.001 to 1000, got ", cap);
   c.qkv = qkv.data_ptr();
   c.qkv_ss = ss;
   c.qkv_sb = sb;

@@ -43,7 +43,7 @@ constexpr int kMaxCtas = 8;                  // portable cluster size
 constexpr int kMaxSteps = 64;                // per CTA: rows of up to 2 Mi tokens
 
 struct Args {
-  const long* ids;        // [B, S] tokens or document ids (nullptr: one document per row)
+  const long* ids;        // [B, S] tokens or document ids
   long ld_ids;
   long eod;
   int by_change;          // 1: a document starts where the id changes; 0: after a token equal to eod
@@ -87,7 +87,7 @@ __device__ __forceinline__ void load_flags(const Args& a, int b, int i0, int len
   uint8_t mark[kPer] = {0, 0, 0, 0};
   long prev = 0;
   const bool whole = i0 + kPer <= a.S;
-  if (a.ids && i0 < a.S) {
+  if (i0 < a.S) {
     const long* p = a.ids + b * a.ld_ids + i0;
     if (i0 > 0) prev = p[-1];
     if (whole && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
@@ -120,7 +120,7 @@ __device__ __forceinline__ void load_flags(const Args& a, int b, int i0, int len
   for (int e = 0; e < kPer; ++e) {
     const int i = i0 + e;
     const long before = e == 0 ? prev : id[e - 1];
-    first[e] = i == 0 || (a.ids && (a.by_change ? id[e] != before : before == a.eod));
+    first[e] = i == 0 || (a.by_change ? id[e] != before : before == a.eod);
     plain[e] = !(i < len && mark[e]);
   }
 }

@@ -35,9 +35,12 @@ struct Mask {
 
 // Tiles [x, y) of the other side that a tile with these bounds needs, and those of them that need no mask: every row
 // sees all of the tile.  (Rows behind the end of the sequence do not count: what they read is zero.)
-__device__ __forceinline__ int2 needed_tiles(const int4& q) {
-  return q.y == 0 ? make_int2(0, 0) : make_int2(q.x / BT, (q.y + BT - 1) / BT);
+// Both are kept within the row, and entries of the order within the batch, so that a table that was captured but not
+// yet written sends nothing out of range.
+__device__ __forceinline__ int2 needed_tiles(const int4& q, int n_t) {
+  return q.y <= 0 ? make_int2(0, 0) : make_int2(max(q.x / BT, 0), min((q.y - 1) / BT + 1, n_t));
 }
+__device__ __forceinline__ int ordered(const int* order, int k, int n) { return min(max(order[k], 0), n - 1); }
 __device__ __forceinline__ int2 whole_tiles(const int4& q) { return make_int2((q.z + BT - 1) / BT, q.w / BT); }
 
 // Key tiles of query tile t of row b.
@@ -48,7 +51,7 @@ __device__ __forceinline__ void key_tiles(const Mask& m, int b, int n_t, int t, 
     return;
   }
   const int4 q = m.qstat[(size_t)b * n_t + t];
-  need = needed_tiles(q);
+  need = needed_tiles(q, n_t);
   whole = whole_tiles(q);
 }
 // Query tiles of key tile t of row b.
@@ -59,7 +62,7 @@ __device__ __forceinline__ void query_tiles(const Mask& m, int b, int n_t, int t
     return;
   }
   const int4 q = m.kstat[(size_t)b * n_t + t];
-  need = needed_tiles(q);
+  need = needed_tiles(q, n_t);
   whole = whole_tiles(q);
 }
 // Which of 32 consecutive rows or columns from `first` on lie in [lo, hi).

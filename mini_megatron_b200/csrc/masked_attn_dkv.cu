@@ -81,7 +81,7 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
   it.part = item - q * a.parts;
   it.hk = q - li * a.nkv;
   if (a.mask.order) {
-    const int e = a.mask.order[li];
+    const int e = ordered(a.mask.order, li, a.B * a.n_t);
     it.b = a.by_tiles.quot(e);
     it.t = e - it.b * a.n_t;
   } else {  // causal rows: the first key tile is seen by the most queries
@@ -541,11 +541,16 @@ __global__ void join_parts_kernel(const float* __restrict__ partial, int parts, 
 // (about three items each, which leaves the heaviest-first order something to balance); the shares' 32-bit sums are
 // joined afterwards.  One K/V head of 128 key tiles (S = 16384, 4 query heads) took DKVONE us as 128 items and
 // DKVSPLIT us with the join as 512.
+//
+// An item of kMaxPairs (query head, query tile) pairs runs for about 0.4 s; waits for the end of an item give up
+// after 2 s, so longer ones are split too.
+static constexpr long kMaxPairs = 1 << 19;
 int masked_attn_dkv_parts(int B, int S, int nh, int nkv, int num_sms) {
   const long items = (long)B * nkv * ((S + mattn::BT - 1) / mattn::BT);
   const int group = nh / nkv;
+  const long n_t = (S + mattn::BT - 1) / mattn::BT;
   for (int p = 1; p < group; ++p)
-    if (group % p == 0 && items * p >= 2L * num_sms) return p;
+    if (group % p == 0 && items * p >= 2L * num_sms && group / p * n_t <= kMaxPairs) return p;
   return group;
 }
 

@@ -80,7 +80,7 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
   Item it;
   it.h = item - li * a.nh;
   if (a.mask.order) {
-    const int e = a.mask.order[li];
+    const int e = ordered(a.mask.order, li, a.B * a.n_t);
     it.b = a.by_tiles.quot(e);
     it.t = e - it.b * a.n_t;
   } else {  // causal rows: the longest first

@@ -84,7 +84,7 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
   it.h = item - li * a.nh;
   int p;
   if (a.mask.order) {
-    const int e = a.mask.order[li];
+    const int e = ordered(a.mask.order, li, a.B * a.n_pairs);
     it.b = a.by_pairs.quot(e);
     p = e - it.b * a.n_pairs;
   } else {  // causal rows: the longest first

@@ -179,7 +179,8 @@ int rotary(const void* x, long x_sb, long x_ss, void* y, long y_sb, long y_ss, i
   a.tokens = B * S;
   a.copy = (x != y);
   // few tokens: one per CTA, so that a short call still spreads over the SMs
-  a.per_cta = (int)std::max(1L, std::min((long)kMaxTokens, a.tokens / (8L * num_sms)));
+  const long fit = 48 * 1024 / ((long)rot * (long)sizeof(float));  // the angles of a CTA's tokens in shared memory
+  a.per_cta = (int)std::max(1L, std::min({(long)kMaxTokens, fit, a.tokens / (8L * num_sms)}));
   const long grid = (a.tokens + a.per_cta - 1) / a.per_cta;
   if (grid > 0x7fffffffL) return -2;
   const size_t smem = (size_t)a.per_cta * rot * sizeof(float);

@@ -15,6 +15,7 @@ without the built extension :func:`native` raises.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import native
 
@@ -61,9 +62,13 @@ def attention_fwd(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, sof
                   softmax_scale=None):
     """``(ctx [B, S, num_heads * head_dim], lse [B, num_heads, S] fp32)`` of masked attention.
 
-    ``plan``: a :class:`~mini_megatron_b200.ops.documents.DocumentPlan` (default: causal).  ``softcap`` up to 1000,
+    ``plan``: a :class:`~mini_megatron_b200.ops.documents.DocumentPlan` (default: causal).  ``softcap`` 0.001 to 1000,
     ``alibi_slopes`` ``[num_heads]`` fp32, ``softmax_scale`` (default ``head_dim ** -0.5``).  On CUDA: bf16, head_dim
-    64 or 128, any length, rows on 16-byte boundaries.
+    64 or 128, up to 4096 heads, any length, rows on 16-byte boundaries.
+
+    Everything in ``qkv`` must be finite, padding too: what a token does not see counts with weight 0, and 0 times an
+    infinity or NaN is NaN.  Statistics and sums are 32-bit; the weights, and in the backward pass the scores'
+    gradients, are rounded to bf16 once, as operands of the tensor cores.
     """
     nkv, cap, scale = _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale)
     if not qkv.is_cuda:
@@ -78,7 +83,7 @@ def attention_bwd(dctx, qkv, ctx, lse, num_heads, head_dim, *, num_kv_heads=None
     CUDA only.  The same inputs give the same bits: no atomics."""
     nkv, cap, scale = _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale)
     return native().masked_attn_bwd(dctx, qkv, ctx, lse, num_heads, nkv, head_dim, None if plan is None else plan.tables,
-                                          alibi_slopes, cap, scale)
+                                    alibi_slopes, cap, scale)
 
 
 class _AttentionFn(torch.autograd.Function):
@@ -90,6 +95,7 @@ class _AttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         qkv, out, lse = ctx.saved_tensors
         return attention_bwd(dout.contiguous(), qkv, out, lse, *ctx.args, **ctx.opts), None, None, None

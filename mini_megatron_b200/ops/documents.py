@@ -26,7 +26,8 @@ from . import native
 
 
 class DocumentPlan:
-    """``positions``, ``start``, ``end``: ``[B, S]`` int32.  ``tables`` belongs to the attention kernels."""
+    """``positions``, ``start``, ``end``: ``[B, S]`` int32.  ``tables`` holds the same intervals as the attention
+    kernels read them: writing to ``start`` or ``end`` does not change what they compute."""
 
     __slots__ = ("positions", "start", "end", "tables", "shape")
 

@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import native
 
@@ -117,6 +118,7 @@ class _RotaryFn(torch.autograd.Function):
         return rotary_fwd(x, rotary, num_heads, positions)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         (positions,) = ctx.saved_tensors
         return rotary_bwd(dy.contiguous(), ctx.rotary, ctx.num_heads, positions), None, None, None

@@ -161,6 +161,39 @@ def test_many_empty_rows(d, nh, nkv, S):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_tables_that_were_never_written(d):
+    """Arbitrary numbers in a plan's tables give arbitrary numbers, inside the tensors; the next call is not affected."""
+    from mini_megatron_b200.ops import check_errors
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    from mini_megatron_b200.ops.documents import DocumentPlan
+    qkv, dctx, plan, _, _ = _case(3, 900, 4, 2, d, 250, False, True, 1.0, "cuda", torch.bfloat16)
+    want = attention_fwd(qkv, 4, d, num_kv_heads=2, plan=plan)
+    want += (attention_bwd(dctx, qkv, *want, 4, d, num_kv_heads=2, plan=plan),)
+    g = torch.Generator().manual_seed(3)
+    for low, high in ((-2 ** 31, 2 ** 31), (-1000, 2000)):
+        tables = torch.randint(low, high, plan.tables.shape, generator=g).to(torch.int32).cuda()
+        other = DocumentPlan(plan.positions, plan.start, plan.end, tables)
+        ctx, lse = attention_fwd(qkv, 4, d, num_kv_heads=2, plan=other)
+        attention_bwd(dctx, qkv, ctx, lse, 4, d, num_kv_heads=2, plan=other)
+        check_errors()
+    got = attention_fwd(qkv, 4, d, num_kv_heads=2, plan=plan)
+    got += (attention_bwd(dctx, qkv, *got, 4, d, num_kv_heads=2, plan=plan),)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    from mini_megatron_b200.ops.attention import attention
+    from mini_megatron_b200.ops.rotary import Rotary, apply_rotary
+    x = torch.randn(1, 40, 192, device="cuda").bfloat16().requires_grad_(True)
+    for y in (attention(x, 1, 64), apply_rotary(x, Rotary(64), 2)):
+        (grad,) = torch.autograd.grad(y.float().pow(2).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            grad.float().sum().backward()
+
+
+@pytest.mark.gpu
 def test_two_graphs_share_nothing():
     """Forward and backward captured twice, replayed alternately on new values, against eager calls."""
     from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
@@ -279,6 +312,8 @@ def test_refusals_gpu():
     x = torch.zeros(2, 4, 384, device="cuda", dtype=torch.bfloat16)
     wide = torch.zeros(2, 4, 400, device="cuda", dtype=torch.bfloat16)
     bad = [((x.float(), 2, 64), {}), ((x, 4, 32), {}), ((x, 2, 64), {"softcap": 1e6}),
+           ((x, 2, 64), {"softcap": 1e-9}), ((x, 2, 64), {"softmax_scale": 1e30}),
+           ((x.new_zeros(1, 1, 3 * 4097 * 64), 4097, 64), {}),
            ((x, 2, 64), {"softmax_scale": 0.0}), ((x, 2, 64), {"softmax_scale": float("nan")}),
            ((x, 2, 64), {"alibi_slopes": torch.ones(3, device="cuda")}),
            ((x, 2, 64), {"alibi_slopes": torch.ones(2)}),

@@ -206,3 +206,22 @@ def test_rotary_frequencies_are_not_copied_in_a_capture():
     finally:
         torch.cuda.is_current_stream_capturing = real
     assert r.turns(x.device).is_cuda
+
+
+@pytest.mark.gpu
+def test_rotary_wide_heads():
+    """Heads of 4096 over many tokens: the angles of four tokens would not fit a CTA's shared memory."""
+    from mini_megatron_b200.ops.rotary import Rotary, rotary_bwd, rotary_fwd
+    rot = Rotary(4096)
+    x = torch.randn(1, 6000, 4096, device="cuda").bfloat16()
+    y = rotary_fwd(x, rot, 1)
+    some = torch.tensor([0, 1, 2999, 5999])
+    want = rotary_fwd(x[:, some].cpu().double(), rot, 1, positions=some)
+    # a' and b' are sums of two products: angle to 2^-24 of a turn (2 pi 2^-24 relative to the pair's length), two
+    # 32-bit roundings, then half a step of bf16
+    size = x[:, some].cpu().double().abs().amax()
+    bound = want.abs() * 2.0 ** -8 + size * 2 * 2.0 ** -20
+    assert ((y[:, some].cpu().double() - want).abs() <= bound).all()
+    back = rotary_bwd(y, rot, 1)
+    # two roundings of bf16, each at most 2^-8 of the pair's length
+    assert ((back.double() - x.double()).abs() <= 4 * 2.0 ** -8 * size.item()).all()
