@@ -243,8 +243,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int sc = 0, pc = 0, ic = 0;  // S issued (s_free phases), P consumed (p_full), items with keys (o_free)
       bool ok = true;
       uint32_t q_addr = 0;
-      // S of the K stage of loop position u; the stage is released either way
-      auto issue_s = [&](int u, bool on) -> bool {
+      // S of the K stage of loop position u; the stage, and after an item's last one Q, are released either way
+      auto issue_s = [&](int u, bool on, bool last) -> bool {
         const int st = u % NS;
         if (!bwait(&k_full[st], (u / NS) & 1, a.err, abort_flag)) return false;
         if (on) {
@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(&s_full[grp]);
         }
         umma_commit(&k_empty[st]);
+        if (last) umma_commit(&q_empty[it % QB]);
         return true;
       };
       auto issue_pv = [&](int u, bool on, bool first, bool last) -> bool {
@@ -284,16 +285,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         q_addr = smem_u32(sQ + (qb * 2 + grp) * C::TILE);
         if (!bwait(&q_full[qb], (it / QB) & 1, a.err, abort_flag)) { ok = false; break; }
         auto on = [&](int j) { return j >= range.x && j < range.y; };
-        if (!issue_s(kv, on(w.lo))) { ok = false; break; }
+        if (!issue_s(kv, on(w.lo), w.lo + 1 == w.hi)) { ok = false; break; }
         for (int j = w.lo; j < w.hi; ++j, ++kv) {
           // d = 64: the next scores first, they only need the softmax to have read the current ones;
           // d = 128: P overwrites S, the next scores follow P V
-          if (SEP && j + 1 < w.hi && !issue_s(kv + 1, on(j + 1))) { ok = false; break; }
+          if (SEP && j + 1 < w.hi && !issue_s(kv + 1, on(j + 1), j + 2 == w.hi)) { ok = false; break; }
           if (!issue_pv(kv, on(j), j == range.x, j == range.y - 1)) { ok = false; break; }
-          if (!SEP && j + 1 < w.hi && !issue_s(kv + 1, on(j + 1))) { ok = false; break; }
+          if (!SEP && j + 1 < w.hi && !issue_s(kv + 1, on(j + 1), j + 2 == w.hi)) { ok = false; break; }
         }
         if (!ok) break;
-        umma_commit(&q_empty[qb]);  // every S of this item has been issued
         ++it;
         if (range.x < range.y) ++ic;
       }
