@@ -54,6 +54,10 @@ struct Cfg {
   static constexpr int ITEM_OFF = OUT_OFF + 4 * 4096;  // [kRing] work items
   static constexpr int BAR_OFF = ITEM_OFF + kRing * 64;
   static constexpr int SMEM = 1024 + BAR_OFF + 512;
+  // Registers: 128 a thread at launch, 65536 in all.  d = 128: an epilogue that reads O 16 columns at a time leaves the
+  // softmax 200 and with them fewer spills (4 x 2048 x 16 causal 74.8 us instead of 77.4, capped 121 instead of 127); at
+  // d = 64 the same split was slower (S = 16384: 240 us instead of 200).
+  static constexpr int SOFTMAX_REGS = D == 128 ? 200 : 192, EPI_REGS = D == 128 ? 56 : 72, EPI_COLS = D == 128 ? 16 : 32;
   static constexpr uint32_t T_S0 = 0, T_S1 = 128, T_O0 = 256, T_O1 = 256 + D;
   static constexpr uint32_t T_P0 = SEP ? 384 : T_S0, T_P1 = SEP ? 448 : T_S1;
 };
@@ -109,6 +113,11 @@ __device__ __forceinline__ Item decode(const Args& a, int item) {
 // Whether the exponentials of the two tiles take turns.
 template <int D>
 constexpr bool kTurns = D == 128;
+
+constexpr int kIssueRegs = 56;
+static_assert(4 * kIssueRegs + 8 * Cfg<64>::SOFTMAX_REGS + 4 * Cfg<64>::EPI_REGS <= 16 * 128 &&
+                  4 * kIssueRegs + 8 * Cfg<128>::SOFTMAX_REGS + 4 * Cfg<128>::EPI_REGS <= 16 * 128,
+              "registers of the launch");
 
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -191,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp < 4) {
-    reg_dec<56>();
+    reg_dec<kIssueRegs>();
     if (warp == 0 && elect_one()) {
       // ---------------------------------------------------------------- TMA
       int kv = 0, it = 0, q_issued = -1;
@@ -315,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp < 12) {
     // ------------------------------------------------------------------ softmax
-    reg_inc<192>();
+    reg_inc<C::SOFTMAX_REGS>();
     const int grp = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;  // query row within the tile (TMEM lane)
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
@@ -469,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ epilogue
-    reg_dec<72>();
+    reg_dec<C::EPI_REGS>();
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     uint8_t* stg = smem + C::OUT_OFF + (warp & 3) * 4096;
@@ -506,20 +515,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float inv = seen ? 1.f / ml.y : 0.f;
         const uint32_t t_o = tmem + (grp == 0 ? C::T_O0 : C::T_O1) + lane_off;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(t_o + c * 32, o);
-          if ((c & 1) == 0 && lane == 0) bulk_wait_read<0>();  // the last store has read the staged rows
+        for (int c = 0; c < D; c += C::EPI_COLS) {
+          uint32_t o[C::EPI_COLS];
+          tmem_ld(t_o + c, o);
+          if (c % 64 == 0 && lane == 0) bulk_wait_read<0>();  // the last store has read the staged rows
           tmem_wait_ld();
           __syncwarp();
-          if (c == D / 32 - 1) warp_arrive(&o_free[grp]);  // O and the statistics are in registers
-          stage_row(stg, 0, lane, (c & 1) * 32, o, inv);
-          if (c & 1) {
+          if (c == D - C::EPI_COLS) warp_arrive(&o_free[grp]);  // O and the statistics are in registers
+          stage_row(stg, 0, lane, c % 64, o, inv);
+          if ((c + C::EPI_COLS) % 64 == 0) {
             fence_proxy_async_smem();
             __syncwarp();
             const int row0 = t * BT + (warp & 3) * 32;
             if (lane == 0 && row0 < a.S) {
-              tma_store_3d(&tm_out, stg, w.h * D + (c / 2) * 64, row0, w.b);
+              tma_store_3d(&tm_out, stg, w.h * D + (c / 64) * 64, row0, w.b);
               bulk_commit();
             }
           }
