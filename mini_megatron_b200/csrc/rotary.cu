@@ -9,13 +9,16 @@
 //
 // Memory bounds it: every value is read and written once.  The angles cost
 // nothing next to that because they depend on the token only: a CTA takes up
-// to 4 tokens (16 x 1024 tokens of 36 heads of 64 in bf16,
-// 151 MB: 33 us with 4, 40 with 1, 36 with 12), computes their r/2 sines and cosines once into shared memory
-// (the turn p f_i in 64 bits, reduced to [-1/2, 1/2] before it is rounded to 32,
-// so a position of millions keeps its angle to 2^-24 of a turn) and then
-// streams all heads of those tokens in 16-byte units, neighbouring threads on
-// neighbouring units; at 32 registers a thread eight CTAs keep an SM's loads in flight (two units
-// a thread at 70 registers: 39 us).  Values are rotated in 32 bits and rounded once.
+// to 4 tokens, copies what is not rotated, computes their r/2 sines and cosines
+// once into shared memory (the turn p f_i in 64 bits, reduced to [-1/2, 1/2]
+// before it is rounded to 32, so a position of millions keeps its angle to 2^-24
+// of a turn) and then streams the rotated heads in 16-byte units, neighbouring
+// threads on neighbouring units.  Values are rotated in 32 bits and rounded once.
+//
+// At 32 registers a thread 16 CTAs of 128 threads keep an SM's loads in flight.
+// 16 x 1024 tokens of 36 heads of 64 in bf16, 24 of them rotated (151 MB): 28.0 us,
+// 5.4 TB/s; 28.5 with 2 tokens, 29.5 with 256 threads, 32.8 with 256 threads, the
+// angles first and the token's row found anew for every unit.  40 registers: 35 us.
 #include "common.cuh"
 #include "ops.h"
 
@@ -24,7 +27,7 @@
 namespace mmb {
 namespace rope {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxTokens = 4;
 
 struct Args {
@@ -70,24 +73,48 @@ struct Vec<float> {
 };
 
 template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 2048 / kThreads) rotary_kernel(const Args a) {
   pdl_trigger();
   constexpr int N = Vec<T>::N;
   extern __shared__ __align__(16) float s_sc[];  // [tokens of this CTA][2][r / 2]: cosines, then sines
+  __shared__ long s_x[kMaxTokens], s_y[kMaxTokens];  // where the tokens' rows begin
+  __shared__ double s_pos[kMaxTokens];
   const int half = a.rot / 2;
   const long t0 = (long)blockIdx.x * a.per_cta;
   const int nt = (int)min((long)a.per_cta, a.tokens - t0);
   pdl_wait();
-  for (int u = threadIdx.x; u < nt * half; u += kThreads) {
-    const int t = u / half, i = u % half;
-    const long tok = t0 + t;
-    const long b = tok / a.S;
-    const int s = (int)(tok % a.S);
+  if (threadIdx.x < nt) {
+    const long tok = t0 + threadIdx.x, b = tok / a.S, s = tok - b * a.S;
+    s_x[threadIdx.x] = b * a.x_sb + s * a.x_ss;
+    s_y[threadIdx.x] = b * a.y_sb + s * a.y_ss;
     double p = (double)s;
     if (a.positions)
       p = a.pos64 ? (double)static_cast<const long*>(a.positions)[b * a.pos_sb + s]
                   : (double)static_cast<const int*>(a.positions)[b * a.pos_sb + s];
-    const double turns = p * a.freqs[i];
+    s_pos[threadIdx.x] = p;
+  }
+  __syncthreads();
+
+  const T* x = static_cast<const T*>(a.x);
+  T* y = static_cast<T*>(a.y);
+  if (a.copy) {  // needs no angles
+    const int tail = (a.d - a.rot) / N, full = a.d / N;
+    const int copies = a.heads_rot * tail + (a.heads - a.heads_rot) * full;
+    for (int u = threadIdx.x; u < nt * copies; u += kThreads) {
+      const int t = u / copies, r = u - t * copies;
+      long off;
+      if (r < a.heads_rot * tail) {
+        const int h = r / tail;
+        off = (long)h * a.d + a.rot + (r - h * tail) * N;
+      } else {
+        off = (long)a.heads_rot * a.d + (long)(r - a.heads_rot * tail) * N;
+      }
+      *reinterpret_cast<uint4*>(y + s_y[t] + off) = *reinterpret_cast<const uint4*>(x + s_x[t] + off);
+    }
+  }
+  for (int u = threadIdx.x; u < nt * half; u += kThreads) {
+    const int t = u / half, i = u - t * half;
+    const double turns = s_pos[t] * a.freqs[i];
     float sn, cs;
     sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
     s_sc[t * a.rot + i] = cs * a.magnitude;
@@ -95,18 +122,14 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const Args a) {
   }
   __syncthreads();
 
-  const T* x = static_cast<const T*>(a.x);
-  T* y = static_cast<T*>(a.y);
   // rotated units: two vectors of one head (halves: one from each; neighbours: two adjacent ones)
   const int per_head = a.rot / (2 * N);
   const int per_tok = per_head * a.heads_rot;
   for (int u = threadIdx.x; u < nt * per_tok; u += kThreads) {
     const int t = u / per_tok, r = u - t * per_tok;
     const int h = r / per_head, g = r - h * per_head;
-    const long tok = t0 + t;
-    const long b = tok / a.S, s = tok - b * a.S;
-    const T* xp = x + b * a.x_sb + s * a.x_ss + (long)h * a.d;
-    T* yp = y + b * a.y_sb + s * a.y_ss + (long)h * a.d;
+    const T* xp = x + s_x[t] + (long)h * a.d;
+    T* yp = y + s_y[t] + (long)h * a.d;
     const int o0 = INTERLEAVED ? 2 * g * N : g * N;
     const int o1 = INTERLEAVED ? o0 + N : o0 + half;
     float v0[N], v1[N], w0[N], w1[N];
@@ -129,23 +152,6 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const Args a) {
     }
     Vec<T>::store(yp + o0, w0);
     Vec<T>::store(yp + o1, w1);
-  }
-  if (!a.copy) return;
-  const int tail = (a.d - a.rot) / N, full = a.d / N;
-  const int copies = a.heads_rot * tail + (a.heads - a.heads_rot) * full;
-  for (int u = threadIdx.x; u < nt * copies; u += kThreads) {
-    const int t = u / copies, r = u - t * copies;
-    long off;
-    if (r < a.heads_rot * tail) {
-      const int h = r / tail;
-      off = (long)h * a.d + a.rot + (r - h * tail) * N;
-    } else {
-      off = (long)a.heads_rot * a.d + (long)(r - a.heads_rot * tail) * N;
-    }
-    const long tok = t0 + t;
-    const long b = tok / a.S, s = tok - b * a.S;
-    *reinterpret_cast<uint4*>(y + b * a.y_sb + s * a.y_ss + off) =
-        *reinterpret_cast<const uint4*>(x + b * a.x_sb + s * a.x_ss + off);
   }
 }
 
@@ -179,12 +185,13 @@ int rotary(const void* x, long x_sb, long x_ss, void* y, long y_sb, long y_ss, i
   a.tokens = B * S;
   a.copy = (x != y);
   // few tokens: one per CTA, so that a short call still spreads over the SMs
-  const long fit = 48 * 1024 / ((long)rot * (long)sizeof(float));  // the angles of a CTA's tokens in shared memory
+  constexpr long kAngles = 47 * 1024;
+  const long fit = kAngles / ((long)rot * (long)sizeof(float));  // the angles of a CTA's tokens in shared memory
   a.per_cta = (int)std::max(1L, std::min({(long)kMaxTokens, fit, a.tokens / (8L * num_sms)}));
   const long grid = (a.tokens + a.per_cta - 1) / a.per_cta;
   if (grid > 0x7fffffffL) return -2;
   const size_t smem = (size_t)a.per_cta * rot * sizeof(float);
-  if (smem > 48 * 1024) return -3;
+  if (smem > (size_t)kAngles) return -3;
   if (is_f32) {
     if (interleaved) launch_k(rotary_kernel<float, true>, (unsigned)grid, kThreads, smem, stream, a);
     else launch_k(rotary_kernel<float, false>, (unsigned)grid, kThreads, smem, stream, a);
