@@ -59,7 +59,7 @@ struct Args {
   int4* kstat;            // [B, n_t] the same of the query intervals
 };
 
-struct Agg {
+struct alignas(16) Agg {
   int ds, lu, stop, nf;  // max document start, max unmarked index, min stopping index, min document start
 };
 
@@ -138,9 +138,9 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
 
   // ---- reduce the chunk, step by step (a row of one step has nothing to carry over)
   const bool alone = n_cta == 1 && n_steps == 1;
+  bool first[kPer], plain[kPer];  // of the last step read
   for (int st = 0; !alone && st < n_steps; ++st) {
     const int i0 = c0 + st * kStep + tid * kPer;
-    bool first[kPer], plain[kPer];
     load_flags(a, b, i0, len, first, plain);
     Agg g{-1, -1, a.S, a.S};
 #pragma unroll
@@ -183,22 +183,16 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
   Agg left{-1, -1, a.S, a.S}, right{-1, -1, a.S, a.S};
   if (n_cta > 1) {
     cluster_sync_all();
-    for (int r = 0; r < n_cta; ++r) {
-      if (r == rank) continue;
-      const uint32_t addr = cluster_addr(&s_cta, r);
-      int ds, lu, stop, nf;
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(ds) : "r"(addr) : "memory");
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(lu) : "r"(addr + 4) : "memory");
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(stop) : "r"(addr + 8) : "memory");
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(nf) : "r"(addr + 12) : "memory");
-      if (r < rank) {
-        left.ds = max(left.ds, ds);
-        left.lu = max(left.lu, lu);
-      } else {
-        right.stop = min(right.stop, stop);
-        right.nf = min(right.nf, nf);
-      }
-    }
+    Agg g{-1, -1, a.S, a.S};  // of CTA `lane`
+    if (lane < n_cta)
+      asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(g.ds), "=r"(g.lu), "=r"(g.stop), "=r"(g.nf)
+                   : "r"(cluster_addr(&s_cta, lane))
+                   : "memory");
+    left.ds = __reduce_max_sync(0xffffffffu, lane < rank ? g.ds : -1);
+    left.lu = __reduce_max_sync(0xffffffffu, lane < rank ? g.lu : -1);
+    right.stop = __reduce_min_sync(0xffffffffu, lane > rank ? g.stop : a.S);
+    right.nf = __reduce_min_sync(0xffffffffu, lane > rank ? g.nf : a.S);
   }
 
   // ---- scan and write, right to left
@@ -210,8 +204,7 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
       lu_left = max(lu_left, s_step[u].lu);
     }
     const int i0 = c0 + st * kStep + tid * kPer;
-    bool first[kPer], plain[kPer];
-    load_flags(a, b, i0, len, first, plain);
+    if (alone || st + 1 < n_steps) load_flags(a, b, i0, len, first, plain);
     int ds[kPer], lu[kPer], stop[kPer], nf[kPer];  // inclusive from the left / first stop and document start > i
     int rd = -1, rl = -1;
 #pragma unroll
