@@ -26,7 +26,8 @@
 // chunk results cross the cluster through distributed shared memory, and a
 // second sweep (right to left) scans and writes.  The work is a few bytes per
 // token: latency bounds it, so the row is spread over CTAs as soon as one CTA
-// would need more than one sweep step (4096 tokens).
+// would need more than one sweep step (4096 tokens).  8 x 32768 tokens: 10.0 us and 4.8 us for the
+// order (2 x 257: 4.8 us), against 0.9 us for the bytes alone.
 #include "common.cuh"
 #include "ops.h"
 

