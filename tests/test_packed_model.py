@@ -1,6 +1,5 @@
 """Plan, rotary positions and masked attention together: as a chain, and inside the GPT and its trainer."""
 import copy
-import os
 
 import pytest
 import torch
@@ -12,9 +11,7 @@ from packed_ref import attention_ref, plan_ref, rotary_ref, row_tensors, split_r
 @pytest.fixture(scope="module", autouse=True)
 def _pg():
     if not dist.is_initialized():
-        os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
-        os.environ.setdefault("MASTER_PORT", "29567")
-        dist.init_process_group("gloo", rank=0, world_size=1)
+        dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)  # no port: workers run side by side
     yield
 
 
