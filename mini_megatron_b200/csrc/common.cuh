@@ -45,6 +45,7 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 // access, which blocks until the previous grid has completed and its writes
 // are visible, so the data dependencies are those of plain stream order.
 // Both instructions are no-ops for a grid launched without the attribute.
+// The kernels of packed rows (document_plan.cu, rotary.cu, masked_attn_*.cu) are always launched so.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -56,27 +57,36 @@ inline bool pdl_enabled() {
   return on;
 }
 
-// Kernel launch: a plain stream-ordered launch, or, with MMB_PDL=1, cudaLaunchKernelEx
-// with the programmatic-serialisation attribute.  Errors are left for the caller's
-// cudaGetLastError().
+// Launch with the programmatic-serialisation attribute (and a cluster size, if any): the kernel may be set up while its
+// predecessor in the stream still runs; it touches memory only behind pdl_wait().
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                            Args&&... args) {
-  if (!pdl_enabled()) {
-    kernel<<<grid, block, smem, stream>>>(std::forward<Args>(args)...);
-    return cudaPeekAtLastError();
-  }
+inline cudaError_t launch_early(int cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                                cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Kernel launch: a plain stream-ordered launch, or, with MMB_PDL=1, an early one.  Errors are left for the caller's
+// cudaGetLastError().
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                            Args&&... args) {
+  if (pdl_enabled()) return launch_early(0, kernel, grid, block, smem, stream, std::forward<Args>(args)...);
+  kernel<<<grid, block, smem, stream>>>(std::forward<Args>(args)...);
+  return cudaPeekAtLastError();
 }
 
 // 2^x with the hardware approximation (ex2.approx; -inf -> 0).

@@ -135,6 +135,8 @@ __global__ void __launch_bounds__(kThreads) document_plan_kernel(const Args a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int c0 = rank * a.chunk, c1 = min(c0 + a.chunk, a.n_t * 128);
   const int n_steps = (c1 - c0 + kStep - 1) / kStep;
+  pdl_trigger();
+  pdl_wait();
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
 
   // ---- reduce the chunk, step by step (a row of one step has nothing to carry over)
@@ -356,7 +358,9 @@ __global__ void __launch_bounds__(kThreads) plan_order_kernel(const OrderArgs a)
     }
     return kBins - 1 - (w >> a.shift);
   };
+  pdl_trigger();
   for (int k = tid; k < kBins; k += kThreads) s_bin[k] = 0;
+  pdl_wait();
   __syncthreads();
   for (int e = tid; e < n; e += kThreads) atomicAdd(&s_bin[bin(e)], 1);
   __syncthreads();
@@ -418,18 +422,7 @@ int document_plan(const long* ids, long ld_ids, long eod, int by_change, const u
   a.kstat = static_cast<int4*>(kstat);
   const int n_cta = (S + a.chunk - 1) / a.chunk;
   if ((long)B * n_cta > INT_MAX) return -2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(B * n_cta));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = n_cta;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, document_plan_kernel, a);
+  const cudaError_t e = launch_early(n_cta, document_plan_kernel, (unsigned)(B * n_cta), kThreads, 0, stream, a);
   // rows of a few tiles: no tile is much heavier than another
   if (e != cudaSuccess || !order) return (int)e;
   OrderArgs o;
@@ -443,7 +436,7 @@ int document_plan(const long* ids, long ld_ids, long eod, int by_change, const u
   o.out[0] = order;
   o.out[1] = order + (size_t)B * o.n_pairs;
   o.out[2] = o.out[1] + (size_t)B * a.n_t;
-  plan_order_kernel<<<3, kThreads, 0, stream>>>(o);
+  launch_early(0, plan_order_kernel, 3, kThreads, 0, stream, o);
   return (int)cudaGetLastError();
 }
 

@@ -512,7 +512,7 @@ int launch(const CUtensorMap& tq, const CUtensorMap& to, const CUtensorMap& td, 
   auto k = masked_attn_dkv_kernel<D, CAP, BIAS>;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, td, a);
+  launch_early(0, k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, td, a);
   return (int)cudaGetLastError();
 }
 
@@ -606,7 +606,7 @@ int masked_attn_dkv(const AttnCall& c, const void* dout, long do_ss, long do_sb,
   if (rc || parts == 1) return rc;
   const long tokens = (long)c.B * c.S, wid = 2L * c.nkv * c.d;
   const long units = tokens * (wid / 8);
-  launch_k(dkv::join_parts_kernel, (unsigned)std::min((units + 255) / 256, 8L * num_sms), 256, 0, stream, partial, parts,
+  launch_early(0, dkv::join_parts_kernel, (unsigned)std::min((units + 255) / 256, 8L * num_sms), 256, 0, stream, partial, parts,
            tokens * wid, tokens, (int)wid, static_cast<__nv_bfloat16*>(dqkv), width, (long)c.nh * c.d);
   return (int)cudaGetLastError();
 }

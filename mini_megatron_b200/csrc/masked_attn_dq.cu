@@ -499,7 +499,7 @@ int row_stats(const AttnCall& c, const void* dout, long do_ss, long do_sb, const
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
   }
-  launch_k(k, (unsigned)grid, 256, smem, stream, static_cast<const __nv_bfloat16*>(dout), do_ss, do_sb,
+  launch_early(0, k, (unsigned)grid, 256, smem, stream, static_cast<const __nv_bfloat16*>(dout), do_ss, do_sb,
            static_cast<const __nv_bfloat16*>(out), lse, c.S, c.nh, n_t, ld);
   return (int)cudaGetLastError();
 }
@@ -509,7 +509,7 @@ int launch(const CUtensorMap& tq, const CUtensorMap& to, const CUtensorMap& td, 
   auto k = masked_attn_dq_kernel<D, CAP, BIAS>;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, td, a);
+  launch_early(0, k, grid, kThreads, Cfg<D>::SMEM, stream, tq, to, td, a);
   return (int)cudaGetLastError();
 }
 

@@ -559,7 +559,7 @@ int launch(const CUtensorMap& tm, const CUtensorMap& to, const Args& a, int grid
   auto k = masked_attn_fwd_kernel<D, CAP, BIAS>;
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  launch_k(k, grid, kThreads, Cfg<D>::SMEM, stream, tm, to, a);
+  launch_early(0, k, grid, kThreads, Cfg<D>::SMEM, stream, tm, to, a);
   return (int)cudaGetLastError();
 }
 

@@ -193,11 +193,11 @@ int rotary(const void* x, long x_sb, long x_ss, void* y, long y_sb, long y_ss, i
   const size_t smem = (size_t)a.per_cta * rot * sizeof(float);
   if (smem > (size_t)kAngles) return -3;
   if (is_f32) {
-    if (interleaved) launch_k(rotary_kernel<float, true>, (unsigned)grid, kThreads, smem, stream, a);
-    else launch_k(rotary_kernel<float, false>, (unsigned)grid, kThreads, smem, stream, a);
+    if (interleaved) launch_early(0, rotary_kernel<float, true>, (unsigned)grid, kThreads, smem, stream, a);
+    else launch_early(0, rotary_kernel<float, false>, (unsigned)grid, kThreads, smem, stream, a);
   } else {
-    if (interleaved) launch_k(rotary_kernel<__nv_bfloat16, true>, (unsigned)grid, kThreads, smem, stream, a);
-    else launch_k(rotary_kernel<__nv_bfloat16, false>, (unsigned)grid, kThreads, smem, stream, a);
+    if (interleaved) launch_early(0, rotary_kernel<__nv_bfloat16, true>, (unsigned)grid, kThreads, smem, stream, a);
+    else launch_early(0, rotary_kernel<__nv_bfloat16, false>, (unsigned)grid, kThreads, smem, stream, a);
   }
   return (int)cudaGetLastError();
 }

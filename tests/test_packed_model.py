@@ -147,6 +147,46 @@ def test_chain_against_64_bits(d, nh, nkv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("S", [300, 1100])
+def test_chain_without_pauses(S):
+    """Buffers rewritten and used over and over without a pause give the bits of calls that are waited for each time:
+    every kernel may be set up before its predecessor has finished, and reads nothing before."""
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    from mini_megatron_b200.ops.documents import document_plan
+    from mini_megatron_b200.ops.rotary import Rotary, rotary_bwd, rotary_fwd
+    B, nh, nkv, d = 2, 4, 2, 64
+    g = torch.Generator().manual_seed(S)
+    rot = Rotary(d, device="cuda")
+    data = [(torch.randint(0, 60, (B, S), generator=g).cuda(),
+             torch.randn(B, S, (nh + 2 * nkv) * d, generator=g).bfloat16().cuda(),
+             torch.randn(B, S, nh * d, generator=g).bfloat16().cuda()) for _ in range(3)]
+    tokens, qkv, dctx = (torch.empty_like(t) for t in data[0])
+
+    def step(k, pause):
+        def wait():
+            if pause:
+                torch.cuda.synchronize()
+        for t, new in zip((tokens, qkv, dctx), data[k % 3]):
+            t.copy_(new)
+        wait()
+        plan = document_plan(tokens, eod=0)
+        wait()
+        rotary_fwd(qkv, rot, nh + nkv, plan.positions, out=qkv)
+        wait()
+        ctx, lse = attention_fwd(qkv, nh, d, num_kv_heads=nkv, plan=plan)
+        wait()
+        grad = attention_bwd(dctx, qkv, ctx, lse, nh, d, num_kv_heads=nkv, plan=plan)
+        wait()
+        return ctx, lse, rotary_bwd(grad, rot, nh + nkv, plan.positions, out=grad)
+
+    want = [step(k, True) for k in range(3)]
+    got = [step(k, False) for k in range(30)]
+    torch.cuda.synchronize()
+    for k, one in enumerate(got):
+        assert all(torch.equal(x, y) for x, y in zip(one, want[k % 3])), k
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", sorted(VARIANTS))
 def test_native_model_matches_cpu(name):
     """Loss and gradients of the native model against the fp32 CPU path on the same weights.
