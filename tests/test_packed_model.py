@@ -187,6 +187,31 @@ def test_chain_without_pauses(S):
 
 
 @pytest.mark.gpu
+def test_activations_beyond_32_bit_offsets():
+    """2.4 G elements: the last rows of the batch get the bits that they get alone."""
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    from mini_megatron_b200.ops.documents import document_plan
+    from mini_megatron_b200.ops.rotary import Rotary, rotary_bwd, rotary_fwd
+    B, S, nh, d = 1600, 1000, 8, 64
+    torch.manual_seed(7)
+    qkv = torch.randn(B, S, 3 * nh * d, device="cuda", dtype=torch.bfloat16)
+    dctx = torch.randn(B, S, nh * d, device="cuda", dtype=torch.bfloat16)
+    tokens = torch.randint(0, 200, (B, S), device="cuda")
+    rot = Rotary(d, device="cuda")
+    assert qkv.numel() > 2 ** 31
+
+    def run(qkv, dctx, tokens):
+        plan = document_plan(tokens, eod=0)
+        x = rotary_fwd(qkv, rot, 2 * nh, plan.positions)
+        ctx, lse = attention_fwd(x, nh, d, plan=plan)
+        grad = attention_bwd(dctx, x, ctx, lse, nh, d, plan=plan)
+        return x[-2:].clone(), ctx[-2:].clone(), lse[-2:].clone(), rotary_bwd(grad, rot, 2 * nh, plan.positions)[-2:].clone()
+
+    whole, alone = run(qkv, dctx, tokens), run(qkv[-2:], dctx[-2:], tokens[-2:])
+    assert all(torch.equal(a, b) for a, b in zip(whole, alone))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", sorted(VARIANTS))
 def test_native_model_matches_cpu(name):
     """Loss and gradients of the native model against the fp32 CPU path on the same weights.
