@@ -18,7 +18,8 @@
 // operand of each of these products is bf16 and the tensor cores take pairs of one type; in 32 bits (tf32) the
 // products would take twice the time and P and dS twice the TMEM columns, which are all in use.  Delta is taken from ctx as
 // it was returned, rounded: the unrounded one would take another pass over the tiles.  Against 64 bits the outputs are
-// off by 0.0021 to 0.0036 (norm of the error over the norm), one rounding of the outputs alone makes 0.0017.
+// off by 0.0021 to 0.0036 (norm of the error over the norm): one rounding of the outputs makes 0.0017, P and dS 0.0016, Delta
+// 0.0005 with even weights to 0.0019 with sharp ones.
 //
 // These kernels, row_stats, rotary and the plans are launched early (launch_early): barriers, TMEM and the first
 // instructions are set up behind the predecessor's last CTAs.  Short calls are made of that: forward and backward of 2
