@@ -103,7 +103,11 @@ class _AttentionFn(torch.autograd.Function):
 
 def attention(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, softcap=None, alibi_slopes=None,
               softmax_scale=None):
-    """Differentiable masked attention: :func:`attention_fwd`'s ``ctx``."""
+    """Differentiable masked attention: :func:`attention_fwd`'s ``ctx``.
+
+    Into a CUDA graph, capture :func:`attention_fwd` and :func:`attention_bwd` rather than an autograd pass over leaves
+    whose eager graph is still alive: autograd would add up their gradients on the stream of that graph.
+    """
     opts = dict(num_kv_heads=num_kv_heads, plan=plan, softcap=softcap, alibi_slopes=alibi_slopes,
                 softmax_scale=softmax_scale)
     if not qkv.is_cuda:
