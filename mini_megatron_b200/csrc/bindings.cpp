@@ -425,6 +425,15 @@ std::vector<Tensor> document_plan(const Tensor& ids, int64_t eod, bool by_change
   return {out.select(0, 0), out.select(0, 1), out.select(0, 2), tables};
 }
 
+// Whether a leaf's gradients would be added up on another stream than the current one: by the node of a graph that
+// was built on that stream and is still alive.
+bool accumulates_elsewhere(const Tensor& leaf) {
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (!node) return false;
+  const auto stream = node->stream();
+  return stream.has_value() && *stream != at::cuda::getCurrentCUDAStream(leaf.device().index()).unwrap();
+}
+
 // ----------------------------------------------------------------- rotary positions
 // x, y [B, S, heads * d] bf16 / fp32 (y may be x; none: a new tensor), positions [B, S] or [S] int32 / int64 or none, freqs [rot / 2] fp64.
 Tensor rotary(const Tensor& x, const c10::optional<Tensor>& out, const c10::optional<Tensor>& positions,
@@ -1097,6 +1106,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("num_sms", &num_sms);
   m.def("document_plan", &document_plan, py::arg("ids"), py::arg("eod"), py::arg("by_change"), py::arg("marks"),
         py::arg("lengths"));
+  m.def("accumulates_elsewhere", &accumulates_elsewhere);
   m.def("document_plan_max_len", &mmb::document_plan_max_len);
   m.def("rotary", &rotary, py::arg("x"), py::arg("out"), py::arg("positions"), py::arg("freqs"), py::arg("magnitude"),
         py::arg("interleaved"), py::arg("head_dim"), py::arg("rotary_dim"), py::arg("num_heads"),

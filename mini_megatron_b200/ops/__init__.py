@@ -46,3 +46,13 @@ def check_errors():
     if code:
         C.clear_error()
         raise RuntimeError(f"device kernel reported error code {code} (bounded wait timed out)")
+
+
+def check_capture(x):
+    """Refuse a leaf in a CUDA graph capture while a graph built on another stream holds its gradient accumulator: the
+    captured backward would make that stream part of the capture, which ends the process."""
+    import torch
+    if (x.is_cuda and x.requires_grad and x.is_leaf and torch.cuda.is_current_stream_capturing()
+            and native().accumulates_elsewhere(x)):
+        raise RuntimeError("an autograd graph of this tensor, built outside of the capture, is still alive: drop it (its "
+                           "outputs and losses) before capturing, or capture the forward and backward operators")

@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import native
+from . import check_capture, native
 
 
 def flash_attn_fwd(qkv, B, S, nh, d):
@@ -105,13 +105,13 @@ def attention(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, softcap
               softmax_scale=None):
     """Differentiable masked attention: :func:`attention_fwd`'s ``ctx``.
 
-    Into a CUDA graph, capture :func:`attention_fwd` and :func:`attention_bwd` rather than an autograd pass over leaves
-    whose eager graph is still alive: autograd would add up their gradients on the stream of that graph.
+    While a CUDA graph is captured, a leaf whose autograd graph from outside of the capture is still alive is refused.
     """
     opts = dict(num_kv_heads=num_kv_heads, plan=plan, softcap=softcap, alibi_slopes=alibi_slopes,
                 softmax_scale=softmax_scale)
     if not qkv.is_cuda:
         return attention_fwd(qkv, num_heads, head_dim, **opts)[0]
+    check_capture(qkv)
     return _AttentionFn.apply(qkv, num_heads, head_dim, opts)
 
 

@@ -14,7 +14,7 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import native
+from . import check_capture, native
 
 SCALINGS = (None, "linear", "ntk", "yarn")
 
@@ -126,6 +126,7 @@ class _RotaryFn(torch.autograd.Function):
 
 def apply_rotary(x, rotary, num_heads, positions=None):
     """:func:`rotary_fwd` as a differentiable operation (out of place)."""
+    check_capture(x)
     return _RotaryFn.apply(x, rotary, num_heads, positions)
 
 

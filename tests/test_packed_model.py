@@ -212,6 +212,32 @@ def test_activations_beyond_32_bit_offsets():
 
 
 @pytest.mark.gpu
+def test_captured_backward_and_a_live_eager_graph():
+    from mini_megatron_b200.ops.attention import attention
+    from mini_megatron_b200.ops.rotary import Rotary, apply_rotary
+    rot = Rotary(64, device="cuda")
+    x = torch.randn(1, 200, 3 * 64, device="cuda").bfloat16().requires_grad_(True)
+    dctx = torch.randn(1, 200, 64, device="cuda").bfloat16()
+
+    def grad():
+        return torch.autograd.grad(attention(apply_rotary(x, rot, 2), 1, 64), x, dctx)[0]
+
+    want = grad()
+    alive = attention(x, 1, 64)
+    for f in (lambda: attention(x, 1, 64), lambda: apply_rotary(x, rot, 2)):
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                f()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = grad()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", sorted(VARIANTS))
 def test_native_model_matches_cpu(name):
     """Loss and gradients of the native model against the fp32 CPU path on the same weights.
