@@ -102,7 +102,7 @@ struct FastDiv {
   __device__ __forceinline__ int quot(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> (31 + l)); }
 };
 
-// Work items travel from one scheduling thread to the roles through a ring in shared memory: decoding an item
+// Work items travel from one scheduling thread (forward) or warp (backward) to the roles through a ring in shared memory: decoding an item
 // (divisions, loads of the mask's tile tables) takes about a thousand cycles, which every role would otherwise
 // spend between two items.
 constexpr int kRing = 4;
@@ -114,19 +114,10 @@ struct Ring {
   // consumer side, item number k: a whole warp / one thread
   __device__ __forceinline__ bool get_warp(Item& w, int k, int* err, volatile int* abort_flag) const;
   __device__ __forceinline__ bool get_thread(Item& w, int k, int* err, volatile int* abort_flag) const;
-  // producer side
+  // producer side: one thread / a whole warp
   __device__ __forceinline__ bool put(const Item& w, int k, int* err, volatile int* abort_flag) const;
   __device__ __forceinline__ bool put_warp(const Item& w, int k, int* err, volatile int* abort_flag) const;
 };
-
-__device__ __forceinline__ void st_shared(uint32_t addr, float v) {
-  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
-__device__ __forceinline__ float ld_shared(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
 
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
@@ -410,6 +401,7 @@ __device__ __forceinline__ void zero_rows(void* p, size_t stride, int rows) {
     *reinterpret_cast<uint4*>(static_cast<char*>(p) + (u / PER) * stride + (u % PER) * 16) = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// N values of one row set to zero.
 template <int N>
 __device__ __forceinline__ void store_zero(__nv_bfloat16* p) {
 #pragma unroll
