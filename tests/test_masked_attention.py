@@ -109,6 +109,33 @@ def test_same_bits_twice_and_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls of different shapes on two streams at the same time give the bits that they give alone."""
+    from mini_megatron_b200.ops import check_errors
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    sets = [(_case(6, 1100, 8, 2, 64, 250, True, True, 1.0, "cuda", torch.bfloat16), 8, 2, 64),
+            (_case(3, 1500, 6, 6, 128, 400, False, True, 1.0, "cuda", torch.bfloat16, seed=9), 6, 6, 128)]
+
+    def call(case, nh, nkv, d):
+        qkv, dctx, plan, _, _ = case
+        ctx, lse = attention_fwd(qkv, nh, d, num_kv_heads=nkv, plan=plan)
+        return ctx, lse, attention_bwd(dctx, qkv, ctx, lse, nh, d, num_kv_heads=nkv, plan=plan)
+
+    want = [call(*c) for c in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(12):
+        for s, c in zip(streams, sets):
+            with torch.cuda.stream(s):
+                got.append(call(*c))
+    torch.cuda.synchronize()
+    check_errors()
+    for k, one in enumerate(got):
+        assert all(torch.equal(x, y) for x, y in zip(one, want[k % 2])), k
+
+
+@pytest.mark.gpu
 def test_strides_and_neighbours():
     """Rows inside wider buffers, a token-major batch; padding gives zeros, what lies around is not read into it."""
     from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
