@@ -544,6 +544,7 @@ mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, c
                     tables->numel() == at_.total,
                 "attention: the plan was made for other rows than qkv's [", B, ", ", S, "] or on another device");
     const int* t = tables->data_ptr<int>();
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t) % 16 == 0, "attention: the plan's tables must lie on a 16-byte boundary");
     c.rows = t + at_.rows;
     c.qstat = t + at_.qstat;
     c.kstat = t + at_.kstat;
@@ -590,6 +591,7 @@ Tensor masked_attn_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out,
   TORCH_CHECK(dout.size(0) == c.B && dout.size(1) == c.S && dout.size(2) == nh * d && out.sizes() == dout.sizes() &&
                   lse.dim() == 3 && lse.size(0) == c.B && lse.size(1) == nh && lse.size(2) == c.S,
               "attention: dctx and ctx must be [B, S, num_heads * head_dim] and lse [B, num_heads, S] of the forward");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0, "attention: ctx must lie on a 16-byte boundary");
   Tensor dqkv = at::empty({c.B, c.S, (nh + 2 * nkv) * d}, qkv.options());
   if (dqkv.numel() == 0) return dqkv;
   Tensor ld = at::empty({c.B, nh, (c.S + 127) / 128, 256}, lse.options());

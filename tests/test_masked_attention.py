@@ -359,3 +359,27 @@ def test_refusals_gpu():
                  (ctx.cpu(), x, ctx, lse), (ctx, x, ctx, lse.cpu())]:
         with pytest.raises(RuntimeError):
             attention_bwd(*args, 2, 64)
+
+
+@pytest.mark.gpu
+def test_tensors_off_the_16_byte_boundary_are_refused():
+    """Views that are contiguous but start inside a 16-byte unit: the kernels read whole units."""
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    from mini_megatron_b200.ops.documents import DocumentPlan, document_plan
+    B, S, nh, d = 2, 700, 2, 64
+    qkv = torch.randn(B, S, 3 * nh * d, device="cuda").bfloat16()
+    dctx = torch.randn(B, S, nh * d, device="cuda").bfloat16()
+    ctx, lse = attention_fwd(qkv, nh, d)
+    for off in (1, 2, 4, 7):
+        moved = torch.zeros(ctx.numel() + 8, device="cuda", dtype=ctx.dtype)[off:off + ctx.numel()].view_as(ctx)
+        moved.copy_(ctx)
+        assert moved.is_contiguous()
+        with pytest.raises(RuntimeError, match="16-byte"):
+            attention_bwd(dctx, qkv, moved, lse, nh, d)
+        with pytest.raises(RuntimeError, match="16-byte"):
+            attention_bwd(moved, qkv, ctx, lse, nh, d)
+    plan = document_plan(torch.ones(B, S, dtype=torch.int64, device="cuda"), eod=0)
+    for off in (1, 2, 3):
+        tables = torch.zeros(plan.tables.numel() + 4, device="cuda", dtype=torch.int32)[off:off + plan.tables.numel()]
+        with pytest.raises(RuntimeError, match="16-byte"):
+            attention_fwd(qkv, nh, d, plan=DocumentPlan(plan.positions, plan.start, plan.end, tables))
