@@ -492,6 +492,7 @@ Tensor rotary(const Tensor& x, const c10::optional<Tensor>& out, const c10::opti
     pp = p.data_ptr();
     pos_sb = p.dim() == 2 ? p.stride(0) : 0;
   }
+  if (out.has_value()) out->unsafeGetTensorImpl()->bump_version();  // graphs that saved it see that it changed
   MMB_CHECK_RC(mmb::rotary(x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(), y.stride(0), y.stride(1), f32, pp,
                            pos64, pos_sb, freqs.data_ptr<double>(), (float)magnitude, inverse ? -1.f : 1.f,
                            interleaved, B, (int)S, (int)d, (int)rot, (int)heads_rot, (int)heads, num_sms(),

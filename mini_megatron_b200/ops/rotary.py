@@ -92,6 +92,9 @@ def _run(x, rotary, num_heads, positions, out, inverse):
     if not x.is_cuda:
         y = _rotary_cpu(x, rotary, num_heads, positions, inverse)
         return y if out is None else out.copy_(y)
+    if out is not None and torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
+        raise RuntimeError("rotary: autograd does not record what is written to out= on CUDA; use apply_rotary for tensors "
+                           "that require a gradient, or torch.no_grad()")
     freqs = rotary._turns.get(x.device)
     if freqs is None:
         freqs = rotary.turns(x.device)
@@ -101,12 +104,16 @@ def _run(x, rotary, num_heads, positions, out, inverse):
 
 def rotary_fwd(x, rotary, num_heads, positions=None, out=None):
     """The first ``num_heads`` heads of ``x`` rotated to ``positions`` (``[B, S]`` or ``[S]`` int32 / int64;
-    default: the index in the row).  ``out=x`` works in place; another ``out`` must not overlap ``x``."""
+    default: the index in the row).  ``out=x`` works in place; another ``out`` must not overlap ``x``.
+
+    On CUDA autograd does not see this call: the result carries no gradient (:func:`apply_rotary` is the differentiable
+    form), and ``out`` is refused for tensors that require one.  A write to ``out`` counts as an in-place operation, so
+    a graph that saved it earlier refuses its backward pass."""
     return _run(x, rotary, num_heads, positions, out, False)
 
 
 def rotary_bwd(dy, rotary, num_heads, positions=None, out=None):
-    """Gradient of :func:`rotary_fwd`: the rotation by the negative angle (``out=dy`` works in place)."""
+    """Gradient of :func:`rotary_fwd`: the rotation by the negative angle (``out=dy`` works in place; autograd: as there)."""
     return _run(dy, rotary, num_heads, positions, out, True)
 
 

@@ -225,3 +225,60 @@ def test_rotary_wide_heads():
     back = rotary_bwd(y, rot, 1)
     # two roundings of bf16, each at most 2^-8 of the pair's length
     assert ((back.double() - x.double()).abs() <= 4 * 2.0 ** -8 * size.item()).all()
+
+
+@pytest.mark.gpu
+def test_rotary_in_place_is_seen_by_autograd():
+    """Writing to ``out`` is refused where a gradient would miss it, and noticed by graphs that saved the tensor."""
+    from mini_megatron_b200.ops.attention import attention
+    from mini_megatron_b200.ops.rotary import Rotary, rotary_bwd, rotary_fwd
+    r = Rotary(64, device="cuda")
+    leaf = torch.randn(1, 40, 192, device="cuda").bfloat16().requires_grad_(True)
+    plain = leaf.detach().clone()
+    inner = leaf * 1
+    for x, out in ((leaf, leaf), (inner, inner), (inner, plain.clone()), (plain, inner)):
+        for fn in (rotary_fwd, rotary_bwd):
+            before, version = out.detach().clone(), out._version
+            with pytest.raises(RuntimeError, match="apply_rotary"):
+                fn(x, r, 2, out=out)
+            assert torch.equal(out, before) and out._version == version
+    # saved by an operator, then overwritten
+    for write in (lambda t: rotary_fwd(t, r, 2, out=t), lambda t: rotary_bwd(t, r, 2, out=t),
+                  lambda t: rotary_fwd(plain, r, 2, out=t)):
+        x = leaf * 1
+        y = attention(x, 1, 64)
+        with torch.no_grad():
+            write(x)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.sum().backward()
+    # a view shares its base's counter; a refused call counts nothing
+    base = plain.clone()
+    version = base._version
+    rotary_fwd(base.view(1, 40, 192), r, 2, out=base.view(1, 40, 192))
+    assert base._version == version + 1
+    with pytest.raises(RuntimeError):
+        rotary_fwd(base, r, 4, out=base)
+    assert base._version == version + 1
+    # without gradients: the values of the call that returns a new tensor
+    want = rotary_fwd(plain, r, 2)
+    with torch.no_grad():
+        assert torch.equal(rotary_fwd(leaf, r, 2, out=leaf.detach().clone()), want)
+        rotary_fwd(leaf, r, 2, out=leaf)
+    assert torch.equal(leaf.detach(), want)
+    with torch.inference_mode():
+        x = plain * 1
+        assert torch.equal(rotary_fwd(x, r, 2, out=x), want)
+
+
+def test_rotary_in_place_gradients_cpu():
+    """On the CPU ``out`` is an ordinary in-place operation: recorded, and refused for leaves."""
+    from mini_megatron_b200.ops.rotary import Rotary, rotary_bwd, rotary_fwd
+    r = Rotary(16)
+    leaf = torch.randn(2, 5, 48, dtype=torch.float64, requires_grad=True)
+    dy = torch.randn(2, 5, 48, dtype=torch.float64)
+    x = leaf * 1
+    rotary_fwd(x, r, 2, out=x)
+    (grad,) = torch.autograd.grad(x, leaf, dy)
+    torch.testing.assert_close(grad, rotary_bwd(dy, r, 2), rtol=1e-12, atol=1e-12)
+    with pytest.raises(RuntimeError):
+        rotary_fwd(leaf, r, 2, out=leaf)
