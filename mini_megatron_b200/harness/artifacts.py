@@ -26,12 +26,13 @@ from pathlib import Path
 import torch
 
 from .bundle import sha256_file
-from .contract import CONTRACT, from_reference_state, full_parameter_names, shard_state
+from .contract import CONTRACT, check_model, from_reference_state, full_parameter_names, shard_state
 
 SCHEMA_VERSION = 1
 
 
 def _model_dict(c):
+    check_model(c)  # the keys below would drop what the contract does not know
     keys = ("num_layers", "hidden_size", "num_attention_heads", "ffn_hidden_size", "max_seq_len", "vocab_size")
     return {k: (c[k] if isinstance(c, dict) else getattr(c, k)) for k in keys}
 

@@ -21,6 +21,8 @@ from __future__ import annotations
 import importlib.util
 from pathlib import Path
 
+from .contract import check_model
+
 REPO = Path(__file__).resolve().parents[2]
 
 
@@ -37,6 +39,7 @@ def mcore_available() -> bool:
 
 def build_mcore_gpt(model_config: dict, tp: int = 1, pp: int = 1, bf16: bool = True):
     """Megatron-Core GPTModel matching the shared contract (requires megatron.core and its parallel state)."""
+    check_model(model_config)
     if not mcore_available():
         raise RuntimeError("Megatron-Core (megatron.core) is not installed in this environment")
     import torch

@@ -48,7 +48,24 @@ def _cfg(model_config, key):
     return getattr(model_config, key)
 
 
+def check_model(model_config, weights_only=False):
+    """Refuse configurations outside of the contract: it knows learned positions and one K/V head per query head, and,
+    for a comparison (not ``weights_only``), plain causal attention."""
+    def get(key, default):
+        value = model_config.get(key) if isinstance(model_config, dict) else getattr(model_config, key, None)
+        return default if value is None else value
+    if get("num_kv_heads", None) not in (None, get("num_attention_heads", None)):
+        raise ValueError("the shared contract has one K/V head per query head: num_kv_heads is not supported")
+    if get("position_embedding", "learned") != "learned":
+        raise ValueError("the shared contract has learned positions: position_embedding is not supported")
+    if not weights_only:
+        for key in ("attn_softcap", "eod_token"):
+            if get(key, None) is not None:
+                raise ValueError(f"the shared contract is plain causal attention: {key} is not supported")
+
+
 def full_parameter_names(model_config) -> list:
+    check_model(model_config, weights_only=True)
     L = _cfg(model_config, "num_layers")
     names = ["embedding.token_embedding.weight", "embedding.position_embedding.weight"]
     for i in range(L):
@@ -58,6 +75,7 @@ def full_parameter_names(model_config) -> list:
 
 def mcore_name_pairs(model_config) -> list:
     """[(name here / in the reference, Megatron-Core GPTModel name)]."""
+    check_model(model_config, weights_only=True)
     pairs = [("embedding.token_embedding.weight", "embedding.word_embeddings.weight"),
              ("embedding.position_embedding.weight", "embedding.position_embeddings.weight"),
              ("ln_f.weight", "decoder.final_layernorm.weight"),
@@ -74,7 +92,7 @@ def is_qkv(name: str) -> bool:
 
 
 def qkv_to_mcore(w: torch.Tensor, num_heads: int) -> torch.Tensor:
-    """Rows ``[all Q | all K | all V]`` -> Megatron-Core's per-head ``[Q_h K_h V_h]``."""
+    """Rows ``[all Q | all K | all V]`` (three equal parts) -> Megatron-Core's per-head ``[Q_h K_h V_h]``."""
     if w.dim() != 2 or w.size(0) % (3 * num_heads):
         raise ValueError("QKV weight must be 2-D with 3 * heads * head_dim rows")
     d = w.size(0) // (3 * num_heads)
@@ -179,6 +197,9 @@ def tp_unshard(shards: list, name: str) -> torch.Tensor:
 def mcore_tp_shard(full_ours: torch.Tensor, name: str, num_heads: int, tp: int, rank: int) -> torch.Tensor:
     """Megatron-Core's TP shard of an unsharded tensor given in this framework's layout."""
     if is_qkv(name):
+        if full_ours.dim() != 2 or full_ours.size(0) != 3 * full_ours.size(1):
+            raise ValueError(f"{name}: {tuple(full_ours.shape)} is not an unsharded [3 * hidden, hidden] QKV weight "
+                             "(shared K/V heads have fewer rows and no form in the shared contract)")
         mc = qkv_to_mcore(full_ours, num_heads)
         rows = mc.size(0) // tp
         return mc.narrow(0, rank * rows, rows).contiguous()
@@ -195,6 +216,7 @@ def stage_layer_range(num_layers: int, pp_rank: int, pp: int):
 
 def stage_parameter_plan(model_config, pp_rank: int, pp: int) -> list:
     """[(full name, stage-local name)] for the parameters stage ``pp_rank`` owns."""
+    check_model(model_config, weights_only=True)
     L = _cfg(model_config, "num_layers")
     start, end = stage_layer_range(L, pp_rank, pp)
     plan = []

@@ -365,3 +365,53 @@ def test_command_lines_end_to_end(tmp_path, capsys, monkeypatch):
     assert legacy.main(["synthetic", str(tmp_path / "syn.pt"), "--num-steps", "2", "--batch-size", "1",
                         "--seq-len", "8"]) == 0
     assert legacy.main(["identity", str(tmp_path / "syn.pt"), str(tmp_path / "id.pt")]) == 0
+
+
+# ----------------------------------------------------------------------------- models outside of the shared contract
+def test_contract_refuses_shared_heads():
+    """1.5 * hidden rows pass as three parts of half-sized heads: without a check the rows are scrambled."""
+    from mini_megatron_b200.config import GPTConfig
+    from mini_megatron_b200.models import build_gpt
+    cfg = GPTConfig(**{**TINY, "num_kv_heads": 1})
+    state = build_gpt(cfg).state_dict()
+    for config in (cfg, cfg.as_dict()):
+        for call in (lambda: contract.to_mcore_state(state, config), lambda: contract.from_mcore_state(state, config),
+                     lambda: contract.mcore_name_pairs(config), lambda: contract.full_parameter_names(config),
+                     lambda: contract.stage_parameter_plan(config, 0, 1),
+                     lambda: contract.shard_state(state, config, 1, 0)):
+            with pytest.raises(ValueError, match="num_kv_heads"):
+                call()
+    name = "decoder.layers.0.attn.qkv.weight"
+    assert state[name].size(0) % (3 * cfg.num_attention_heads) == 0
+    with pytest.raises(ValueError, match="unsharded"):
+        contract.mcore_tp_shard(state[name], name, cfg.num_attention_heads, 2, 0)
+
+
+def test_contract_refuses_other_positions_and_masks(tmp_path):
+    from mini_megatron_b200.config import GPTConfig
+    from mini_megatron_b200.harness import baselines
+    for kw, word in [(dict(position_embedding="rotary"), "position_embedding"),
+                     (dict(position_embedding="alibi"), "position_embedding"), (dict(num_kv_heads=2), "num_kv_heads"),
+                     (dict(attn_softcap=30.0), "attn_softcap"), (dict(eod_token=0), "eod_token")]:
+        cfg = GPTConfig(**{**TINY, **kw})
+        with pytest.raises(ValueError, match=word):
+            freeze(tmp_path / "artifact", cfg)
+        with pytest.raises(ValueError, match=word):
+            baselines.build_mcore_gpt(cfg.as_dict())
+        assert not (tmp_path / "artifact").exists()
+        if word == "position_embedding":
+            with pytest.raises(ValueError, match=word):
+                contract.full_parameter_names(cfg)
+
+
+def test_contract_takes_plain_models_as_before():
+    from mini_megatron_b200.config import GPTConfig
+    from mini_megatron_b200.models import build_gpt
+    cfg = GPTConfig(**{**TINY, "num_kv_heads": TINY["num_attention_heads"]})
+    state = build_gpt(cfg).state_dict()
+    for config in (cfg, cfg.as_dict(), GPTConfig(**TINY), TINY):
+        back = contract.from_mcore_state(contract.to_mcore_state(state, config), config)
+        assert set(back) == set(state) and all(torch.equal(back[k], state[k]) for k in state)
+    name = "decoder.layers.0.attn.qkv.weight"
+    parts = [contract.mcore_tp_shard(state[name], name, cfg.num_attention_heads, 2, r) for r in range(2)]
+    assert torch.equal(contract.qkv_from_mcore(torch.cat(parts), cfg.num_attention_heads), state[name])
