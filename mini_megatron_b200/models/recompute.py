@@ -8,7 +8,9 @@ import torch
 import torch.utils.checkpoint
 
 
-def checkpoint(layer, x):
+def checkpoint(layer, x, plan=None):
+    """``layer(x, plan=plan)`` that keeps only ``x`` (and the plan of packed rows) for the backward pass."""
     if x.is_cuda and hasattr(layer, "native_forward"):
-        return layer.native_forward(x, recompute=True)
-    return torch.utils.checkpoint.checkpoint(layer._forward, x, use_reentrant=False)
+        return layer.native_forward(x, recompute=True, plan=plan)
+    args = (x,) if plan is None else (x, plan)
+    return torch.utils.checkpoint.checkpoint(layer._forward, *args, use_reentrant=False)

@@ -297,3 +297,25 @@ def test_trainer_graph_recompute_and_eager_agree():
     for other in (("on", False), ("off", True)):
         for a, b in zip(runs["off", False], runs[other]):
             assert abs(a - b) < 2e-3 * abs(a), runs
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_recomputed_layer_takes_the_plan(device):
+    """A checkpointed layer attends inside the documents, like the layer itself."""
+    from mini_megatron_b200.models.recompute import checkpoint
+    from mini_megatron_b200.ops.documents import document_plan
+    from mini_megatron_b200.optim import make_param_buffer
+    layer = _build(_cfg(position_embedding="alibi", num_kv_heads=2)).decoder.layers[0].to(device)
+    if device == "cuda":
+        make_param_buffer(layer)
+    tokens = torch.randint(0, 9, (2, 140), generator=torch.Generator().manual_seed(2)).to(device)
+    plan = document_plan(tokens, eod=3)
+    x = torch.randn(2, 140, 256, generator=torch.Generator().manual_seed(3)).to(device)
+    outs = []
+    for run in (lambda z: layer(z, plan=plan), lambda z: checkpoint(layer, z, plan)):
+        leaf = x.clone().requires_grad_(True)
+        y = run(leaf)
+        (grad,) = torch.autograd.grad(y.square().sum(), leaf)
+        outs.append((y.detach(), grad))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert not torch.equal(outs[0][0], checkpoint(layer, x).detach())
