@@ -64,8 +64,8 @@ class Attention(nn.Module):
         if spec.alibi:
             from ..ops.attention import alibi_slopes
             first = pg.tp_rank() * self.num_heads
-            self.register_buffer("alibi_slopes", alibi_slopes(num_heads)[first:first + self.num_heads].clone(),
-                                 persistent=False)
+            self._slopes = alibi_slopes(num_heads)[first:first + self.num_heads].clone()
+            self.register_buffer("alibi_slopes", self._slopes.clone(), persistent=False)
         else:
             self.alibi_slopes = None
         # stride 3: each TP rank holds an equal subset of Q, K and V heads
@@ -73,6 +73,12 @@ class Attention(nn.Module):
                                         stride=3 if kv_heads == num_heads else 1,
                                         sequence_parallel=sequence_parallel)
         self.o = RowParallelLinear(hidden_size, hidden_size, bias=False, sequence_parallel=sequence_parallel)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.alibi_slopes is not None:  # constants of 32 bits, whatever type the parameters are turned into
+            self.alibi_slopes = self._slopes.to(self.alibi_slopes.device)
+        return self
 
     def plain(self, plan):
         """Whether this is causal attention without anything else."""

@@ -319,3 +319,15 @@ def test_recomputed_layer_takes_the_plan(device):
         outs.append((y.detach(), grad))
     assert all(torch.equal(a, b) for a, b in zip(*outs))
     assert not torch.equal(outs[0][0], checkpoint(layer, x).detach())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_slopes_keep_their_bits(dtype):
+    """Turning a model into another type does not round the distance bias: 12 slopes are no powers of two."""
+    from mini_megatron_b200.ops.attention import alibi_slopes
+    model = _build(_cfg(position_embedding="alibi", hidden_size=12 * 8, num_attention_heads=12))
+    for turned in (model.to(dtype), copy.deepcopy(model), model.float()):
+        for layer in turned.decoder.layers:
+            assert layer.attn.alibi_slopes.dtype == torch.float32
+            assert torch.equal(layer.attn.alibi_slopes, alibi_slopes(12))
+    assert not any("alibi" in k for k in model.state_dict())
