@@ -90,6 +90,8 @@ def parse_args(argv=None):
     p.add_argument("--weight-decay", type=float, default=cfgmod.WEIGHT_DECAY)
     p.add_argument("--save", type=str, default=None)
     p.add_argument("--load", type=str, default=None)
+    p.add_argument("--load-other-attention", action="store_true",
+                   help="load weights of a model with another attention variant (positions, cap, heads)")
     p.add_argument("--identity-labels", action="store_true", help="labels = tokens (the reference's default task)")
     p.add_argument("--reference-pp-semantics", action="store_true")
     return p.parse_args(argv)
@@ -163,7 +165,8 @@ def main(argv=None):
     mpu = trainer.mpu
     start_step = 0
     if args.load:
-        start_step = load_distributed_checkpoint(args.load, *trainer.state_for_checkpoint(), mpu=mpu, device=device)
+        start_step = load_distributed_checkpoint(args.load, *trainer.state_for_checkpoint(), mpu=mpu, device=device,
+                                                 allow_other_attention=args.load_other_attention)
     it = data_iterator(args, args.micro_batch_size, S, mcfg.vocab_size, mpu["dp_rank"], m)
     is_reporter = mpu["pp_rank"] == mpu["pp_size"] - 1 and mpu["tp_rank"] == 0 and mpu["dp_rank"] == 0
     warm = 0 if args.reference_pp_semantics else args.warmup_steps

@@ -56,6 +56,7 @@ class Attention(nn.Module):
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         if kv_heads != num_heads and tp > 1:
             raise ValueError("shared K/V heads need TP size 1: the QKV weight is sharded in equal Q, K and V parts")
+        self.all_heads, self.all_kv_heads = num_heads, kv_heads  # of every tensor-parallel rank together
         self.num_heads = num_heads // tp
         self.num_kv_heads = kv_heads // tp
         self.head_dim = hidden_size // num_heads
@@ -84,6 +85,12 @@ class Attention(nn.Module):
         """Whether this is causal attention without anything else."""
         return (plan is None and self.spec.rotary is None and not self.spec.alibi and self.spec.softcap is None
                 and self.num_kv_heads == self.num_heads)
+
+    def description(self):
+        """What the weights' shapes do not say about this attention, as plain values (tensor-parallel ranks agree)."""
+        rotary = self.spec.rotary
+        return dict(num_heads=self.all_heads, num_kv_heads=self.all_kv_heads, alibi=bool(self.spec.alibi),
+                    softcap=self.spec.softcap, rotary=None if rotary is None else rotary.description)
 
     def options(self, plan):
         """Arguments of the masked attention operators."""

@@ -50,6 +50,13 @@ class Rotary:
         if scaling == "yarn" and (not original_max_positions or not beta_fast > beta_slow > 0):
             raise ValueError("yarn scaling needs original_max_positions and beta_fast > beta_slow > 0")
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, bool(interleaved)
+        # what the rotation is a function of, for checkpoints
+        self.description = dict(rotary_dim=rotary_dim, base=float(base), interleaved=bool(interleaved), scaling=scaling)
+        if scaling is not None:
+            self.description["factor"] = float(factor)
+        if scaling == "yarn":
+            self.description.update(original_max_positions=original_max_positions, beta_fast=float(beta_fast),
+                                    beta_slow=float(beta_slow))
         self.magnitude = 1.0
         if scaling == "ntk":
             base = base * factor ** (rotary_dim / (rotary_dim - 2))

@@ -8,7 +8,8 @@ layout exactly (checkpoint.py:5-21): ``{"model_state", "optimizer_state",
 (dp, pp, tp) run needs: one file per (tp, pp) model shard written by DP rank
 0, one optimizer file per DP rank when the optimizer state is sharded
 (ZeRO-1), a JSON manifest with the topology and a SHA-256 of every file.  The
-loader validates the topology and the checksums and raises
+loader validates the topology, the checksums and the attention variant (heads,
+score cap, distance bias, rotary frequencies: what no weight's shape shows) and raises
 ``CheckpointError`` on any mismatch or truncated file.  Writes go to a
 temporary name and are renamed into place, so a crash never leaves a
 half-written file under the final name.  The bf16 GEMM shadows are rebuilt
@@ -85,6 +86,16 @@ def _topology(mpu):
     return {"tp": mpu["tp_size"], "pp": mpu["pp_size"], "dp": mpu["dp_size"]}
 
 
+def _attention(model):
+    """Descriptions of the model's attention layers, one of each kind, or None where there are none."""
+    from ..models.transformer import Attention
+    kinds = []
+    for m in model.modules():
+        if isinstance(m, Attention) and m.description() not in kinds:
+            kinds.append(m.description())
+    return kinds or None
+
+
 def save_distributed_checkpoint(directory, model, optimizer, scheduler, step, mpu=None, sharded_optimizer=False):
     """Write this rank's part of a distributed checkpoint.
 
@@ -115,7 +126,7 @@ def save_distributed_checkpoint(directory, model, optimizer, scheduler, step, mp
         written = {k: v for w in allw for k, v in w.items()}
     if not dist.is_initialized() or dist.get_rank() == 0:
         manifest = {"schema_version": SCHEMA_VERSION, "step": step, "topology": _topology(mpu),
-                    "sharded_optimizer": bool(sharded_optimizer), "files": written}
+                    "sharded_optimizer": bool(sharded_optimizer), "attention": _attention(model), "files": written}
         tmp = os.path.join(directory, "manifest.json.tmp")
         with open(tmp, "w") as f:
             json.dump(manifest, f, indent=1, sort_keys=True)
@@ -124,7 +135,14 @@ def save_distributed_checkpoint(directory, model, optimizer, scheduler, step, mp
         dist.barrier()
 
 
-def load_distributed_checkpoint(directory, model, optimizer, scheduler, mpu=None, device="cpu"):
+def load_distributed_checkpoint(directory, model, optimizer, scheduler, mpu=None, device="cpu",
+                                allow_other_attention=False):
+    """Load what :func:`save_distributed_checkpoint` wrote and return its step.
+
+    Weights of a model with another attention variant have the same shapes but another meaning: they are refused, unless
+    ``allow_other_attention`` says that the change is meant (stretched rotary positions, for one).  Checkpoints from
+    before the variant was recorded are loaded without this check.
+    """
     mpath = os.path.join(directory, "manifest.json")
     try:
         with open(mpath) as f:
@@ -135,6 +153,9 @@ def load_distributed_checkpoint(directory, model, optimizer, scheduler, mpu=None
         raise CheckpointError(f"unsupported checkpoint schema {manifest.get('schema_version')}")
     if manifest["topology"] != _topology(mpu):
         raise CheckpointError(f"checkpoint topology {manifest['topology']} != current {_topology(mpu)}")
+    saved, current = manifest.get("attention"), _attention(model)
+    if saved and current and saved != current and not allow_other_attention:
+        raise CheckpointError(f"checkpoint attention {saved} != the model's {current} (allow_other_attention loads it)")
     model_name, optim_name = _names(mpu)
     if not manifest["sharded_optimizer"]:
         optim_name = optim_name.rsplit("_dp", 1)[0] + "_dp000.pt"

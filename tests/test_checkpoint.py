@@ -175,3 +175,46 @@ def test_checkpoints_interchange_with_the_reference(tmp_path, direction):
     _train_one(dst_model, dst_opt, dst_sched)
     for a, b in zip(src_model.state_dict().values(), dst_model.state_dict().values()):
         torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-6)
+
+
+def test_checkpoints_of_another_attention_variant_are_refused(tmp_path):
+    """Cap, positions and head count leave the weights' shapes alone: the manifest says what they were trained with."""
+    import dataclasses
+    from mini_megatron_b200.config import PRESETS
+    from mini_megatron_b200.models import build_gpt
+    from mini_megatron_b200.utils.checkpoint import (CheckpointError, load_distributed_checkpoint,
+                                                     save_distributed_checkpoint)
+    rot = dict(position_embedding="rotary")
+    yarn = dict(rot, rotary_scaling="yarn", rotary_factor=4.0, rotary_original_max_positions=16)
+
+    def parts(kw):
+        torch.manual_seed(3)
+        model = build_gpt(dataclasses.replace(PRESETS["tiny"], **kw))
+        opt = torch.optim.SGD(model.parameters(), lr=1e-3)
+        return model, opt, torch.optim.lr_scheduler.LambdaLR(opt, lambda s: 1.0)
+
+    pairs = [(dict(), dict(attn_softcap=30.0)), (dict(attn_softcap=30.0), dict(attn_softcap=20.0)),
+             (dict(), dict(num_attention_heads=2)), (rot, dict(position_embedding="alibi")),
+             (rot, dict(rot, rotary_base=500000.0)), (rot, dict(rot, rotary_percent=0.5)),
+             (rot, dict(rot, rotary_interleaved=True)), (rot, yarn), (yarn, dict(yarn, rotary_factor=8.0))]
+    for k, (saved, other) in enumerate(pairs):
+        where = str(tmp_path / str(k))
+        save_distributed_checkpoint(where, *parts(saved), 5)
+        assert load_distributed_checkpoint(where, *parts(saved)) == 5
+        with pytest.raises(CheckpointError, match="attention"):
+            load_distributed_checkpoint(where, *parts(other))
+        assert load_distributed_checkpoint(where, *parts(other), allow_other_attention=True) == 5
+    # equal variants in other words; a manifest without the entry
+    where = str(tmp_path / "same")
+    save_distributed_checkpoint(where, *parts(rot), 6)
+    assert load_distributed_checkpoint(where, *parts(dict(rot, rotary_factor=4.0, num_kv_heads=4, eod_token=3))) == 6
+    man = json.load(open(tmp_path / "same" / "manifest.json"))
+    del man["attention"]
+    json.dump(man, open(tmp_path / "same" / "manifest.json", "w"))
+    assert load_distributed_checkpoint(where, *parts(dict(position_embedding="alibi"))) == 6
+
+
+def test_command_line_can_load_another_variant():
+    import main
+    assert main.parse_args([]).load_other_attention is False
+    assert main.parse_args(["--load-other-attention"]).load_other_attention is True
