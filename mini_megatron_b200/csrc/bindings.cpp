@@ -525,7 +525,8 @@ mmb::AttnCall attn_call(const Tensor& qkv, int64_t nh, int64_t nkv, int64_t d, c
   const int64_t B = qkv.size(0), S = qkv.size(1);
   TORCH_CHECK(qkv.size(2) == (nh + 2 * nkv) * d, "attention: qkv's last dimension must be (num_heads + 2 num_kv_heads)",
               " * head_dim = ", (nh + 2 * nkv) * d, ", got ", qkv.size(2));
-  TORCH_CHECK(S <= INT_MAX - 256 && B <= INT_MAX && nh <= 4096, "attention: at most 4096 heads, got ", nh);
+  TORCH_CHECK(S <= 128 * mmb::kAttnMaxTiles, "attention: rows of at most ", 128 * mmb::kAttnMaxTiles, " tokens, got ", S);
+  TORCH_CHECK(B <= INT_MAX && nh <= 4096, "attention: at most 4096 heads, got ", nh);
   // in 32 bits neither the scale nor its quotient by the cap overflows or vanishes
   TORCH_CHECK(scale >= 1e-15 && scale <= 1e15, "attention: softmax_scale must be from 1e-15 to 1e15, got ", scale);
   TORCH_CHECK(cap == 0 || (cap >= 1e-3 && cap <= 1000), "attention: softcap must be from 0.001 to 1000, got ", cap);
@@ -1117,6 +1118,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("masked_attn_fwd", &masked_attn_fwd, py::arg("qkv"), py::arg("num_heads"), py::arg("num_kv_heads"),
         py::arg("head_dim"), py::arg("tables"), py::arg("slopes"), py::arg("cap"),
         py::arg("scale"));
+  m.def("masked_attn_dkv_parts", &mmb::masked_attn_dkv_parts, py::arg("B"), py::arg("S"), py::arg("num_heads"),
+        py::arg("num_kv_heads"), py::arg("num_sms"), "shares that the query heads of a K/V head are cut into");
   m.def("masked_attn_bwd", &masked_attn_bwd, py::arg("dctx"), py::arg("qkv"), py::arg("ctx"), py::arg("lse"),
         py::arg("num_heads"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("tables"), py::arg("slopes"), py::arg("cap"), py::arg("scale"));
   m.def("flash_attn_fwd", &flash_attn_fwd);

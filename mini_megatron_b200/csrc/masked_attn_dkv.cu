@@ -545,15 +545,15 @@ __global__ void join_parts_kernel(const float* __restrict__ partial, int parts, 
 // joined afterwards.  One K/V head of 128 key tiles (S = 16384, 4 query heads) took 551 us as 128 items and
 // 247 us with the join as 512.
 //
-// An item of kMaxPairs (query head, query tile) pairs runs for about 0.4 s; waits for the end of an item give up
-// after 2 s, so longer ones are split too.
-static constexpr long kMaxPairs = 1 << 19;
+// Waits for the end of an item give up after 2 s.  A (query head, query tile) pair takes 1.2 us (d = 64) to 3.4 us (d = 128,
+// scores beyond the cap, distance bias), in loops of seconds under the power limit, so an item of kAttnMaxTiles of them ends
+// within 0.9 s; longer ones are split too.
 int masked_attn_dkv_parts(int B, int S, int nh, int nkv, int num_sms) {
   const long items = (long)B * nkv * ((S + mattn::BT - 1) / mattn::BT);
   const int group = nh / nkv;
   const long n_t = (S + mattn::BT - 1) / mattn::BT;
   for (int p = 1; p < group; ++p)
-    if (group % p == 0 && items * p >= 2L * num_sms && group / p * n_t <= kMaxPairs) return p;
+    if (group % p == 0 && items * p >= 2L * num_sms && group / p * n_t <= kAttnMaxTiles) return p;
   return group;
 }
 

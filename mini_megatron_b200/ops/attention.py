@@ -64,7 +64,7 @@ def attention_fwd(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, sof
 
     ``plan``: a :class:`~mini_megatron_b200.ops.documents.DocumentPlan` (default: causal).  ``softcap`` 0.001 to 1000,
     ``alibi_slopes`` ``[num_heads]`` fp32, ``softmax_scale`` (default ``head_dim ** -0.5``).  On CUDA: bf16, head_dim
-    64 or 128, up to 4096 heads, any length, rows on 16-byte boundaries.
+    64 or 128, up to 4096 heads, rows of up to 32 Mi tokens (2 Mi with a plan) on 16-byte boundaries.
 
     Everything in ``qkv`` must be finite, padding too: what a token does not see counts with weight 0, and 0 times an
     infinity or NaN is NaN.  Statistics and sums are 32-bit; the weights, and in the backward pass the scores'

@@ -383,3 +383,29 @@ def test_tensors_off_the_16_byte_boundary_are_refused():
         tables = torch.zeros(plan.tables.numel() + 4, device="cuda", dtype=torch.int32)[off:off + plan.tables.numel()]
         with pytest.raises(RuntimeError, match="16-byte"):
             attention_fwd(qkv, nh, d, plan=DocumentPlan(plan.positions, plan.start, plan.end, tables))
+
+
+@pytest.mark.gpu
+def test_rows_whose_items_outlast_the_waits_are_refused():
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    qkv = torch.empty(1, 2 ** 25 + 1, 192, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="tokens"):
+        attention_fwd(qkv, 1, 64)
+    ctx = qkv[..., :64]
+    with pytest.raises(RuntimeError, match="tokens"):
+        attention_bwd(ctx, qkv, ctx, torch.empty(1, 1, 8, device="cuda"), 1, 64)
+
+
+def test_shares_of_query_heads():
+    """The cut of a K/V head's query heads: whole heads, items that end well before a wait gives up, work for every SM."""
+    native = pytest.importorskip("mini_megatron_b200._C", reason="extension not built")
+    for S in (1, 128, 129, 1999, 4096, 16384, 2 ** 17, 2 ** 21, 2 ** 25):
+        for nkv in (1, 2, 3, 8, 64):
+            for group in (1, 2, 3, 4, 6, 8, 16, 32, 60, 64, 4096 // nkv):
+                for B in (1, 3, 40):
+                    n_t = (S + 127) // 128
+                    parts = native.masked_attn_dkv_parts(B, S, nkv * group, nkv, 148)
+                    assert 1 <= parts <= group and group % parts == 0
+                    assert group // parts * n_t <= 2 ** 18
+                    smaller = [p for p in range(1, parts) if group % p == 0]
+                    assert all(B * nkv * n_t * p < 2 * 148 or group // p * n_t > 2 ** 18 for p in smaller)
