@@ -409,3 +409,36 @@ def test_shares_of_query_heads():
                     assert group // parts * n_t <= 2 ** 18
                     smaller = [p for p in range(1, parts) if group % p == 0]
                     assert all(B * nkv * n_t * p < 2 * 148 or group // p * n_t > 2 ** 18 for p in smaller)
+
+
+# B, S, nh, nkv, d, mean document, prefix, pad, cap, alibi, shares (148 SMs)
+SHARED = [
+    (3, 1999, 16, 4, 64, 700, True, True, 0.0, True, 2),
+    (3, 1999, 16, 4, 128, 700, False, True, 30.0, False, 2),
+    (2, 2000, 24, 2, 64, None, False, False, 20.0, True, 6),
+    (2, 2000, 48, 4, 64, 400, False, True, 0.0, False, 3),
+    (1, 1999, 48, 8, 128, 500, True, False, 0.0, True, 3),
+    (1, 1200, 64, 8, 128, None, False, False, 0.0, True, 4),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,nh,nkv,d,doc,prefix,pad,cap,alibi,shares", SHARED)
+def test_some_of_a_group_in_every_share(B, S, nh, nkv, d, doc, prefix, pad, cap, alibi, shares):
+    """Items that walk several query heads and leave their sums to be joined."""
+    from mini_megatron_b200.ops import check_errors, native
+    from mini_megatron_b200.ops.attention import attention_bwd, attention_fwd
+    assert native().masked_attn_dkv_parts(B, S, nh, nkv, native().num_sms()) == shares and 1 < shares < nh // nkv
+    qkv, dctx, plan, start, end = _case(B, S, nh, nkv, d, doc, prefix, pad, 1.5, "cuda", torch.bfloat16, seed=11)
+    slopes = _slopes(nh, "cuda") if alibi else None
+    opts = dict(num_kv_heads=nkv, plan=plan, softcap=cap or None, alibi_slopes=slopes)
+    ctx, lse = attention_fwd(qkv, nh, d, **opts)
+    dqkv = attention_bwd(dctx, qkv, ctx, lse, nh, d, **opts)
+    check_errors()
+    for b in range(B):   # a row at a time: the 64-bit form holds several [S, S] tensors a head
+        s, e = (None, None) if start is None else (start[b:b + 1], end[b:b + 1])
+        (r_ctx, r_lse, r_grad), (b_ctx, b_lse, b_grad) = attention_ref(qkv[b:b + 1], dctx[b:b + 1], nh, nkv, d, s, e,
+                                                                      cap, slopes)
+        _near(ctx[b:b + 1], r_ctx, b_ctx, "ctx")
+        _near(lse[b:b + 1], r_lse, b_lse, "lse")
+        _near(dqkv[b:b + 1], r_grad, b_grad, "dqkv")
