@@ -61,31 +61,36 @@ def _whole(name):
     return model.state_dict(), logits.detach(), {n: p.grad for n, p in model.named_parameters()}
 
 
-def _tp_worker(rank, world, name, sp, state):
+def _tp_worker(rank, world, sp, states):
     from mini_megatron_b200.models import build_gpt
     from mini_megatron_b200.parallel import process_groups as pg
     from mini_megatron_b200.parallel.data_parallel import allreduce_sequence_parallel_grads
     mpu = pg.init_model_parallel(world, 1, sp)
     pg.set_model_parallel(mpu)
-    model = build_gpt(_config(name)).double()
-    model.load_state_dict({n: _shard(state[n], n, world, rank) for n in model.state_dict()})
     tokens, dlogits = _batch()
-    logits = model(tokens)
-    logits.backward(dlogits.chunk(world, -1)[rank])
-    if sp:
-        allreduce_sequence_parallel_grads([p for p in model.parameters() if getattr(p, "sequence_parallel_grad", False)],
-                                          mpu["tp_group"])
+    out = {}
+    for name, state in states.items():
+        model = build_gpt(_config(name)).double()
+        model.load_state_dict({n: _shard(state[n], n, world, rank) for n in model.state_dict()})
+        logits = model(tokens)
+        logits.backward(dlogits.chunk(world, -1)[rank])
+        if sp:
+            allreduce_sequence_parallel_grads([p for p in model.parameters()
+                                               if getattr(p, "sequence_parallel_grad", False)], mpu["tp_group"])
+        out[name] = logits.detach(), {n: p.grad for n, p in model.named_parameters()}
     pg.set_model_parallel(None)
-    return logits.detach(), {n: p.grad for n, p in model.named_parameters()}
+    return out
 
 
 @pytest.mark.parametrize("sp", [False, True])
-@pytest.mark.parametrize("name", sorted(VARIANTS))
-def test_two_tensor_parallel_ranks(name, sp):
-    state, want, grads = _whole(name)
-    for rank, (logits, got) in enumerate(run_ranks(_tp_worker, 2, name, sp, state)):
-        # sums of about a hundred terms in 64 bits, in another order: 2^-53 * 100 a step, a dozen steps
-        torch.testing.assert_close(logits, want.chunk(2, -1)[rank], rtol=1e-9, atol=1e-9)
-        assert set(got) == set(grads)
-        for n, g in got.items():
-            torch.testing.assert_close(g, _shard(grads[n], n, 2, rank), rtol=1e-9, atol=1e-9, msg=n)
+def test_two_tensor_parallel_ranks(sp):
+    whole = {name: _whole(name) for name in VARIANTS}
+    results = run_ranks(_tp_worker, 2, sp, {name: w[0] for name, w in whole.items()})
+    for rank, result in enumerate(results):
+        for name, (logits, got) in result.items():
+            _, want, grads = whole[name]
+            # sums of about a hundred terms in 64 bits, in another order: 2^-53 * 100 a step, a dozen steps
+            torch.testing.assert_close(logits, want.chunk(2, -1)[rank], rtol=1e-9, atol=1e-9, msg=name)
+            assert set(got) == set(grads)
+            for n, g in got.items():
+                torch.testing.assert_close(g, _shard(grads[n], n, 2, rank), rtol=1e-9, atol=1e-9, msg=f"{name} {n}")
