@@ -30,14 +30,30 @@ int num_sms() {
   return n;
 }
 
-// One device error word per device; kernels record bounded-wait timeouts here.
+// One device error word per device; kernels record bounded-wait timeouts here.  It is allocated and cleared outside of
+// any stream, so that a first call inside a graph capture neither puts the word into the graph's memory nor has every
+// replay clear what earlier kernels recorded.
 int* error_word() {
-  static std::vector<Tensor> words;
+  static std::vector<int*> words;
   const int dev = at::cuda::current_device();
-  if ((int)words.size() <= dev) words.resize(dev + 1);
-  if (!words[dev].defined())
-    words[dev] = at::zeros({4}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, dev));
-  return words[dev].data_ptr<int>();
+  if ((int)words.size() <= dev) words.resize(dev + 1, nullptr);
+  if (!words[dev]) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    int* word = nullptr;
+    cudaStream_t side = nullptr;
+    cudaError_t e = cudaMalloc(&word, 4 * sizeof(int));
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, 4 * sizeof(int), side);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(side);
+    if (side) cudaStreamDestroy(side);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess && word) cudaFree(word);
+    C10_CUDA_CHECK(e);
+    C10_CUDA_CHECK(back);
+    words[dev] = word;
+  }
+  return words[dev];
 }
 
 int64_t get_error() {

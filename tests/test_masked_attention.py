@@ -442,3 +442,42 @@ def test_some_of_a_group_in_every_share(B, S, nh, nkv, d, doc, prefix, pad, cap,
         _near(ctx[b:b + 1], r_ctx, b_ctx, "ctx")
         _near(lse[b:b + 1], r_lse, b_lse, "lse")
         _near(dqkv[b:b + 1], r_grad, b_grad, "dqkv")
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+from mini_megatron_b200.ops import check_errors, native
+from mini_megatron_b200.ops.attention import attention_fwd
+x = torch.randn(1, 300, 192, device="cuda").bfloat16()
+junk = [torch.full((4,), 77, device="cuda", dtype=torch.int32) for _ in range(8)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ctx, lse = attention_fwd(x, 1, 64)
+check_errors()                       # nothing has run yet
+native().set_error(7)
+g.replay()
+torch.cuda.synchronize()
+assert native().get_error() == 7     # a replay does not clear what was recorded before it
+native().clear_error()
+g.replay()
+check_errors()
+want = attention_fwd(x, 1, 64)
+assert torch.equal(ctx, want[0]) and torch.equal(lse, want[1])
+del g, ctx, lse
+torch.cuda.empty_cache()
+attention_fwd(x, 1, 64)
+check_errors()
+print("fine")
+"""
+
+
+@pytest.mark.gpu
+def test_first_call_inside_a_capture_keeps_the_error_word():
+    """In a process of its own: the word that kernels report to does not belong to the graph."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], capture_output=True, text=True, timeout=300,
+                         cwd=root, env=dict(os.environ, PYTHONPATH=root))
+    assert run.returncode == 0 and run.stdout.strip() == "fine", run.stdout + run.stderr
