@@ -231,6 +231,7 @@ void embedding_fwd(const Tensor& ids, const Tensor& wte, const c10::optional<Ten
   const float* p = nullptr;
   if (wpe.has_value()) {
     check_f32(*wpe, "wpe");
+    TORCH_CHECK(S <= wpe->size(0), "rows of ", S, " tokens are longer than the position table (", wpe->size(0), ")");
     p = wpe->data_ptr<float>();
   }
   const int rc = mmb::embedding_fwd(ids.data_ptr<int64_t>(), wte.data_ptr<float>(), p, out.data_ptr<float>(),
@@ -245,6 +246,7 @@ void embedding_bwd(const Tensor& ids, const Tensor& dout, Tensor& dwte, const c1
   float* p = nullptr;
   if (dwpe.has_value()) {
     check_f32(*dwpe, "dwpe");
+    TORCH_CHECK(S <= dwpe->size(0), "rows of ", S, " tokens are longer than the position table (", dwpe->size(0), ")");
     p = dwpe->data_ptr<float>();
   }
   const int rc = mmb::embedding_bwd(ids.data_ptr<int64_t>(), dout.data_ptr<float>(), dwte.data_ptr<float>(), p,

@@ -331,3 +331,19 @@ def test_slopes_keep_their_bits(dtype):
             assert layer.attn.alibi_slopes.dtype == torch.float32
             assert torch.equal(layer.attn.alibi_slopes, alibi_slopes(12))
     assert not any("alibi" in k for k in model.state_dict())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_rows_longer_than_the_position_table_are_refused(device):
+    """Any row length runs, but a learned table ends at max_seq_len; models without one have no such end."""
+    ids = torch.zeros(1, 300, dtype=torch.int64, device=device)
+    model = _build(_cfg(max_seq_len=256)).to(device)
+    with pytest.raises((IndexError, RuntimeError)):
+        model(ids)
+    assert model(ids[:, :256]).shape[:2] == (1, 256)
+    if device == "cuda":
+        from mini_megatron_b200.ops import native
+        dwte, dwpe = torch.zeros(512, 256, device=device), torch.zeros(256, 256, device=device)
+        with pytest.raises(RuntimeError, match="position table"):
+            native().embedding_bwd(ids.view(-1), torch.zeros(300, 256, device=device), dwte, dwpe, 1, 300, 0, 512)
+    assert _build(_cfg(max_seq_len=256, position_embedding="rotary")).to(device)(ids).shape[:2] == (1, 300)
