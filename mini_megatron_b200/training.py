@@ -130,7 +130,7 @@ class Trainer:
         pg.set_model_parallel(self.mpu)
         mpu = self.mpu
         self.seq_len = cfg.seq_len or cfg.model.max_seq_len
-        if self.seq_len > cfg.model.max_seq_len:
+        if self.seq_len > cfg.model.max_seq_len and cfg.model.position_embedding == "learned":
             raise ValueError("seq_len exceeds the position table")
         sp = self.mpu["sequence_parallel"]
         if sp and self.seq_len % cfg.tp:

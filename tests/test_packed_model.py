@@ -347,3 +347,17 @@ def test_rows_longer_than_the_position_table_are_refused(device):
         with pytest.raises(RuntimeError, match="position table"):
             native().embedding_bwd(ids.view(-1), torch.zeros(300, 256, device=device), dwte, dwpe, 1, 300, 0, 512)
     assert _build(_cfg(max_seq_len=256, position_embedding="rotary")).to(device)(ids).shape[:2] == (1, 300)
+
+
+def test_trainer_row_length_without_a_position_table():
+    from mini_megatron_b200.parallel import process_groups as pg
+    from mini_megatron_b200.training import TrainConfig, Trainer, synthetic_batch
+    small = dict(num_layers=1, hidden_size=32, num_attention_heads=2, ffn_hidden_size=64, max_seq_len=16, vocab_size=50)
+    for pos in ("rotary", "alibi"):
+        t = Trainer(TrainConfig(model=_cfg(**small, position_embedding=pos), micro_batch_size=2, seq_len=24), device="cpu")
+        assert torch.isfinite(t.train_step(*synthetic_batch(1, 2, 24, 50)))
+        t.destroy()
+        pg.set_model_parallel(None)
+    with pytest.raises(ValueError, match="position table"):
+        Trainer(TrainConfig(model=_cfg(**small), micro_batch_size=2, seq_len=24), device="cpu")
+    pg.set_model_parallel(None)
