@@ -62,7 +62,8 @@ class GPTConfig:
     rotary_factor: float = 1.0               # ... by this factor
     rotary_original_max_positions: int | None = None
     attn_softcap: float | None = None        # scores become cap * tanh(score / cap)
-    eod_token: int | None = None             # rows are packed documents that end with this token
+    eod_token: int | None = None             # rows are packed documents that end with this token (learned
+                                             # positions still count along the row, rotary ones restart)
 
     @property
     def head_dim(self) -> int:
@@ -84,7 +85,9 @@ class GPTConfig:
         return L * per_layer + 2 * v * h + table + 2 * h
 
     def flops_per_token(self, seq_len: int) -> float:
-        """Training FLOPs per token (fwd + bwd, causal attention counted at half)."""
+        """Training FLOPs per token (fwd + bwd, causal attention counted at half).
+
+        Every row counts as one document: for packed documents, which see less, this is an upper bound."""
         h, f, L, v = self.hidden_size, self.ffn_hidden_size, self.num_layers, self.vocab_size
         qkv = (self.num_attention_heads + 2 * self.kv_heads) * self.head_dim
         dense = 2 * (qkv * h + h * h + 2 * h * f) * L + 2 * h * v

@@ -243,7 +243,9 @@ class GPT(nn.Module):
     overwritten by its gradient during backward.
 
     With ``eod_token`` rows are packed documents: attention stays inside a document
-    and rotary positions restart with it.  ``forward(..., plan=...)`` takes another
+    and rotary positions restart with it.  A learned position table does not: its rows
+    are those of the index in the row, so a document's logits depend on where it lies
+    (with rotary positions or a distance bias they are the ones it has alone).  ``forward(..., plan=...)`` takes another
     :class:`~mini_megatron_b200.ops.documents.DocumentPlan` instead (prefixes, padding).
     """
 

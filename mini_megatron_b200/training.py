@@ -61,7 +61,10 @@ def make_lr_lambda(warmup_steps, num_steps):
 
 
 def compute_mfu(model, seq_len, micro_batch_size, tp, pp, elapsed, num_steps, peak_flops=None):
-    """Reference MFU formula (main.py:46-66) with the peak as a parameter (B200 dense bf16 by default)."""
+    """Reference MFU formula (main.py:46-66) with the peak as a parameter (B200 dense bf16 by default).
+
+    It counts whole rows and as many K/V heads as query heads: with packed documents or shared heads it reads too high.
+    """
     L, h, V = model["num_layers"], model["hidden_size"], model["vocab_size"]
     B, s = micro_batch_size, seq_len
     ws = int(os.environ.get("WORLD_SIZE", "1"))

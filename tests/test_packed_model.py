@@ -361,3 +361,18 @@ def test_trainer_row_length_without_a_position_table():
     with pytest.raises(ValueError, match="position table"):
         Trainer(TrainConfig(model=_cfg(**small), micro_batch_size=2, seq_len=24), device="cpu")
     pg.set_model_parallel(None)
+
+
+def test_learned_positions_count_along_a_packed_row():
+    """A document behind others gets the logits that it has alone with the table's rows from where it begins."""
+    model = _build(_cfg(eod_token=3)).double()
+    g = torch.Generator().manual_seed(5)
+    docs = [torch.cat([torch.randint(4, 500, (n - 1,), generator=g), torch.tensor([3])]) for n in (9, 1, 30)]
+    logits = model(torch.cat(docs)[None])[0].detach()
+    table = model.embedding.position_embedding.weight
+    rows, at = table.detach().clone(), 0
+    for doc in docs:
+        with torch.no_grad():
+            table.copy_(rows.roll(-at, 0))
+        torch.testing.assert_close(logits[at:at + len(doc)], model(doc[None])[0].detach(), rtol=1e-9, atol=1e-9)
+        at += len(doc)
