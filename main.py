@@ -71,7 +71,8 @@ def parse_args(argv=None):
     p.add_argument("--rotary-factor", type=float, help="how far --rotary-scaling stretches the original positions")
     p.add_argument("--rotary-original-max-positions", type=int)
     p.add_argument("--attn-softcap", type=float, help="cap attention scores: cap * tanh(score / cap)")
-    p.add_argument("--eod-token", type=int, help="rows are packed documents that end with this token (pp = 1; learned positions count along the row)")
+    p.add_argument("--eod-token", type=int, help="rows are packed documents that end with this token (pp = 1; learned "
+                                                 "positions count along the row)")
     p.add_argument("--num-microbatches", type=int, default=1)
     p.add_argument("--sequence-parallel", action="store_true")
     p.add_argument("--zero1", action="store_true")

@@ -44,8 +44,10 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 // predecessor.  Each kernel calls pdl_wait() before its first global-memory
 // access, which blocks until the previous grid has completed and its writes
 // are visible, so the data dependencies are those of plain stream order.
-// Both instructions are no-ops for a grid launched without the attribute.
-// The kernels of packed rows (document_plan.cu, rotary.cu, masked_attn_*.cu) are always launched so.
+// The attribute belongs to the kernel that is launched early: pdl_wait() does
+// nothing in a plainly launched grid, but its pdl_trigger() lets a following
+// kernel that carries the attribute be set up while it still runs.
+// The kernels of packed rows (document_plan.cu, rotary.cu, masked_attn_*.cu) always carry it.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

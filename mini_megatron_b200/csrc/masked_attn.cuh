@@ -17,13 +17,16 @@
 // Roundings to 16 bits, besides the outputs: P, as operand of P V and of dV, and dS, as operand of dQ and dK.  The other
 // operand of each of these products is bf16 and the tensor cores take pairs of one type; in 32 bits (tf32) the
 // products would take twice the time and P and dS twice the TMEM columns, which are all in use.  Delta is taken from ctx as
-// it was returned, rounded: the unrounded one would take another pass over the tiles.  Against 64 bits the outputs are
+// it was returned, rounded.  The forward's epilogue has the unrounded O and could write what the rounding took off as a
+// second bf16 tensor for row_stats to add (25 MB each way at 16 x 1024 tokens, 12 heads of 64: about 8 us of 210); it does
+// not, because the backward is a function of ctx and lse alone.  Against 64 bits the outputs are
 // off by 0.0021 to 0.0036 (norm of the error over the norm): one rounding of the outputs makes 0.0017, P and dS 0.0016, Delta
 // 0.0005 with even weights to 0.0019 with sharp ones.
 //
 // These kernels, row_stats, rotary and the plans are launched early (launch_early): barriers, TMEM and the first
 // instructions are set up behind the predecessor's last CTAs.  Short calls are made of that: forward and backward of 2
-// rows of a few hundred tokens 28.8 -> 20.7 us, S = 16384 719 -> 702 us.  An early CTA holds all of its SM's TMEM while it
+// rows of 77 tokens 28.7 -> 22.5 us, S = 16384 719 -> 702 us.  The predecessor may be any kernel that triggers, plainly
+// launched ones among them; all of its CTAs have started by then.  An early CTA holds all of its SM's TMEM while it
 // waits; the predecessor cannot be kept from its own by that, because no kernel that uses TMEM fits beside 200 KB
 // of shared memory on one SM.
 #pragma once
@@ -185,7 +188,8 @@ __device__ __forceinline__ float2 cap_tanh(float2 s, const Score& k) {
   const float2 e = add2(exp2_pair(mul2(s, pair(k.twice))), pair(1.f));
   return fma2(make_float2(rcp_approx(e.x), rcp_approx(e.y)), pair(-2.f), pair(1.f));
 }
-// Whether every |u| of the warp's N scores a thread is at most 1 (false for a NaN).
+// Whether every |u| of the warp's N scores a thread is at most 1.  The maximum passes over a NaN, which may so be taken for
+// a small score; either form of tanh keeps it a NaN.
 template <int N>
 __device__ __forceinline__ bool cap_small(const uint32_t (&s)[N], const Score& k) {
   float m[4] = {0.f, 0.f, 0.f, 0.f};

@@ -40,7 +40,10 @@ def flash_attn_bwd(dctx, qkv, ctx, lse, B, S, nh, d):
 
 
 def alibi_slopes(num_heads):
-    """``[num_heads]`` fp32: ``2 ** (-8 (h + 1) / num_heads)``, the geometric slopes of linear distance biases."""
+    """``[num_heads]`` fp32: ``2 ** (-8 (h + 1) / num_heads)``, the geometric slopes of linear distance biases.
+
+    The series is the same for every head count; models whose slopes for a count that is no power of two were taken
+    from the series of neighbouring powers pass their own."""
     return torch.tensor([2.0 ** (-8.0 * (h + 1) / num_heads) for h in range(num_heads)], dtype=torch.float32)
 
 
@@ -68,7 +71,8 @@ def attention_fwd(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, sof
 
     Everything in ``qkv`` must be finite, padding too: what a token does not see counts with weight 0, and 0 times an
     infinity or NaN is NaN.  Statistics and sums are 32-bit; the weights, and in the backward pass the scores'
-    gradients, are rounded to bf16 once, as operands of the tensor cores.
+    gradients, are rounded to bf16 once, as operands of the tensor cores.  On CUDA autograd does not see this call:
+    :func:`attention` is the differentiable form.
     """
     nkv, cap, scale = _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale)
     if not qkv.is_cuda:
@@ -80,7 +84,7 @@ def attention_fwd(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, sof
 def attention_bwd(dctx, qkv, ctx, lse, num_heads, head_dim, *, num_kv_heads=None, plan=None, softcap=None,
                   alibi_slopes=None, softmax_scale=None):
     """``dqkv`` (layout of ``qkv``, contiguous) from the gradient of ``ctx`` and what :func:`attention_fwd` returned.
-    CUDA only.  The same inputs give the same bits: no atomics."""
+    CUDA only.  The same inputs give the same bits: no atomics.  ``dctx`` has to be finite in padding too, like ``qkv``."""
     nkv, cap, scale = _options(qkv, num_heads, head_dim, num_kv_heads, plan, softcap, alibi_slopes, softmax_scale)
     return native().masked_attn_bwd(dctx, qkv, ctx, lse, num_heads, nkv, head_dim, None if plan is None else plan.tables,
                                     alibi_slopes, cap, scale)
