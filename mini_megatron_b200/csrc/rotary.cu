@@ -19,6 +19,7 @@
 // 16 x 1024 tokens of 36 heads of 64 in bf16, 24 of them rotated (151 MB): 28.0 us,
 // 5.4 TB/s; 28.5 with 2 tokens, 29.5 with 256 threads, 32.8 with 256 threads, the
 // angles first and the token's row found anew for every unit.  40 registers: 35 us.
+// The same in fp32 (302 MB): 50.2 us, 6.0 TB/s.
 #include "common.cuh"
 #include "ops.h"
 
