@@ -25,7 +25,7 @@ CLASSIFIERS = (
     ("fused_dp_optimizer", re.compile(r"dp_rs_adamw_ag", re.I)),
     ("fused_tp_collective", re.compile(r"tp_rs_reduce|tp_ag_push|ln_fwd_push|EPI_PUSH|, 7>", re.I)),
     ("fused_adamw", re.compile(r"adamw_kernel|FusedAdamMathFunctor|multi_tensor_apply_kernel", re.I)),
-    ("attention", re.compile(r"flash|fmha|scaled_dot_product|attn_", re.I)),
+    ("attention", re.compile(r"flash|fmha|scaled_dot_product|attn_|mattn::|rope::|docplan::", re.I)),
     ("gemm", re.compile(r"gemm|cutlass|cublas|nvjet|matmul|sm100_xmma|sm90_xmma", re.I)),
     ("layernorm", re.compile(r"ln_fwd|ln_bwd|ln_param|layer_norm|LayerNorm|GammaBeta", re.I)),
     ("cross_entropy", re.compile(r"ce_fwd|ce_bwd|cross_entropy|SoftMax|softmax|nll_loss", re.I)),

@@ -415,3 +415,12 @@ def test_contract_takes_plain_models_as_before():
     name = "decoder.layers.0.attn.qkv.weight"
     parts = [contract.mcore_tp_shard(state[name], name, cfg.num_attention_heads, 2, r) for r in range(2)]
     assert torch.equal(contract.qkv_from_mcore(torch.cat(parts), cfg.num_attention_heads), state[name])
+
+
+@pytest.mark.parametrize("name", ["void mmb::mattn::fwd::masked_attn_fwd_kernel<64, false, false>(...)",
+                                  "void mmb::mattn::dq::row_stats_kernel<64>(...)",
+                                  "mmb::mattn::dkv::join_parts_kernel(...)",
+                                  "void mmb::rope::rotary_kernel<__nv_bfloat16, true>(...)",
+                                  "mmb::docplan::document_plan_kernel(...)", "mmb::docplan::plan_order_kernel(...)"])
+def test_kernels_of_packed_rows_are_classified(name):
+    assert kernels.classify(name) == "attention"
