@@ -70,7 +70,9 @@ def attention_fwd(qkv, num_heads, head_dim, *, num_kv_heads=None, plan=None, sof
     64 or 128, up to 4096 heads, rows of up to 32 Mi tokens (2 Mi with a plan) on 16-byte boundaries.
 
     Everything in ``qkv`` must be finite, padding too: what a token does not see counts with weight 0, and 0 times an
-    infinity or NaN is NaN.  Statistics and sums are 32-bit; the weights, and in the backward pass the scores'
+    infinity or NaN is NaN.  Scores are 32-bit: one of size x is known to x / 2^24.  The gradients take the weights from
+    ``lse``, so x / 2^22 is their relative error as well, below bf16's for scores up to 10^4; ctx and lse are right up to
+    10^8, and from 2^31 on nothing is.  Statistics and sums are 32-bit; the weights, and in the backward pass the scores'
     gradients, are rounded to bf16 once, as operands of the tensor cores.  On CUDA autograd does not see this call:
     :func:`attention` is the differentiable form.
     """

@@ -481,3 +481,33 @@ def test_first_call_inside_a_capture_keeps_the_error_word():
     run = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], capture_output=True, text=True, timeout=300,
                          cwd=root, env=dict(os.environ, PYTHONPATH=root))
     assert run.returncode == 0 and run.stdout.strip() == "fine", run.stdout + run.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e8])
+@pytest.mark.parametrize("alibi", [False, True])
+def test_very_large_scores(d, size, alibi):
+    """Rows whose scores lie far apart see one key: ctx is its value and lse its score, however large the scores."""
+    from mini_megatron_b200.ops.attention import attention_fwd
+    qkv, _, plan, start, end = _case(2, 500, 2, 1, d, 200, True, True, 1.0, "cuda", torch.bfloat16, seed=21)
+    slopes = _slopes(2, "cuda") if alibi else None
+    scale = size / 4 / d ** 0.5          # q.k is a normal number times sqrt(d): the largest of a row about 4
+    ctx, lse = attention_fwd(qkv, 2, d, num_kv_heads=1, plan=plan, alibi_slopes=slopes, softmax_scale=scale)
+    q, k, v = (t.double() for t in qkv.view(2, 500, 4, d).transpose(1, 2).split([2, 1, 1], 1))
+    at = torch.arange(500, device="cuda")
+    x = q @ k.transpose(-1, -2) * scale
+    if alibi:
+        x = x - slopes.double().view(2, 1, 1) * (at[:, None] - at).abs()
+    x = x.masked_fill(~((at >= start[..., None]) & (at < end[..., None]))[:, None], float("-inf"))
+    top = x.topk(2, -1)
+    # a 32-bit sum of d products and the scaling: off by at most 2^-23 (d + 4) of the products' size, which is below 64 d^0.5
+    off = 2.0 ** -23 * (d + 4) * scale * 64 * d ** 0.5
+    clear = top.values[..., 0] - top.values[..., 1] > 2 * off + 20   # the second key weighs less than e^-20
+    assert clear.sum() > 0.8 * 2 * (end > start).sum()
+    want = v.expand(2, 2, 500, d).gather(2, top.indices[..., :1].expand(-1, -1, -1, d))
+    got = ctx.view(2, 500, 2, d).transpose(1, 2).double()
+    err = (got - want).abs()
+    # the key's weight and ctx are rounded once each
+    assert (err <= 2.02 * 2.0 ** -8 * want.abs() + 2.0 ** -20)[clear].all()
+    assert ((lse.double() - top.values[..., 0]).abs() <= off + 2.0 ** -21 * top.values[..., 0].abs() + 1e-6)[clear].all()
